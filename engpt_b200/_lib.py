@@ -61,6 +61,13 @@ SIGNATURES = {
     "engpt_project_row_grad": (_i, [_p, _p, _i, _i64, _i64, _p]),
     "engpt_project_column_grad": (_i, [_p, _p, _i, _i64, _i64, _p, _p]),
     "engpt_column_scratch_floats": (_i64, [_i64, _i64]),
+    "engpt_advance_block_tables": (_i, [_p, _p, _p, _i, _p, _i64, _i, _p, _i, _p, _i, _i, _p, _p, _p]),
+    "engpt_qkv_append": (_i, [_p, _i, _p, _p, _p, _i, _i, _p, _f, _f, _i64, _i, _i, _p, _p, _p, _p, _p, _p, _i, _i,
+                              _p]),
+    "engpt_write_kv_pages": (_i, [_p, _p, _p, _i, _i64, _i, _i, _p, _p, _p, _p, _i, _i, _p]),
+    "engpt_paged_attention_floats": (_i64, [_i, _i, _i, _i, _i, _i, _i]),
+    "engpt_paged_attention": (_i, [_p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _i64, _i, _p, _f, _p, _p,
+                                   _p]),
 }
 CE_NOALLOC_MAX_ROWS = 262144
 

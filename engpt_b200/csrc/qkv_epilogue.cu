@@ -32,6 +32,39 @@ struct QkvArgs {
   int layout;  // ENGPT_QKV_BTHD, ENGPT_QKV_BHTD or ENGPT_QKV_INPLACE
 };
 
+// Where the tokens of engpt_qkv_append stand and where their k and v go (q goes to QkvArgs::q, [n, H, Dh]).
+struct PagedDst {
+  const int* positions;   // [n] rotary row of each token
+  const int* slots;       // [n] cache slot, -1: none
+  int rope_rows;
+  int64_t n_slots;        // num_pages * page_size
+  int page_size;
+  int64_t ks[3], vs[3];   // element strides: page, head, slot
+};
+
+// Rotary row of token n, or -1 for a position outside the tables (recorded).
+__device__ __forceinline__ int paged_position(const PagedDst& d, int64_t n) {
+  const int p = d.positions[n];
+  if (p >= 0 && p < d.rope_rows) return p;
+  record_device_error(ENGPT_ERR_ARG, 42);
+  return -1;
+}
+
+// Cache slot of token n, or -1 for none; a slot outside the pool is recorded.
+__device__ __forceinline__ int paged_slot(const PagedDst& d, int64_t n) {
+  const int s = d.slots[n];
+  if (s >= 0 && s < d.n_slots) return s;
+  if (s != -1) record_device_error(ENGPT_ERR_ARG, 43);
+  return -1;
+}
+
+// Element offset of (slot, head) in the key (part 1) or value (part 2) pool.
+__device__ __forceinline__ int64_t paged_offset(const PagedDst& d, int part, int slot, int h) {
+  const int page = slot / d.page_size, off = slot - page * d.page_size;
+  const int64_t* s = part == 1 ? d.ks : d.vs;
+  return page * s[0] + h * s[1] + off * s[2];
+}
+
 // Element offset of row (token n, part s, head h) in the output of part s.
 // Token index n < 2^31 (checked on the host), so the (b, t) split is 32-bit.
 __device__ __forceinline__ int64_t out_offset(const QkvArgs& a, int64_t n, int s, int h) {
@@ -92,8 +125,9 @@ __device__ __forceinline__ void store8<float>(float* p, const float* x) {
 constexpr int kQkvTok = 2;
 constexpr int kQkvMaxHalf = 128;   // rotary pairs staged per token (head_dim <= 256)
 
-template <typename T, int LPR>
-__global__ void __launch_bounds__(768, 2) qkv_vec_kernel(QkvArgs a) {
+// PAGED (engpt_qkv_append): every token has its own rotary row, and k and v go to its cache slot.
+template <typename T, int LPR, bool PAGED>
+__global__ void __launch_bounds__(768, 2) qkv_vec_kernel(QkvArgs a, PagedDst d) {
   __shared__ __align__(16) float s_cos[kQkvTok][kQkvMaxHalf];
   __shared__ __align__(16) float s_sin[kQkvTok][kQkvMaxHalf];
   constexpr bool kFast = sizeof(T) == 2;
@@ -119,15 +153,28 @@ __global__ void __launch_bounds__(768, 2) qkv_vec_kernel(QkvArgs a) {
       rho[k] = 1.f;
     }
   }
+  int pos[kQkvTok], slot[kQkvTok];
+  if (PAGED) {
+#pragma unroll
+    for (int k = 0; k < kQkvTok; ++k) {
+      pos[k] = n0 + k < ntok ? paged_position(d, n0 + k) : -1;
+      slot[k] = n0 + k < ntok ? paged_slot(d, n0 + k) : -1;
+    }
+  }
   // rotary rows of the CTA's tokens -> shared memory
   const int half = a.rope_half;
-  const int t0 = n0 % a.T;
+  const int t0 = PAGED ? 0 : n0 % a.T;
   for (int pi = threadIdx.y * blockDim.x + threadIdx.x; pi < half; pi += blockDim.x * blockDim.y) {
 #pragma unroll
     for (int k = 0; k < kQkvTok; ++k) {
       int t = t0 + k;
-      while (t >= a.T) t -= a.T;  // tokens of the next sequence
-      const bool live = n0 + k < ntok;
+      bool live = n0 + k < ntok;
+      if (PAGED) {
+        t = pos[k];
+        live = t >= 0;
+      } else {
+        while (t >= a.T) t -= a.T;  // tokens of the next sequence
+      }
       s_cos[k][pi] = live ? a.cos_tab[(int64_t)t * half + pi] : 1.f;
       s_sin[k][pi] = live ? a.sin_tab[(int64_t)t * half + pi] : 0.f;
     }
@@ -188,7 +235,19 @@ __global__ void __launch_bounds__(768, 2) qkv_vec_kernel(QkvArgs a) {
         for (int i = 0; i < 8; ++i) outv[i] = (x[i] * inv_den) * scl[i];
       }
     }
-    store8<T>(inplace ? src + k * tok_stride : base + out_offset(a, n, s, h) + e0, outv);
+    if (PAGED) {
+      if (s == 0) {
+        if (pos[k] < 0) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) outv[i] = 0.f;
+        }
+        store8<T>(base + ((int64_t)n * a.H + h) * a.Dh + e0, outv);
+      } else if (pos[k] >= 0 && slot[k] >= 0) {
+        store8<T>(base + paged_offset(d, s, slot[k], h) + e0, outv);
+      }
+    } else {
+      store8<T>(inplace ? src + k * tok_stride : base + out_offset(a, n, s, h) + e0, outv);
+    }
   }
 }
 
@@ -204,8 +263,8 @@ __device__ __forceinline__ void stf(T* p, int64_t i, float v) {
 }
 
 // Generic path: any Dh.  One warp per (token, q|k|v, head) row.
-template <typename T>
-__global__ void __launch_bounds__(256) qkv_generic_kernel(QkvArgs a) {
+template <typename T, bool PAGED>
+__global__ void __launch_bounds__(256) qkv_generic_kernel(QkvArgs a, PagedDst d) {
   const int lane = threadIdx.x & 31;
   const int64_t task = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
   const int64_t ntask = (int64_t)a.B * a.T * 3 * a.H;
@@ -215,7 +274,25 @@ __global__ void __launch_bounds__(256) qkv_generic_kernel(QkvArgs a) {
   const int s = (int)(ns % 3);
   const int64_t n = ns / 3;
   const T* src = reinterpret_cast<const T*>(a.qkv) + task * (int64_t)a.Dh;
-  T* dst = reinterpret_cast<T*>(s == 0 ? a.q : (s == 1 ? a.k : a.v)) + out_offset(a, n, s, h);
+  T* dst = reinterpret_cast<T*>(s == 0 ? a.q : (s == 1 ? a.k : a.v));
+  int t = 0;
+  if (PAGED) {
+    t = paged_position(d, n);
+    const int slot = s == 0 ? -1 : paged_slot(d, n);
+    if (s == 0) {
+      dst += (n * a.H + h) * (int64_t)a.Dh;
+      if (t < 0) {
+        for (int e = lane; e < a.Dh; e += 32) stf<T>(dst, e, 0.f);
+        return;
+      }
+    } else {
+      if (t < 0 || slot < 0) return;
+      dst += paged_offset(d, s, slot, h);
+    }
+  } else {
+    dst += out_offset(a, n, s, h);
+    t = (int)(n % a.T);
+  }
   const float rho = a.rho[n];
   if (s == 2) {
     for (int e = lane; e < a.Dh; e += 32) stf<T>(dst, e, ldf<T>(src, e) / rho);
@@ -229,7 +306,6 @@ __global__ void __launch_bounds__(256) qkv_generic_kernel(QkvArgs a) {
   ss = warp_sum_xor<32>(ss);
   float den = sqrtf(ss);
   if (a.eps > 0.f) den = fmaxf(den, rho * a.eps);
-  const int t = (int)(n % a.T);
   const float* sc = a.qk_scale + (int64_t)h * a.Dh;
   const int npairs = (a.Dh + 1) / 2;
   for (int p = lane; p < npairs; p += 32) {
@@ -245,6 +321,51 @@ __global__ void __launch_bounds__(256) qkv_generic_kernel(QkvArgs a) {
       if (e + 1 < a.Dh) stf<T>(dst, e + 1, (ldf<T>(src, e + 1) / den) * (sc[e + 1] * a.qk_mult));
     }
   }
+}
+
+// The vector kernel where heads, alignment and (for a cache) strides allow 16-byte accesses, else the generic one.
+template <bool PAGED>
+static int launch_qkv(const QkvArgs& a, const PagedDst& d, int dtype, const char* what, cudaStream_t st) {
+  const int B = a.B, T = a.T, H = a.H, Dh = a.Dh, rope_half = a.rope_half;
+  const int64_t ntask = (int64_t)B * T * 3 * H;
+  const int esz = dtype == ENGPT_BF16 ? 2 : 4;
+  bool vec_ok = (Dh == 8 || Dh == 16 || Dh == 32 || Dh == 64 || Dh == 128 || Dh == 256) &&
+                rope_half <= kQkvMaxHalf && rope_half % 4 == 0 &&
+                aligned(a.qkv, 16) && aligned(a.q, 16) && aligned(a.k, 16) && aligned(a.v, 16) &&
+                aligned(a.qk_scale, 16) && (rope_half == 0 || (aligned(a.cos_tab, 16) && aligned(a.sin_tab, 16))) &&
+                ((int64_t)Dh * esz) % 16 == 0;
+  if (PAGED)
+    for (int i = 0; i < 3; ++i) vec_ok = vec_ok && (d.ks[i] * esz) % 16 == 0 && (d.vs[i] * esz) % 16 == 0;
+  const int threads_per_token = 3 * H * (Dh / 8);
+  if (vec_ok && threads_per_token <= 768 && threads_per_token % 32 == 0) {
+    const int lpr = Dh / 8;
+    ENGPT_REQUIRE((int64_t)B * T <= 0x7fffffffLL, ENGPT_ERR_SHAPE, "%s: too large", what);
+    const int64_t blocks = ((int64_t)B * T + kQkvTok - 1) / kQkvTok;
+#define ENGPT_QKV_LAUNCH(L)                                                                                  \
+  case L:                                                                                                    \
+    if (dtype == ENGPT_BF16)                                                                                 \
+      qkv_vec_kernel<__nv_bfloat16, L, PAGED><<<(unsigned)blocks, dim3(H * L, 3), 0, st>>>(a, d);             \
+    else                                                                                                     \
+      qkv_vec_kernel<float, L, PAGED><<<(unsigned)blocks, dim3(H * L, 3), 0, st>>>(a, d);                     \
+    break;
+    switch (lpr) {
+      ENGPT_QKV_LAUNCH(1)
+      ENGPT_QKV_LAUNCH(2)
+      ENGPT_QKV_LAUNCH(4)
+      ENGPT_QKV_LAUNCH(8)
+      ENGPT_QKV_LAUNCH(16)
+      ENGPT_QKV_LAUNCH(32)
+      default:
+        return set_error(ENGPT_ERR_UNSUPPORTED, "%s: lpr %d", what, lpr);
+    }
+#undef ENGPT_QKV_LAUNCH
+  } else {
+    const int64_t blocks = (ntask * 32 + 255) / 256;
+    ENGPT_REQUIRE(blocks <= 0x7fffffffLL, ENGPT_ERR_SHAPE, "%s: too large", what);
+    if (dtype == ENGPT_BF16) qkv_generic_kernel<__nv_bfloat16, PAGED><<<(unsigned)blocks, 256, 0, st>>>(a, d);
+    else qkv_generic_kernel<float, PAGED><<<(unsigned)blocks, 256, 0, st>>>(a, d);
+  }
+  return check_launch(what);
 }
 
 }  // namespace engpt
@@ -274,42 +395,37 @@ extern "C" int engpt_qkv_postprocess(const void* qkv, int dtype, const float* rh
   ENGPT_REQUIRE(rope_half == 0 || (cos_tab && sin_tab), ENGPT_ERR_ARG, "qkv_postprocess: null rope table");
   QkvArgs a{qkv, rho, cos_tab, sin_tab, rope_half, qk_scale, qk_mult, norm_eps, B, T, H, Dh, q_out, k_out, v_out,
             out_layout};
-  const int64_t ntask = (int64_t)B * T * 3 * H;
-  cudaStream_t st = as_stream(stream);
-  const int esz = dtype == ENGPT_BF16 ? 2 : 4;
-  const bool vec_ok = (Dh == 8 || Dh == 16 || Dh == 32 || Dh == 64 || Dh == 128 || Dh == 256) &&
-                      rope_half <= kQkvMaxHalf && rope_half % 4 == 0 &&
-                      aligned(qkv, 16) && aligned(q_out, 16) && aligned(k_out, 16) && aligned(v_out, 16) &&
-                      aligned(qk_scale, 16) && (rope_half == 0 || (aligned(cos_tab, 16) && aligned(sin_tab, 16))) &&
-                      ((int64_t)Dh * esz) % 16 == 0;
-  const int threads_per_token = 3 * H * (Dh / 8);
-  if (vec_ok && threads_per_token <= 768 && threads_per_token % 32 == 0) {
-    const int lpr = Dh / 8;
-    ENGPT_REQUIRE((int64_t)B * T <= 0x7fffffffLL, ENGPT_ERR_SHAPE, "qkv_postprocess: too large");
-    const int64_t blocks = ((int64_t)B * T + kQkvTok - 1) / kQkvTok;
-#define ENGPT_QKV_LAUNCH(L)                                                                                  \
-  case L:                                                                                                    \
-    if (dtype == ENGPT_BF16)                                                                                 \
-      qkv_vec_kernel<__nv_bfloat16, L><<<(unsigned)blocks, dim3(H * L, 3), 0, st>>>(a);                       \
-    else                                                                                                     \
-      qkv_vec_kernel<float, L><<<(unsigned)blocks, dim3(H * L, 3), 0, st>>>(a);                               \
-    break;
-    switch (lpr) {
-      ENGPT_QKV_LAUNCH(1)
-      ENGPT_QKV_LAUNCH(2)
-      ENGPT_QKV_LAUNCH(4)
-      ENGPT_QKV_LAUNCH(8)
-      ENGPT_QKV_LAUNCH(16)
-      ENGPT_QKV_LAUNCH(32)
-      default:
-        return set_error(ENGPT_ERR_UNSUPPORTED, "qkv_postprocess: lpr %d", lpr);
-    }
-#undef ENGPT_QKV_LAUNCH
-  } else {
-    const int64_t blocks = (ntask * 32 + 255) / 256;
-    ENGPT_REQUIRE(blocks <= 0x7fffffffLL, ENGPT_ERR_SHAPE, "qkv_postprocess: too large");
-    if (dtype == ENGPT_BF16) qkv_generic_kernel<__nv_bfloat16><<<(unsigned)blocks, 256, 0, st>>>(a);
-    else qkv_generic_kernel<float><<<(unsigned)blocks, 256, 0, st>>>(a);
+  return launch_qkv<false>(a, PagedDst{}, dtype, "qkv_postprocess", as_stream(stream));
+}
+
+extern "C" int engpt_qkv_append(const void* qkv, int dtype, const float* rho, const float* cos_tab,
+                                const float* sin_tab, int rope_rows, int rope_half, const float* qk_scale,
+                                float qk_mult, float norm_eps, int64_t n, int H, int Dh, const int* positions,
+                                const int* slots, void* q_out, void* k_pages, void* v_pages,
+                                const int64_t* page_strides, int num_pages, int page_size, void* stream) {
+  clear_error();
+  ENGPT_REQUIRE(n >= 0 && n <= 0x7fffffffLL && H > 0 && Dh > 0, ENGPT_ERR_SHAPE, "qkv_append: n=%lld H=%d Dh=%d",
+                (long long)n, H, Dh);
+  ENGPT_REQUIRE(rope_half >= 0 && 2 * rope_half <= Dh && rope_rows >= 0, ENGPT_ERR_SHAPE,
+                "qkv_append: rope_half=%d rope_rows=%d Dh=%d", rope_half, rope_rows, Dh);
+  ENGPT_REQUIRE(num_pages >= 0 && page_size > 0 && (int64_t)num_pages * page_size <= 0x7fffffffLL, ENGPT_ERR_SHAPE,
+                "qkv_append: num_pages=%d page_size=%d", num_pages, page_size);
+  ENGPT_REQUIRE(dtype == ENGPT_BF16 || dtype == ENGPT_F32, ENGPT_ERR_DTYPE, "qkv_append: dtype %d", dtype);
+  if (n == 0) return ENGPT_OK;
+  ENGPT_REQUIRE(qkv && rho && qk_scale && q_out && k_pages && v_pages && positions && slots && page_strides,
+                ENGPT_ERR_ARG, "qkv_append: null pointer");
+  ENGPT_REQUIRE(rope_half == 0 || (cos_tab && sin_tab), ENGPT_ERR_ARG, "qkv_append: null rope table");
+  QkvArgs a{qkv, rho, cos_tab, sin_tab, rope_half, qk_scale, qk_mult, norm_eps, 1, (int)n, H, Dh, q_out, k_pages,
+            v_pages, ENGPT_QKV_BTHD};
+  PagedDst d;
+  d.positions = positions;
+  d.slots = slots;
+  d.rope_rows = rope_rows;
+  d.n_slots = (int64_t)num_pages * page_size;
+  d.page_size = page_size;
+  for (int i = 0; i < 3; ++i) {
+    d.ks[i] = page_strides[i];
+    d.vs[i] = page_strides[3 + i];
   }
-  return check_launch("qkv_postprocess");
+  return launch_qkv<true>(a, d, dtype, "qkv_append", as_stream(stream));
 }

@@ -332,6 +332,85 @@ ENGPT_API int engpt_cross_entropy(const void* logits, int dtype, int64_t rows, i
 ENGPT_API int engpt_cross_entropy_noalloc(const void* logits, int dtype, int64_t rows, int64_t vocab,
                                           int64_t ld, const int64_t* targets, float* loss_out, void* stream);
 
+/*
+ * Paged key-value cache for decoding.  The reference has no cache (its
+ * forwards are whole sequences); these entry points are what generation from
+ * an EfficientNGPT needs next to them.
+ *
+ * The cache of one layer is two page pools, keys and values, [num_pages, kv
+ * heads, page_size, Dh] with element strides (page, head, slot) and a
+ * contiguous Dh axis.  Request b's row of the block table [B, table_width]
+ * lists its pages in order; its token at position p is in slot
+ * block_table[b, p / page_size] * page_size + p % page_size.  A slot of -1
+ * means none.  All indices are int32; num_pages * page_size < 2^31.
+ *
+ * engpt_advance_block_tables makes one step of the allocator on the device,
+ * in place on lengths [B] (tokens in the cache), block_table (row stride
+ * table_stride), the stack of free pages free_pages [num_pages] and its size
+ * free_count [1]:
+ *   1. every row b with finished[b] != 0 (finished may be NULL) pushes its
+ *      ceil(lengths[b] / page_size) pages, rows in order, pages in order, and
+ *      its length becomes 0;
+ *   2. every row takes pages for new_tokens[b] more tokens from the top of the
+ *      stack, rows in order, and lengths[b] grows by new_tokens[b];
+ *   3. slots and positions [B, max_new] receive the slot and the position of
+ *      each new token; -1 and 0 behind a row's last one.
+ * Table entries behind a row's pages are left as they were.  A row is refused
+ * (no pages, length and table unchanged, its slots -1, ENGPT_ERR_ARG in the
+ * device status word) if new_tokens[b] is negative or above max_new, if the
+ * table row is too short for it (site 40), or if the stack has too few pages
+ * left for it and the rows before it (site 41).  B <= 8192.
+ */
+ENGPT_API int engpt_advance_block_tables(int* lengths, const int* new_tokens, const unsigned char* finished, int B,
+                                         int* block_table, int64_t table_stride, int table_width, int* free_pages,
+                                         int num_pages, int* free_count, int page_size, int max_new, int* slots,
+                                         int* positions, void* stream);
+
+/*
+ * engpt_qkv_postprocess with explicit positions and the cache as the place of
+ * k and v: qkv [n, 3, H, Dh] contiguous raw projection rows, rho [n],
+ * positions [n] (rows of cos_tab/sin_tab [rope_rows, rope_half]), slots [n].
+ * q_out [n, H, Dh]; k and v go to their slots of k_pages and v_pages
+ * (page_strides: 6 int64, k page, head, slot, then v), which must be distinct;
+ * a row with slot -1 only gets its q.  A row whose position or slot is out of
+ * range is recorded (ENGPT_ERR_ARG, sites 42 and 43): nothing is written to
+ * the cache for it, and for a position its q is zero.
+ */
+ENGPT_API int engpt_qkv_append(const void* qkv, int dtype, const float* rho, const float* cos_tab,
+                               const float* sin_tab, int rope_rows, int rope_half, const float* qk_scale,
+                               float qk_mult, float norm_eps, int64_t n, int H, int Dh, const int* positions,
+                               const int* slots, void* q_out, void* k_pages, void* v_pages,
+                               const int64_t* page_strides, int num_pages, int page_size, void* stream);
+
+/*
+ * Copies finished k and v rows [n, H, Dh] (element strides kv_strides: 4
+ * int64, k row, k head, v row, v head; contiguous Dh) into their cache slots.
+ * Slots as for engpt_qkv_append.
+ */
+ENGPT_API int engpt_write_kv_pages(const void* k, const void* v, const int64_t* kv_strides, int dtype, int64_t n,
+                                   int H, int Dh, const int* slots, void* k_pages, void* v_pages,
+                                   const int64_t* page_strides, int num_pages, int page_size, void* stream);
+
+/*
+ * Attention of one new token per request over its cached keys and values:
+ * o[b, h] = sum_j softmax_j(scale q[b, h] . k_j) v_j over the first lengths[b]
+ * tokens of request b, query head h reading kv head h / (H / Hkv).  q [B, H,
+ * Dh] with element strides q_strides (2 int64: row, head), o [B, H, Dh]
+ * contiguous.  A row of length 0 (or below) gives zeros; what lies in the
+ * cache behind a row's length is never used.  A length above table_width *
+ * page_size or a page outside the pool is recorded (ENGPT_ERR_ARG, site 44)
+ * and its keys count as absent.  Dh <= 256.  workspace: scratch of
+ * engpt_paged_attention_floats(...) floats, 16-byte aligned, owned by this
+ * call until its kernels have run; it needs no initial value.
+ */
+ENGPT_API int64_t engpt_paged_attention_floats(int dtype, int B, int H, int Hkv, int Dh, int table_width,
+                                               int page_size);
+ENGPT_API int engpt_paged_attention(const void* q, const int64_t* q_strides, const void* k_pages,
+                                    const void* v_pages, const int64_t* page_strides, int dtype, int B, int H,
+                                    int Hkv, int Dh, int num_pages, int page_size, const int* block_table,
+                                    int64_t table_stride, int table_width, const int* lengths, float scale, void* o,
+                                    float* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

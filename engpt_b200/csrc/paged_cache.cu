@@ -8,12 +8,14 @@
 //
 // write_kv_pages: a gathered copy, bound by HBM.
 #include "common.cuh"
+#include "sm100_ptx.cuh"
 
 namespace engpt {
 namespace paged {
 
-constexpr int kTableThreads = 1024;
-constexpr int kMaxRows = 8192;   // three ints of shared memory per row
+constexpr int kMaxRows = 8192;      // five ints of shared memory per row
+constexpr int kTableCluster = 8;    // CTAs of a large launch
+constexpr int kPiece = 128;         // pages that a warp pushes at a time (four loads in flight per lane)
 
 struct TableArgs {
   int* lengths;
@@ -32,138 +34,171 @@ struct TableArgs {
   int* positions;
 };
 
-// Exclusive prefix sum over the CTA's threads (thread order), with the total.
-__device__ __forceinline__ int64_t block_exclusive_sum(int v, int64_t* s_warp, int64_t& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t x = v;
+__device__ __forceinline__ int64_t warp_inclusive_sum(int64_t x, int lane) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
-  if (lane == 31) s_warp[warp] = x;
-  __syncthreads();
-  if (warp == 0) {
-    int64_t w = s_warp[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += y;
-    }
-    s_warp[lane] = w;
-  }
-  __syncthreads();
-  const int64_t before = warp ? s_warp[warp - 1] : 0;
-  total = s_warp[31];
-  __syncthreads();
-  return before + x - v;
+  return x;
 }
 
-__global__ void __launch_bounds__(kTableThreads) advance_tables_kernel(TableArgs a) {
+// One step of the allocator by one cluster (of one CTA for a small step).  Every CTA reads all rows and forms all
+// prefix sums for itself; the cluster shares the copying of freed pages and, behind a barrier (everything that the
+// step overwrites has been read), the new tokens, U consecutive ones of a row per thread.  Latency bound: two
+// dependent trips to memory before the barrier, two behind it.
+template <int U>
+__global__ void __launch_bounds__(1024) advance_tables_kernel(TableArgs a, int ctas) {
   extern __shared__ int s_rows[];
-  int* s_len = s_rows;              // length after the release
-  int* s_off = s_rows + a.B;        // pages pushed, then pages taken, by the rows before
-  int* s_new = s_rows + 2 * a.B;    // new tokens; -1: refused
-  __shared__ int64_t s_warp[32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int* s_len = s_rows;               // length after the release
+  int* s_new = s_rows + a.B;         // new tokens; -1: refused
+  int* s_off = s_rows + 2 * a.B;     // pages taken by the rows before
+  int* s_held = s_rows + 3 * a.B;    // pages to push
+  int* s_push = s_rows + 4 * a.B;    // pages pushed by the rows before
+  __shared__ int64_t s_warp[2][32];
+  __shared__ int s_taken;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
+  const int rank = blockIdx.x;       // the grid is one cluster
+  const bool first = rank == 0;      // records what every CTA sees
 
+  if (tid == 0) s_taken = 0;
   int n_free = *a.free_count;
   if (n_free < 0 || n_free > a.P) {
-    if (tid == 0) record_device_error(ENGPT_ERR_ARG, 40);
+    if (first && tid == 0) record_device_error(ENGPT_ERR_ARG, 40);
     n_free = n_free < 0 ? 0 : a.P;
   }
-  // 1. finished rows push their pages
-  int64_t pushed = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kTableThreads) {
+  int64_t pushed = 0, needed = 0;
+  for (int b0 = 0; b0 < a.B; b0 += threads) {
     const int b = b0 + tid;
-    int len = 0, held = 0;
+    int held = 0, need = 0;
     if (b < a.B) {
-      len = max(a.lengths[b], 0);
-      if (a.finished && a.finished[b]) held = min((int)(((int64_t)len + a.ps - 1) / a.ps), a.W);
-    }
-    int64_t total;
-    const int64_t off = block_exclusive_sum(held, s_warp, total) + pushed;
-    pushed += total;
-    if (b < a.B) {
-      s_len[b] = len;
-      s_off[b] = (int)min(off, (int64_t)0x7fffffff);
-    }
-  }
-  __syncthreads();
-  if (a.finished) {
-    for (int b = warp; b < a.B; b += kTableThreads / 32) {
-      if (!a.finished[b]) continue;
-      const int held = min((int)(((int64_t)s_len[b] + a.ps - 1) / a.ps), a.W);
-      const int* row = a.table + b * a.table_stride;
-      for (int j = lane; j < held; j += 32) {
-        const int64_t at = (int64_t)n_free + s_off[b] + j;
-        if (at < a.P) a.free_pages[at] = row[j];
-        else record_device_error(ENGPT_ERR_ARG, 40);
+      int len = max(a.lengths[b], 0), fresh = a.new_tokens[b];
+      if (a.finished && a.finished[b]) {
+        held = min((int)(((int64_t)len + a.ps - 1) / a.ps), a.W);
+        len = 0;
       }
-      __syncwarp();
-      if (lane == 0) s_len[b] = 0;
-    }
-    __syncthreads();
-  }
-  n_free = (int)min((int64_t)n_free + pushed, (int64_t)a.P);
-  // 2. pages for the new tokens
-  int64_t need_before = 0;
-  int taken = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kTableThreads) {
-    const int b = b0 + tid;
-    int need = 0, fresh = 0;
-    if (b < a.B) {
-      fresh = a.new_tokens[b];
-      const int64_t len = s_len[b], end = len + fresh;
+      const int64_t end = (int64_t)len + fresh;
       if (fresh < 0 || fresh > a.max_new || end > (int64_t)a.W * a.ps) {
-        record_device_error(ENGPT_ERR_ARG, 40);
+        if (first) record_device_error(ENGPT_ERR_ARG, 40);
         fresh = -1;
       } else {
-        need = (int)((end + a.ps - 1) / a.ps - (len + a.ps - 1) / a.ps);
+        need = (int)((uint32_t)(end + a.ps - 1) / (uint32_t)a.ps - ((uint32_t)len + a.ps - 1) / (uint32_t)a.ps);
       }
-    }
-    int64_t total;
-    const int64_t off = block_exclusive_sum(need, s_warp, total) + need_before;
-    need_before += total;
-    if (need > 0 && off + need > n_free) {   // off grows with b: once the stack is short it stays short
-      record_device_error(ENGPT_ERR_ARG, 41);
-      fresh = -1;
-      need = 0;
-    }
-    int64_t got;
-    block_exclusive_sum(need, s_warp, got);
-    taken += (int)got;
-    if (b < a.B) {
-      s_off[b] = (int)min(off, (int64_t)0x7fffffff);
+      s_len[b] = len;
       s_new[b] = fresh;
+      s_held[b] = held;
     }
+    const int64_t xh = warp_inclusive_sum(held, lane), xn = warp_inclusive_sum(need, lane);
+    if (lane == 31) {
+      s_warp[0][warp] = xh;
+      s_warp[1][warp] = xn;
+    }
+    __syncthreads();
+    if (warp < 2) {
+      const int64_t v = lane < warps ? s_warp[warp][lane] : 0;
+      s_warp[warp][lane] = warp_inclusive_sum(v, lane);
+    }
+    __syncthreads();
+    if (b < a.B) {
+      const int64_t most = 0x7fffffff;
+      s_push[b] = (int)min(pushed + (warp ? s_warp[0][warp - 1] : 0) + xh - held, most);
+      s_off[b] = (int)min(needed + (warp ? s_warp[1][warp - 1] : 0) + xn - need, most);
+      // (whether the stack is deep enough for the row is known when everything has been pushed, below)
+    }
+    pushed += s_warp[0][31];
+    needed += s_warp[1][31];
+    __syncthreads();
   }
-  __syncthreads();
-  // 3. slots and positions; the first token of a page enters the page into the table
-  const int64_t tokens = (int64_t)a.B * a.max_new;
-  for (int64_t t = tid; t < tokens; t += kTableThreads) {
-    const int b = (int)(t / a.max_new), i = (int)(t - (int64_t)b * a.max_new);
-    int slot = -1, pos = 0;
-    if (i < s_new[b]) {
-      const int len = s_len[b];
-      pos = len + i;
-      const int j = pos / a.ps, r = pos - j * a.ps;
-      const int have = (int)(((int64_t)len + a.ps - 1) / a.ps);
-      int* entry = a.table + b * a.table_stride + j;
-      int page;
-      if (j < have) {
-        page = *entry;
-      } else {
-        page = a.free_pages[n_free - 1 - s_off[b] - (j - have)];
-        if (r == 0) *entry = page;
+  // finished rows push their pages, a warp per piece of a row
+  if (pushed > 0) {
+    const int pieces = (a.W + kPiece - 1) / kPiece;
+    const int64_t total = (int64_t)a.B * pieces;
+    for (int64_t i = rank * warps + warp; i < total; i += (int64_t)ctas * warps) {
+      const int b = total <= 0xffffffffLL ? (int)((uint32_t)i / (uint32_t)pieces) : (int)(i / pieces);
+      const int j0 = (int)(i - (int64_t)b * pieces) * kPiece;
+      const int held = s_held[b];
+      if (j0 >= held) continue;
+      const int* row = a.table + b * a.table_stride;
+      int page[kPiece / 32];
+#pragma unroll
+      for (int k = 0; k < kPiece / 32; ++k) {
+        const int j = j0 + k * 32 + lane;
+        page[k] = j < held ? row[j] : 0;
       }
-      slot = page * a.ps + r;
+#pragma unroll
+      for (int k = 0; k < kPiece / 32; ++k) {
+        const int j = j0 + k * 32 + lane;
+        const int64_t at = (int64_t)n_free + s_push[b] + j;
+        if (j < held) {
+          if (at < a.P) a.free_pages[at] = page[k];
+          else record_device_error(ENGPT_ERR_ARG, 40);
+        }
+      }
     }
-    a.slots[t] = slot;
-    a.positions[t] = pos;
   }
-  for (int b = tid; b < a.B; b += kTableThreads) a.lengths[b] = s_len[b] + max(s_new[b], 0);
-  if (tid == 0) *a.free_count = n_free - taken;
+  n_free = (int)min((int64_t)n_free + pushed, (int64_t)a.P);
+  // rows that the stack is too short for.  The sums grow with the row, so the rows behind the first one that found
+  // too few pages get none either, and the pages taken are those up to the last row that was served.
+  for (int b = tid; b < a.B; b += threads) {
+    const int len = s_len[b], fresh = s_new[b];
+    if (fresh <= 0) continue;
+    const int need = (int)(((uint32_t)len + fresh + a.ps - 1) / (uint32_t)a.ps - ((uint32_t)len + a.ps - 1) / (uint32_t)a.ps);
+    if (need == 0) continue;
+    if ((int64_t)s_off[b] + need > n_free) {
+      if (first) record_device_error(ENGPT_ERR_ARG, 41);
+      s_new[b] = -1;
+    } else if (needed > n_free) {
+      atomicMax(&s_taken, s_off[b] + need);
+    }
+  }
+  if (ctas > 1) sm100::cluster_sync_all();
+  else __syncthreads();
+  // slots and positions; the first token of a page enters the page into the table
+  const uint32_t per_row = (uint32_t)a.max_new / U;
+  const uint32_t total = (uint32_t)a.B * per_row;
+  for (uint32_t t = rank * threads + tid; t < total; t += ctas * threads) {
+    const uint32_t b = per_row == 1 ? t : t / per_row;
+    const int i0 = (int)(t - b * per_row) * U;
+    const int fresh = s_new[b], len = s_len[b];
+    int slot[U], pos[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      slot[u] = -1;
+      pos[u] = 0;
+    }
+    if (i0 < fresh) {
+      const int have = (int)(((uint32_t)len + a.ps - 1) / (uint32_t)a.ps);
+      int j = (int)((uint32_t)(len + i0) / (uint32_t)a.ps), r = len + i0 - j * a.ps;
+      int* entry = a.table + b * a.table_stride;
+      const int* stack = a.free_pages + (n_free - 1 - s_off[b]);
+      int page = j < have ? entry[j] : stack[have - j];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i0 + u < fresh) {
+          if (r == a.ps) {
+            ++j;
+            r = 0;
+            page = stack[have - j];
+          }
+          if (r == 0) entry[j] = page;
+          slot[u] = page * a.ps + r;
+          pos[u] = len + i0 + u;
+          ++r;
+        }
+      }
+    }
+    if constexpr (U == 4) {
+      reinterpret_cast<int4*>(a.slots)[t] = make_int4(slot[0], slot[1], slot[2], slot[3]);
+      reinterpret_cast<int4*>(a.positions)[t] = make_int4(pos[0], pos[1], pos[2], pos[3]);
+    } else {
+      a.slots[t] = slot[0];
+      a.positions[t] = pos[0];
+    }
+  }
+  if (first) {
+    for (int b = tid; b < a.B; b += threads) a.lengths[b] = s_len[b] + max(s_new[b], 0);
+    if (tid == 0) *a.free_count = n_free - (needed > n_free ? s_taken : (int)needed);
+  }
 }
 
 // ------------------------------------------------------------------ write
@@ -229,10 +264,30 @@ extern "C" int engpt_advance_block_tables(int* lengths, const int* new_tokens, c
                 ENGPT_ERR_ARG, "advance_block_tables: null pointer");
   TableArgs a{lengths, new_tokens, finished, B, block_table, table_stride, table_width, free_pages, num_pages,
               free_count, page_size, max_new, slots, positions};
-  const size_t smem = sizeof(int) * 3 * (size_t)B;
-  if (smem > 48 * 1024)
-    cudaFuncSetAttribute(advance_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  advance_tables_kernel<<<1, kTableThreads, smem, as_stream(stream)>>>(a);
+  ENGPT_REQUIRE((int64_t)B * max_new <= 0x7fffffffLL, ENGPT_ERR_SHAPE, "advance_block_tables: B=%d max_new=%d", B,
+                max_new);
+  const bool vec = max_new % 4 == 0 && aligned(slots, 16) && aligned(positions, 16);
+  // A step of a few hundred rows is one small CTA (less to start); longer ones share the tokens and the freed pages
+  // over a cluster.
+  const bool small = B <= 256 && (int64_t)B * max_new <= 1024;
+  const int ctas = small ? 1 : kTableCluster;
+  const size_t smem = sizeof(int) * 5 * (size_t)B;
+  auto kern = vec ? advance_tables_kernel<4> : advance_tables_kernel<1>;
+  cudaError_t e = cudaSuccess;
+  if (smem > 40 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(small ? 256 : 1024);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = as_stream(stream);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kern, a, ctas);
+  if (e != cudaSuccess) return set_error(ENGPT_ERR_LAUNCH, "advance_block_tables: %s", cudaGetErrorString(e));
   return check_launch("advance_block_tables");
 }
 

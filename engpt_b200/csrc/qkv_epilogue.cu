@@ -38,23 +38,21 @@ struct PagedDst {
   const int* slots;       // [n] cache slot, -1: none
   int rope_rows;
   int64_t n_slots;        // num_pages * page_size
-  int page_size;
+  int page_size, page_shift;   // page_shift: log2(page_size), or -1
   int64_t ks[3], vs[3];   // element strides: page, head, slot
 };
 
-// Rotary row of token n, or -1 for a position outside the tables (recorded).
-__device__ __forceinline__ int paged_position(const PagedDst& d, int64_t n) {
-  const int p = d.positions[n];
+// A token's rotary row p as given, or -1 for one outside the tables (recorded).
+__device__ __forceinline__ int checked_position(const PagedDst& d, int p) {
   if (p >= 0 && p < d.rope_rows) return p;
   record_device_error(ENGPT_ERR_ARG, 42);
   return -1;
 }
 
-// Cache slot of token n, or -1 for none; a slot outside the pool is recorded.
-__device__ __forceinline__ int paged_slot(const PagedDst& d, int64_t n) {
-  const int s = d.slots[n];
-  if (s >= 0 && s < d.n_slots) return s;
-  if (s != -1) record_device_error(ENGPT_ERR_ARG, 43);
+// A token's cache slot as given, or -1 for none; a slot outside the pool is recorded.
+__device__ __forceinline__ int checked_slot(const PagedDst& d, int slot) {
+  if (slot >= 0 && slot < d.n_slots) return slot;
+  if (slot != -1) record_device_error(ENGPT_ERR_ARG, 43);
   return -1;
 }
 
@@ -125,9 +123,8 @@ __device__ __forceinline__ void store8<float>(float* p, const float* x) {
 constexpr int kQkvTok = 2;
 constexpr int kQkvMaxHalf = 128;   // rotary pairs staged per token (head_dim <= 256)
 
-// PAGED (engpt_qkv_append): every token has its own rotary row, and k and v go to its cache slot.
-template <typename T, int LPR, bool PAGED>
-__global__ void __launch_bounds__(768, 2) qkv_vec_kernel(QkvArgs a, PagedDst d) {
+template <typename T, int LPR>
+__global__ void __launch_bounds__(768, 2) qkv_vec_kernel(QkvArgs a) {
   __shared__ __align__(16) float s_cos[kQkvTok][kQkvMaxHalf];
   __shared__ __align__(16) float s_sin[kQkvTok][kQkvMaxHalf];
   constexpr bool kFast = sizeof(T) == 2;
@@ -153,28 +150,15 @@ __global__ void __launch_bounds__(768, 2) qkv_vec_kernel(QkvArgs a, PagedDst d) 
       rho[k] = 1.f;
     }
   }
-  int pos[kQkvTok], slot[kQkvTok];
-  if (PAGED) {
-#pragma unroll
-    for (int k = 0; k < kQkvTok; ++k) {
-      pos[k] = n0 + k < ntok ? paged_position(d, n0 + k) : -1;
-      slot[k] = n0 + k < ntok ? paged_slot(d, n0 + k) : -1;
-    }
-  }
   // rotary rows of the CTA's tokens -> shared memory
   const int half = a.rope_half;
-  const int t0 = PAGED ? 0 : n0 % a.T;
+  const int t0 = n0 % a.T;
   for (int pi = threadIdx.y * blockDim.x + threadIdx.x; pi < half; pi += blockDim.x * blockDim.y) {
 #pragma unroll
     for (int k = 0; k < kQkvTok; ++k) {
       int t = t0 + k;
-      bool live = n0 + k < ntok;
-      if (PAGED) {
-        t = pos[k];
-        live = t >= 0;
-      } else {
-        while (t >= a.T) t -= a.T;  // tokens of the next sequence
-      }
+      while (t >= a.T) t -= a.T;  // tokens of the next sequence
+      const bool live = n0 + k < ntok;
       s_cos[k][pi] = live ? a.cos_tab[(int64_t)t * half + pi] : 1.f;
       s_sin[k][pi] = live ? a.sin_tab[(int64_t)t * half + pi] : 0.f;
     }
@@ -235,18 +219,125 @@ __global__ void __launch_bounds__(768, 2) qkv_vec_kernel(QkvArgs a, PagedDst d) 
         for (int i = 0; i < 8; ++i) outv[i] = (x[i] * inv_den) * scl[i];
       }
     }
-    if (PAGED) {
+    store8<T>(inplace ? src + k * tok_stride : base + out_offset(a, n, s, h) + e0, outv);
+  }
+}
+
+// engpt_qkv_append: the same arithmetic (bit for bit) with a rotary row of its own for every token, q to [n, H, Dh]
+// and k and v to the token's cache slot.  A thread owns one 8-element slice of a head and does its q, k and v: they
+// share the position, the slot, rho, the rotary row and (q and k) the scales.  It walks over tokens with the next
+// token's rows in flight while it works on the current one.  The rotary rows, the same for all heads of a token, come
+// through L1; nothing waits on a CTA barrier.
+template <typename T>
+struct AppendRow {
+  Raw8<T> x[3];
+  float rho;
+  int pos, slot;
+  __device__ __forceinline__ void load(const QkvArgs& a, const PagedDst& d, const T* src, int64_t part, int n) {
+    const T* p = src + n * (3 * part);
+#pragma unroll
+    for (int s = 0; s < 3; ++s) x[s].load(p + s * part);
+    rho = a.rho[n];
+    pos = d.positions[n];
+    slot = d.slots[n];
+  }
+};
+
+constexpr int kAppendCtas = 16;   // CTAs per SM of a launch whose CTAs walk over several tokens
+
+// MIN: CTAs per SM that the registers have to leave room for.
+template <typename T, int LPR, int MIN>
+__global__ void __launch_bounds__(128, MIN) append_vec_kernel(QkvArgs a, PagedDst d) {
+  constexpr bool kFast = sizeof(T) == 2;
+  const int idx = blockIdx.y * 128 + threadIdx.x;      // (head, slice)
+  const bool mine = idx < a.H * LPR;
+  const int h = mine ? idx / LPR : 0;
+  const int e0 = (idx % LPR) * 8;
+  const int64_t part = (int64_t)a.H * a.Dh;            // elements from q to k and from k to v
+  const T* src = reinterpret_cast<const T*>(a.qkv) + (int64_t)h * a.Dh + e0;
+  T* q_dst = reinterpret_cast<T*>(a.q) + (int64_t)h * a.Dh + e0;
+  T* k_dst = reinterpret_cast<T*>(a.k) + h * d.ks[1] + e0;
+  T* v_dst = reinterpret_cast<T*>(a.v) + h * d.vs[1] + e0;
+  const int p0 = e0 >> 1;                              // first rotary pair (a multiple of 4)
+  const bool rot = p0 < a.rope_half;                   // so is rope_half: 4 pairs rotate together or not at all
+  float scl[8];
+  {
+    const float* sc = a.qk_scale + (int64_t)h * a.Dh + e0;
+    const float4 s0 = __ldg(reinterpret_cast<const float4*>(sc));
+    const float4 s1 = __ldg(reinterpret_cast<const float4*>(sc + 4));
+    const float v[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) scl[i] = v[i] * a.qk_mult;
+  }
+  AppendRow<T> next;
+  int n = blockIdx.x;
+  next.load(a, d, src, part, n);                       // (a thread without a slice of its own walks head 0)
+  for (; n < a.T; n += gridDim.x) {
+    const AppendRow<T> row = next;
+    const bool turn = rot && (unsigned)row.pos < (unsigned)d.rope_rows;
+    float4 c4 = make_float4(1.f, 1.f, 1.f, 1.f), s4 = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (turn) {
+      c4 = __ldg(reinterpret_cast<const float4*>(a.cos_tab + (int64_t)row.pos * a.rope_half + p0));
+      s4 = __ldg(reinterpret_cast<const float4*>(a.sin_tab + (int64_t)row.pos * a.rope_half + p0));
+    }
+    if (n + (int64_t)gridDim.x < a.T) next.load(a, d, src, part, n + gridDim.x);
+    float ss[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      float x[8];
+      row.x[s].to_float(x);
+      ss[s] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss[s] = fmaf(x[i], x[i], ss[s]);
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) ss[s] += __shfl_xor_sync(0xffffffffu, ss[s], o);
+    }
+    if (!mine) continue;
+    const bool placed = checked_position(d, row.pos) >= 0;
+    const int slot = checked_slot(d, row.slot);
+    const int page = d.page_shift >= 0 ? slot >> d.page_shift : slot / d.page_size;
+    const int off = slot - page * d.page_size;
+    const bool keep = placed && slot >= 0;
+#pragma unroll
+    for (int s = 0; s < 3; ++s) {
+      float x[8], outv[8];
+      row.x[s].to_float(x);
+      if (s == 2) {
+        const float inv_rho = kFast ? __fdividef(1.0f, row.rho) : 1.0f / row.rho;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) outv[i] = x[i] * inv_rho;
+      } else {
+        float inv_den;
+        if (kFast) {
+          inv_den = rsqrtf(ss[s]);
+          if (a.eps > 0.f) inv_den = fminf(inv_den, __fdividef(1.0f, row.rho * a.eps));
+        } else {
+          float den = sqrtf(ss[s]);
+          if (a.eps > 0.f) den = fmaxf(den, row.rho * a.eps);
+          inv_den = 1.0f / den;
+        }
+        if (rot) {
+          const float c[4] = {c4.x, c4.y, c4.z, c4.w}, sn[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float xe = x[2 * i], xo = x[2 * i + 1];
+            outv[2 * i] = ((xe * c[i] - xo * sn[i]) * inv_den) * scl[2 * i];
+            outv[2 * i + 1] = ((xe * sn[i] + xo * c[i]) * inv_den) * scl[2 * i + 1];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) outv[i] = (x[i] * inv_den) * scl[i];
+        }
+      }
       if (s == 0) {
-        if (pos[k] < 0) {
+        if (!placed) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) outv[i] = 0.f;
         }
-        store8<T>(base + ((int64_t)n * a.H + h) * a.Dh + e0, outv);
-      } else if (pos[k] >= 0 && slot[k] >= 0) {
-        store8<T>(base + paged_offset(d, s, slot[k], h) + e0, outv);
+        store8<T>(q_dst + n * part, outv);
+      } else if (keep) {
+        store8<T>(s == 1 ? k_dst + page * d.ks[0] + off * d.ks[2] : v_dst + page * d.vs[0] + off * d.vs[2], outv);
       }
-    } else {
-      store8<T>(inplace ? src + k * tok_stride : base + out_offset(a, n, s, h) + e0, outv);
     }
   }
 }
@@ -277,8 +368,8 @@ __global__ void __launch_bounds__(256) qkv_generic_kernel(QkvArgs a, PagedDst d)
   T* dst = reinterpret_cast<T*>(s == 0 ? a.q : (s == 1 ? a.k : a.v));
   int t = 0;
   if (PAGED) {
-    t = paged_position(d, n);
-    const int slot = s == 0 ? -1 : paged_slot(d, n);
+    t = checked_position(d, d.positions[n]);
+    const int slot = s == 0 ? -1 : checked_slot(d, d.slots[n]);
     if (s == 0) {
       dst += (n * a.H + h) * (int64_t)a.Dh;
       if (t < 0) {
@@ -323,49 +414,38 @@ __global__ void __launch_bounds__(256) qkv_generic_kernel(QkvArgs a, PagedDst d)
   }
 }
 
-// The vector kernel where heads, alignment and (for a cache) strides allow 16-byte accesses, else the generic one.
+// 16-byte accesses to q, k, v and the tables are possible.
+static bool vec_access(const QkvArgs& a, int esz) {
+  const int Dh = a.Dh;
+  return (Dh == 8 || Dh == 16 || Dh == 32 || Dh == 64 || Dh == 128 || Dh == 256) && a.rope_half <= kQkvMaxHalf &&
+         a.rope_half % 4 == 0 && aligned(a.qkv, 16) && aligned(a.q, 16) && aligned(a.k, 16) && aligned(a.v, 16) &&
+         aligned(a.qk_scale, 16) && (a.rope_half == 0 || (aligned(a.cos_tab, 16) && aligned(a.sin_tab, 16))) &&
+         ((int64_t)Dh * esz) % 16 == 0;
+}
+
 template <bool PAGED>
-static int launch_qkv(const QkvArgs& a, const PagedDst& d, int dtype, const char* what, cudaStream_t st) {
-  const int B = a.B, T = a.T, H = a.H, Dh = a.Dh, rope_half = a.rope_half;
-  const int64_t ntask = (int64_t)B * T * 3 * H;
-  const int esz = dtype == ENGPT_BF16 ? 2 : 4;
-  bool vec_ok = (Dh == 8 || Dh == 16 || Dh == 32 || Dh == 64 || Dh == 128 || Dh == 256) &&
-                rope_half <= kQkvMaxHalf && rope_half % 4 == 0 &&
-                aligned(a.qkv, 16) && aligned(a.q, 16) && aligned(a.k, 16) && aligned(a.v, 16) &&
-                aligned(a.qk_scale, 16) && (rope_half == 0 || (aligned(a.cos_tab, 16) && aligned(a.sin_tab, 16))) &&
-                ((int64_t)Dh * esz) % 16 == 0;
-  if (PAGED)
-    for (int i = 0; i < 3; ++i) vec_ok = vec_ok && (d.ks[i] * esz) % 16 == 0 && (d.vs[i] * esz) % 16 == 0;
-  const int threads_per_token = 3 * H * (Dh / 8);
-  if (vec_ok && threads_per_token <= 768 && threads_per_token % 32 == 0) {
-    const int lpr = Dh / 8;
-    ENGPT_REQUIRE((int64_t)B * T <= 0x7fffffffLL, ENGPT_ERR_SHAPE, "%s: too large", what);
-    const int64_t blocks = ((int64_t)B * T + kQkvTok - 1) / kQkvTok;
-#define ENGPT_QKV_LAUNCH(L)                                                                                  \
-  case L:                                                                                                    \
-    if (dtype == ENGPT_BF16)                                                                                 \
-      qkv_vec_kernel<__nv_bfloat16, L, PAGED><<<(unsigned)blocks, dim3(H * L, 3), 0, st>>>(a, d);             \
-    else                                                                                                     \
-      qkv_vec_kernel<float, L, PAGED><<<(unsigned)blocks, dim3(H * L, 3), 0, st>>>(a, d);                     \
-    break;
-    switch (lpr) {
-      ENGPT_QKV_LAUNCH(1)
-      ENGPT_QKV_LAUNCH(2)
-      ENGPT_QKV_LAUNCH(4)
-      ENGPT_QKV_LAUNCH(8)
-      ENGPT_QKV_LAUNCH(16)
-      ENGPT_QKV_LAUNCH(32)
-      default:
-        return set_error(ENGPT_ERR_UNSUPPORTED, "%s: lpr %d", what, lpr);
-    }
-#undef ENGPT_QKV_LAUNCH
-  } else {
-    const int64_t blocks = (ntask * 32 + 255) / 256;
-    ENGPT_REQUIRE(blocks <= 0x7fffffffLL, ENGPT_ERR_SHAPE, "%s: too large", what);
-    if (dtype == ENGPT_BF16) qkv_generic_kernel<__nv_bfloat16, PAGED><<<(unsigned)blocks, 256, 0, st>>>(a, d);
-    else qkv_generic_kernel<float, PAGED><<<(unsigned)blocks, 256, 0, st>>>(a, d);
-  }
+static int launch_generic(const QkvArgs& a, const PagedDst& d, int dtype, const char* what, cudaStream_t st) {
+  const int64_t ntask = (int64_t)a.B * a.T * 3 * a.H;
+  const int64_t blocks = (ntask * 32 + 255) / 256;
+  ENGPT_REQUIRE(blocks <= 0x7fffffffLL, ENGPT_ERR_SHAPE, "%s: too large", what);
+  if (dtype == ENGPT_BF16) qkv_generic_kernel<__nv_bfloat16, PAGED><<<(unsigned)blocks, 256, 0, st>>>(a, d);
+  else qkv_generic_kernel<float, PAGED><<<(unsigned)blocks, 256, 0, st>>>(a, d);
   return check_launch(what);
+}
+
+template <typename T, int LPR>
+static void launch_append(const QkvArgs& a, const PagedDst& d, cudaStream_t st) {
+  const int y = ceil_div((int64_t)a.H * LPR, 128);
+  // A token per CTA for a few tokens; else kAppendCtas per SM that walk, in bf16 with the registers held to 8 resident
+  // CTAs per SM for more rows in flight: 8188 tokens of 16 heads of 128 take 36 us so (5.6 TB/s), 39 with 6 resident
+  // CTAs, 44 without a limit, 46 with a token per CTA.  fp32 rows are twice as long and would spill at 8.
+  const int64_t most = (int64_t)num_sms() * kAppendCtas / y;
+  if (a.T <= most) {
+    append_vec_kernel<T, LPR, 1><<<dim3((unsigned)a.T, (unsigned)y), 128, 0, st>>>(a, d);
+    return;
+  }
+  append_vec_kernel<T, LPR, sizeof(T) == 2 ? 8 : 1>
+      <<<dim3((unsigned)(most > 0 ? most : 1), (unsigned)y), 128, 0, st>>>(a, d);
 }
 
 }  // namespace engpt
@@ -395,7 +475,34 @@ extern "C" int engpt_qkv_postprocess(const void* qkv, int dtype, const float* rh
   ENGPT_REQUIRE(rope_half == 0 || (cos_tab && sin_tab), ENGPT_ERR_ARG, "qkv_postprocess: null rope table");
   QkvArgs a{qkv, rho, cos_tab, sin_tab, rope_half, qk_scale, qk_mult, norm_eps, B, T, H, Dh, q_out, k_out, v_out,
             out_layout};
-  return launch_qkv<false>(a, PagedDst{}, dtype, "qkv_postprocess", as_stream(stream));
+  cudaStream_t st = as_stream(stream);
+  const bool vec_ok = vec_access(a, dtype == ENGPT_BF16 ? 2 : 4);
+  const int threads_per_token = 3 * H * (Dh / 8);
+  if (vec_ok && threads_per_token <= 768 && threads_per_token % 32 == 0) {
+    const int lpr = Dh / 8;
+    ENGPT_REQUIRE((int64_t)B * T <= 0x7fffffffLL, ENGPT_ERR_SHAPE, "qkv_postprocess: too large");
+    const int64_t blocks = ((int64_t)B * T + kQkvTok - 1) / kQkvTok;
+#define ENGPT_QKV_LAUNCH(L)                                                                                  \
+  case L:                                                                                                    \
+    if (dtype == ENGPT_BF16)                                                                                 \
+      qkv_vec_kernel<__nv_bfloat16, L><<<(unsigned)blocks, dim3(H * L, 3), 0, st>>>(a);                       \
+    else                                                                                                     \
+      qkv_vec_kernel<float, L><<<(unsigned)blocks, dim3(H * L, 3), 0, st>>>(a);                               \
+    break;
+    switch (lpr) {
+      ENGPT_QKV_LAUNCH(1)
+      ENGPT_QKV_LAUNCH(2)
+      ENGPT_QKV_LAUNCH(4)
+      ENGPT_QKV_LAUNCH(8)
+      ENGPT_QKV_LAUNCH(16)
+      ENGPT_QKV_LAUNCH(32)
+      default:
+        return set_error(ENGPT_ERR_UNSUPPORTED, "qkv_postprocess: lpr %d", lpr);
+    }
+#undef ENGPT_QKV_LAUNCH
+    return check_launch("qkv_postprocess");
+  }
+  return launch_generic<false>(a, PagedDst{}, dtype, "qkv_postprocess", st);
 }
 
 extern "C" int engpt_qkv_append(const void* qkv, int dtype, const float* rho, const float* cos_tab,
@@ -423,9 +530,35 @@ extern "C" int engpt_qkv_append(const void* qkv, int dtype, const float* rho, co
   d.rope_rows = rope_rows;
   d.n_slots = (int64_t)num_pages * page_size;
   d.page_size = page_size;
+  d.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size) : -1;
   for (int i = 0; i < 3; ++i) {
     d.ks[i] = page_strides[i];
     d.vs[i] = page_strides[3 + i];
   }
-  return launch_qkv<true>(a, d, dtype, "qkv_append", as_stream(stream));
+  const int esz = dtype == ENGPT_BF16 ? 2 : 4;
+  bool vec = vec_access(a, esz) && H <= 65535;
+  for (int i = 0; i < 3; ++i) {
+    // the stride of an axis of one element is never used, and may be anything
+    if ((i == 0 ? num_pages : i == 1 ? H : page_size) == 1) d.ks[i] = d.vs[i] = 0;
+    vec = vec && d.ks[i] * esz % 16 == 0 && d.vs[i] * esz % 16 == 0;
+  }
+  cudaStream_t st = as_stream(stream);
+  if (!vec) return launch_generic<true>(a, d, dtype, "qkv_append", st);
+#define ENGPT_APPEND_LAUNCH(L)                                       \
+  case 8 * L:                                                        \
+    if (dtype == ENGPT_BF16) launch_append<__nv_bfloat16, L>(a, d, st); \
+    else launch_append<float, L>(a, d, st);                          \
+    break;
+  switch (Dh) {
+    ENGPT_APPEND_LAUNCH(1)
+    ENGPT_APPEND_LAUNCH(2)
+    ENGPT_APPEND_LAUNCH(4)
+    ENGPT_APPEND_LAUNCH(8)
+    ENGPT_APPEND_LAUNCH(16)
+    ENGPT_APPEND_LAUNCH(32)
+    default:
+      return set_error(ENGPT_ERR_UNSUPPORTED, "qkv_append: head_dim %d", Dh);
+  }
+#undef ENGPT_APPEND_LAUNCH
+  return check_launch("qkv_append");
 }

@@ -11,6 +11,7 @@
 #include "sm100_ptx.cuh"
 
 #include <cudaTypedefs.h>
+#include <math.h>
 
 namespace engpt {
 namespace paged {
@@ -236,51 +237,51 @@ int dispatch_simt(const AttnArgs& a, bool vec, cudaStream_t st) {
 
 // ------------------------------------------------------------------ tensor-core kernel (bf16, head_dim 64 or 128)
 //
-// A tile is KT keys of one kv head (KT * D = 4096: 8 KB of keys, 8 KB of values).  The tiles of all (row, kv head)
-// pairs form one list, cut into equal contiguous ranges, one per warp ("worker") of a persistent grid, so the load
-// is even whatever the lengths.  A warp fetches its own tiles through its own ring of STAGES tiles in shared memory:
-// TMA boxes of R rows (R divides the page size) at the page that the block table names, 128-byte swizzled, one
-// mbarrier per stage; no warp waits for another one until the end.
+// A tile is KT keys of one kv head, TILE bytes of keys and as many of values.  The tiles of all (row, kv head) pairs
+// form one list, cut into equal contiguous ranges, one per warp ("worker") of a persistent grid, so the load is even
+// whatever the lengths.  A warp fetches its own tiles through its own ring of STAGES tiles in shared memory: TMA
+// boxes of R rows (R divides the page size) at the page that the block table names, 128-byte swizzled, one mbarrier
+// per stage; no warp waits for another one until the end.
 //
 // Per tile, with up to 8 query heads of the kv head as rows 0-7 of the 16-row mma.sync operand:
 //   S = Q K^T (rows 8-15 are zero), p = 2^(S scale - m), and O += P V with P's bf16 value in rows 0-7 and the
 //   remainder p - bf16(p), again as bf16, in rows 8-15: adding the two halves of O at the end gives the product
 //   with weights of 16 mantissa bits for the price of the otherwise idle half of the operand.
-// The products are far from bounding anything here (64 mma.sync of 16x8x16 per 16 KB), which is why this is not
-// built on tcgen05: its 128-row operand would be 1/128 to 1/16 full and would need TMEM round trips for P.
+// The products do not bound anything here (64 mma.sync of 16x8x16 per 16 KB), which is why this is not built on
+// tcgen05: its 128-row operand would be 1/128 to 1/16 full and P would take a trip through TMEM.
 //
-// A range that begins or ends inside a pair leaves a part (o, m, l).  Pairs within one CTA are joined by the warp
-// that holds their beginning, after a CTA barrier; a pair that runs over CTAs by decode_join_mma_kernel.
+// A range that begins or ends inside a pair leaves a part (o, m, l) in shared memory.  After a CTA barrier the parts
+// of a pair are joined by the warp that holds its first one; a pair that runs over CTAs leaves one part per CTA in
+// the workspace, joined by decode_join_list_kernel.
+constexpr int kWarps = 8;
+constexpr int kStages = 1;
+constexpr int kTileBytes = 8192;        // one of K, V
+
 template <int D>
 struct Mma {
-  static constexpr int KT = 4096 / D;
+  static constexpr int KT = kTileBytes / (2 * D);
   static constexpr int NT = KT / 8;     // 8-key tiles
   static constexpr int KC = KT / 16;    // 16-key steps of P V
   static constexpr int DK = D / 16;     // 16-dim steps of Q K^T
   static constexpr int DN = D / 8;      // 8-dim tiles of O
 };
-constexpr int kTileBytes = 8192;        // one of K, V
-constexpr int kWarps = 4;
-constexpr int kStages = 3;
 
 struct MmaArgs {
   const __nv_bfloat16* q;
   int64_t q_row, q_head;
   int B, H, G, HQ, QG;     // HQ: (kv head, group of up to 8 query heads) per row; QG: such groups per kv head
   int rows;                // query heads per group, min(G, 8)
-  int P, ps, R, r_shift;   // R = 2^r_shift keys per box
+  int P, ps, ps_shift;     // ps_shift: log2(page size), or -1
+  int R, r_shift;          // R = 2^r_shift keys per box
   const int* table;
   int64_t table_stride;
   int W;
   const int* lengths;
-  float scale_log2;
+  float scale_log2;        // |scale| log2(e)
+  uint32_t q_flip;         // sign bits to flip in q for a negative scale
   __nv_bfloat16* o;
-  float* work;             // [workers][2][rows][D + 2], then one Meta per CTA
+  float* work;             // [CTAs][2][rows][D + 2]
   int stages;
-};
-
-struct Meta {
-  int b, h, first, last;   // pair and its workers; first < 0: none
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
@@ -293,10 +294,9 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t* r) {
 }
 __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-               "{%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // p as bf16 plus the bf16 of what that rounding left.
@@ -306,14 +306,19 @@ __device__ __forceinline__ void split_bf16x2(float x, float y, uint32_t& hi, uin
   lo = sm100::pack_bf16x2(x - hx, y - hy);
 }
 
-// Usable length of row b without recording (the kernel's prologue records once).
-__device__ __forceinline__ int clip_length(const MmaArgs& a, int b) {
-  return (int)min((int64_t)max(a.lengths[b], 0), (int64_t)a.W * a.ps);
+// Usable length of row b (a length beyond the table is recorded once, by the kernel's prologue).
+__device__ __forceinline__ int clip_length(const MmaArgs& a, int len) {
+  return (int)min((int64_t)max(len, 0), (int64_t)a.W * a.ps);
 }
 
-// Position in the list of tiles: tile t of T of (row b of length len, head group h).
+// Position in the list of tiles: tile t of T of (row b of length len, head group h of kv head hk).
 struct Cursor {
-  int b, h, t, T, len;
+  int b, h, t, T, len, hk;
+};
+
+// A box of the tile to come: its page (-1: past the length, -2: outside the pool) and first row in the page.
+struct Box {
+  int page, off;
 };
 
 template <int D>
@@ -323,37 +328,40 @@ struct Worker {
   const CUtensorMap *mk, *mv;
   uint32_t ring;            // this warp's stages in shared memory
   uint32_t bars;            // its mbarriers
-  int* masks;               // valid boxes of the tile in each stage
-  volatile int* abort_flag;
+  int* masks;               // copied boxes of the tile in each stage
   int lane;
 
   __device__ __forceinline__ void enter_row(Cursor& c) const {
-    c.len = c.b < a.B ? clip_length(a, c.b) : 0;
+    c.len = c.b < a.B ? clip_length(a, a.lengths[c.b]) : 0;
     c.T = (c.len + C::KT - 1) / C::KT;
   }
 
   __device__ __forceinline__ void advance(Cursor& c) const {
     if (++c.t < c.T) return;
     c.t = 0;
-    if (++c.h < a.HQ) return;
-    c.h = 0;
+    ++c.h;
+    if (c.h < a.HQ) {
+      c.hk = c.h / a.QG;
+      return;
+    }
+    c.h = c.hk = 0;
     do {
       ++c.b;
       enter_row(c);
     } while (c.b < a.B && c.T == 0);
   }
 
-  // Page of box `lane` of the cursor's tile: -1 past the length, -2 outside the pool.
-  __device__ __forceinline__ int box_page(const Cursor& c) const {
+  __device__ __forceinline__ Box find_box(const Cursor& c) const {
     const int key = c.t * C::KT + lane * a.R;
-    if (lane * a.R >= C::KT || key >= c.len) return -1;
-    const int page = a.table[c.b * a.table_stride + key / a.ps];
-    return page >= 0 && page < a.P ? page : -2;
+    if (lane * a.R >= C::KT || key >= c.len) return Box{-1, 0};
+    const int j = a.ps_shift >= 0 ? key >> a.ps_shift : key / a.ps;
+    const int page = a.table[c.b * a.table_stride + j];
+    return Box{page >= 0 && page < a.P ? page : -2, key - j * a.ps};
   }
 
   // Start the copies of the cursor's tile into stage s.
-  __device__ __forceinline__ void issue(const Cursor& c, int page, int s) const {
-    const uint32_t mask = __ballot_sync(0xffffffffu, page >= 0);
+  __device__ __forceinline__ void issue(const Cursor& c, const Box& x, int s) const {
+    const uint32_t mask = __ballot_sync(0xffffffffu, x.page >= 0);
     const uint32_t bar = bars + 8 * s;
     const uint32_t box = a.R * 128;
     if (lane == 0) {
@@ -361,18 +369,17 @@ struct Worker {
       sm100::mbar_expect_tx(bar, __popc(mask) * box * (D / 64) * 2);
     }
     __syncwarp();
-    if (page >= 0) {
-      const int key = c.t * C::KT + lane * a.R;
-      const int off = key % a.ps, hk = c.h / a.QG;
+    if (x.page >= 0) {
       const uint32_t dst = ring + s * 2 * kTileBytes + lane * box;
 #pragma unroll
       for (int half = 0; half < D / 64; ++half) {
-        sm100::tma_load_4d(dst + half * C::KT * 128, mk, half * 64, off, hk, page, bar);
-        sm100::tma_load_4d(dst + half * C::KT * 128 + kTileBytes, mv, half * 64, off, hk, page, bar);
+        sm100::tma_load_4d(dst + half * C::KT * 128, mk, half * 64, x.off, c.hk, x.page, bar);
+        sm100::tma_load_4d(dst + half * C::KT * 128 + kTileBytes, mv, half * 64, x.off, c.hk, x.page, bar);
       }
-    } else if (page == -2) {
+    } else if (x.page == -2) {
       record_device_error(ENGPT_ERR_ARG, 44);
     }
+    __syncwarp();
   }
 
   // A wait ran out: let the copies still in flight land (bounded) before the CTA's shared memory goes away.
@@ -388,7 +395,7 @@ struct Worker {
 };
 
 // The running state of one pair: rows 0-7 of S and O in the mma layout (row lane / 4, columns 2 (lane % 4) + {0, 1}
-// of each 8-column tile).
+// of each 8-column tile).  m is in units of the raw product q.k.
 template <int D>
 struct State {
   float o[Mma<D>::DN][4];
@@ -411,64 +418,60 @@ __device__ __forceinline__ void load_query(const MmaArgs& a, int b, int h, int l
   const __nv_bfloat16* q = a.q + b * a.q_row + head * a.q_head + 2 * t;
 #pragma unroll
   for (int k = 0; k < Mma<D>::DK; ++k) {
-    qa[k][0] = live ? *reinterpret_cast<const uint32_t*>(q + k * 16) : 0u;
-    qa[k][1] = live ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 8) : 0u;
+    qa[k][0] = live ? *reinterpret_cast<const uint32_t*>(q + k * 16) ^ a.q_flip : 0u;
+    qa[k][1] = live ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 8) ^ a.q_flip : 0u;
   }
 }
 
-// One tile: scores, softmax step, P V.  `live` keys from the tile's start are below the length; boxes whose bit of
-// `mask` is unset were not copied.
-template <int D>
+// One tile: scores, softmax step, P V.  WHOLE: all its keys count.  Otherwise `live` keys from the tile's start are
+// below the length, and boxes whose bit of `mask` is unset were not copied.
+template <int D, bool WHOLE>
 __device__ __forceinline__ void tile_step(const MmaArgs& a, uint32_t sk, const uint32_t (*qa)[2], State<D>& st,
                                           int live, uint32_t mask, int lane) {
   using C = Mma<D>;
   const uint32_t sv = sk + kTileBytes;
   const int r8 = lane & 7, q4 = lane >> 3, t = lane & 3;
-  const bool whole = live >= C::KT && mask == (1u << (C::KT >> a.r_shift)) - 1u;
-  float s[C::NT][4];
-#pragma unroll
-  for (int n = 0; n < C::NT; ++n) {
-    s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-    for (int kp = 0; kp < C::DK / 2; ++kp) {
-      uint32_t b[4];
-      const int c = kp * 4 + q4;
-      ldsm4(sk + (c >> 3) * (C::KT * 128) + (n * 8 + r8) * 128 + (((c & 7) ^ r8) << 4), b);
-      mma16816(s[n], qa[2 * kp][0], 0u, qa[2 * kp][1], 0u, b[0], b[1]);
-      mma16816(s[n], qa[2 * kp + 1][0], 0u, qa[2 * kp + 1][1], 0u, b[2], b[3]);
-    }
-  }
-  if (!whole) {
-    // absent keys: score -inf (weight 0), and values 0, as the weight would not cancel a stale NaN or infinity
-#pragma unroll
-    for (int n = 0; n < C::NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int key = n * 8 + 2 * t + i;
-        if (key >= live || !((mask >> (key >> a.r_shift)) & 1u)) s[n][i] = -INFINITY;
-        else s[n][i] *= a.scale_log2;
-      }
+  if (!WHOLE) {
+    // absent values become 0: their weight 0 would not cancel a stale NaN or infinity
     for (int i = lane; i < C::KT * (D / 64) * 8; i += 32) {   // 16-byte pieces: half, key, piece
       const int key = (i >> 3) % C::KT;
       if (key >= live || !((mask >> (key >> a.r_shift)) & 1u))
         asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(sv + i * 16), "r"(0u) : "memory");
     }
     __syncwarp();
-  } else {
+  }
+  float s[C::NT][4];
 #pragma unroll
-    for (int n = 0; n < C::NT; ++n) {
-      s[n][0] *= a.scale_log2;
-      s[n][1] *= a.scale_log2;
-    }
+  for (int n = 0; n < C::NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+  for (int kp = 0; kp < C::DK / 2; ++kp) {
+    uint32_t b[C::NT][4];
+    const int c = kp * 4 + q4;
+#pragma unroll
+    for (int n = 0; n < C::NT; ++n)
+      ldsm4(sk + (c >> 3) * (C::KT * 128) + (n * 8 + r8) * 128 + (((c & 7) ^ r8) << 4), b[n]);
+#pragma unroll
+    for (int n = 0; n < C::NT; ++n) mma16816(s[n], qa[2 * kp][0], 0u, qa[2 * kp][1], 0u, b[n][0], b[n][1]);
+#pragma unroll
+    for (int n = 0; n < C::NT; ++n) mma16816(s[n], qa[2 * kp + 1][0], 0u, qa[2 * kp + 1][1], 0u, b[n][2], b[n][3]);
+  }
+  if (!WHOLE) {
+#pragma unroll
+    for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int key = n * 8 + 2 * t + i;
+        if (key >= live || !((mask >> (key >> a.r_shift)) & 1u)) s[n][i] = -INFINITY;
+      }
   }
   float mx = st.m;
 #pragma unroll
   for (int n = 0; n < C::NT; ++n) mx = fmaxf(mx, fmaxf(s[n][0], s[n][1]));
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-  const float ms = mx == -INFINITY ? 0.f : mx;
-  const float corr = sm100::ex2_approx(st.m - ms);
+  const float ms = mx == -INFINITY ? 0.f : mx * a.scale_log2;
   if (__any_sync(0xffffffffu, mx > st.m)) {
+    const float corr = st.m == -INFINITY ? 0.f : sm100::ex2_approx(st.m * a.scale_log2 - ms);
 #pragma unroll
     for (int i = 0; i < C::DN; ++i)
 #pragma unroll
@@ -476,35 +479,44 @@ __device__ __forceinline__ void tile_step(const MmaArgs& a, uint32_t sk, const u
     st.l *= corr;
     st.m = mx;
   }
+  uint32_t hi[C::KC][2], lo[C::KC][2];
+  float sum[2] = {0.f, 0.f};
+#pragma unroll
+  for (int n = 0; n < C::NT; ++n) {
+    float p[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      p[i] = sm100::ex2_approx(fmaf(s[n][i], a.scale_log2, -ms));
+      if (!WHOLE && s[n][i] == -INFINITY) p[i] = 0.f;   // (the product is NaN for a scale of 0)
+      sum[i] += p[i];
+    }
+    split_bf16x2(p[0], p[1], hi[n >> 1][n & 1], lo[n >> 1][n & 1]);
+  }
+  st.l += sum[0] + sum[1];
 #pragma unroll
   for (int j = 0; j < C::KC; ++j) {
-    float p[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      p[i] = sm100::ex2_approx(s[2 * j + (i >> 1)][i & 1] - ms);
-      st.l += p[i];
-    }
-    uint32_t h0, l0, h1, l1;
-    split_bf16x2(p[0], p[1], h0, l0);
-    split_bf16x2(p[2], p[3], h1, l1);
     const int key = j * 16 + (q4 & 1) * 8 + r8;
+    uint32_t b[C::DN / 2][4];
 #pragma unroll
     for (int dp = 0; dp < C::DN / 2; ++dp) {
-      uint32_t b[4];
       const int c = 2 * dp + (q4 >> 1);
-      ldsm4_t(sv + (c >> 3) * (C::KT * 128) + key * 128 + (((c & 7) ^ r8) << 4), b);
-      mma16816(st.o[2 * dp], h0, l0, h1, l1, b[0], b[1]);
-      mma16816(st.o[2 * dp + 1], h0, l0, h1, l1, b[2], b[3]);
+      ldsm4_t(sv + (c >> 3) * (C::KT * 128) + key * 128 + (((c & 7) ^ r8) << 4), b[dp]);
+    }
+#pragma unroll
+    for (int dp = 0; dp < C::DN / 2; ++dp) {
+      mma16816(st.o[2 * dp], hi[j][0], lo[j][0], hi[j][1], lo[j][1], b[dp][0], b[dp][1]);
+      mma16816(st.o[2 * dp + 1], hi[j][0], lo[j][0], hi[j][1], lo[j][1], b[dp][2], b[dp][3]);
     }
   }
-  if (!whole) sm100::fence_proxy_async_smem();   // the zeros above, before a later copy into this stage
+  if (!WHOLE) sm100::fence_proxy_async_smem();   // the zeros above, before a later copy into this stage
 }
 
-// The pair's sums of this lane: o (both halves of the operand added) and l over the row's four lanes.
+// The pair's sums of this lane: o (both halves of the operand added) and l over the row's four lanes; m in base-2 units.
 template <int D>
-__device__ __forceinline__ void finish_rows(State<D>& st) {
+__device__ __forceinline__ void finish_rows(const MmaArgs& a, State<D>& st) {
   st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
   st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
+  if (st.m != -INFINITY) st.m *= a.scale_log2;
 #pragma unroll
   for (int i = 0; i < Mma<D>::DN; ++i) {
     st.o[i][0] += st.o[i][2];
@@ -534,21 +546,47 @@ __device__ __forceinline__ void store_rows(const MmaArgs& a, const State<D>& st,
     *reinterpret_cast<uint32_t*>(o + i * 8) = sm100::pack_bf16x2(st.o[i][0] * inv, st.o[i][1] * inv);
 }
 
-// Joins parts (one per index i < n, at part(i)) of a pair, one warp, and stores the rows.
+// Joins row r of n <= 8 parts (part(i): its rows) by one warp: into the output, or as one part at `to`.  Lane i holds
+// part i's weight, and all loads are independent.
 template <int D, typename F>
-__device__ __forceinline__ void join_rows(const MmaArgs& a, int b, int h, int n, F part, int lane) {
+__device__ __forceinline__ void join_row(const MmaArgs& a, int b, int h, int r, int n, F part, float* to, int lane) {
   constexpr int E = D / 32;
-  for (int r = 0; r < a.rows && (h % a.QG) * 8 + r < a.G; ++r) {
-    float mx = -INFINITY;
-    for (int i = 0; i < n; ++i) mx = fmaxf(mx, part(i)[r * (D + 2) + D]);
-    float o[E] = {}, l = 0.f;
-    for (int i = 0; i < n; ++i) {
-      const float* p = part(i) + r * (D + 2);
-      const float w = join_weight(p[D], mx);
-      l = fmaf(p[D + 1], w, l);
+  if ((h % a.QG) * 8 + r >= a.G) return;
+  float m = -INFINITY, l = 0.f;
+  if (lane < n) {
+    const float2 ml = *reinterpret_cast<const float2*>(part(lane) + r * (D + 2) + D);
+    m = ml.x;
+    l = ml.y;
+  }
+  float mx = m;
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = fmaf(p[lane + 32 * e], w, o[e]);
+  for (int k = 4; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+  mx = __shfl_sync(0xffffffffu, mx, 0);
+  const float w = join_weight(m, mx);
+  l *= w;
+#pragma unroll
+  for (int k = 4; k > 0; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
+  l = __shfl_sync(0xffffffffu, l, 0);
+  float x[8][E], o[E] = {};
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[k][e] = k < n ? part(k)[r * (D + 2) + lane + 32 * e] : 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float wk = __shfl_sync(0xffffffffu, w, k);
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = fmaf(x[k][e], wk, o[e]);
+  }
+  if (to) {
+    to += r * (D + 2);
+#pragma unroll
+    for (int e = 0; e < E; ++e) to[lane + 32 * e] = o[e];
+    if (lane == 0) {
+      to[D] = mx;
+      to[D + 1] = l;
     }
+  } else {
     const float inv = l == 0.f ? 0.f : 1.f / l;
     __nv_bfloat16* dst = a.o + ((int64_t)b * a.H + (h / a.QG) * a.G + (h % a.QG) * 8 + r) * D;
 #pragma unroll
@@ -556,10 +594,76 @@ __device__ __forceinline__ void join_rows(const MmaArgs& a, int b, int h, int n,
   }
 }
 
-// LIST: the persistent form over the list of tiles.  Otherwise one CTA per pair (its tiles dealt to the four warps
-// in contiguous shares, joined in shared memory): no prefix sums, no second launch.
-template <int D, bool LIST>
-__global__ void __launch_bounds__(kWarps * 32) decode_mma_kernel(MmaArgs a, const __grid_constant__ CUtensorMap mk,
+// Floats of shared memory for one part of each warp.
+template <int D>
+__host__ __device__ constexpr int part_floats(int rows) {
+  return rows * (D + 2);
+}
+
+// First tile of every row, s_start[0 .. B] (exclusive prefix sums of a row's tiles times HQ), by a CTA of `threads`
+// threads; returns their number.  For up to 32 rows every warp forms the same sums for itself (the warps write the
+// same numbers) and keeps row `lane`'s length and first tile in `len` and `start`: no barrier before the first copy.
+template <int KT>
+__device__ __forceinline__ int list_starts(const MmaArgs& a, int* s_start, int* s_scan, int threads, bool record,
+                                           int& len, int& start) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int carry = 0;
+  for (int b0 = 0; b0 < a.B; b0 += threads) {
+    const int b = b0 + (a.B <= 32 ? lane : tid);
+    len = 0;
+    if (b < a.B) {
+      len = a.lengths[b];
+      if (record && len > (int64_t)a.W * a.ps) record_device_error(ENGPT_ERR_ARG, 44);
+      len = clip_length(a, len);
+    }
+    const int v = (len + KT - 1) / KT * a.HQ;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (a.B <= 32) {
+      start = x - v;
+      if (lane < a.B) s_start[lane] = start;
+      carry = __shfl_sync(0xffffffffu, x, 31);
+      if (lane == 0) s_start[a.B] = carry;
+      __syncwarp();
+      return carry;
+    }
+    if (lane == 31) s_scan[warp] = x;
+    __syncthreads();
+    int before = carry, total = 0;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      if (i < warp) before += s_scan[i];
+      total += s_scan[i];
+    }
+    if (b < a.B) s_start[b] = before + x - v;
+    carry += total;
+    __syncthreads();
+  }
+  if (tid == 0) s_start[a.B] = carry;
+  __syncthreads();
+  return carry;
+}
+
+// Last row whose first tile is <= f (rows without tiles share their successor's start).
+__device__ __forceinline__ int list_row(const MmaArgs& a, const int* s_start, int f, int start) {
+  const int lane = threadIdx.x & 31;
+  if (a.B <= 32) return 31 - __clz(__ballot_sync(0xffffffffu, lane < a.B && start <= f));
+  int lo = 0, hi = a.B;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (s_start[mid] <= f) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// The persistent form over the list of tiles.
+template <int D>
+__global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(MmaArgs a, const __grid_constant__ CUtensorMap mk,
                                                                  const __grid_constant__ CUtensorMap mv) {
   using C = Mma<D>;
   extern __shared__ uint8_t smem_raw[];
@@ -568,115 +672,80 @@ __global__ void __launch_bounds__(kWarps * 32) decode_mma_kernel(MmaArgs a, cons
   const int ring_bytes = a.stages * 2 * kTileBytes;
   uint8_t* tail = ring_ptr + kWarps * ring_bytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(tail);                       // [kWarps][stages]
-  int* masks = reinterpret_cast<int*>(bars + kWarps * a.stages);            // [kWarps][stages]
-  int* s_abort = masks + kWarps * a.stages;
-  int* s_scan = s_abort + 1;                                                // [kWarps]
-  int* s_start = s_scan + kWarps;                                           // LIST: [B + 1] first tile of each row
+  const int pf = part_floats<D>(a.rows);
+  float* s_part = reinterpret_cast<float*>(bars + kWarps * a.stages);       // [kWarps] first part of each warp
+  int* masks = reinterpret_cast<int*>(s_part + kWarps * pf);                // [kWarps][stages]
+  int* s_start = masks + kWarps * a.stages;                                 // [B + 1] first tile of each row
+  __shared__ int s_abort, s_scan[kWarps], s_head[kWarps], s_tail[kWarps], s_over[kWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   Worker<D> w{a, &mk, &mv, base + warp * ring_bytes, sm100::smem_u32(bars + warp * a.stages), masks + warp * a.stages,
-              s_abort, lane};
+              lane};
   if (lane == 0) {
     for (int s = 0; s < a.stages; ++s) sm100::mbar_init(w.bars + 8 * s, 1);
     sm100::fence_mbar_init();
+    s_abort = 0;         // (every warp: a wait may set it only seconds later)
+    s_head[warp] = s_tail[warp] = -1;
+  }
+  if (tid == 0) {
     sm100::tma_prefetch_desc(&mk);
     sm100::tma_prefetch_desc(&mv);
   }
-  if (tid == 0) *s_abort = 0;
+  __syncwarp();
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // nothing of an earlier kernel has been touched before
 
   // this worker's range of the list [f0, f1) and its first tile
   const int worker = blockIdx.x * kWarps + warp;
-  int f0, f1, per = 0;
+  int row_len = 0, row_start = 0;
+  const int total = list_starts<C::KT>(a, s_start, s_scan, kWarps * 32, blockIdx.x == 0, row_len, row_start);
+  const int workers = gridDim.x * kWarps;
+  const int per = (int)(((uint32_t)total + workers - 1) / (uint32_t)workers);
+  const int f0 = (int)min((int64_t)total, (int64_t)worker * per), f1 = (int)min((int64_t)total, (int64_t)f0 + per);
   Cursor c;
-  if (LIST) {
-    // first tile of every row: exclusive prefix sums of tiles(b) * HQ
-    int carry = 0;
-    for (int b0 = 0; b0 < a.B; b0 += kWarps * 32) {
-      const int b = b0 + tid;
-      int v = 0;
-      if (b < a.B) {
-        if (blockIdx.x == 0 && a.lengths[b] > (int64_t)a.W * a.ps) record_device_error(ENGPT_ERR_ARG, 44);
-        v = (clip_length(a, b) + C::KT - 1) / C::KT * a.HQ;
-      }
-      int x = v;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      if (lane == 31) s_scan[warp] = x;
-      __syncthreads();
-      int before = carry, total = 0;
-#pragma unroll
-      for (int i = 0; i < kWarps; ++i) {
-        if (i < warp) before += s_scan[i];
-        total += s_scan[i];
-      }
-      if (b < a.B) s_start[b] = before + x - v;
-      carry += total;
-      __syncthreads();
-    }
-    if (tid == 0) s_start[a.B] = carry;
-    __syncthreads();
-    const int workers = gridDim.x * kWarps;
-    per = (carry + workers - 1) / workers;
-    f0 = (int)min((int64_t)carry, (int64_t)worker * per);
-    f1 = min(carry, f0 + per);
-    // last row whose first tile is <= f0 (rows without tiles share their successor's start)
-    int lo = 0, hi = a.B;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s_start[mid] <= f0) lo = mid;
-      else hi = mid;
-    }
-    c.b = lo;
-    w.enter_row(c);
-    const int in = f0 - s_start[lo], T = max(c.T, 1);
-    c.h = in / T;
-    c.t = in - c.h * T;
+  c.b = list_row(a, s_start, f0, row_start);
+  if (a.B <= 32) {
+    c.len = __shfl_sync(0xffffffffu, row_len, c.b);
+    c.T = (c.len + C::KT - 1) / C::KT;
   } else {
-    c.b = blockIdx.x / a.HQ;
-    c.h = blockIdx.x - c.b * a.HQ;
-    if (tid == 0 && c.h == 0 && a.lengths[c.b] > (int64_t)a.W * a.ps) record_device_error(ENGPT_ERR_ARG, 44);
     w.enter_row(c);
-    per = (c.T + kWarps - 1) / kWarps;
-    f0 = min(c.T, warp * per);
-    f1 = min(c.T, f0 + per);
-    c.t = f0;
-    __syncthreads();   // *s_abort
   }
-
-  // rows without keys
-  if (LIST) {
-    for (int64_t i = blockIdx.x * (int64_t)(kWarps * 32) + tid; i < (int64_t)a.B * a.H; i += (int64_t)gridDim.x * kWarps * 32) {
-      const int b = (int)(i / a.H);
-      if (s_start[b + 1] == s_start[b])
-        for (int e = 0; e < D; e += 8) *reinterpret_cast<uint4*>(a.o + i * D + e) = make_uint4(0u, 0u, 0u, 0u);
-    }
-  }
+  const uint32_t in = f0 - s_start[c.b], T = max(c.T, 1);
+  c.h = (int)(in / T);
+  c.t = (int)(in - c.h * T);
+  c.hk = c.h / a.QG;
 
   // fill the ring
-  int n_issued = min(f1 - f0, a.stages);
+  const int n_issued = min(f1 - f0, a.stages);
   Cursor ci = c;
-  int page = n_issued > 0 ? w.box_page(ci) : -1;
+  Box box = n_issued > 0 ? w.find_box(ci) : Box{-1, 0};
   for (int s = 0; s < n_issued; ++s) {
     Cursor cn = ci;
     w.advance(cn);
-    const int pn = f0 + s + 1 < f1 ? w.box_page(cn) : -1;
-    w.issue(ci, page, s);
+    const Box next = f0 + s + 1 < f1 ? w.find_box(cn) : Box{-1, 0};
+    w.issue(ci, box, s);
     ci = cn;
-    page = pn;
+    box = next;
   }
 
-  const int pair_tiles = c.T;   // one CTA per pair: its tiles
+  // the joining kernel may start: it reads nothing of this one before this one has ended
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // rows without keys
+  for (int64_t i = blockIdx.x * (int64_t)(kWarps * 32) + tid; i < (int64_t)a.B * a.H;
+       i += (int64_t)gridDim.x * kWarps * 32) {
+    const int b = (int)(i / a.H);
+    if (s_start[b + 1] == s_start[b])
+      for (int e = 0; e < D; e += 8) *reinterpret_cast<uint4*>(a.o + i * D + e) = make_uint4(0u, 0u, 0u, 0u);
+  }
+
+  float* part = s_part + warp * pf;                                         // a pair that began before this range
+  float* tail_part = reinterpret_cast<float*>(ring_ptr + warp * ring_bytes);   // one that ends behind it (ring unused)
   State<D> st;
   st.reset();
   uint32_t qa[C::DK][2];
   uint32_t phases = 0;
-  bool fresh = true;          // the next tile begins a segment
-  bool ok = true, cut = false;
-  int t0 = 0, my_last = 0;
-  Cursor mine = c;            // the pair whose beginning this worker holds and whose end it does not
+  bool fresh = true;                // the next tile begins a segment
+  int t0 = 0;
   int s = 0;
   for (int f = f0; f < f1; ++f) {
     if (fresh) {
@@ -684,97 +753,226 @@ __global__ void __launch_bounds__(kWarps * 32) decode_mma_kernel(MmaArgs a, cons
       t0 = c.t;
       fresh = false;
     }
-    if (!__all_sync(0xffffffffu, sm100::mbar_wait(w.bars + 8 * s, (phases >> s) & 1u, s_abort, 45))) {
+    if (!__all_sync(0xffffffffu, sm100::mbar_wait(w.bars + 8 * s, (phases >> s) & 1u, &s_abort, 45))) {
       w.drain(s, min(f1 - f, a.stages), phases);
-      ok = false;
-      break;
+      break;   // (the pair keeps no part of this warp: its rows are wrong, and the status word says so)
     }
     phases ^= 1u << s;
-    tile_step<D>(a, w.ring + s * 2 * kTileBytes, qa, st, c.len - c.t * C::KT, (uint32_t)w.masks[s], lane);
+    const uint32_t sk = w.ring + s * 2 * kTileBytes, mask = (uint32_t)w.masks[s];
+    const int live = c.len - c.t * C::KT;
+    if (live >= C::KT && mask == (1u << (C::KT >> a.r_shift)) - 1u)
+      tile_step<D, true>(a, sk, qa, st, live, mask, lane);
+    else
+      tile_step<D, false>(a, sk, qa, st, live, mask, lane);
     __syncwarp();
     if (f + a.stages < f1) {
-      w.issue(ci, page, s);
+      w.issue(ci, box, s);
       w.advance(ci);
-      page = f + a.stages + 1 < f1 ? w.box_page(ci) : -1;
+      box = f + a.stages + 1 < f1 ? w.find_box(ci) : Box{-1, 0};
     }
     if (++s == a.stages) s = 0;
     const bool pair_end = c.t + 1 == c.T;
     if (pair_end || f + 1 == f1) {
-      finish_rows<D>(st);
-      if (LIST) {
-        if (t0 == 0 && pair_end) {
-          store_rows<D>(a, st, c.b, c.h, lane);
-        } else {
-          store_part<D>(a, st, a.work + ((int64_t)worker * 2 + (t0 == 0 ? 1 : 0)) * a.rows * (D + 2), lane);
-          if (t0 == 0) {
-            cut = true;
-            mine = c;
-            my_last = (s_start[c.b] + (c.h + 1) * c.T - 1) / per;
-          }
+      finish_rows<D>(a, st);
+      if (t0 == 0 && pair_end) {
+        store_rows<D>(a, st, c.b, c.h, lane);
+      } else if (t0 == 0) {
+        store_part<D>(a, st, tail_part, lane);   // the last tile of the range: every stage has been read
+        if (lane == 0) {
+          s_tail[warp] = c.b * a.HQ + c.h;
+          s_over[warp] = s_start[c.b] + (int64_t)(c.h + 1) * c.T > (int64_t)(blockIdx.x + 1) * kWarps * per;
         }
-        st.reset();
-        fresh = true;
+      } else {
+        store_part<D>(a, st, part, lane);
+        if (lane == 0) s_head[warp] = c.b * a.HQ + c.h;
       }
+      st.reset();
+      fresh = true;
     }
     w.advance(c);
   }
 
-  if (LIST) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    __shared__ Meta s_meta;
-    if (tid == 0) s_meta.first = -1;
-    __syncthreads();   // every worker's parts are written
-    if (cut && ok) {
-      if (my_last / kWarps == (int)blockIdx.x) {
-        const int first = worker, rows = a.rows;
-        const float* work = a.work;
-        join_rows<D>(a, mine.b, mine.h, my_last - first + 1,
-                     [=](int i) { return work + ((int64_t)(first + i) * 2 + (i == 0 ? 1 : 0)) * rows * (D + 2); }, lane);
-      } else if (lane == 0) {
-        s_meta = Meta{mine.b, mine.h, worker, my_last};   // at most one pair runs over the CTA's end
-      }
-    }
-    __syncthreads();
-    if (tid == 0) {
-      Meta* metas = reinterpret_cast<Meta*>(a.work + (int64_t)gridDim.x * kWarps * 2 * a.rows * (D + 2));
-      metas[blockIdx.x] = s_meta;
-    }
+  float* out = a.work + (int64_t)blockIdx.x * 2 * pf;
+  __syncthreads();   // every worker's parts are written
+  // Groups of parts of one pair: those that begin in warp g, and the one that comes in from an earlier CTA (g = -1:
+  // warps 0, 1, ..).  With few rows a warp joins its own group (the last warp the incoming one too); with 8 all warps
+  // share each group's rows.
+  auto join_group = [&](int g, int r0, int step) {
+    const int pair = g < 0 ? s_head[0] : s_tail[g];
+    if (pair < 0) return;
+    const int w0 = max(g, 0);
+    int n = g < 0 ? 0 : 1;
+    while (w0 + n < kWarps && s_head[w0 + n] == pair) ++n;
+    const float* first = g < 0 ? s_part : reinterpret_cast<const float*>(ring_ptr + g * ring_bytes);
+    const float* rest = s_part + g * pf;
+    float* to = g < 0 ? out : (s_over[g] ? out + pf : nullptr);   // at most one pair runs over the CTA's end
+    const int b = pair / a.HQ, h = pair - b * a.HQ;
+    for (int r = r0; r < a.rows; r += step)
+      join_row<D>(a, b, h, r, n, [=](int i) { return i == 0 ? first : (g < 0 ? first : rest) + i * pf; }, to, lane);
+  };
+  if (a.rows < kWarps) {
+    join_group(warp, 0, 1);
+    if (warp == kWarps - 1) join_group(-1, 0, 1);
   } else {
-    // parts in each warp's own (by now unused) ring memory
-    float* part = reinterpret_cast<float*>(ring_ptr + warp * ring_bytes);
-    if (f0 >= f1) finish_rows<D>(st);
-    const int n = per > 0 ? (pair_tiles + per - 1) / per : 0;
-    __syncwarp();
-    if (n > 1 && ok) store_part<D>(a, st, part, lane);
-    __syncthreads();
-    const int b = blockIdx.x / a.HQ, h = blockIdx.x - b * a.HQ;
-    if (warp == 0 && ok) {
-      if (n <= 1)
-        store_rows<D>(a, st, b, h, lane);
-      else
-        join_rows<D>(a, b, h, n, [=](int i) { return reinterpret_cast<const float*>(ring_ptr + i * ring_bytes); }, lane);
-    }
+    for (int g = -1; g < kWarps; ++g) join_group(g, warp, kWarps);
   }
 }
 
-// Pairs that run over the end of a CTA of decode_mma_kernel: one CTA per such end, a warp's share of the parts each.
+// One cluster of `cs` CTAs per pair: tile t goes to warp t mod (cs * kWarps) of the cluster, whose parts are joined
+// through shared memory, then through the shared memory of the cluster's first CTA.  No prefix sums, no second
+// launch, and the first page look-up does not wait for the length: the form for short rows and for few pairs.
 template <int D>
-__global__ void __launch_bounds__(256) decode_join_mma_kernel(MmaArgs a, int ctas) {
-  constexpr int E = D / 32, NW = 8;
-  __shared__ float s_o[NW][D];
-  __shared__ float s_m[NW], s_l[NW];
+__global__ void __launch_bounds__(kWarps * 32) decode_pair_kernel(MmaArgs a, const __grid_constant__ CUtensorMap mk,
+                                                                  const __grid_constant__ CUtensorMap mv, int cs) {
+  using C = Mma<D>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (sm100::smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* ring_ptr = smem_raw + (base - sm100::smem_u32(smem_raw));
+  const int ring_bytes = a.stages * 2 * kTileBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring_ptr + kWarps * ring_bytes);   // [kWarps][stages]
+  const int pf = part_floats<D>(a.rows);
+  float* s_part = reinterpret_cast<float*>(bars + kWarps * a.stages);             // [kWarps] the warps' parts
+  float* s_cta = s_part + kWarps * pf;                                            // [cs] the CTAs' parts (rank 0)
+  int* masks = reinterpret_cast<int*>(s_cta + cs * pf);                           // [kWarps][stages]
+  __shared__ int s_abort;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (cs > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+
+  const int pair = blockIdx.x / cs, rank = blockIdx.x - pair * cs;
+  const int me = rank * kWarps + warp, step = cs * kWarps;
+  Worker<D> w{a, &mk, &mv, base + warp * ring_bytes, sm100::smem_u32(bars + warp * a.stages), masks + warp * a.stages,
+              lane};
+  Cursor c;
+  c.b = pair / a.HQ;
+  c.h = pair - c.b * a.HQ;
+  c.hk = c.h / a.QG;
+  c.t = me;
+  if (lane == 0) {
+    for (int s = 0; s < a.stages; ++s) sm100::mbar_init(w.bars + 8 * s, 1);
+    sm100::fence_mbar_init();
+    s_abort = 0;                        // (every warp: a wait may set it only seconds later)
+    if (warp == 0) {
+      sm100::tma_prefetch_desc(&mk);
+      sm100::tma_prefetch_desc(&mv);
+    }
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // nothing of an earlier kernel has been touched before
+  const int len = a.lengths[c.b];
+  c.len = c.T = a.W * a.ps;             // the look-up is bounded by the table row; the length cuts it below
+  Box box = w.find_box(c);
+  if (me == 0 && c.h == 0 && lane == 0 && len > (int64_t)a.W * a.ps) record_device_error(ENGPT_ERR_ARG, 44);
+  uint32_t qa[C::DK][2];
+  load_query<D>(a, c.b, c.h, lane, qa);
+  __syncwarp();
+  c.len = clip_length(a, len);
+  c.T = (c.len + C::KT - 1) / C::KT;
+  if (c.t * C::KT + lane * a.R >= c.len) box.page = -1;
+  const int n = c.T > me ? (c.T - me + step - 1) / step : 0;   // this warp's tiles
+  Cursor ci = c;
+  for (int i = 0; i < min(n, a.stages); ++i) {
+    w.issue(ci, box, i);
+    ci.t += step;
+    box = i + 1 < n ? w.find_box(ci) : Box{-1, 0};
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  State<D> st;
+  st.reset();
+  uint32_t phases = 0;
+  bool ok = true;
+  int s = 0;
+  for (int i = 0; i < n; ++i, c.t += step) {
+    if (!__all_sync(0xffffffffu, sm100::mbar_wait(w.bars + 8 * s, (phases >> s) & 1u, &s_abort, 46))) {
+      w.drain(s, min(n - i, a.stages), phases);
+      ok = false;
+      break;
+    }
+    phases ^= 1u << s;
+    const uint32_t sk = w.ring + s * 2 * kTileBytes, mask = (uint32_t)w.masks[s];
+    const int live = c.len - c.t * C::KT;
+    if (live >= C::KT && mask == (1u << (C::KT >> a.r_shift)) - 1u)
+      tile_step<D, true>(a, sk, qa, st, live, mask, lane);
+    else
+      tile_step<D, false>(a, sk, qa, st, live, mask, lane);
+    __syncwarp();
+    if (i + a.stages < n) {
+      w.issue(ci, box, s);
+      ci.t += step;
+      box = i + a.stages + 1 < n ? w.find_box(ci) : Box{-1, 0};
+    }
+    if (++s == a.stages) s = 0;
+  }
+  finish_rows<D>(a, st);
+
+  if (c.T <= 1) {
+    if (me == 0 && ok) store_rows<D>(a, st, c.b, c.h, lane);
+    if (cs > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    return;
+  }
+  const int mine = min(max(c.T - rank * kWarps, 0), kWarps);   // this CTA's warps with tiles
+  if (warp < mine && ok) store_part<D>(a, st, s_part + warp * pf, lane);
+  __syncthreads();
+  const float* parts = s_part;
+  if (cs == 1) {
+    for (int r = warp; r < a.rows; r += kWarps)
+      join_row<D>(a, c.b, c.h, r, mine, [=](int i) { return parts + i * pf; }, nullptr, lane);
+    return;
+  }
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // every CTA of the cluster has started
+  if (mine > 0) {
+    float* to;
+    asm("mapa.u64 %0, %1, %2;" : "=l"(to) : "l"(s_cta + rank * pf), "r"(0));
+    for (int r = warp; r < a.rows; r += kWarps)
+      join_row<D>(a, c.b, c.h, r, mine, [=](int i) { return parts + i * pf; }, to, lane);
+  }
+  sm100::cluster_sync_all();
+  if (rank == 0) {
+    const float* ctas = s_cta;
+    const int k = min(cs, (c.T + kWarps - 1) / kWarps);                 // CTAs with tiles
+    for (int r = warp; r < a.rows; r += kWarps)
+      join_row<D>(a, c.b, c.h, r, k, [=](int i) { return ctas + i * pf; }, nullptr, lane);
+  }
+}
+
+// Pairs that run over the end of a CTA of decode_list_kernel: one CTA per such end, a warp's share of the parts each.
+// It starts while that kernel runs (whose CTAs have by then waited for all earlier work) and finds its pair from the
+// lengths; only the parts have to wait.
+template <int D>
+__global__ void __launch_bounds__(kWarps * 32) decode_join_list_kernel(MmaArgs a) {
+  constexpr int E = D / 32;
+  extern __shared__ int s_start[];
+  __shared__ float s_o[kWarps][D];
+  __shared__ float s_m[kWarps], s_l[kWarps];
+  __shared__ int s_scan[kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  int row_len = 0, row_start = 0;
+  const int total = list_starts<Mma<D>::KT>(a, s_start, s_scan, kWarps * 32, false, row_len, row_start);
+  const int workers = gridDim.x * kWarps;
+  const int64_t per = (int64_t)kWarps * (((uint32_t)total + workers - 1) / (uint32_t)workers);   // tiles of a CTA
+  const int64_t end = (blockIdx.x + 1) * per;   // the first tile of the next CTA
+  int first = 0, n = 0, b = 0, h = 0;
+  if (end < total) {
+    b = list_row(a, s_start, (int)end, row_start);
+    const int T = (s_start[b + 1] - s_start[b]) / a.HQ;
+    h = ((int)end - s_start[b]) / T;
+    const int64_t from = s_start[b] + (int64_t)h * T;
+    if (from < end && from >= end - per) {      // it begins in this CTA and runs over its end
+      first = blockIdx.x;
+      n = (int)((from + T - 1) / per) - first + 1;
+    }
+  }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const Meta mt = reinterpret_cast<const Meta*>(a.work + (int64_t)ctas * kWarps * 2 * a.rows * (D + 2))[blockIdx.x];
-  if (mt.first < 0) return;
-  const int n = mt.last - mt.first + 1;
-  for (int r = 0; r < a.rows && (mt.h % a.QG) * 8 + r < a.G; ++r) {
+  const int pf = part_floats<D>(a.rows);
+  const int rows = n > 0 ? min(a.rows, a.G - (h % a.QG) * 8) : 0;
+  for (int r = 0; r < rows; ++r) {
     float m = -INFINITY, l = 0.f, o[E] = {};
-    for (int i = warp; i < n; i += NW) {
-      const float* p = a.work + (((int64_t)(mt.first + i) * 2 + (i == 0 ? 1 : 0)) * a.rows + r) * (D + 2);
-      const float pm = p[D], mx = fmaxf(m, pm);
-      const float w0 = join_weight(m, mx), w1 = join_weight(pm, mx);
-      l = l * w0 + p[D + 1] * w1;
+#pragma unroll 4
+    for (int i = warp; i < n; i += kWarps) {
+      const float* p = a.work + ((int64_t)(first + i) * 2 + (i == 0 ? 1 : 0)) * pf + r * (D + 2);
+      const float2 ml = *reinterpret_cast<const float2*>(p + D);
+      const float mx = fmaxf(m, ml.x);
+      const float w0 = join_weight(m, mx), w1 = join_weight(ml.x, mx);
+      l = l * w0 + ml.y * w1;
 #pragma unroll
       for (int e = 0; e < E; ++e) o[e] = o[e] * w0 + p[lane + 32 * e] * w1;
       m = mx;
@@ -790,15 +988,15 @@ __global__ void __launch_bounds__(256) decode_join_mma_kernel(MmaArgs a, int cta
     if (threadIdx.x < D) {
       float mx = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < NW; ++i) mx = fmaxf(mx, s_m[i]);
+      for (int i = 0; i < kWarps; ++i) mx = fmaxf(mx, s_m[i]);
       float lx = 0.f, ox = 0.f;
 #pragma unroll
-      for (int i = 0; i < NW; ++i) {
+      for (int i = 0; i < kWarps; ++i) {
         const float wgt = join_weight(s_m[i], mx);
         lx = fmaf(s_l[i], wgt, lx);
         ox = fmaf(s_o[i][threadIdx.x], wgt, ox);
       }
-      a.o[((int64_t)mt.b * a.H + (mt.h / a.QG) * a.G + (mt.h % a.QG) * 8 + r) * D + threadIdx.x] =
+      a.o[((int64_t)b * a.H + (h / a.QG) * a.G + (h % a.QG) * 8 + r) * D + threadIdx.x] =
           __float2bfloat16_rn(lx == 0.f ? 0.f : ox / lx);
     }
   }
@@ -831,7 +1029,11 @@ static int page_map(CUtensorMap* m, const void* base, int D, int ps, int heads, 
   return ENGPT_OK;
 }
 
-inline int tile_keys(int D) { return 4096 / D; }
+constexpr int kPairTiles = 2;
+constexpr int kPairMin = 100;
+constexpr int kWideClusters = 10;   // clusters of 8 CTAs of this size that surely run at once
+
+inline int tile_keys(int D) { return kTileBytes / (2 * D); }
 
 inline int64_t most_tiles(int D, int table_width, int page_size) {
   return ((int64_t)table_width * page_size + tile_keys(D) - 1) / tile_keys(D);
@@ -843,39 +1045,76 @@ inline bool mma_sizes(int dtype, int B, int H, int Hkv, int D, int table_width, 
          B * (int64_t)H * most_tiles(D, table_width, page_size) < (1ll << 31);
 }
 
-// One CTA per pair while the longest row that the table can hold has at most this many tiles per warp.
-constexpr int kPairTiles = 2;
-
-inline bool mma_list(int D, int table_width, int page_size) {
-  return most_tiles(D, table_width, page_size) > kPairTiles * kWarps;
+// CTAs per pair of the pair form, or 0 for the list form.  The pair form starts and ends faster (at 16 pairs of 16
+// tiles 5.0 against 7.0 us) but is only good in one wave of CTAs (512 pairs of 8 tiles: 23 against 17 us) and does not
+// balance; its clusters are the widest that one wave takes, as long as every warp gets a tile.  With fewer than
+// kPairMin CTAs it leaves memory bandwidth unused, which pays up to kPairTiles tiles per warp (16 pairs of 64 / 128
+// tiles: 8.9 / 13.4 us against 9.1 / 12.7).
+inline int pair_ctas(int B, int H, int Hkv, int D, int table_width, int page_size) {
+  const int64_t pairs = (int64_t)B * Hkv * ((H / Hkv + 7) / 8);
+  const int64_t tiles = most_tiles(D, table_width, page_size);
+  const int sms = num_sms();
+  if (pairs > sms) return 0;
+  int cs = 8;
+  while (cs > 1 && pairs * cs > (cs == 8 ? kWideClusters * 8 : sms)) cs >>= 1;
+  while (cs > 1 && tiles <= kWarps * (cs / 2)) cs >>= 1;
+  return pairs * cs >= kPairMin || tiles <= kPairTiles * kWarps * cs ? cs : 0;
 }
 
 inline int64_t mma_floats(int H, int Hkv, int D) {
   const int rows = H / Hkv < 8 ? H / Hkv : 8;
-  return (int64_t)num_sms() * (kWarps * 2 * (int64_t)rows * (D + 2) + 4);
+  return (int64_t)num_sms() * 2 * rows * (D + 2);
 }
 
-template <int D, bool LIST>
-int launch_mma_kernel(const MmaArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t st) {
-  auto kern = decode_mma_kernel<D, LIST>;
-  const size_t smem = 1024 + (size_t)kWarps * a.stages * (2 * kTileBytes + 12) + 8 + 4 * kWarps +
-                      (LIST ? 4 * ((size_t)a.B + 1) : 0);
+template <int D>
+size_t mma_smem(const MmaArgs& a, int parts) {
+  return 1024 + (size_t)kWarps * a.stages * (2 * kTileBytes + 12) + 4 * (size_t)parts * part_floats<D>(a.rows);
+}
+
+template <int D>
+int launch_pair(const MmaArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int cs, cudaStream_t st) {
+  auto kern = decode_pair_kernel<D>;
+  const size_t smem = mma_smem<D>(a, kWarps + cs);
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((int64_t)a.B * a.HQ * cs));
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cs;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cs > 1 ? 2 : 1;
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kern, a, mk, mv, cs);
+  if (e != cudaSuccess) return set_error(ENGPT_ERR_LAUNCH, "paged_attention: %s", cudaGetErrorString(e));
+  return ENGPT_OK;
+}
+
+template <int D>
+int launch_list(const MmaArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t st) {
+  auto kern = decode_list_kernel<D>;
+  const size_t smem = mma_smem<D>(a, kWarps) + 4 * ((size_t)a.B + 1);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return set_error(ENGPT_ERR_LAUNCH, "paged_attention: %s", cudaGetErrorString(e));
-  const unsigned grid = LIST ? (unsigned)num_sms() : (unsigned)((int64_t)a.B * a.HQ);
-  kern<<<grid, kWarps * 32, smem, st>>>(a, mk, mv);
-  int rc = check_launch("paged_attention");
-  if (rc || !LIST) return rc;
+  // both kernels may be started before what runs ahead of them has ended; they wait for it on the device
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3((unsigned)num_sms());
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, decode_join_mma_kernel<D>, a, (int)grid);
+  e = cudaLaunchKernelEx(&cfg, kern, a, mk, mv);
+  if (e != cudaSuccess) return set_error(ENGPT_ERR_LAUNCH, "paged_attention: %s", cudaGetErrorString(e));
+  cfg.dynamicSmemBytes = 4 * ((size_t)a.B + 1);
+  e = cudaLaunchKernelEx(&cfg, decode_join_list_kernel<D>, a);
   if (e != cudaSuccess) return set_error(ENGPT_ERR_LAUNCH, "paged_attention (join): %s", cudaGetErrorString(e));
   return check_launch("paged_attention (join)");
 }
@@ -896,6 +1135,7 @@ int launch_mma(const AttnArgs& x, int Hkv, cudaStream_t st) {
   a.rows = x.G < 8 ? x.G : 8;
   a.P = x.P;
   a.ps = x.ps;
+  a.ps_shift = (x.ps & (x.ps - 1)) == 0 ? __builtin_ctz((unsigned)x.ps) : -1;
   a.r_shift = 3;
   while (x.ps % (2 << a.r_shift) == 0 && (2 << a.r_shift) <= tile_keys(D)) ++a.r_shift;
   a.R = 1 << a.r_shift;
@@ -903,19 +1143,17 @@ int launch_mma(const AttnArgs& x, int Hkv, cudaStream_t st) {
   a.table_stride = x.table_stride;
   a.W = x.W;
   a.lengths = x.lengths;
-  a.scale_log2 = x.scale_log2;
+  a.scale_log2 = fabsf(x.scale_log2);
+  a.q_flip = x.scale_log2 < 0.f ? 0x80008000u : 0u;
   a.o = reinterpret_cast<__nv_bfloat16*>(x.o);
   a.work = x.work;
   CUtensorMap mk, mv;
   if ((rc = page_map(&mk, x.k_pages, D, x.ps, Hkv, x.P, x.ks, a.R))) return rc;
   if ((rc = page_map(&mv, x.v_pages, D, x.ps, Hkv, x.P, x.vs, a.R))) return rc;
-  if (mma_list(D, x.W, x.ps)) {
-    a.stages = kStages;
-    return launch_mma_kernel<D, true>(a, mk, mv, st);
-  }
-  const int64_t per = (most_tiles(D, x.W, x.ps) + kWarps - 1) / kWarps;
-  a.stages = per < 1 ? 1 : (per < kStages ? (int)per : kStages);
-  return launch_mma_kernel<D, false>(a, mk, mv, st);
+  const int cs = pair_ctas(x.B, x.H, Hkv, D, x.W, x.ps);
+  a.stages = kStages;
+  if (cs == 0) return launch_list<D>(a, mk, mv, st);
+  return launch_pair<D>(a, mk, mv, cs, st);
 }
 
 }  // namespace paged
@@ -931,7 +1169,7 @@ extern "C" int64_t engpt_paged_attention_floats(int dtype, int B, int H, int Hkv
   const int64_t simt = splits > 1 ? (int64_t)B * H * splits * (Dh + 2) : 0;
   if (!mma_sizes(dtype, B, H, Hkv, Dh, table_width, page_size)) return simt;
   // strides and alignment decide at the call which of the two kernels runs
-  const int64_t mma = mma_list(Dh, table_width, page_size) ? mma_floats(H, Hkv, Dh) : 0;
+  const int64_t mma = pair_ctas(B, H, Hkv, Dh, table_width, page_size) == 0 ? mma_floats(H, Hkv, Dh) : 0;
   return simt > mma ? simt : mma;
 }
 

@@ -70,19 +70,42 @@ __device__ __forceinline__ void load_vec(const T* p, float* x) {
 
 constexpr int kThreads = 128;
 constexpr int kGroups = kThreads / 8;
+constexpr int kSimtCluster = 8;
 
 // m2 - m for the joining weights; a part without keys has m = -inf and weighs nothing.
 __device__ __forceinline__ float join_weight(float m_part, float m) {
   return m_part == -INFINITY ? 0.f : sm100::ex2_approx(m_part - m);
 }
 
-// CUDA-core kernel: any head_dim up to 256, fp32 or bf16, any strides.  Eight lanes share a key (each owns NC
-// pieces of VEC elements, VEC = 16 bytes where the addresses allow it); a lane group keeps its own m, l and o
-// over every kGroups-th key of the CTA's range, and the groups join through shared memory at the end.
-template <typename T, int VEC, int NC>
+// The splits' parts ([splits][Dh + 2]: o, m, l) of row and head bh, joined by one CTA into the output.
+template <typename T>
+__device__ __forceinline__ void join_parts(const AttnArgs& a, const float* part, int64_t bh) {
+  const int step = a.Dh + 2;
+  float mx = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) mx = fmaxf(mx, part[s * step + a.Dh]);
+  float lx = 0.f;
+  for (int s = 0; s < a.splits; ++s) lx = fmaf(part[s * step + a.Dh + 1], join_weight(part[s * step + a.Dh], mx), lx);
+  for (int e = threadIdx.x; e < a.Dh; e += kThreads) {
+    float ox = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < a.splits; ++s) ox = fmaf(part[s * step + e], join_weight(part[s * step + a.Dh], mx), ox);
+    store1(reinterpret_cast<T*>(a.o) + bh * a.Dh + e, lx == 0.f ? 0.f : ox / lx);
+  }
+}
+
+// CUDA-core kernel: any head_dim up to 256, fp32 or bf16, any strides.  Eight lanes share a key (each owns NC pieces
+// of VEC elements, VEC = 16 bytes where the addresses allow it); a lane group keeps its own m, l and o over every
+// kGroups-th key of the CTA's range, U keys in flight at a time, and the groups join through shared memory.  The
+// `splits` CTAs of a (row, head) are a cluster while there are at most 8 and join in the shared memory of the first;
+// otherwise they leave parts in the workspace for decode_join_kernel.
+template <typename T, int VEC, int NC, int U>
 __global__ void __launch_bounds__(kThreads) decode_simt_kernel(AttnArgs a) {
   const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int sub = threadIdx.x & 7, grp = threadIdx.x >> 3;
+  const bool cluster = a.splits > 1 && a.splits <= kSimtCluster;
+  if (cluster) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // nothing of an earlier kernel has been touched before
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int len = row_length(a, b);
   // this CTA's keys [j0, j1)
   const int64_t chunk = ((int64_t)len + a.splits - 1) / a.splits;
@@ -107,43 +130,49 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(AttnArgs a) {
       for (int i = 0; i < VEC; ++i) qf[c * VEC + i] *= a.scale_log2;
     }
   }
-  for (int jb = j0; jb < j1; jb += kGroups) {   // CTA-uniform trip count: the shuffles need whole warps
-    const int j = jb + grp;
-    bool live = j < j1;
-    int page = 0, off = 0;
-    if (live) {
+  for (int jb = j0; jb < j1; jb += U * kGroups) {   // CTA-uniform trip count: the shuffles need whole warps
+    int page[U], off[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = jb + u * kGroups + grp;
       const int pj = j / a.ps;
-      off = j - pj * a.ps;
-      page = row[pj];
-      if (page < 0 || page >= a.P) {
+      off[u] = j - pj * a.ps;
+      page[u] = j < j1 ? row[pj] : -1;
+      if (j >= j1) off[u] = -1;                     // no key, as opposed to a bad page
+    }
+    float kf[U][NC * VEC], vf[U][NC * VEC];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool live = page[u] >= 0 && page[u] < a.P;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int e = (c * 8 + sub) * VEC;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) kf[u][c * VEC + i] = vf[u][c * VEC + i] = 0.f;
+        if (live && e < a.Dh) {
+          load_vec<T, VEC>(kp + page[u] * a.ks[0] + off[u] * a.ks[2] + e, kf[u] + c * VEC);
+          load_vec<T, VEC>(vp + page[u] * a.vs[0] + off[u] * a.vs[2] + e, vf[u] + c * VEC);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < NC * VEC; ++i) s = fmaf(qf[i], kf[u][i], s);
+#pragma unroll
+      for (int w = 4; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+      if (page[u] >= 0 && page[u] < a.P) {
+        const float mn = fmaxf(m, s);
+        const float ms = mn == -INFINITY ? 0.f : mn;
+        const float corr = sm100::ex2_approx(m - ms), p = sm100::ex2_approx(s - ms);
+        m = mn;
+        l = fmaf(l, corr, p);
+#pragma unroll
+        for (int i = 0; i < NC * VEC; ++i) o[i] = fmaf(o[i], corr, p * vf[u][i]);
+      } else if (off[u] >= 0) {
         record_device_error(ENGPT_ERR_ARG, 44);
-        live = false;
       }
-    }
-    float kf[NC * VEC], vf[NC * VEC];
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int e = (c * 8 + sub) * VEC;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) kf[c * VEC + i] = vf[c * VEC + i] = 0.f;
-      if (live && e < a.Dh) {
-        load_vec<T, VEC>(kp + page * a.ks[0] + off * a.ks[2] + e, kf + c * VEC);
-        load_vec<T, VEC>(vp + page * a.vs[0] + off * a.vs[2] + e, vf + c * VEC);
-      }
-    }
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < NC * VEC; ++i) s = fmaf(qf[i], kf[i], s);
-#pragma unroll
-    for (int w = 4; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-    if (live) {
-      const float mn = fmaxf(m, s);
-      const float ms = mn == -INFINITY ? 0.f : mn;
-      const float corr = sm100::ex2_approx(m - ms), p = sm100::ex2_approx(s - ms);
-      m = mn;
-      l = fmaf(l, corr, p);
-#pragma unroll
-      for (int i = 0; i < NC * VEC; ++i) o[i] = fmaf(o[i], corr, p * vf[i]);
     }
   }
   // join the CTA's lane groups
@@ -151,6 +180,7 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(AttnArgs a) {
   float* s_o = sm;                       // [kGroups][Dh]
   float* s_m = sm + kGroups * a.Dh;      // [kGroups]
   float* s_l = s_m + kGroups;
+  float* s_cta = s_l + kGroups;          // cluster: [splits][Dh + 2] (first CTA)
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int e = (c * 8 + sub) * VEC;
@@ -164,17 +194,26 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(AttnArgs a) {
     s_l[grp] = l;
   }
   __syncthreads();
-  float mx = -INFINITY;
+  float wgt[kGroups], mx = -INFINITY, lx = 0.f;
+#pragma unroll
   for (int g = 0; g < kGroups; ++g) mx = fmaxf(mx, s_m[g]);
-  float lx = 0.f;
-  for (int g = 0; g < kGroups; ++g) lx += s_l[g] * join_weight(s_m[g], mx);
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    wgt[g] = join_weight(s_m[g], mx);
+    lx = fmaf(s_l[g], wgt[g], lx);
+  }
   const int64_t bh = (int64_t)b * a.H + h;
   float* part = a.work + (bh * a.splits + split) * (a.Dh + 2);
+  if (cluster) {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // every CTA of the cluster has started
+    asm("mapa.u64 %0, %1, %2;" : "=l"(part) : "l"(s_cta + split * (a.Dh + 2)), "r"(0));
+  }
   for (int e = threadIdx.x; e < a.Dh; e += kThreads) {
     float ox = 0.f;
-    for (int g = 0; g < kGroups; ++g) ox = fmaf(s_o[g * a.Dh + e], join_weight(s_m[g], mx), ox);
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) ox = fmaf(s_o[g * a.Dh + e], wgt[g], ox);
     if (a.splits == 1)
-      store1(reinterpret_cast<T*>(a.o) + bh * a.Dh + e, len == 0 || lx == 0.f ? 0.f : ox / lx);
+      store1(reinterpret_cast<T*>(a.o) + bh * a.Dh + e, lx == 0.f ? 0.f : ox / lx);
     else
       part[e] = ox;
   }
@@ -182,23 +221,17 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(AttnArgs a) {
     part[a.Dh] = mx;
     part[a.Dh + 1] = lx;
   }
+  if (cluster) {
+    sm100::cluster_sync_all();
+    if (split == 0) join_parts<T>(a, s_cta, bh);
+  }
 }
 
 // Joins the parts of one (row, head) per CTA.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) decode_join_kernel(AttnArgs a) {
-  const int64_t bh = blockIdx.x;
-  const float* part = a.work + bh * a.splits * (a.Dh + 2);
-  const int step = a.Dh + 2;
-  float mx = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) mx = fmaxf(mx, part[s * step + a.Dh]);
-  float lx = 0.f;
-  for (int s = 0; s < a.splits; ++s) lx += part[s * step + a.Dh + 1] * join_weight(part[s * step + a.Dh], mx);
-  for (int e = threadIdx.x; e < a.Dh; e += kThreads) {
-    float ox = 0.f;
-    for (int s = 0; s < a.splits; ++s) ox = fmaf(part[s * step + e], join_weight(part[s * step + a.Dh], mx), ox);
-    store1(reinterpret_cast<T*>(a.o) + bh * a.Dh + e, lx == 0.f ? 0.f : ox / lx);
-  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  join_parts<T>(a, a.work + (int64_t)blockIdx.x * a.splits * (a.Dh + 2), blockIdx.x);
 }
 
 // Key splits of a launch: about four CTAs per SM, at least 128 keys each at the longest length the table holds.
@@ -207,35 +240,55 @@ inline int simt_splits(int B, int H, int64_t most) {
   int64_t s = rows > 0 ? (4 * 148 + rows - 1) / rows : 1;
   const int64_t by_len = (most + 127) / 128;
   if (s > by_len) s = by_len;
+  if (s > kSimtCluster && s < 2 * kSimtCluster) s = kSimtCluster;   // (one launch instead of two)
   if (s > 256) s = 256;
   return s < 1 ? 1 : (int)s;
 }
 
-template <typename T, int VEC, int NC>
+template <typename T, int VEC, int NC, int U>
 int launch_simt(const AttnArgs& a, cudaStream_t st) {
-  const size_t smem = sizeof(float) * (size_t)(kGroups * (a.Dh + 2));
-  decode_simt_kernel<T, VEC, NC><<<dim3(a.splits, a.H, a.B), kThreads, smem, st>>>(a);
-  int rc = check_launch("paged_attention");
-  if (rc || a.splits == 1) return rc;
-  decode_join_kernel<T><<<(unsigned)((int64_t)a.B * a.H), kThreads, 0, st>>>(a);
-  return check_launch("paged_attention (join)");
+  const bool cluster = a.splits > 1 && a.splits <= kSimtCluster;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.splits, a.H, a.B);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = sizeof(float) * (size_t)((kGroups + (cluster ? a.splits : 0)) * (a.Dh + 2));
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = a.splits;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster ? 2 : 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, decode_simt_kernel<T, VEC, NC, U>, a);
+  if (e == cudaSuccess && a.splits > kSimtCluster) {
+    cfg.gridDim = dim3((unsigned)((int64_t)a.B * a.H));
+    cfg.dynamicSmemBytes = 0;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, decode_join_kernel<T>, a);
+  }
+  if (e != cudaSuccess) return set_error(ENGPT_ERR_LAUNCH, "paged_attention: %s", cudaGetErrorString(e));
+  return check_launch("paged_attention");
 }
 
 template <typename T>
 int dispatch_simt(const AttnArgs& a, bool vec, cudaStream_t st) {
   constexpr int V = 16 / (int)sizeof(T);
   const int nc = vec ? (a.Dh + 8 * V - 1) / (8 * V) : (a.Dh + 7) / 8;
-  if (vec) {
-    if (nc <= 1) return launch_simt<T, V, 1>(a, st);
-    if (nc <= 2) return launch_simt<T, V, 2>(a, st);
-    if (nc <= 4) return launch_simt<T, V, 4>(a, st);
-    if (sizeof(T) == 4) return launch_simt<T, V, 8>(a, st);
+  if (vec) {   // U: 16 elements of keys and of values in flight per lane, at least one key
+    if (nc <= 1) return launch_simt<T, V, 1, 16 / V>(a, st);
+    if (nc <= 2) return launch_simt<T, V, 2, sizeof(T) == 4 ? 2 : 1>(a, st);
+    if (nc <= 4) return launch_simt<T, V, 4, 1>(a, st);
+    if (sizeof(T) == 4) return launch_simt<T, V, 8, 1>(a, st);
   }
-  if (nc <= 8) return launch_simt<T, 1, 8>(a, st);
-  return launch_simt<T, 1, 32>(a, st);
+  if (nc <= 8) return launch_simt<T, 1, 8, 2>(a, st);
+  return launch_simt<T, 1, 32, 1>(a, st);
 }
 
-// ------------------------------------------------------------------ tensor-core kernel (bf16, head_dim 64 or 128)
+// ------------------------------------------------------------------ tensor-core kernel (bf16, head_dim up to 128)
+//
+// Built for a width D of 64 or 128; a smaller head_dim is padded with zeros by TMA, in shared memory only.
 //
 // A tile is KT keys of one kv head, TILE bytes of keys and as many of values.  The tiles of all (row, kv head) pairs
 // form one list, cut into equal contiguous ranges, one per warp ("worker") of a persistent grid, so the load is even
@@ -269,6 +322,7 @@ struct Mma {
 struct MmaArgs {
   const __nv_bfloat16* q;
   int64_t q_row, q_head;
+  int dim;                 // head_dim, at most D and a multiple of 8; TMA fills the columns behind it with zeros
   int B, H, G, HQ, QG;     // HQ: (kv head, group of up to 8 query heads) per row; QG: such groups per kv head
   int rows;                // query heads per group, min(G, 8)
   int P, ps, ps_shift;     // ps_shift: log2(page size), or -1
@@ -418,8 +472,8 @@ __device__ __forceinline__ void load_query(const MmaArgs& a, int b, int h, int l
   const __nv_bfloat16* q = a.q + b * a.q_row + head * a.q_head + 2 * t;
 #pragma unroll
   for (int k = 0; k < Mma<D>::DK; ++k) {
-    qa[k][0] = live ? *reinterpret_cast<const uint32_t*>(q + k * 16) ^ a.q_flip : 0u;
-    qa[k][1] = live ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 8) ^ a.q_flip : 0u;
+    qa[k][0] = live && k * 16 < a.dim ? *reinterpret_cast<const uint32_t*>(q + k * 16) ^ a.q_flip : 0u;
+    qa[k][1] = live && k * 16 + 8 < a.dim ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 8) ^ a.q_flip : 0u;
   }
 }
 
@@ -539,11 +593,11 @@ __device__ __forceinline__ void store_rows(const MmaArgs& a, const State<D>& st,
   const int g = lane >> 2, t = lane & 3;
   const int in = (h % a.QG) * 8 + g;
   if (g >= a.rows || in >= a.G) return;
-  __nv_bfloat16* o = a.o + ((int64_t)b * a.H + (h / a.QG) * a.G + in) * D + 2 * t;
+  __nv_bfloat16* o = a.o + ((int64_t)b * a.H + (h / a.QG) * a.G + in) * a.dim + 2 * t;
   const float inv = st.l == 0.f ? 0.f : 1.f / st.l;
 #pragma unroll
   for (int i = 0; i < Mma<D>::DN; ++i)
-    *reinterpret_cast<uint32_t*>(o + i * 8) = sm100::pack_bf16x2(st.o[i][0] * inv, st.o[i][1] * inv);
+    if (i * 8 < a.dim) *reinterpret_cast<uint32_t*>(o + i * 8) = sm100::pack_bf16x2(st.o[i][0] * inv, st.o[i][1] * inv);
 }
 
 // Joins row r of n <= 8 parts (part(i): its rows) by one warp: into the output, or as one part at `to`.  Lane i holds
@@ -588,9 +642,10 @@ __device__ __forceinline__ void join_row(const MmaArgs& a, int b, int h, int r, 
     }
   } else {
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    __nv_bfloat16* dst = a.o + ((int64_t)b * a.H + (h / a.QG) * a.G + (h % a.QG) * 8 + r) * D;
+    __nv_bfloat16* dst = a.o + ((int64_t)b * a.H + (h / a.QG) * a.G + (h % a.QG) * 8 + r) * a.dim;
 #pragma unroll
-    for (int e = 0; e < E; ++e) dst[lane + 32 * e] = __float2bfloat16_rn(o[e] * inv);
+    for (int e = 0; e < E; ++e)
+      if (lane + 32 * e < a.dim) dst[lane + 32 * e] = __float2bfloat16_rn(o[e] * inv);
   }
 }
 
@@ -735,7 +790,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(MmaArgs a, con
        i += (int64_t)gridDim.x * kWarps * 32) {
     const int b = (int)(i / a.H);
     if (s_start[b + 1] == s_start[b])
-      for (int e = 0; e < D; e += 8) *reinterpret_cast<uint4*>(a.o + i * D + e) = make_uint4(0u, 0u, 0u, 0u);
+      for (int e = 0; e < a.dim; e += 8) *reinterpret_cast<uint4*>(a.o + i * a.dim + e) = make_uint4(0u, 0u, 0u, 0u);
   }
 
   float* part = s_part + warp * pf;                                         // a pair that began before this range
@@ -985,7 +1040,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_join_list_kernel(MmaArgs a
       s_l[warp] = l;
     }
     __syncthreads();
-    if (threadIdx.x < D) {
+    if (threadIdx.x < a.dim) {
       float mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < kWarps; ++i) mx = fmaxf(mx, s_m[i]);
@@ -996,7 +1051,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_join_list_kernel(MmaArgs a
         lx = fmaf(s_l[i], wgt, lx);
         ox = fmaf(s_o[i][threadIdx.x], wgt, ox);
       }
-      a.o[((int64_t)b * a.H + (h / a.QG) * a.G + (h % a.QG) * 8 + r) * D + threadIdx.x] =
+      a.o[((int64_t)b * a.H + (h / a.QG) * a.G + (h % a.QG) * 8 + r) * a.dim + threadIdx.x] =
           __float2bfloat16_rn(lx == 0.f ? 0.f : ox / lx);
     }
   }
@@ -1033,7 +1088,9 @@ constexpr int kPairTiles = 2;
 constexpr int kPairMin = 100;
 constexpr int kWideClusters = 10;   // clusters of 8 CTAs of this size that surely run at once
 
-inline int tile_keys(int D) { return kTileBytes / (2 * D); }
+// Width of the tensor-core kernels for a head_dim, and keys of their tiles.
+inline int mma_width(int dim) { return dim <= 64 ? 64 : 128; }
+inline int tile_keys(int dim) { return kTileBytes / (2 * mma_width(dim)); }
 
 inline int64_t most_tiles(int D, int table_width, int page_size) {
   return ((int64_t)table_width * page_size + tile_keys(D) - 1) / tile_keys(D);
@@ -1041,7 +1098,7 @@ inline int64_t most_tiles(int D, int table_width, int page_size) {
 
 // Does a launch of these sizes go to the tensor-core kernel (strides and alignment apart)?
 inline bool mma_sizes(int dtype, int B, int H, int Hkv, int D, int table_width, int page_size) {
-  return dtype == ENGPT_BF16 && (D == 64 || D == 128) && page_size % 8 == 0 && B <= 8192 &&
+  return dtype == ENGPT_BF16 && D <= 128 && D % 8 == 0 && page_size % 8 == 0 && B <= 8192 &&
          B * (int64_t)H * most_tiles(D, table_width, page_size) < (1ll << 31);
 }
 
@@ -1063,7 +1120,7 @@ inline int pair_ctas(int B, int H, int Hkv, int D, int table_width, int page_siz
 
 inline int64_t mma_floats(int H, int Hkv, int D) {
   const int rows = H / Hkv < 8 ? H / Hkv : 8;
-  return (int64_t)num_sms() * 2 * rows * (D + 2);
+  return (int64_t)num_sms() * 2 * rows * (mma_width(D) + 2);
 }
 
 template <int D>
@@ -1126,6 +1183,7 @@ int launch_mma(const AttnArgs& x, int Hkv, cudaStream_t st) {
   MmaArgs a;
   a.q = reinterpret_cast<const __nv_bfloat16*>(x.q);
   a.q_row = x.q_row;
+  a.dim = x.Dh;
   a.q_head = x.q_head;
   a.B = x.B;
   a.H = x.H;
@@ -1148,8 +1206,8 @@ int launch_mma(const AttnArgs& x, int Hkv, cudaStream_t st) {
   a.o = reinterpret_cast<__nv_bfloat16*>(x.o);
   a.work = x.work;
   CUtensorMap mk, mv;
-  if ((rc = page_map(&mk, x.k_pages, D, x.ps, Hkv, x.P, x.ks, a.R))) return rc;
-  if ((rc = page_map(&mv, x.v_pages, D, x.ps, Hkv, x.P, x.vs, a.R))) return rc;
+  if ((rc = page_map(&mk, x.k_pages, x.Dh, x.ps, Hkv, x.P, x.ks, a.R))) return rc;
+  if ((rc = page_map(&mv, x.v_pages, x.Dh, x.ps, Hkv, x.P, x.vs, a.R))) return rc;
   const int cs = pair_ctas(x.B, x.H, Hkv, D, x.W, x.ps);
   a.stages = kStages;
   if (cs == 0) return launch_list<D>(a, mk, mv, st);
@@ -1166,7 +1224,7 @@ extern "C" int64_t engpt_paged_attention_floats(int dtype, int B, int H, int Hkv
                                                 int page_size) {
   if (B <= 0 || H <= 0 || Hkv <= 0 || Dh <= 0 || table_width < 0 || page_size <= 0) return 0;
   const int splits = simt_splits(B, H, (int64_t)table_width * page_size);
-  const int64_t simt = splits > 1 ? (int64_t)B * H * splits * (Dh + 2) : 0;
+  const int64_t simt = splits > kSimtCluster ? (int64_t)B * H * splits * (Dh + 2) : 0;
   if (!mma_sizes(dtype, B, H, Hkv, Dh, table_width, page_size)) return simt;
   // strides and alignment decide at the call which of the two kernels runs
   const int64_t mma = pair_ctas(B, H, Hkv, Dh, table_width, page_size) == 0 ? mma_floats(H, Hkv, Dh) : 0;
@@ -1230,6 +1288,6 @@ extern "C" int engpt_paged_attention(const void* q, const int64_t* q_strides, co
   }
   cudaStream_t st = as_stream(stream);
   if (vec && positive && num_pages > 0 && mma_sizes(dtype, B, H, Hkv, Dh, table_width, page_size))
-    return Dh == 64 ? launch_mma<64>(a, Hkv, st) : launch_mma<128>(a, Hkv, st);
+    return mma_width(Dh) == 64 ? launch_mma<64>(a, Hkv, st) : launch_mma<128>(a, Hkv, st);
   return dtype == ENGPT_BF16 ? dispatch_simt<__nv_bfloat16>(a, vec, st) : dispatch_simt<float>(a, vec, st);
 }

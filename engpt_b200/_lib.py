@@ -99,6 +99,27 @@ def load() -> ctypes.CDLL:
         return lib
 
 
+def raise_status(name: str, rc: int, msg: str) -> None:
+    raise EngptError(name, rc, msg)
+
+
+_native = None
+
+
+def native():
+    """The compiled binding ``engpt_b200._native`` (``csrc/bindings.cpp``); raises if it has not been built."""
+    global _native
+    if _native is None:
+        load()
+        try:
+            from . import _native as mod
+        except ImportError as e:
+            raise RuntimeError(f"engpt_b200 binding not found or not loadable ({e}); build it with "
+                               "`python -m engpt_b200.build`") from e
+        _native = mod
+    return _native
+
+
 def call(name: str, *args) -> None:
     lib = load()
     rc = getattr(lib, name)(*args)

@@ -1,4 +1,4 @@
-"""Build ``libengpt_b200.so`` (all CUDA sources under ``csrc/``) for sm_100a.
+"""Build ``libengpt_b200.so`` (all CUDA sources under ``csrc/``) for sm_100a and the torch binding ``_native.so``.
 
 The library is built in-tree next to this file so that it travels with the
 source tree.  ``python -m engpt_b200.build`` (or ``build()``) recompiles the
@@ -18,6 +18,7 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libengpt_b200.so")
+NATIVE = os.path.join(HERE, "_native.so")     # Python module of csrc/bindings.cpp, linked against LIB
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -79,7 +80,34 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> str:
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
         os.replace(tmp, LIB)
+    build_native(force)
     return LIB
+
+
+def build_native(force: bool = False) -> str:
+    """The torch binding ``engpt_b200._native`` (host code only), for the running interpreter and its torch."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    src = os.path.join(CSRC, "bindings.cpp")
+    newest = max(os.path.getmtime(p) for p in (src, os.path.join(INCLUDE, "engpt_b200.h"), torch.__file__))
+    if not force and os.path.exists(NATIVE) and os.path.getmtime(NATIVE) >= newest:
+        return NATIVE
+    torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cuda_include = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
+    includes = [*cpp_extension.include_paths(), cuda_include, sysconfig.get_paths()["include"]]
+    tmp = NATIVE + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-isystem{p}" for p in includes), src, "-o", tmp,
+           f"-L{HERE}", "-l:libengpt_b200.so", f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+           "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src}:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, NATIVE)
+    return NATIVE
 
 
 if __name__ == "__main__":

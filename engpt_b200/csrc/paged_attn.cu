@@ -94,13 +94,13 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, const float* part,
 }
 
 // CUDA-core kernel: any head_dim up to 256, fp32 or bf16, any strides.  Eight lanes share a key (each owns NC pieces
-// of VEC elements, VEC = 16 bytes where the addresses allow it); a lane group keeps its own m, l and o over every
-// kGroups-th key of the CTA's range, U keys in flight at a time, and the groups join through shared memory.  The
-// `splits` CTAs of a (row, head) are a cluster while there are at most 8 and join in the shared memory of the first;
-// otherwise they leave parts in the workspace for decode_join_kernel.
-template <typename T, int VEC, int NC, int U>
+// of VEC elements, VEC = 16 bytes where the addresses allow it); a lane group keeps its own m, l and o of HG query
+// heads of one kv head over every kGroups-th key of the CTA's range, U keys in flight at a time, and the groups join
+// through shared memory.  The `splits` CTAs of a row and its heads are a cluster while there are at most 8 and join in
+// the shared memory of the first; otherwise they leave parts in the workspace for decode_join_kernel.
+template <typename T, int VEC, int NC, int U, int HG>
 __global__ void __launch_bounds__(kThreads) decode_simt_kernel(AttnArgs a) {
-  const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int split = blockIdx.x, h0 = blockIdx.y * HG, b = blockIdx.z;
   const int sub = threadIdx.x & 7, grp = threadIdx.x >> 3;
   const bool cluster = a.splits > 1 && a.splits <= kSimtCluster;
   if (cluster) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
@@ -111,23 +111,27 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(AttnArgs a) {
   const int64_t chunk = ((int64_t)len + a.splits - 1) / a.splits;
   const int j0 = (int)min((int64_t)len, split * chunk), j1 = (int)min((int64_t)len, j0 + chunk);
 
-  const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_row + h * a.q_head;
-  const int hk = h / a.G;
+  const int hk = h0 / a.G;
   const T* kp = reinterpret_cast<const T*>(a.k_pages) + hk * a.ks[1];
   const T* vp = reinterpret_cast<const T*>(a.v_pages) + hk * a.vs[1];
   const int* row = a.table + b * a.table_stride;
 
-  float qf[NC * VEC], o[NC * VEC];
-  float m = -INFINITY, l = 0.f;
+  float qf[HG][NC * VEC], o[HG][NC * VEC], m[HG], l[HG];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int e = (c * 8 + sub) * VEC;
+  for (int g = 0; g < HG; ++g) {
+    const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_row + (h0 + g) * a.q_head;
+    m[g] = -INFINITY;
+    l[g] = 0.f;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) qf[c * VEC + i] = o[c * VEC + i] = 0.f;
-    if (e < a.Dh) {
-      load_vec<T, VEC>(q + e, qf + c * VEC);
+    for (int c = 0; c < NC; ++c) {
+      const int e = (c * 8 + sub) * VEC;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) qf[c * VEC + i] *= a.scale_log2;
+      for (int i = 0; i < VEC; ++i) qf[g][c * VEC + i] = o[g][c * VEC + i] = 0.f;
+      if (e < a.Dh) {
+        load_vec<T, VEC>(q + e, qf[g] + c * VEC);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) qf[g][c * VEC + i] *= a.scale_log2;
+      }
     }
   }
   for (int jb = j0; jb < j1; jb += U * kGroups) {   // CTA-uniform trip count: the shuffles need whole warps
@@ -157,73 +161,90 @@ __global__ void __launch_bounds__(kThreads) decode_simt_kernel(AttnArgs a) {
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float s = 0.f;
+      float s[HG];
 #pragma unroll
-      for (int i = 0; i < NC * VEC; ++i) s = fmaf(qf[i], kf[u][i], s);
+      for (int g = 0; g < HG; ++g) {
+        s[g] = 0.f;
 #pragma unroll
-      for (int w = 4; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+        for (int i = 0; i < NC * VEC; ++i) s[g] = fmaf(qf[g][i], kf[u][i], s[g]);
+      }
+#pragma unroll
+      for (int w = 4; w > 0; w >>= 1)
+#pragma unroll
+        for (int g = 0; g < HG; ++g) s[g] += __shfl_xor_sync(0xffffffffu, s[g], w);
       if (page[u] >= 0 && page[u] < a.P) {
-        const float mn = fmaxf(m, s);
-        const float ms = mn == -INFINITY ? 0.f : mn;
-        const float corr = sm100::ex2_approx(m - ms), p = sm100::ex2_approx(s - ms);
-        m = mn;
-        l = fmaf(l, corr, p);
 #pragma unroll
-        for (int i = 0; i < NC * VEC; ++i) o[i] = fmaf(o[i], corr, p * vf[u][i]);
+        for (int g = 0; g < HG; ++g) {
+          const float mn = fmaxf(m[g], s[g]);
+          const float ms = mn == -INFINITY ? 0.f : mn;
+          const float corr = sm100::ex2_approx(m[g] - ms), p = sm100::ex2_approx(s[g] - ms);
+          m[g] = mn;
+          l[g] = fmaf(l[g], corr, p);
+#pragma unroll
+          for (int i = 0; i < NC * VEC; ++i) o[g][i] = fmaf(o[g][i], corr, p * vf[u][i]);
+        }
       } else if (off[u] >= 0) {
         record_device_error(ENGPT_ERR_ARG, 44);
       }
     }
   }
-  // join the CTA's lane groups
+  // join the CTA's lane groups, head by head
   extern __shared__ float sm[];
-  float* s_o = sm;                       // [kGroups][Dh]
-  float* s_m = sm + kGroups * a.Dh;      // [kGroups]
-  float* s_l = s_m + kGroups;
-  float* s_cta = s_l + kGroups;          // cluster: [splits][Dh + 2] (first CTA)
+  float* s_o = sm;                           // [kGroups][Dh]
+  float* s_m = sm + kGroups * a.Dh;          // [HG][kGroups]
+  float* s_l = s_m + HG * kGroups;
+  float* s_cta = s_l + HG * kGroups;         // cluster: [HG][splits][Dh + 2] (first CTA)
+  if (sub == 0) {
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int e = (c * 8 + sub) * VEC;
-    if (e < a.Dh) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) s_o[grp * a.Dh + e + i] = o[c * VEC + i];
+    for (int g = 0; g < HG; ++g) {
+      s_m[g * kGroups + grp] = m[g];
+      s_l[g * kGroups + grp] = l[g];
     }
   }
-  if (sub == 0) {
-    s_m[grp] = m;
-    s_l[grp] = l;
-  }
-  __syncthreads();
-  float wgt[kGroups], mx = -INFINITY, lx = 0.f;
+  if (cluster) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // every CTA has started
 #pragma unroll
-  for (int g = 0; g < kGroups; ++g) mx = fmaxf(mx, s_m[g]);
+  for (int g = 0; g < HG; ++g) {
+    if (g > 0) __syncthreads();
 #pragma unroll
-  for (int g = 0; g < kGroups; ++g) {
-    wgt[g] = join_weight(s_m[g], mx);
-    lx = fmaf(s_l[g], wgt[g], lx);
-  }
-  const int64_t bh = (int64_t)b * a.H + h;
-  float* part = a.work + (bh * a.splits + split) * (a.Dh + 2);
-  if (cluster) {
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // every CTA of the cluster has started
-    asm("mapa.u64 %0, %1, %2;" : "=l"(part) : "l"(s_cta + split * (a.Dh + 2)), "r"(0));
-  }
-  for (int e = threadIdx.x; e < a.Dh; e += kThreads) {
-    float ox = 0.f;
+    for (int c = 0; c < NC; ++c) {
+      const int e = (c * 8 + sub) * VEC;
+      if (e < a.Dh) {
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) ox = fmaf(s_o[g * a.Dh + e], wgt[g], ox);
-    if (a.splits == 1)
-      store1(reinterpret_cast<T*>(a.o) + bh * a.Dh + e, lx == 0.f ? 0.f : ox / lx);
-    else
-      part[e] = ox;
-  }
-  if (a.splits > 1 && threadIdx.x == 0) {
-    part[a.Dh] = mx;
-    part[a.Dh + 1] = lx;
+        for (int i = 0; i < VEC; ++i) s_o[grp * a.Dh + e + i] = o[g][c * VEC + i];
+      }
+    }
+    __syncthreads();
+    float wgt[kGroups], mx = -INFINITY, lx = 0.f;
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) mx = fmaxf(mx, s_m[g * kGroups + k]);
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+      wgt[k] = join_weight(s_m[g * kGroups + k], mx);
+      lx = fmaf(s_l[g * kGroups + k], wgt[k], lx);
+    }
+    const int64_t bh = (int64_t)b * a.H + h0 + g;
+    float* part = a.work + (bh * a.splits + split) * (a.Dh + 2);
+    if (cluster)
+      asm("mapa.u64 %0, %1, %2;" : "=l"(part) : "l"(s_cta + (g * a.splits + split) * (a.Dh + 2)), "r"(0));
+    for (int e = threadIdx.x; e < a.Dh; e += kThreads) {
+      float ox = 0.f;
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) ox = fmaf(s_o[k * a.Dh + e], wgt[k], ox);
+      if (a.splits == 1)
+        store1(reinterpret_cast<T*>(a.o) + bh * a.Dh + e, lx == 0.f ? 0.f : ox / lx);
+      else
+        part[e] = ox;
+    }
+    if (a.splits > 1 && threadIdx.x == 0) {
+      part[a.Dh] = mx;
+      part[a.Dh + 1] = lx;
+    }
   }
   if (cluster) {
     sm100::cluster_sync_all();
-    if (split == 0) join_parts<T>(a, s_cta, bh);
+    if (split == 0)
+      for (int g = 0; g < HG; ++g)
+        join_parts<T>(a, s_cta + g * a.splits * (a.Dh + 2), (int64_t)b * a.H + h0 + g);
   }
 }
 
@@ -234,24 +255,26 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(AttnArgs a) {
   join_parts<T>(a, a.work + (int64_t)blockIdx.x * a.splits * (a.Dh + 2), blockIdx.x);
 }
 
-// Key splits of a launch: about four CTAs per SM, at least 128 keys each at the longest length the table holds.
+// Key splits of a launch: about four CTAs per SM, at least 64 keys each at the longest length the table holds.  One
+// cluster rather than a second launch where that leaves a CTA no more than 256 keys.
 inline int simt_splits(int B, int H, int64_t most) {
   const int64_t rows = (int64_t)B * H;
-  int64_t s = rows > 0 ? (4 * 148 + rows - 1) / rows : 1;
-  const int64_t by_len = (most + 127) / 128;
+  int64_t s = rows > 0 ? (4 * (int64_t)num_sms() + rows - 1) / rows : 1;
+  const int64_t by_len = (most + 63) / 64;
   if (s > by_len) s = by_len;
-  if (s > kSimtCluster && s < 2 * kSimtCluster) s = kSimtCluster;   // (one launch instead of two)
+  if (s > kSimtCluster && most <= 256 * kSimtCluster) s = kSimtCluster;
   if (s > 256) s = 256;
   return s < 1 ? 1 : (int)s;
 }
 
-template <typename T, int VEC, int NC, int U>
+template <typename T, int VEC, int NC, int U, int HG>
 int launch_simt(const AttnArgs& a, cudaStream_t st) {
   const bool cluster = a.splits > 1 && a.splits <= kSimtCluster;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.splits, a.H, a.B);
+  cfg.gridDim = dim3(a.splits, a.H / HG, a.B);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(float) * (size_t)((kGroups + (cluster ? a.splits : 0)) * (a.Dh + 2));
+  cfg.dynamicSmemBytes =
+      sizeof(float) * (size_t)(kGroups * (a.Dh + 2 * HG) + (cluster ? HG * a.splits * (a.Dh + 2) : 0));
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -261,7 +284,7 @@ int launch_simt(const AttnArgs& a, cudaStream_t st) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster ? 2 : 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, decode_simt_kernel<T, VEC, NC, U>, a);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, decode_simt_kernel<T, VEC, NC, U, HG>, a);
   if (e == cudaSuccess && a.splits > kSimtCluster) {
     cfg.gridDim = dim3((unsigned)((int64_t)a.B * a.H));
     cfg.dynamicSmemBytes = 0;
@@ -272,18 +295,31 @@ int launch_simt(const AttnArgs& a, cudaStream_t st) {
   return check_launch("paged_attention");
 }
 
+// Query heads that share a kv head and one reading of its keys: 4, 2 or 1 (8 fp32 rows of 1024 tokens, 32 heads on 4
+// of 128: 28 us with four heads per reading, 41 with one).
+template <typename T, int VEC, int NC, int U>
+int launch_simt_heads(const AttnArgs& a, cudaStream_t st) {
+  if (a.G % 4 == 0) return launch_simt<T, VEC, NC, U, 4>(a, st);
+  if (a.G % 2 == 0) return launch_simt<T, VEC, NC, U, 2>(a, st);
+  return launch_simt<T, VEC, NC, U, 1>(a, st);
+}
+
 template <typename T>
 int dispatch_simt(const AttnArgs& a, bool vec, cudaStream_t st) {
   constexpr int V = 16 / (int)sizeof(T);
   const int nc = vec ? (a.Dh + 8 * V - 1) / (8 * V) : (a.Dh + 7) / 8;
-  if (vec) {   // U: 16 elements of keys and of values in flight per lane, at least one key
-    if (nc <= 1) return launch_simt<T, V, 1, 16 / V>(a, st);
-    if (nc <= 2) return launch_simt<T, V, 2, sizeof(T) == 4 ? 2 : 1>(a, st);
-    if (nc <= 4) return launch_simt<T, V, 4, 1>(a, st);
-    if (sizeof(T) == 4) return launch_simt<T, V, 8, 1>(a, st);
+  if (vec && sizeof(T) == 4) {
+    if (nc <= 1) return launch_simt_heads<T, V, 1, 4>(a, st);
+    if (nc <= 2) return launch_simt_heads<T, V, 2, 4>(a, st);
+    if (nc <= 4) return launch_simt_heads<T, V, 4, 2>(a, st);
+    return launch_simt<T, V, 8, 1, 1>(a, st);
   }
-  if (nc <= 8) return launch_simt<T, 1, 8, 2>(a, st);
-  return launch_simt<T, 1, 32, 1>(a, st);
+  if (vec) {   // bf16 comes here with a head_dim above 128, or pages of an odd size
+    if (nc <= 2) return launch_simt<T, V, 2, 2, 1>(a, st);
+    return launch_simt<T, V, 4, 1, 1>(a, st);
+  }
+  if (nc <= 8) return launch_simt<T, 1, 8, 2, 1>(a, st);
+  return launch_simt<T, 1, 32, 1, 1>(a, st);
 }
 
 // ------------------------------------------------------------------ tensor-core kernel (bf16, head_dim up to 128)

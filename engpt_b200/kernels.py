@@ -14,7 +14,6 @@ reference never reuse ``qkv``).
 
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Optional, Tuple
 
@@ -350,44 +349,7 @@ def project_column_grad_(weight: Tensor, grad: Tensor) -> None:
 
 
 # ------------------------------------------------------------ paged key-value cache
-def _index(t: Tensor, name: str, shape: Optional[tuple], dev: torch.device) -> None:
-    """An int32 index tensor of the given shape on the cache's device, contiguous."""
-    if t.dtype != torch.int32 or (shape is not None and tuple(t.shape) != shape) or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor" + (f" of shape {shape}" if shape else "")
-                         + f", got {t.dtype} {tuple(t.shape)}")
-    if t.device != dev:
-        raise RuntimeError("engpt_b200 ops: all tensors must be on the same device")
-
-
-def _pools(k_pages: Tensor, v_pages: Tensor) -> Tuple[int, int, int, int]:
-    """Checks a cache's two page pools; (num_pages, kv heads, page_size, head_dim)."""
-    if not k_pages.is_cuda or not v_pages.is_cuda:
-        raise RuntimeError("engpt_b200 ops run on CUDA tensors only (no CPU fallback)")
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
-        raise ValueError("k_pages and v_pages must share a shape [num_pages, kv_heads, page_size, head_dim] and dtype")
-    if k_pages.device != v_pages.device:
-        raise RuntimeError("engpt_b200 ops: all tensors must be on the same device")
-    if (k_pages.shape[3] > 1 and (k_pages.stride(3) != 1 or v_pages.stride(3) != 1)):
-        raise ValueError("k_pages and v_pages need a contiguous head_dim axis")
-    return tuple(k_pages.shape)
-
-
-def _page_strides(k_pages: Tensor, v_pages: Tensor) -> "ctypes.Array":
-    return (ctypes.c_int64 * 6)(*k_pages.stride()[:3], *v_pages.stride()[:3])
-
-
-def _table(block_table: Tensor, rows: int, dev: torch.device) -> None:
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != rows or (
-            block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError("block_table must be int32 [batch, pages per request] with contiguous rows")
-    if block_table.device != dev:
-        raise RuntimeError("engpt_b200 ops: all tensors must be on the same device")
-
-
-def _table_stride(block_table: Tensor) -> int:
-    return block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1]
-
-
+# Argument checks and launches are in the compiled binding (csrc/bindings.cpp).
 @torch.no_grad()
 def advance_block_tables(lengths: Tensor, new_tokens: Tensor, block_table: Tensor, free_pages: Tensor,
                          free_count: Tensor, *, page_size: int, max_new: int, finished: Optional[Tensor] = None
@@ -396,43 +358,19 @@ def advance_block_tables(lengths: Tensor, new_tokens: Tensor, block_table: Tenso
 
     ``lengths`` ``[B]`` (tokens of each request in the cache), ``block_table``
     ``[B, W]``, the stack ``free_pages`` ``[num_pages]`` and its size
-    ``free_count`` ``[1]`` are updated in place.  Rows with ``finished`` set
-    first give all their pages back and become empty; then every row takes
-    the pages that ``new_tokens[b]`` more tokens need, rows in order.
-    ``slots`` and ``positions`` are int32 ``[B, max_new]``: a token's place in
-    the cache (``page * page_size + offset``) and in its sequence; ``-1`` and
-    0 behind a row's last new token.
+    ``free_count`` ``[1]``, all int32, are updated in place.  Rows with
+    ``finished`` (bool ``[B]``) set first give all their pages back and become
+    empty; then every row takes the pages that ``new_tokens[b]`` more tokens
+    need, rows in order.  ``slots`` and ``positions`` are int32 ``[B,
+    max_new]``: a token's place in the cache (``page * page_size + offset``)
+    and in its sequence; ``-1`` and 0 behind a row's last new token.
 
     A row whose request cannot be met (more than ``max_new`` tokens, a table
     row too short, no pages left) is refused whole: its length stays, its
     slots are ``-1``, and ``engpt_b200._lib.raise_on_device_status`` reports it.
     """
-    if not lengths.is_cuda:
-        raise RuntimeError("engpt_b200 ops run on CUDA tensors only (no CPU fallback)")
-    dev, bsz = lengths.device, lengths.shape[0]
-    _index(lengths, "lengths", (bsz,), dev)
-    _index(new_tokens, "new_tokens", (bsz,), dev)
-    _table(block_table, bsz, dev)
-    if free_pages.dim() != 1:
-        raise ValueError("free_pages must have shape [num_pages]")
-    _index(free_pages, "free_pages", None, dev)
-    _index(free_count, "free_count", (1,), dev)
-    if finished is not None:
-        if finished.dtype not in (torch.bool, torch.uint8) or tuple(finished.shape) != (bsz,) or \
-                not finished.is_contiguous():
-            raise ValueError("finished must be a contiguous bool or uint8 tensor [batch]")
-        if finished.device != dev:
-            raise RuntimeError("engpt_b200 ops: all tensors must be on the same device")
-    if page_size < 1 or max_new < 0:
-        raise ValueError("page_size must be positive and max_new not negative")
-    out = torch.empty(2, bsz, max_new, device=dev, dtype=torch.int32)
-    slots, positions = out[0], out[1]
-    with torch.cuda.device(dev):
-        _lib.call("engpt_advance_block_tables", lengths.data_ptr(), new_tokens.data_ptr(), _lib.ptr(finished), bsz,
-                  block_table.data_ptr(), _table_stride(block_table), block_table.shape[1], free_pages.data_ptr(),
-                  free_pages.shape[0], free_count.data_ptr(), page_size, max_new, slots.data_ptr(),
-                  positions.data_ptr(), _lib.stream_handle(dev))
-    return slots, positions
+    return _lib.native().advance_block_tables(lengths, new_tokens, block_table, free_pages, free_count, page_size,
+                                              max_new, finished)
 
 
 def qkv_append_from_carried(qkv: Tensor, rho: Tensor, cos: Tensor, sin: Tensor, qk_scale: Tensor, norm_eps: float,
@@ -443,66 +381,21 @@ def qkv_append_from_carried(qkv: Tensor, rho: Tensor, cos: Tensor, sin: Tensor, 
     ``qkv`` ``[..., 3, H, Dh]`` holds raw projection rows of carried ``Y`` with
     radii ``rho`` ``[...]``; ``positions`` ``[...]`` selects each token's rotary
     row and ``slots`` ``[...]`` its place in ``k_pages`` / ``v_pages``
-    ``[num_pages, H, page_size, Dh]`` (``-1``: k and v are not kept).  Slots
-    other than ``-1`` must be distinct.  Returns q ``[..., H, Dh]``.
+    ``[num_pages, H, page_size, Dh]`` (``-1``: k and v are not kept), both
+    int32.  Slots other than ``-1`` must be distinct.  Returns q ``[..., H,
+    Dh]``; the scale applied to q and k is ``qk_scale * qk_mult``.
     """
-    num_pages, kv_heads, page_size, dim = _pools(k_pages, v_pages)
-    dev = k_pages.device
-    _require_cuda(k_pages, qkv, rho, cos, sin, qk_scale)
-    _forward_only(qkv, rho, cos, sin, qk_scale)
-    if qkv.dim() < 3 or tuple(qkv.shape[-3:]) != (3, kv_heads, dim) or qkv.dtype != k_pages.dtype:
-        raise ValueError("qkv must have shape [..., 3, H, Dh] and the cache's heads, head_dim and dtype")
-    lead = tuple(qkv.shape[:-3])
-    if tuple(rho.shape) != lead:
-        raise ValueError("rho must have qkv's leading shape")
-    if tuple(qk_scale.shape) != (kv_heads, dim):
-        raise ValueError("qk_scale must have shape [n_head, head_dim]")
-    half = dim // 2
-    if cos.dim() != 2 or cos.shape[1] != half or sin.shape != cos.shape:
-        raise ValueError("cos/sin must have shape [T, head_dim // 2]")
-    _index(positions, "positions", lead, dev)
-    _index(slots, "slots", lead, dev)
-    qkv = qkv.contiguous()
-    q = torch.empty(*lead, kv_heads, dim, device=dev, dtype=qkv.dtype)
-    rho, cos, sin, qk_scale = _f32c(rho), _f32c(cos), _f32c(sin), _f32c(qk_scale)
-    with torch.cuda.device(dev):
-        _lib.call("engpt_qkv_append", qkv.data_ptr(), _lib.dtype_code(qkv.dtype), rho.data_ptr(), cos.data_ptr(),
-                  sin.data_ptr(), cos.shape[0], half, qk_scale.data_ptr(), float(qk_mult), float(norm_eps),
-                  rho.numel(), kv_heads, dim, positions.data_ptr(), slots.data_ptr(), q.data_ptr(),
-                  k_pages.data_ptr(), v_pages.data_ptr(), _page_strides(k_pages, v_pages), num_pages, page_size,
-                  _lib.stream_handle(dev))
-    return q
+    return _lib.native().qkv_append(qkv, rho, cos, sin, qk_scale, norm_eps, positions, slots, k_pages, v_pages,
+                                    qk_mult)
 
 
-def _kv_rows(t: Tensor, name: str) -> Tensor:
-    """``[..., H, Dh]`` as ``[n, H, Dh]`` rows with a contiguous last axis (a view where the strides allow it)."""
-    t = t.reshape(-1, t.shape[-2], t.shape[-1])
-    return t if t.stride(2) == 1 or t.shape[2] <= 1 else t.contiguous()
-
-
-@torch.no_grad()
 def write_kv_pages(k: Tensor, v: Tensor, slots: Tensor, k_pages: Tensor, v_pages: Tensor) -> None:
     """Copy finished k and v ``[..., H, Dh]`` into their cache slots (``slots`` ``[...]`` int32, ``-1``: none).
 
     k and v may be views into the packed ``[B, T, 3, H, Dh]`` projection.
     Slots other than ``-1`` must be distinct.
     """
-    num_pages, kv_heads, page_size, dim = _pools(k_pages, v_pages)
-    dev = k_pages.device
-    _require_cuda(k_pages, k, v)
-    if k.dim() < 2 or k.shape != v.shape or tuple(k.shape[-2:]) != (kv_heads, dim):
-        raise ValueError("k and v must share a shape [..., H, Dh] with the cache's heads and head_dim")
-    if k.dtype != k_pages.dtype or v.dtype != k_pages.dtype:
-        raise ValueError("k and v must have the cache's dtype")
-    _index(slots, "slots", tuple(k.shape[:-2]), dev)
-    if slots.numel() == 0:
-        return
-    k, v = _kv_rows(k, "k"), _kv_rows(v, "v")
-    strides = (ctypes.c_int64 * 4)(k.stride(0), k.stride(1), v.stride(0), v.stride(1))
-    with torch.cuda.device(dev):
-        _lib.call("engpt_write_kv_pages", k.data_ptr(), v.data_ptr(), strides, _lib.dtype_code(k.dtype), k.shape[0],
-                  kv_heads, dim, slots.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                  _page_strides(k_pages, v_pages), num_pages, page_size, _lib.stream_handle(dev))
+    _lib.native().write_kv_pages(k, v, slots, k_pages, v_pages)
 
 
 def paged_sdpa(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: Tensor, lengths: Tensor, *,
@@ -510,31 +403,10 @@ def paged_sdpa(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: Tensor,
     """Attention of one new token per request over its cached keys and values; returns ``[B, H, Dh]``.
 
     ``softmax(scale * q k^T) v`` over the first ``lengths[b]`` tokens of the
-    pages in ``block_table[b]``; query head ``h`` reads kv head
-    ``h // (H // kv_heads)``.  A row of length 0 gives zeros.  Whatever lies in
-    the cache behind a row's length (stale or NaN) has no effect.
+    pages in ``block_table[b]`` (int32, as ``advance_block_tables`` keeps them);
+    query head ``h`` reads kv head ``h // (H // kv_heads)``.  A row of length 0
+    gives zeros.  Whatever lies in the cache behind a row's length (stale or
+    NaN) has no effect.  ``k_pages`` and ``v_pages`` are ``[num_pages, kv_heads,
+    page_size, Dh]`` with any strides and a contiguous last axis.
     """
-    num_pages, kv_heads, page_size, dim = _pools(k_pages, v_pages)
-    dev = k_pages.device
-    _require_cuda(k_pages, q)
-    _forward_only(q, k_pages, v_pages)
-    if q.dim() != 3 or q.shape[2] != dim or q.dtype != k_pages.dtype:
-        raise ValueError("q must have shape [batch, n_head, head_dim] and the cache's head_dim and dtype")
-    bsz, heads = q.shape[0], q.shape[1]
-    if heads == 0 or kv_heads == 0 or heads % kv_heads:
-        raise ValueError("the number of query heads must be a multiple of the cache's heads")
-    _index(lengths, "lengths", (bsz,), dev)
-    _table(block_table, bsz, dev)
-    if q.stride(2) != 1 and dim > 1:
-        q = q.contiguous()
-    o = torch.empty(bsz, heads, dim, device=dev, dtype=q.dtype)
-    code, width = _lib.dtype_code(q.dtype), block_table.shape[1]
-    strides = (ctypes.c_int64 * 2)(q.stride(0), q.stride(1))
-    with torch.cuda.device(dev):
-        floats = _lib.load().engpt_paged_attention_floats(code, bsz, heads, kv_heads, dim, width, page_size)
-        work = torch.empty(floats, device=dev, dtype=torch.float32) if floats else None
-        _lib.call("engpt_paged_attention", q.data_ptr(), strides, k_pages.data_ptr(), v_pages.data_ptr(),
-                  _page_strides(k_pages, v_pages), code, bsz, heads, kv_heads, dim, num_pages, page_size,
-                  block_table.data_ptr(), _table_stride(block_table), width, lengths.data_ptr(), float(scale),
-                  o.data_ptr(), _lib.ptr(work), _lib.stream_handle(dev))
-    return o
+    return _lib.native().paged_sdpa(q, k_pages, v_pages, block_table, lengths, scale)

@@ -8,6 +8,8 @@ Drop-in names for the reference package:
 * ``engpt_b200.kernels`` -- the engpt.kernels hot-path ops on CUDA kernels
 * ``torch.ops.engpt_b200.*`` -- the three hot-path ops as registered
   PyTorch operators (``engpt_b200.torch_ops``)
+* ``PagedDecoder`` / ``PagedKVCache`` -- generation with a paged key-value
+  cache (``engpt_b200.decode``; the reference has none)
 * ``patch_reference(engpt_pkg)`` -- rebinds the hot-path ops inside an
   imported reference package so its own model calls the CUDA kernels
 """
@@ -18,6 +20,8 @@ from .config import ModelConfig
 from .models import EfficientNGPT, EfficientNGPTBlock
 from . import kernels
 from . import torch_ops  # registers torch.ops.engpt_b200.{qkv_postprocess_from_carried, causal_sdpa, carried_residual_gauge}
+from .decode import PagedDecoder, PagedKVCache
 from .integration import patch_reference
 
-__all__ = ["EfficientNGPT", "EfficientNGPTBlock", "ModelConfig", "kernels", "patch_reference", "__version__"]
+__all__ = ["EfficientNGPT", "EfficientNGPTBlock", "ModelConfig", "PagedDecoder", "PagedKVCache", "kernels",
+           "patch_reference", "__version__"]

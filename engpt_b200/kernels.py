@@ -350,7 +350,6 @@ def project_column_grad_(weight: Tensor, grad: Tensor) -> None:
 
 # ------------------------------------------------------------ paged key-value cache
 # Argument checks and launches are in the compiled binding (csrc/bindings.cpp).
-@torch.no_grad()
 def advance_block_tables(lengths: Tensor, new_tokens: Tensor, block_table: Tensor, free_pages: Tensor,
                          free_count: Tensor, *, page_size: int, max_new: int, finished: Optional[Tensor] = None
                          ) -> Tuple[Tensor, Tensor]:

@@ -410,8 +410,11 @@ class EfficientNGPT(nn.Module):
     @torch.no_grad()
     def _run(self, idx: Optional[Tensor] = None, y: Optional[Tensor] = None, rho: Optional[Tensor] = None,
              targets: Optional[Tensor] = None,
-             layer_callback: Optional[Callable[[int, Tensor, Tensor], None]] = None
-             ) -> Tuple[Tensor, Optional[Tensor]]:
+             layer_callback: Optional[Callable[[int, Tensor, Tensor], None]] = None,
+             kv_callback: Optional[Callable[[int, Tensor, Tensor], None]] = None,
+             head_rows: Optional[Tensor] = None) -> Tuple[Tensor, Optional[Tensor]]:
+        # kv_callback(layer, k, v): a layer's post-processed keys and values [B, T, H, Dh] (views of the workspace);
+        # head_rows: the output head for these rows of the [B*T] token list only, logits [len(head_rows), V]
         cfg = self.cfg
         dev = self.token_emb.weight.device
         if dev.type != "cuda":
@@ -502,6 +505,8 @@ class EfficientNGPT(nn.Module):
                               ws.cos.data_ptr(), ws.sin.data_ptr(), Dh // 2, s_qk.data_ptr(),
                               float(blk.qk_mult), float(cfg.norm_eps), bsz, seq_len, Hl, Dh, None, None, None,
                               _lib.QKV_INPLACE, st)
+                if kv_callback is not None:
+                    kv_callback(i, ws.k, ws.v)
                 if self.attn_timer is not None:
                     self.attn_timer("start")
                 if self.attn_impl == _lib.ATTN_AUTO:
@@ -571,6 +576,8 @@ class EfficientNGPT(nn.Module):
             # logits are computed into a [N, V_pad] buffer and returned as the [B, T, V] view of its
             # first V columns (row stride V_pad); values are those of the [N, V] product
             vp = ws.vocab_pad
+            if head_rows is not None:
+                return torch.mm(ws.x.index_select(0, head_rows), ws.w_head.t())[:, :cfg.vocab_size], None
             logits_buf = torch.empty(n, vp, device=dev, dtype=ws.act)
             loss = None
             if targets is not None and targets.ndim != 2:
@@ -593,6 +600,11 @@ class EfficientNGPT(nn.Module):
             if self.contiguous_logits:
                 logits = logits.contiguous()
         return logits, loss
+
+    def decoder(self, max_batch: int, num_pages: int, **kwargs) -> "PagedDecoder":
+        """A decoder over a paged key-value cache for generating from this model (``engpt_b200.decode``)."""
+        from .decode import PagedDecoder
+        return PagedDecoder(self, max_batch, num_pages, **kwargs)
 
     def last_hidden(self) -> Tensor:
         """Represented state ``Y / rho`` after the last block of the latest forward, ``[B, T, d]``.

@@ -122,3 +122,17 @@ def test_c_entry_points_check_before_any_launch():
     assert at(p, two, p, p, six, 1, 2, 4, 2, 64, 4, 16, p, 4, 5, p, 1.0, p, p, None) == 1
     assert at(p, two, p, p, six, 1, 0, 4, 2, 64, 4, 16, p, 5, 5, p, 1.0, p, p, None) == 0
     assert b"paged_attention" in lib.engpt_last_error() or lib.engpt_last_error() == b""
+
+
+def test_cache_and_decoder_refuse_the_cpu():
+    from engpt_b200 import EfficientNGPT, ModelConfig, PagedKVCache
+    from tests.helpers import SMALL
+    cfg = ModelConfig(**SMALL)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        PagedKVCache(cfg, 2, 4, device="cpu")
+    with pytest.raises(ValueError):
+        PagedKVCache(cfg, 2, 0)
+    with pytest.raises(NotImplementedError):
+        PagedKVCache(cfg, 2, 4, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        EfficientNGPT(cfg).decoder(2, 4)

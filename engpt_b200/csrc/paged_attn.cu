@@ -343,6 +343,7 @@ int dispatch_simt(const AttnArgs& a, bool vec, cudaStream_t st) {
 // of a pair are joined by the warp that holds its first one; a pair that runs over CTAs leaves one part per CTA in
 // the workspace, joined by decode_join_list_kernel.
 constexpr int kWarps = 8;
+constexpr int kPairWarps = 4;           // of the form with a cluster per pair
 constexpr int kStages = 1;
 constexpr int kTileBytes = 8192;        // one of K, V
 
@@ -636,9 +637,9 @@ __device__ __forceinline__ void store_rows(const MmaArgs& a, const State<D>& st,
     if (i * 8 < a.dim) *reinterpret_cast<uint32_t*>(o + i * 8) = sm100::pack_bf16x2(st.o[i][0] * inv, st.o[i][1] * inv);
 }
 
-// Joins row r of n <= 8 parts (part(i): its rows) by one warp: into the output, or as one part at `to`.  Lane i holds
+// Joins row r of n <= N parts (part(i): its rows) by one warp: into the output, or as one part at `to`.  Lane i holds
 // part i's weight, and all loads are independent.
-template <int D, typename F>
+template <int D, int N, typename F>
 __device__ __forceinline__ void join_row(const MmaArgs& a, int b, int h, int r, int n, F part, float* to, int lane) {
   constexpr int E = D / 32;
   if ((h % a.QG) * 8 + r >= a.G) return;
@@ -650,20 +651,20 @@ __device__ __forceinline__ void join_row(const MmaArgs& a, int b, int h, int r, 
   }
   float mx = m;
 #pragma unroll
-  for (int k = 4; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+  for (int k = N / 2; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
   mx = __shfl_sync(0xffffffffu, mx, 0);
   const float w = join_weight(m, mx);
   l *= w;
 #pragma unroll
-  for (int k = 4; k > 0; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
+  for (int k = N / 2; k > 0; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
   l = __shfl_sync(0xffffffffu, l, 0);
-  float x[8][E], o[E] = {};
+  float x[N][E], o[E] = {};
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
+  for (int k = 0; k < N; ++k)
 #pragma unroll
     for (int e = 0; e < E; ++e) x[k][e] = k < n ? part(k)[r * (D + 2) + lane + 32 * e] : 0.f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
+  for (int k = 0; k < N; ++k) {
     const float wk = __shfl_sync(0xffffffffu, w, k);
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = fmaf(x[k][e], wk, o[e]);
@@ -899,7 +900,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(MmaArgs a, con
     float* to = g < 0 ? out : (s_over[g] ? out + pf : nullptr);   // at most one pair runs over the CTA's end
     const int b = pair / a.HQ, h = pair - b * a.HQ;
     for (int r = r0; r < a.rows; r += step)
-      join_row<D>(a, b, h, r, n, [=](int i) { return i == 0 ? first : (g < 0 ? first : rest) + i * pf; }, to, lane);
+      join_row<D, kWarps>(a, b, h, r, n, [=](int i) { return i == 0 ? first : (g < 0 ? first : rest) + i * pf; }, to, lane);
   };
   if (a.rows < kWarps) {
     join_group(warp, 0, 1);
@@ -909,28 +910,28 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(MmaArgs a, con
   }
 }
 
-// One cluster of `cs` CTAs per pair: tile t goes to warp t mod (cs * kWarps) of the cluster, whose parts are joined
+// One cluster of `cs` CTAs per pair: tile t goes to warp t mod (cs * kPairWarps) of the cluster, whose parts are joined
 // through shared memory, then through the shared memory of the cluster's first CTA.  No prefix sums, no second
 // launch, and the first page look-up does not wait for the length: the form for short rows and for few pairs.
 template <int D>
-__global__ void __launch_bounds__(kWarps * 32) decode_pair_kernel(MmaArgs a, const __grid_constant__ CUtensorMap mk,
+__global__ void __launch_bounds__(kPairWarps * 32) decode_pair_kernel(MmaArgs a, const __grid_constant__ CUtensorMap mk,
                                                                   const __grid_constant__ CUtensorMap mv, int cs) {
   using C = Mma<D>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (sm100::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* ring_ptr = smem_raw + (base - sm100::smem_u32(smem_raw));
   const int ring_bytes = a.stages * 2 * kTileBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring_ptr + kWarps * ring_bytes);   // [kWarps][stages]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring_ptr + kPairWarps * ring_bytes);   // [kPairWarps][stages]
   const int pf = part_floats<D>(a.rows);
-  float* s_part = reinterpret_cast<float*>(bars + kWarps * a.stages);             // [kWarps] the warps' parts
-  float* s_cta = s_part + kWarps * pf;                                            // [cs] the CTAs' parts (rank 0)
-  int* masks = reinterpret_cast<int*>(s_cta + cs * pf);                           // [kWarps][stages]
+  float* s_part = reinterpret_cast<float*>(bars + kPairWarps * a.stages);             // [kPairWarps] the warps' parts
+  float* s_cta = s_part + kPairWarps * pf;                                            // [cs] the CTAs' parts (rank 0)
+  int* masks = reinterpret_cast<int*>(s_cta + cs * pf);                           // [kPairWarps][stages]
   __shared__ int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (cs > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
   const int pair = blockIdx.x / cs, rank = blockIdx.x - pair * cs;
-  const int me = rank * kWarps + warp, step = cs * kWarps;
+  const int me = rank * kPairWarps + warp, step = cs * kPairWarps;
   Worker<D> w{a, &mk, &mv, base + warp * ring_bytes, sm100::smem_u32(bars + warp * a.stages), masks + warp * a.stages,
               lane};
   Cursor c;
@@ -999,28 +1000,28 @@ __global__ void __launch_bounds__(kWarps * 32) decode_pair_kernel(MmaArgs a, con
     if (cs > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     return;
   }
-  const int mine = min(max(c.T - rank * kWarps, 0), kWarps);   // this CTA's warps with tiles
+  const int mine = min(max(c.T - rank * kPairWarps, 0), kPairWarps);   // this CTA's warps with tiles
   if (warp < mine && ok) store_part<D>(a, st, s_part + warp * pf, lane);
   __syncthreads();
   const float* parts = s_part;
   if (cs == 1) {
-    for (int r = warp; r < a.rows; r += kWarps)
-      join_row<D>(a, c.b, c.h, r, mine, [=](int i) { return parts + i * pf; }, nullptr, lane);
+    for (int r = warp; r < a.rows; r += kPairWarps)
+      join_row<D, kPairWarps>(a, c.b, c.h, r, mine, [=](int i) { return parts + i * pf; }, nullptr, lane);
     return;
   }
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // every CTA of the cluster has started
   if (mine > 0) {
     float* to;
     asm("mapa.u64 %0, %1, %2;" : "=l"(to) : "l"(s_cta + rank * pf), "r"(0));
-    for (int r = warp; r < a.rows; r += kWarps)
-      join_row<D>(a, c.b, c.h, r, mine, [=](int i) { return parts + i * pf; }, to, lane);
+    for (int r = warp; r < a.rows; r += kPairWarps)
+      join_row<D, kPairWarps>(a, c.b, c.h, r, mine, [=](int i) { return parts + i * pf; }, to, lane);
   }
   sm100::cluster_sync_all();
   if (rank == 0) {
     const float* ctas = s_cta;
-    const int k = min(cs, (c.T + kWarps - 1) / kWarps);                 // CTAs with tiles
-    for (int r = warp; r < a.rows; r += kWarps)
-      join_row<D>(a, c.b, c.h, r, k, [=](int i) { return ctas + i * pf; }, nullptr, lane);
+    const int k = min(cs, (c.T + kPairWarps - 1) / kPairWarps);                 // CTAs with tiles
+    for (int r = warp; r < a.rows; r += kPairWarps)
+      join_row<D, 8>(a, c.b, c.h, r, k, [=](int i) { return ctas + i * pf; }, nullptr, lane);
   }
 }
 
@@ -1120,10 +1121,6 @@ static int page_map(CUtensorMap* m, const void* base, int D, int ps, int heads, 
   return ENGPT_OK;
 }
 
-constexpr int kPairTiles = 2;
-constexpr int kPairMin = 100;
-constexpr int kWideClusters = 10;   // clusters of 8 CTAs of this size that surely run at once
-
 // Width of the tensor-core kernels for a head_dim, and keys of their tiles.
 inline int mma_width(int dim) { return dim <= 64 ? 64 : 128; }
 inline int tile_keys(int dim) { return kTileBytes / (2 * mma_width(dim)); }
@@ -1138,20 +1135,25 @@ inline bool mma_sizes(int dtype, int B, int H, int Hkv, int D, int table_width, 
          B * (int64_t)H * most_tiles(D, table_width, page_size) < (1ll << 31);
 }
 
-// CTAs per pair of the pair form, or 0 for the list form.  The pair form starts and ends faster (at 16 pairs of 16
-// tiles 5.0 against 7.0 us) but is only good in one wave of CTAs (512 pairs of 8 tiles: 23 against 17 us) and does not
-// balance; its clusters are the widest that one wave takes, as long as every warp gets a tile.  With fewer than
-// kPairMin CTAs it leaves memory bandwidth unused, which pays up to kPairTiles tiles per warp (16 pairs of 64 / 128
-// tiles: 8.9 / 13.4 us against 9.1 / 12.7).
+// CTAs per pair of the pair form, or 0 for the list form.
+//
+// The pair form starts and ends faster (an empty launch takes some 3 us, the list form's two 5.5) but does not balance
+// rows of different length, so it has to be one wave of CTAs.  Its clusters are the widest that run at once: 8 CTAs up
+// to one per SM in all (16 pairs of 32 tiles: 4.9 us with 8, 5.8 with 4, 8.3 with 2), 4 or 2 up to two per SM (64 pairs
+// of 32 tiles: 10.6 us with 4, 12.1 with 2, 15.3 with 8 in three waves; list 13.1); narrower where a warp would be
+// without a tile.  Its warps take their tiles one after the other, 2 us each, where the list form spreads them over all
+// SMs at 16 KB / 6.2 TB/s = 1/380 us each: with t tiles per warp the pair form is taken while 2 (t - 1) <= 2 + pairs *
+// tiles / 380 (16 pairs of 128 tiles: 12.3 against 13.0 us, 8 pairs of 128: 10.7 against 9.6, 16 pairs of 256: 19.2
+// against 18.5).
 inline int pair_ctas(int B, int H, int Hkv, int D, int table_width, int page_size) {
   const int64_t pairs = (int64_t)B * Hkv * ((H / Hkv + 7) / 8);
   const int64_t tiles = most_tiles(D, table_width, page_size);
   const int sms = num_sms();
-  if (pairs > sms) return 0;
-  int cs = 8;
-  while (cs > 1 && pairs * cs > (cs == 8 ? kWideClusters * 8 : sms)) cs >>= 1;
-  while (cs > 1 && tiles <= kWarps * (cs / 2)) cs >>= 1;
-  return pairs * cs >= kPairMin || tiles <= kPairTiles * kWarps * cs ? cs : 0;
+  if (pairs > 2 * sms) return 0;
+  int cs = pairs * 8 <= sms ? 8 : pairs * 4 <= 2 * sms ? 4 : pairs * 2 <= 2 * sms ? 2 : 1;
+  while (cs > 1 && tiles <= kPairWarps * (cs / 2)) cs >>= 1;
+  const int64_t per_warp = (tiles + kPairWarps * cs - 1) / (kPairWarps * cs);
+  return 2 * (per_warp - 1) <= 2 + pairs * tiles / 380 ? cs : 0;
 }
 
 inline int64_t mma_floats(int H, int Hkv, int D) {
@@ -1160,18 +1162,18 @@ inline int64_t mma_floats(int H, int Hkv, int D) {
 }
 
 template <int D>
-size_t mma_smem(const MmaArgs& a, int parts) {
-  return 1024 + (size_t)kWarps * a.stages * (2 * kTileBytes + 12) + 4 * (size_t)parts * part_floats<D>(a.rows);
+size_t mma_smem(const MmaArgs& a, int warps, int parts) {
+  return 1024 + (size_t)warps * a.stages * (2 * kTileBytes + 12) + 4 * (size_t)parts * part_floats<D>(a.rows);
 }
 
 template <int D>
 int launch_pair(const MmaArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int cs, cudaStream_t st) {
   auto kern = decode_pair_kernel<D>;
-  const size_t smem = mma_smem<D>(a, kWarps + cs);
+  const size_t smem = mma_smem<D>(a, kPairWarps, kPairWarps + cs);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((int64_t)a.B * a.HQ * cs));
-  cfg.blockDim = dim3(kWarps * 32);
+  cfg.blockDim = dim3(kPairWarps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -1190,7 +1192,7 @@ int launch_pair(const MmaArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, 
 template <int D>
 int launch_list(const MmaArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t st) {
   auto kern = decode_list_kernel<D>;
-  const size_t smem = mma_smem<D>(a, kWarps) + 4 * ((size_t)a.B + 1);
+  const size_t smem = mma_smem<D>(a, kWarps, kWarps) + 4 * ((size_t)a.B + 1);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return set_error(ENGPT_ERR_LAUNCH, "paged_attention: %s", cudaGetErrorString(e));
   // both kernels may be started before what runs ahead of them has ended; they wait for it on the device

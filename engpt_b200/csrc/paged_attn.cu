@@ -1144,7 +1144,8 @@ inline bool mma_sizes(int dtype, int B, int H, int Hkv, int D, int table_width, 
 // without a tile.  Its warps take their tiles one after the other, 2 us each, where the list form spreads them over all
 // SMs at 16 KB / 6.2 TB/s = 1/380 us each: with t tiles per warp the pair form is taken while 2 (t - 1) <= 2 + pairs *
 // tiles / 380 (16 pairs of 128 tiles: 12.3 against 13.0 us, 8 pairs of 128: 10.7 against 9.6, 16 pairs of 256: 19.2
-// against 18.5).
+// against 18.5), and, as the rows of a batch may differ and the longest one decides, with at most 4 tiles per warp if
+// there are several rows (8 rows of 16 pairs of 32 tiles: 15.4 us against the list's 17.0 if all are that long).
 inline int pair_ctas(int B, int H, int Hkv, int D, int table_width, int page_size) {
   const int64_t pairs = (int64_t)B * Hkv * ((H / Hkv + 7) / 8);
   const int64_t tiles = most_tiles(D, table_width, page_size);
@@ -1153,6 +1154,7 @@ inline int pair_ctas(int B, int H, int Hkv, int D, int table_width, int page_siz
   int cs = pairs * 8 <= sms ? 8 : pairs * 4 <= 2 * sms ? 4 : pairs * 2 <= 2 * sms ? 2 : 1;
   while (cs > 1 && tiles <= kPairWarps * (cs / 2)) cs >>= 1;
   const int64_t per_warp = (tiles + kPairWarps * cs - 1) / (kPairWarps * cs);
+  if (B > 1 && per_warp > 4) return 0;
   return 2 * (per_warp - 1) <= 2 + pairs * tiles / 380 ? cs : 0;
 }
 

@@ -407,7 +407,8 @@ struct Cursor {
   int b, h, t, T, len, hk;
 };
 
-// A box of the tile to come: its page (-1: past the length, -2: outside the pool) and first row in the page.
+// A box of the tile to come: its page as the table has it (looked at only when the copy is issued, so that nothing
+// waits for the look-up before) and first row in the page, -1 for a box past the length.
 struct Box {
   int page, off;
 };
@@ -444,15 +445,15 @@ struct Worker {
 
   __device__ __forceinline__ Box find_box(const Cursor& c) const {
     const int key = c.t * C::KT + lane * a.R;
-    if (lane * a.R >= C::KT || key >= c.len) return Box{-1, 0};
+    if (lane * a.R >= C::KT || key >= c.len) return Box{0, -1};
     const int j = a.ps_shift >= 0 ? key >> a.ps_shift : key / a.ps;
-    const int page = a.table[c.b * a.table_stride + j];
-    return Box{page >= 0 && page < a.P ? page : -2, key - j * a.ps};
+    return Box{a.table[c.b * a.table_stride + j], key - j * a.ps};
   }
 
   // Start the copies of the cursor's tile into stage s.
   __device__ __forceinline__ void issue(const Cursor& c, const Box& x, int s) const {
-    const uint32_t mask = __ballot_sync(0xffffffffu, x.page >= 0);
+    const bool here = x.off >= 0 && (unsigned)x.page < (unsigned)a.P;
+    const uint32_t mask = __ballot_sync(0xffffffffu, here);
     const uint32_t bar = bars + 8 * s;
     const uint32_t box = a.R * 128;
     if (lane == 0) {
@@ -460,14 +461,14 @@ struct Worker {
       sm100::mbar_expect_tx(bar, __popc(mask) * box * (D / 64) * 2);
     }
     __syncwarp();
-    if (x.page >= 0) {
+    if (here) {
       const uint32_t dst = ring + s * 2 * kTileBytes + lane * box;
 #pragma unroll
       for (int half = 0; half < D / 64; ++half) {
         sm100::tma_load_4d(dst + half * C::KT * 128, mk, half * 64, x.off, c.hk, x.page, bar);
         sm100::tma_load_4d(dst + half * C::KT * 128 + kTileBytes, mv, half * 64, x.off, c.hk, x.page, bar);
       }
-    } else if (x.page == -2) {
+    } else if (x.off >= 0) {   // a page outside the pool
       record_device_error(ENGPT_ERR_ARG, 44);
     }
     __syncwarp();
@@ -809,11 +810,11 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(MmaArgs a, con
   // fill the ring
   const int n_issued = min(f1 - f0, a.stages);
   Cursor ci = c;
-  Box box = n_issued > 0 ? w.find_box(ci) : Box{-1, 0};
+  Box box = n_issued > 0 ? w.find_box(ci) : Box{0, -1};
   for (int s = 0; s < n_issued; ++s) {
     Cursor cn = ci;
     w.advance(cn);
-    const Box next = f0 + s + 1 < f1 ? w.find_box(cn) : Box{-1, 0};
+    const Box next = f0 + s + 1 < f1 ? w.find_box(cn) : Box{0, -1};
     w.issue(ci, box, s);
     ci = cn;
     box = next;
@@ -860,7 +861,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(MmaArgs a, con
     if (f + a.stages < f1) {
       w.issue(ci, box, s);
       w.advance(ci);
-      box = f + a.stages + 1 < f1 ? w.find_box(ci) : Box{-1, 0};
+      box = f + a.stages + 1 < f1 ? w.find_box(ci) : Box{0, -1};
     }
     if (++s == a.stages) s = 0;
     const bool pair_end = c.t + 1 == c.T;
@@ -958,13 +959,13 @@ __global__ void __launch_bounds__(kPairWarps * 32) decode_pair_kernel(MmaArgs a,
   __syncwarp();
   c.len = clip_length(a, len);
   c.T = (c.len + C::KT - 1) / C::KT;
-  if (c.t * C::KT + lane * a.R >= c.len) box.page = -1;
+  if (c.t * C::KT + lane * a.R >= c.len) box.off = -1;
   const int n = c.T > me ? (c.T - me + step - 1) / step : 0;   // this warp's tiles
   Cursor ci = c;
   for (int i = 0; i < min(n, a.stages); ++i) {
     w.issue(ci, box, i);
     ci.t += step;
-    box = i + 1 < n ? w.find_box(ci) : Box{-1, 0};
+    box = i + 1 < n ? w.find_box(ci) : Box{0, -1};
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   State<D> st;
@@ -989,7 +990,7 @@ __global__ void __launch_bounds__(kPairWarps * 32) decode_pair_kernel(MmaArgs a,
     if (i + a.stages < n) {
       w.issue(ci, box, s);
       ci.t += step;
-      box = i + a.stages + 1 < n ? w.find_box(ci) : Box{-1, 0};
+      box = i + a.stages + 1 < n ? w.find_box(ci) : Box{0, -1};
     }
     if (++s == a.stages) s = 0;
   }

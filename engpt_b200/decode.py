@@ -224,7 +224,8 @@ class PagedDecoder:
             raise ValueError(f"active must be a bool tensor of shape [{b}]")
         new = self._ones if active is None else active.to(device=self.device, dtype=torch.int32, non_blocking=True)
         idx = idx.to(device=self.device, dtype=torch.int64, non_blocking=True)
-        with torch.cuda.device(self.device):
+        # (the compute type is the decoder's, whatever autocast region the caller is in)
+        with torch.cuda.device(self.device), torch.autocast("cuda", enabled=False):
             if self.cuda_graphs:
                 if self._graph is None:
                     self._graph = _StepGraph(self)

@@ -103,6 +103,20 @@ def test_graphed_steps_equal_eager_steps(cuda, dtype):
     assert torch.equal(runs[0][0][on], runs[1][0][on])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("outer", [torch.bfloat16, torch.float16])
+def test_an_outer_autocast_region_changes_nothing(cuda, dtype, outer):
+    cfg = CFGS["dh64"]
+    model = model_on(cuda, "dh64")
+    idx = tokens(cfg, (2, 12), 3)
+    logits = []
+    for enabled in (False, True):
+        dec = model.decoder(2, 4, page_size=16, dtype=dtype)
+        with torch.autocast("cuda", dtype=outer, enabled=enabled):
+            logits.append([dec.prefill(idx[:, :10]), dec.step(idx[:, 10]), dec.step(idx[:, 11])])
+    assert all(torch.equal(a, b) for a, b in zip(*logits))
+
+
 def test_requests_come_and_go(cuda):
     """Rows are released and refilled while others decode; every request sees only its own tokens."""
     cfg = CFGS["dh64"]

@@ -304,6 +304,56 @@ def test_attention_lengths(cuda, dtype, dim, page):
     check_attention(attention_inputs(LENGTHS, 4, 4, dim, page, dtype, seed=dim + page))
 
 
+@pytest.mark.parametrize("dim,page", [(8, 8), (24, 16), (40, 64), (96, 8), (104, 40), (120, 128), (136, 16), (7, 16)])
+def test_attention_other_head_dims_bf16(cuda, dim, page):
+    """Head dims that are padded in shared memory, and the ones next to them that are not."""
+    check_attention(attention_inputs([0, 1, 100, 257, 33], 4, 2, dim, page, torch.bfloat16, seed=dim))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128, 80])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-30, 3.0])
+def test_attention_scales(cuda, dtype, dim, scale):
+    args = attention_inputs([0, 5, 64, 333], 3, 3, dim, 16, dtype, seed=dim)
+    check_attention(args[:5] + (scale,))
+
+
+def test_attention_more_rows_than_the_list_takes(cuda):
+    """9000 rows: beyond the tensor-core kernels' prefix sums."""
+    bsz, page, heads, dim = 9000, 16, 2, 64
+    rng = np.random.default_rng(1)
+    lengths = rng.integers(0, 40, bsz).tolist()
+    pool = sum(R.pages_of(n, page) for n in lengths)
+    table, _ = R.random_table(lengths, page, 3, pool, rng)
+    gen = torch.Generator(device="cuda").manual_seed(bsz)
+    kp, vp = (torch.randn(pool, heads, page, dim, generator=gen, device="cuda").bfloat16() for _ in range(2))
+    q = torch.randn(bsz, heads, dim, generator=gen, device="cuda").bfloat16()
+    check_attention((q, kp, vp, table.cuda(), torch.tensor(lengths, dtype=torch.int32, device=cuda), 0.125))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv_heads", [(16, 16), (16, 2)])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("bsz,width_tokens", [(1, 64), (1, 512), (1, 2048), (1, 8192), (3, 512), (3, 2048), (12, 1024),
+                                              (20, 512), (40, 256)])
+def test_attention_every_form_with_short_and_long_rows(cuda, dtype, heads, kv_heads, dim, bsz, width_tokens):
+    """The table's width decides the form (clusters of 1 to 8 CTAs, the list); the rows themselves may be of any length
+    within it, the last one as long as the table allows."""
+    page = 64
+    rng = np.random.default_rng(bsz + width_tokens)
+    lengths = [int(x) for x in rng.integers(0, 130, bsz)]
+    lengths[-1] = width_tokens
+    pool = sum(R.pages_of(n, page) for n in lengths) + 1
+    table, _ = R.random_table(lengths, page, width_tokens // page, pool, rng)
+    gen = torch.Generator(device="cuda").manual_seed(bsz)
+    kp, vp = (torch.randn(pool, kv_heads, page, dim, generator=gen, device="cuda").to(dtype) for _ in range(2))
+    q = torch.randn(bsz, heads, dim, generator=gen, device="cuda").to(dtype)
+    lens = torch.tensor(lengths, dtype=torch.int32, device=cuda)
+    check_attention((q, kp, vp, table.cuda(), lens, 0.125))
+    lens[-1] = 3          # the same form, nothing left of the long row
+    check_attention((q, kp, vp, table.cuda(), lens, 0.125))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("heads,kv_heads", [(1, 1), (6, 2), (8, 1), (16, 2), (12, 1), (40, 2), (5, 5)])
 @pytest.mark.parametrize("dim", [64, 128, 48])

@@ -249,6 +249,10 @@ constexpr int kAppendCtas = 16;   // CTAs per SM of a launch whose CTAs walk ove
 template <typename T, int LPR, int MIN>
 __global__ void __launch_bounds__(128, MIN) append_vec_kernel(QkvArgs a, PagedDst d) {
   constexpr bool kFast = sizeof(T) == 2;
+  // started ahead of the end of what runs before (usually the projection), and so may be what follows (usually the
+  // attention over the pages): each waits on the device for its predecessor's results
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int idx = blockIdx.y * 128 + threadIdx.x;      // (head, slice)
   const bool mine = idx < a.H * LPR;
   const int h = mine ? idx / LPR : 0;
@@ -440,12 +444,19 @@ static void launch_append(const QkvArgs& a, const PagedDst& d, cudaStream_t st) 
   // CTAs per SM for more rows in flight: 8188 tokens of 16 heads of 128 take 36 us so (5.6 TB/s), 39 with 6 resident
   // CTAs, 44 without a limit, 46 with a token per CTA.  fp32 rows are twice as long and would spill at 8.
   const int64_t most = (int64_t)num_sms() * kAppendCtas / y;
-  if (a.T <= most) {
-    append_vec_kernel<T, LPR, 1><<<dim3((unsigned)a.T, (unsigned)y), 128, 0, st>>>(a, d);
-    return;
-  }
-  append_vec_kernel<T, LPR, sizeof(T) == 2 ? 8 : 1>
-      <<<dim3((unsigned)(most > 0 ? most : 1), (unsigned)y), 128, 0, st>>>(a, d);
+  const bool walk = a.T > most;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(walk ? (most > 0 ? most : 1) : a.T), (unsigned)y);
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  // (a launch error is picked up by check_launch)
+  if (walk) cudaLaunchKernelEx(&cfg, append_vec_kernel<T, LPR, sizeof(T) == 2 ? 8 : 1>, a, d);
+  else cudaLaunchKernelEx(&cfg, append_vec_kernel<T, LPR, 1>, a, d);
 }
 
 }  // namespace engpt

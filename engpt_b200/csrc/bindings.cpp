@@ -91,7 +91,9 @@ Pools check_pools(const Tensor& k, const Tensor& v) {
   return p;
 }
 
-Tensor f32c(const Tensor& t) { return t.to(at::kFloat).contiguous(); }
+Tensor f32c(const Tensor& t) {
+  return t.scalar_type() == at::kFloat && t.is_contiguous() ? t : t.to(at::kFloat).contiguous();
+}
 
 void* stream_of(const c10::Device& dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 

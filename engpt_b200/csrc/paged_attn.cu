@@ -53,10 +53,11 @@ __device__ __forceinline__ void store1<__nv_bfloat16>(__nv_bfloat16* p, float v)
 
 template <typename T, int VEC>
 __device__ __forceinline__ void load_vec(const T* p, float* x) {
+  // (coherent loads: the kernel may have been started while an earlier one was still writing the pages)
   if constexpr (VEC == 8) {
-    unpack8(ld_stream(p), x);
+    unpack8(ld_once(p), x);
   } else if constexpr (VEC == 4) {
-    const uint4 r = ld_stream(p);
+    const uint4 r = ld_once(p);
     x[0] = __uint_as_float(r.x);
     x[1] = __uint_as_float(r.y);
     x[2] = __uint_as_float(r.z);
@@ -71,6 +72,7 @@ __device__ __forceinline__ void load_vec(const T* p, float* x) {
 constexpr int kThreads = 128;
 constexpr int kGroups = kThreads / 8;
 constexpr int kSimtCluster = 8;
+constexpr int64_t kMostKeys = 0x7fffffff - 4096;   // of a row: key indices are ints and run a tile or two past it
 
 // m2 - m for the joining weights; a part without keys has m = -inf and weighs nothing.
 __device__ __forceinline__ float join_weight(float m_part, float m) {
@@ -328,7 +330,7 @@ int dispatch_simt(const AttnArgs& a, bool vec, cudaStream_t st) {
 //
 // A tile is KT keys of one kv head, TILE bytes of keys and as many of values.  The tiles of all (row, kv head) pairs
 // form one list, cut into equal contiguous ranges, one per warp ("worker") of a persistent grid, so the load is even
-// whatever the lengths.  A warp fetches its own tiles through its own ring of STAGES tiles in shared memory: TMA
+// whatever the lengths.  A warp fetches its own tiles through its own ring of kStages tiles in shared memory: TMA
 // boxes of R rows (R divides the page size) at the page that the block table names, 128-byte swizzled, one mbarrier
 // per stage; no warp waits for another one until the end.
 //
@@ -342,8 +344,12 @@ int dispatch_simt(const AttnArgs& a, bool vec, cudaStream_t st) {
 // A range that begins or ends inside a pair leaves a part (o, m, l) in shared memory.  After a CTA barrier the parts
 // of a pair are joined by the warp that holds its first one; a pair that runs over CTAs leaves one part per CTA in
 // the workspace, joined by decode_join_list_kernel.
+//
+// Warps, stages and tiles are what 64 rows of up to 4096 tokens (16 heads of 64) run best with: eight warps with one
+// 16 KB stage each 87 us, which leaves a warp idle while its copies fly but has seven others; 10 or 12 such warps 90
+// and 89, six or four with two stages 101 and 105, eight with two stages of 8 KB 97.
 constexpr int kWarps = 8;
-constexpr int kPairWarps = 4;           // of the form with a cluster per pair
+constexpr int kPairWarps = 4;           // of the form with a cluster per pair: several CTAs per SM
 constexpr int kStages = 1;
 constexpr int kTileBytes = 8192;        // one of K, V
 
@@ -1284,7 +1290,7 @@ extern "C" int engpt_paged_attention(const void* q, const int64_t* q_strides, co
   ENGPT_REQUIRE(B <= 65535 && H <= 65535, ENGPT_ERR_SHAPE, "paged_attention: B=%d H=%d (at most 65535)", B, H);
   ENGPT_REQUIRE(num_pages >= 0 && page_size > 0 && (int64_t)num_pages * page_size <= 0x7fffffffLL, ENGPT_ERR_SHAPE,
                 "paged_attention: num_pages=%d page_size=%d", num_pages, page_size);
-  ENGPT_REQUIRE(table_width >= 0 && table_stride >= table_width && (int64_t)table_width * page_size <= 0x7fffffffLL,
+  ENGPT_REQUIRE(table_width >= 0 && table_stride >= table_width && (int64_t)table_width * page_size <= kMostKeys,
                 ENGPT_ERR_SHAPE, "paged_attention: table_width=%d page_size=%d", table_width, page_size);
   ENGPT_REQUIRE(dtype == ENGPT_BF16 || dtype == ENGPT_F32, ENGPT_ERR_DTYPE, "paged_attention: dtype %d", dtype);
   if (B == 0) return ENGPT_OK;

@@ -233,7 +233,7 @@ struct AppendRow {
   Raw8<T> x[3];
   float rho;
   int pos, slot;
-  __device__ __forceinline__ void load(const QkvArgs& a, const PagedDst& d, const T* src, int64_t part, int n) {
+  __device__ __forceinline__ void load(const QkvArgs& a, const PagedDst& d, const T* src, int64_t part, int64_t n) {
     const T* p = src + n * (3 * part);
 #pragma unroll
     for (int s = 0; s < 3; ++s) x[s].load(p + s * part);
@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(128, MIN) append_vec_kernel(QkvArgs a, PagedDs
     for (int i = 0; i < 8; ++i) scl[i] = v[i] * a.qk_mult;
   }
   AppendRow<T> next;
-  int n = blockIdx.x;
+  int64_t n = blockIdx.x;
   next.load(a, d, src, part, n);                       // (a thread without a slice of its own walks head 0)
   for (; n < a.T; n += gridDim.x) {
     const AppendRow<T> row = next;
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(128, MIN) append_vec_kernel(QkvArgs a, PagedDs
       c4 = __ldg(reinterpret_cast<const float4*>(a.cos_tab + (int64_t)row.pos * a.rope_half + p0));
       s4 = __ldg(reinterpret_cast<const float4*>(a.sin_tab + (int64_t)row.pos * a.rope_half + p0));
     }
-    if (n + (int64_t)gridDim.x < a.T) next.load(a, d, src, part, n + gridDim.x);
+    if (n + gridDim.x < a.T) next.load(a, d, src, part, n + gridDim.x);
     float ss[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {

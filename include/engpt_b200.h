@@ -398,8 +398,8 @@ ENGPT_API int engpt_write_kv_pages(const void* k, const void* v, const int64_t* 
  * Dh] with element strides q_strides (2 int64: row, head), o [B, H, Dh]
  * contiguous.  A row of length 0 (or below) gives zeros; what lies in the
  * cache behind a row's length is never used.  A length above table_width *
- * page_size or a page outside the pool is recorded (ENGPT_ERR_ARG, site 44)
- * and its keys count as absent.  Dh <= 256.  workspace: scratch of
+ * page_size (at most 2^31 - 4097) or a page outside the pool is recorded
+ * (ENGPT_ERR_ARG, site 44) and its keys count as absent.  Dh <= 256.  workspace: scratch of
  * engpt_paged_attention_floats(...) floats, 16-byte aligned, owned by this
  * call until its kernels have run; it needs no initial value.
  */

@@ -328,9 +328,9 @@ int dispatch_simt(const AttnArgs& a, bool vec, cudaStream_t st) {
 //
 // Built for a width D of 64 or 128; a smaller head_dim is padded with zeros by TMA, in shared memory only.
 //
-// A tile is KT keys of one kv head, TILE bytes of keys and as many of values.  The tiles of all (row, kv head) pairs
-// form one list, cut into equal contiguous ranges, one per warp ("worker") of a persistent grid, so the load is even
-// whatever the lengths.  A warp fetches its own tiles through its own ring of kStages tiles in shared memory: TMA
+// A tile is KT keys of one kv head, kTileBytes of keys and as many of values.  The tiles of all (row, kv head) pairs
+// form one list, cut into contiguous ranges of equal cost, one per warp ("worker") of a persistent grid, so the load is
+// even whatever the lengths: a tile costs kTileUnits and the end of a pair kEndUnits more.  A warp fetches its own tiles through its own ring of kStages tiles in shared memory: TMA
 // boxes of R rows (R divides the page size) at the page that the block table names, 128-byte swizzled, one mbarrier
 // per stage; no warp waits for another one until the end.
 //
@@ -352,6 +352,10 @@ constexpr int kWarps = 8;
 constexpr int kPairWarps = 4;           // of the form with a cluster per pair: several CTAs per SM
 constexpr int kStages = 1;
 constexpr int kTileBytes = 8192;        // one of K, V
+constexpr int kTileUnits = 2, kEndUnits = 1;
+
+// Units of a pair of T tiles.
+__host__ __device__ constexpr int pair_units(int T) { return T > 0 ? T * kTileUnits + kEndUnits : 0; }
 
 template <int D>
 struct Mma {
@@ -408,9 +412,9 @@ __device__ __forceinline__ int clip_length(const MmaArgs& a, int len) {
   return (int)min((int64_t)max(len, 0), (int64_t)a.W * a.ps);
 }
 
-// Position in the list of tiles: tile t of T of (row b of length len, head group h of kv head hk).
+// Position in the list of tiles: tile t of T of (row b of length len, head group h of kv head hk), at unit u.
 struct Cursor {
-  int b, h, t, T, len, hk;
+  int b, h, t, T, len, hk, u;
 };
 
 // A box of the tile to come: its page as the table has it (looked at only when the copy is issued, so that nothing
@@ -435,7 +439,9 @@ struct Worker {
   }
 
   __device__ __forceinline__ void advance(Cursor& c) const {
+    c.u += kTileUnits;
     if (++c.t < c.T) return;
+    c.u += kEndUnits;
     c.t = 0;
     ++c.h;
     if (c.h < a.HQ) {
@@ -699,7 +705,7 @@ __host__ __device__ constexpr int part_floats(int rows) {
   return rows * (D + 2);
 }
 
-// First tile of every row, s_start[0 .. B] (exclusive prefix sums of a row's tiles times HQ), by a CTA of `threads`
+// First unit of every row, s_start[0 .. B] (exclusive prefix sums of a row's units times HQ), by a CTA of `threads`
 // threads; returns their number.  For up to 32 rows every warp forms the same sums for itself (the warps write the
 // same numbers) and keeps row `lane`'s length and first tile in `len` and `start`: no barrier before the first copy.
 template <int KT>
@@ -715,7 +721,7 @@ __device__ __forceinline__ int list_starts(const MmaArgs& a, int* s_start, int* 
       if (record && len > (int64_t)a.W * a.ps) record_device_error(ENGPT_ERR_ARG, 44);
       len = clip_length(a, len);
     }
-    const int v = (len + KT - 1) / KT * a.HQ;
+    const int v = pair_units((len + KT - 1) / KT) * a.HQ;
     int x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -747,7 +753,14 @@ __device__ __forceinline__ int list_starts(const MmaArgs& a, int* s_start, int* 
   return carry;
 }
 
-// Last row whose first tile is <= f (rows without tiles share their successor's start).
+// Units of a worker; at least a tile's, so that no worker between two others of a pair is without one of its tiles.
+__device__ __forceinline__ int worker_units(int total) {
+  const uint32_t workers = gridDim.x * kWarps;
+  return max(kTileUnits, (int)(((uint32_t)total + workers - 1) / workers));
+}
+
+// Last row whose first unit is <= f (rows without tiles share their successor's start).
+// (A cut that gives every worker its exact share, i * total / workers, was slower: it cuts more pairs.)
 __device__ __forceinline__ int list_row(const MmaArgs& a, const int* s_start, int f, int start) {
   const int lane = threadIdx.x & 31;
   if (a.B <= 32) return 31 - __clz(__ballot_sync(0xffffffffu, lane < a.B && start <= f));
@@ -793,35 +806,42 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(MmaArgs a, con
   __syncwarp();
   asm volatile("griddepcontrol.wait;" ::: "memory");   // nothing of an earlier kernel has been touched before
 
-  // this worker's range of the list [f0, f1) and its first tile
+  // this worker's range [u0, u1) of the list's units and its first tile: the tiles that begin in the range are its own
   const int worker = blockIdx.x * kWarps + warp;
   int row_len = 0, row_start = 0;
   const int total = list_starts<C::KT>(a, s_start, s_scan, kWarps * 32, blockIdx.x == 0, row_len, row_start);
-  const int workers = gridDim.x * kWarps;
-  const int per = (int)(((uint32_t)total + workers - 1) / (uint32_t)workers);
-  const int f0 = (int)min((int64_t)total, (int64_t)worker * per), f1 = (int)min((int64_t)total, (int64_t)f0 + per);
+  const int per = worker_units(total);
+  const int u0 = (int)min((int64_t)total, (int64_t)worker * per), u1 = (int)min((int64_t)total, (int64_t)u0 + per);
   Cursor c;
-  c.b = list_row(a, s_start, f0, row_start);
+  c.b = list_row(a, s_start, u0, row_start);
   if (a.B <= 32) {
     c.len = __shfl_sync(0xffffffffu, row_len, c.b);
     c.T = (c.len + C::KT - 1) / C::KT;
   } else {
     w.enter_row(c);
   }
-  const uint32_t in = f0 - s_start[c.b], T = max(c.T, 1);
-  c.h = (int)(in / T);
-  c.t = (int)(in - c.h * T);
+  const uint32_t in = u0 - s_start[c.b], span = max(pair_units(c.T), 1);
+  c.h = (int)(in / span);
+  c.t = (int)(in - c.h * span + kTileUnits - 1) / kTileUnits;   // the first tile that begins in the range
   c.hk = c.h / a.QG;
+  c.u = s_start[c.b] + c.h * (int)span + c.t * kTileUnits;
+  if (u0 >= u1) {
+    c.u = u1;            // nothing to do
+  } else if (c.t >= c.T) {
+    c.t = c.T - 1;       // the range begins in the end of a pair: on to the next one
+    c.u -= kTileUnits;
+    w.advance(c);
+  }
 
-  // fill the ring
-  const int n_issued = min(f1 - f0, a.stages);
+  // fill the ring: ci is the next tile to fetch
   Cursor ci = c;
-  Box box = n_issued > 0 ? w.find_box(ci) : Box{0, -1};
-  for (int s = 0; s < n_issued; ++s) {
+  Box box = ci.u < u1 ? w.find_box(ci) : Box{0, -1};
+  int in_flight = 0;
+  for (; in_flight < a.stages && ci.u < u1; ++in_flight) {
     Cursor cn = ci;
     w.advance(cn);
-    const Box next = f0 + s + 1 < f1 ? w.find_box(cn) : Box{0, -1};
-    w.issue(ci, box, s);
+    const Box next = cn.u < u1 ? w.find_box(cn) : Box{0, -1};
+    w.issue(ci, box, in_flight);
     ci = cn;
     box = next;
   }
@@ -846,14 +866,14 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(MmaArgs a, con
   bool fresh = true;                // the next tile begins a segment
   int t0 = 0;
   int s = 0;
-  for (int f = f0; f < f1; ++f) {
+  while (c.u < u1) {
     if (fresh) {
       load_query<D>(a, c.b, c.h, lane, qa);
       t0 = c.t;
       fresh = false;
     }
     if (!__all_sync(0xffffffffu, sm100::mbar_wait(w.bars + 8 * s, (phases >> s) & 1u, &s_abort, 45))) {
-      w.drain(s, min(f1 - f, a.stages), phases);
+      w.drain(s, in_flight, phases);
       break;   // (the pair keeps no part of this warp: its rows are wrong, and the status word says so)
     }
     phases ^= 1u << s;
@@ -864,14 +884,18 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(MmaArgs a, con
     else
       tile_step<D, false>(a, sk, qa, st, live, mask, lane);
     __syncwarp();
-    if (f + a.stages < f1) {
+    --in_flight;
+    if (ci.u < u1) {
       w.issue(ci, box, s);
+      ++in_flight;
       w.advance(ci);
-      box = f + a.stages + 1 < f1 ? w.find_box(ci) : Box{0, -1};
+      box = ci.u < u1 ? w.find_box(ci) : Box{0, -1};
     }
     if (++s == a.stages) s = 0;
     const bool pair_end = c.t + 1 == c.T;
-    if (pair_end || f + 1 == f1) {
+    Cursor cn = c;
+    w.advance(cn);
+    if (pair_end || cn.u >= u1) {
       finish_rows<D>(a, st);
       if (t0 == 0 && pair_end) {
         store_rows<D>(a, st, c.b, c.h, lane);
@@ -879,7 +903,8 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(MmaArgs a, con
         store_part<D>(a, st, tail_part, lane);   // the last tile of the range: every stage has been read
         if (lane == 0) {
           s_tail[warp] = c.b * a.HQ + c.h;
-          s_over[warp] = s_start[c.b] + (int64_t)(c.h + 1) * c.T > (int64_t)(blockIdx.x + 1) * kWarps * per;
+          // does its last tile begin behind this CTA's units?
+          s_over[warp] = (int64_t)c.u + (c.T - 1 - c.t) * kTileUnits >= (int64_t)(blockIdx.x + 1) * kWarps * per;
         }
       } else {
         store_part<D>(a, st, part, lane);
@@ -888,7 +913,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(MmaArgs a, con
       st.reset();
       fresh = true;
     }
-    w.advance(c);
+    c = cn;
   }
 
   float* out = a.work + (int64_t)blockIdx.x * 2 * pf;
@@ -1046,18 +1071,17 @@ __global__ void __launch_bounds__(kWarps * 32) decode_join_list_kernel(MmaArgs a
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   int row_len = 0, row_start = 0;
   const int total = list_starts<Mma<D>::KT>(a, s_start, s_scan, kWarps * 32, false, row_len, row_start);
-  const int workers = gridDim.x * kWarps;
-  const int64_t per = (int64_t)kWarps * (((uint32_t)total + workers - 1) / (uint32_t)workers);   // tiles of a CTA
-  const int64_t end = (blockIdx.x + 1) * per;   // the first tile of the next CTA
+  const int64_t per = (int64_t)kWarps * worker_units(total);   // of a CTA
+  const int64_t end = (blockIdx.x + 1) * per;   // the first unit of the next CTA
   int first = 0, n = 0, b = 0, h = 0;
   if (end < total) {
     b = list_row(a, s_start, (int)end, row_start);
-    const int T = (s_start[b + 1] - s_start[b]) / a.HQ;
-    h = ((int)end - s_start[b]) / T;
-    const int64_t from = s_start[b] + (int64_t)h * T;
-    if (from < end && from >= end - per) {      // it begins in this CTA and runs over its end
+    const int span = (s_start[b + 1] - s_start[b]) / a.HQ;
+    h = ((int)end - s_start[b]) / span;
+    const int64_t from = s_start[b] + (int64_t)h * span, to = from + span - kEndUnits - kTileUnits;   // first, last tile
+    if (from < end && from >= end - per && to >= end) {      // it begins in this CTA and runs over its end
       first = blockIdx.x;
-      n = (int)((from + T - 1) / per) - first + 1;
+      n = (int)(to / per) - first + 1;
     }
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -1139,7 +1163,7 @@ inline int64_t most_tiles(int D, int table_width, int page_size) {
 // Does a launch of these sizes go to the tensor-core kernel (strides and alignment apart)?
 inline bool mma_sizes(int dtype, int B, int H, int Hkv, int D, int table_width, int page_size) {
   return dtype == ENGPT_BF16 && D <= 128 && D % 8 == 0 && page_size % 8 == 0 && B <= 8192 &&
-         B * (int64_t)H * most_tiles(D, table_width, page_size) < (1ll << 31);
+         B * (int64_t)H * (kTileUnits * most_tiles(D, table_width, page_size) + kEndUnits) < (1ll << 31);
 }
 
 // CTAs per pair of the pair form, or 0 for the list form.

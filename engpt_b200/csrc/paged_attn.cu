@@ -330,7 +330,7 @@ int dispatch_simt(const AttnArgs& a, bool vec, cudaStream_t st) {
 //
 // A tile is KT keys of one kv head, kTileBytes of keys and as many of values.  The tiles of all (row, kv head) pairs
 // form one list, cut into contiguous ranges of equal cost, one per warp ("worker") of a persistent grid, so the load is
-// even whatever the lengths: a tile costs kTileUnits and the end of a pair kEndUnits more.  A warp fetches its own tiles through its own ring of kStages tiles in shared memory: TMA
+// even whatever the lengths.  A warp fetches its own tiles through its own ring of kStages tiles in shared memory: TMA
 // boxes of R rows (R divides the page size) at the page that the block table names, 128-byte swizzled, one mbarrier
 // per stage; no warp waits for another one until the end.
 //
@@ -352,11 +352,6 @@ constexpr int kWarps = 8;
 constexpr int kPairWarps = 4;           // of the form with a cluster per pair: several CTAs per SM
 constexpr int kStages = 1;
 constexpr int kTileBytes = 8192;        // one of K, V
-constexpr int kTileUnits = 2, kEndUnits = 1;
-
-// Units of a pair of T tiles.
-__host__ __device__ constexpr int pair_units(int T) { return T > 0 ? T * kTileUnits + kEndUnits : 0; }
-
 template <int D>
 struct Mma {
   static constexpr int KT = kTileBytes / (2 * D);
@@ -383,7 +378,13 @@ struct MmaArgs {
   __nv_bfloat16* o;
   float* work;             // [CTAs][2][rows][D + 2]
   int stages;
+  int tile_units, end_units;   // list form: cost of a tile and of a pair's end
 };
+
+// Units of a pair of T tiles.
+__device__ __forceinline__ int pair_units(const MmaArgs& a, int T) {
+  return T > 0 ? T * a.tile_units + a.end_units : 0;
+}
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -439,9 +440,9 @@ struct Worker {
   }
 
   __device__ __forceinline__ void advance(Cursor& c) const {
-    c.u += kTileUnits;
+    c.u += a.tile_units;
     if (++c.t < c.T) return;
-    c.u += kEndUnits;
+    c.u += a.end_units;
     c.t = 0;
     ++c.h;
     if (c.h < a.HQ) {
@@ -721,7 +722,7 @@ __device__ __forceinline__ int list_starts(const MmaArgs& a, int* s_start, int* 
       if (record && len > (int64_t)a.W * a.ps) record_device_error(ENGPT_ERR_ARG, 44);
       len = clip_length(a, len);
     }
-    const int v = pair_units((len + KT - 1) / KT) * a.HQ;
+    const int v = pair_units(a, (len + KT - 1) / KT) * a.HQ;
     int x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -754,9 +755,9 @@ __device__ __forceinline__ int list_starts(const MmaArgs& a, int* s_start, int* 
 }
 
 // Units of a worker; at least a tile's, so that no worker between two others of a pair is without one of its tiles.
-__device__ __forceinline__ int worker_units(int total) {
-  const uint32_t workers = gridDim.x * kWarps;
-  return max(kTileUnits, (int)(((uint32_t)total + workers - 1) / workers));
+__device__ __forceinline__ int worker_units(const MmaArgs& a, int total, int ctas) {
+  const uint32_t workers = ctas * kWarps;
+  return max(a.tile_units, (int)(((uint32_t)total + workers - 1) / workers));
 }
 
 // Last row whose first unit is <= f (rows without tiles share their successor's start).
@@ -810,7 +811,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(MmaArgs a, con
   const int worker = blockIdx.x * kWarps + warp;
   int row_len = 0, row_start = 0;
   const int total = list_starts<C::KT>(a, s_start, s_scan, kWarps * 32, blockIdx.x == 0, row_len, row_start);
-  const int per = worker_units(total);
+  const int per = worker_units(a, total, gridDim.x);
   const int u0 = (int)min((int64_t)total, (int64_t)worker * per), u1 = (int)min((int64_t)total, (int64_t)u0 + per);
   Cursor c;
   c.b = list_row(a, s_start, u0, row_start);
@@ -820,16 +821,16 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(MmaArgs a, con
   } else {
     w.enter_row(c);
   }
-  const uint32_t in = u0 - s_start[c.b], span = max(pair_units(c.T), 1);
+  const uint32_t in = u0 - s_start[c.b], span = max(pair_units(a, c.T), 1);
   c.h = (int)(in / span);
-  c.t = (int)(in - c.h * span + kTileUnits - 1) / kTileUnits;   // the first tile that begins in the range
+  c.t = (int)((in - c.h * span + a.tile_units - 1) / (uint32_t)a.tile_units);   // the first tile that begins in the range
   c.hk = c.h / a.QG;
-  c.u = s_start[c.b] + c.h * (int)span + c.t * kTileUnits;
+  c.u = s_start[c.b] + c.h * (int)span + c.t * a.tile_units;
   if (u0 >= u1) {
     c.u = u1;            // nothing to do
   } else if (c.t >= c.T) {
     c.t = c.T - 1;       // the range begins in the end of a pair: on to the next one
-    c.u -= kTileUnits;
+    c.u -= a.tile_units;
     w.advance(c);
   }
 
@@ -904,7 +905,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(MmaArgs a, con
         if (lane == 0) {
           s_tail[warp] = c.b * a.HQ + c.h;
           // does its last tile begin behind this CTA's units?
-          s_over[warp] = (int64_t)c.u + (c.T - 1 - c.t) * kTileUnits >= (int64_t)(blockIdx.x + 1) * kWarps * per;
+          s_over[warp] = (int64_t)c.u + (c.T - 1 - c.t) * a.tile_units >= (int64_t)(blockIdx.x + 1) * kWarps * per;
         }
       } else {
         store_part<D>(a, st, part, lane);
@@ -1057,11 +1058,12 @@ __global__ void __launch_bounds__(kPairWarps * 32) decode_pair_kernel(MmaArgs a,
   }
 }
 
-// Pairs that run over the end of a CTA of decode_list_kernel: one CTA per such end, a warp's share of the parts each.
+// Pairs that run over the end of a CTA of decode_list_kernel: a CTA per pair and row of its query heads, or per CTA
+// end and row if there are more pairs than CTAs (of `ctas`); every warp takes a share of the parts.
 // It starts while that kernel runs (whose CTAs have by then waited for all earlier work) and finds its pair from the
 // lengths; only the parts have to wait.
 template <int D>
-__global__ void __launch_bounds__(kWarps * 32) decode_join_list_kernel(MmaArgs a) {
+__global__ void __launch_bounds__(kWarps * 32) decode_join_list_kernel(MmaArgs a, int ctas) {
   constexpr int E = D / 32;
   extern __shared__ int s_start[];
   __shared__ float s_o[kWarps][D];
@@ -1071,23 +1073,34 @@ __global__ void __launch_bounds__(kWarps * 32) decode_join_list_kernel(MmaArgs a
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   int row_len = 0, row_start = 0;
   const int total = list_starts<Mma<D>::KT>(a, s_start, s_scan, kWarps * 32, false, row_len, row_start);
-  const int64_t per = (int64_t)kWarps * worker_units(total);   // of a CTA
-  const int64_t end = (blockIdx.x + 1) * per;   // the first unit of the next CTA
+  const int64_t per = (int64_t)kWarps * worker_units(a, total, ctas);   // of a CTA
   int first = 0, n = 0, b = 0, h = 0;
-  if (end < total) {
-    b = list_row(a, s_start, (int)end, row_start);
+  if ((int)gridDim.x < ctas) {                        // pair blockIdx.x
+    b = blockIdx.x / a.HQ;
+    h = blockIdx.x - b * a.HQ;
     const int span = (s_start[b + 1] - s_start[b]) / a.HQ;
-    h = ((int)end - s_start[b]) / span;
-    const int64_t from = s_start[b] + (int64_t)h * span, to = from + span - kEndUnits - kTileUnits;   // first, last tile
-    if (from < end && from >= end - per && to >= end) {      // it begins in this CTA and runs over its end
-      first = blockIdx.x;
+    const int64_t from = s_start[b] + (int64_t)h * span, to = from + span - a.end_units - a.tile_units;   // first, last tile
+    if (span > 0 && from / per < to / per) {
+      first = (int)(from / per);
       n = (int)(to / per) - first + 1;
+    }
+  } else {                                            // the pair that runs over the end of CTA blockIdx.x
+    const int64_t end = (blockIdx.x + 1) * per;       // the first unit of the next CTA
+    if (end < total) {
+      b = list_row(a, s_start, (int)end, row_start);
+      const int span = (s_start[b + 1] - s_start[b]) / a.HQ;
+      h = ((int)end - s_start[b]) / span;
+      const int64_t from = s_start[b] + (int64_t)h * span, to = from + span - a.end_units - a.tile_units;
+      if (from < end && from >= end - per && to >= end) {   // it begins in this CTA
+        first = blockIdx.x;
+        n = (int)(to / per) - first + 1;
+      }
     }
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int pf = part_floats<D>(a.rows);
-  const int rows = n > 0 ? min(a.rows, a.G - (h % a.QG) * 8) : 0;
-  for (int r = 0; r < rows; ++r) {
+  const int r = blockIdx.y;
+  if (n > 0 && (h % a.QG) * 8 + r < a.G) {
     float m = -INFINITY, l = 0.f, o[E] = {};
 #pragma unroll 4
     for (int i = warp; i < n; i += kWarps) {
@@ -1100,7 +1113,6 @@ __global__ void __launch_bounds__(kWarps * 32) decode_join_list_kernel(MmaArgs a
       for (int e = 0; e < E; ++e) o[e] = o[e] * w0 + p[lane + 32 * e] * w1;
       m = mx;
     }
-    __syncthreads();
 #pragma unroll
     for (int e = 0; e < E; ++e) s_o[warp][lane + 32 * e] = o[e];
     if (lane == 0) {
@@ -1163,7 +1175,7 @@ inline int64_t most_tiles(int D, int table_width, int page_size) {
 // Does a launch of these sizes go to the tensor-core kernel (strides and alignment apart)?
 inline bool mma_sizes(int dtype, int B, int H, int Hkv, int D, int table_width, int page_size) {
   return dtype == ENGPT_BF16 && D <= 128 && D % 8 == 0 && page_size % 8 == 0 && B <= 8192 &&
-         B * (int64_t)H * (kTileUnits * most_tiles(D, table_width, page_size) + kEndUnits) < (1ll << 31);
+         B * (int64_t)H * (2 * most_tiles(D, table_width, page_size) + 1) < (1ll << 31);
 }
 
 // CTAs per pair of the pair form, or 0 for the list form.
@@ -1241,8 +1253,10 @@ int launch_list(const MmaArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, 
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, kern, a, mk, mv);
   if (e != cudaSuccess) return set_error(ENGPT_ERR_LAUNCH, "paged_attention: %s", cudaGetErrorString(e));
+  const int64_t pairs = (int64_t)a.B * a.HQ;
+  cfg.gridDim = dim3((unsigned)(pairs < num_sms() ? pairs : num_sms()), a.rows);
   cfg.dynamicSmemBytes = 4 * ((size_t)a.B + 1);
-  e = cudaLaunchKernelEx(&cfg, decode_join_list_kernel<D>, a);
+  e = cudaLaunchKernelEx(&cfg, decode_join_list_kernel<D>, a, num_sms());
   if (e != cudaSuccess) return set_error(ENGPT_ERR_LAUNCH, "paged_attention (join): %s", cudaGetErrorString(e));
   return check_launch("paged_attention (join)");
 }
@@ -1281,6 +1295,12 @@ int launch_mma(const AttnArgs& x, int Hkv, cudaStream_t st) {
   if ((rc = page_map(&mv, x.v_pages, x.Dh, x.ps, Hkv, x.P, x.vs, a.R))) return rc;
   const int cs = pair_ctas(x.B, x.H, Hkv, D, x.W, x.ps);
   a.stages = kStages;
+  // The end of a pair costs a worker about half a tile (its sums and stores, and tiles that are partly empty).  It is
+  // counted once workers see such ends often (256 rows of 1 to 512 tokens: 51.8 us, 63.8 without); with few pairs the
+  // ranges are whole tiles, which cuts fewer pairs (32 rows of 512 tokens, 16 heads: 16.9 us, 18.5 with).
+  const bool ends = 2 * (int64_t)x.B * a.HQ > (int64_t)num_sms() * kWarps;
+  a.tile_units = ends ? 2 : 1;
+  a.end_units = ends ? 1 : 0;
   if (cs == 0) return launch_list<D>(a, mk, mv, st);
   return launch_pair<D>(a, mk, mv, cs, st);
 }

@@ -243,20 +243,28 @@ struct AppendRow {
   }
 };
 
-constexpr int kAppendCtas = 16;   // CTAs per SM of a launch whose CTAs walk over several tokens
+constexpr int kAppendThreads = 2048;   // per SM in a launch whose CTAs walk over several tokens
 
-// MIN: CTAs per SM that the registers have to leave room for.
-template <typename T, int LPR, int MIN>
+// MIN: CTAs per SM that the registers have to leave room for.  WIDE: the plain case, a token's heads fill whole CTAs
+// and Dh = 8 LPR.  Otherwise a CTA takes several tokens side by side, and rows may be shorter than their LPR lanes (a power
+// of two, for the butterfly): the lanes behind a row add nothing.
+template <typename T, int LPR, int MIN, bool WIDE>
 __global__ void __launch_bounds__(128, MIN) append_vec_kernel(QkvArgs a, PagedDst d) {
   constexpr bool kFast = sizeof(T) == 2;
   // started ahead of the end of what runs before (usually the projection), and so may be what follows (usually the
   // attention over the pages): each waits on the device for its predecessor's results
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int idx = blockIdx.y * 128 + threadIdx.x;      // (head, slice)
-  const bool mine = idx < a.H * LPR;
-  const int h = mine ? idx / LPR : 0;
-  const int e0 = (idx % LPR) * 8;
+  const int lanes = a.H * LPR, tokens = WIDE || lanes >= 128 ? 1 : 128 / lanes;
+  const int idx = blockIdx.y * blockDim.x + threadIdx.x;   // (token of the CTA's, head, slice)
+  const int sub = tokens > 1 ? idx / lanes : 0;
+  bool mine = tokens > 1 ? sub < tokens : idx < lanes;
+  const int h = mine ? (idx - sub * lanes) / LPR : 0;
+  int e0 = (idx % LPR) * 8;
+  if (!WIDE && e0 >= a.Dh) {
+    e0 = 0;
+    mine = false;
+  }
   const int64_t part = (int64_t)a.H * a.Dh;            // elements from q to k and from k to v
   const T* src = reinterpret_cast<const T*>(a.qkv) + (int64_t)h * a.Dh + e0;
   T* q_dst = reinterpret_cast<T*>(a.q) + (int64_t)h * a.Dh + e0;
@@ -274,9 +282,12 @@ __global__ void __launch_bounds__(128, MIN) append_vec_kernel(QkvArgs a, PagedDs
     for (int i = 0; i < 8; ++i) scl[i] = v[i] * a.qk_mult;
   }
   AppendRow<T> next;
-  int64_t n = blockIdx.x;
-  next.load(a, d, src, part, n);                       // (a thread without a slice of its own walks head 0)
-  for (; n < a.T; n += gridDim.x) {
+  const int64_t step = (int64_t)gridDim.x * tokens;
+  int64_t n0 = (int64_t)blockIdx.x * tokens;           // the CTA's first token: the trip count is the same for all lanes
+  // (a thread without a slice or a token of its own loads another one's)
+  next.load(a, d, src, part, WIDE || n0 + sub < a.T ? n0 + sub : a.T - 1);
+  for (; n0 < a.T; n0 += step) {
+    const int64_t n = n0 + sub;
     const AppendRow<T> row = next;
     const bool turn = rot && (unsigned)row.pos < (unsigned)d.rope_rows;
     float4 c4 = make_float4(1.f, 1.f, 1.f, 1.f), s4 = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -284,7 +295,7 @@ __global__ void __launch_bounds__(128, MIN) append_vec_kernel(QkvArgs a, PagedDs
       c4 = __ldg(reinterpret_cast<const float4*>(a.cos_tab + (int64_t)row.pos * a.rope_half + p0));
       s4 = __ldg(reinterpret_cast<const float4*>(a.sin_tab + (int64_t)row.pos * a.rope_half + p0));
     }
-    if (n + gridDim.x < a.T) next.load(a, d, src, part, n + gridDim.x);
+    if (n + step < a.T) next.load(a, d, src, part, n + step);
     float ss[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -293,10 +304,11 @@ __global__ void __launch_bounds__(128, MIN) append_vec_kernel(QkvArgs a, PagedDs
       ss[s] = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss[s] = fmaf(x[i], x[i], ss[s]);
+      if (!WIDE && !mine) ss[s] = 0.f;
 #pragma unroll
       for (int o = LPR / 2; o > 0; o >>= 1) ss[s] += __shfl_xor_sync(0xffffffffu, ss[s], o);
     }
-    if (!mine) continue;
+    if (!mine || (!WIDE && n >= a.T)) continue;
     const bool placed = checked_position(d, row.pos) >= 0;
     const int slot = checked_slot(d, row.slot);
     const int page = d.page_shift >= 0 ? slot >> d.page_shift : slot / d.page_size;
@@ -419,12 +431,15 @@ __global__ void __launch_bounds__(256) qkv_generic_kernel(QkvArgs a, PagedDst d)
 }
 
 // 16-byte accesses to q, k, v and the tables are possible.
+static bool vec_aligned(const QkvArgs& a) {
+  return aligned(a.qkv, 16) && aligned(a.q, 16) && aligned(a.k, 16) && aligned(a.v, 16) && aligned(a.qk_scale, 16) &&
+         (a.rope_half == 0 || (aligned(a.cos_tab, 16) && aligned(a.sin_tab, 16)));
+}
+
 static bool vec_access(const QkvArgs& a, int esz) {
   const int Dh = a.Dh;
   return (Dh == 8 || Dh == 16 || Dh == 32 || Dh == 64 || Dh == 128 || Dh == 256) && a.rope_half <= kQkvMaxHalf &&
-         a.rope_half % 4 == 0 && aligned(a.qkv, 16) && aligned(a.q, 16) && aligned(a.k, 16) && aligned(a.v, 16) &&
-         aligned(a.qk_scale, 16) && (a.rope_half == 0 || (aligned(a.cos_tab, 16) && aligned(a.sin_tab, 16))) &&
-         ((int64_t)Dh * esz) % 16 == 0;
+         a.rope_half % 4 == 0 && vec_aligned(a) && ((int64_t)Dh * esz) % 16 == 0;
 }
 
 template <bool PAGED>
@@ -439,15 +454,20 @@ static int launch_generic(const QkvArgs& a, const PagedDst& d, int dtype, const 
 
 template <typename T, int LPR>
 static void launch_append(const QkvArgs& a, const PagedDst& d, cudaStream_t st) {
-  const int y = ceil_div((int64_t)a.H * LPR, 128);
-  // A token per CTA for a few tokens; else kAppendCtas per SM that walk, in bf16 with the registers held to 8 resident
+  // CTAs of a size that divides a token's lanes, or of 128 threads with several tokens or idle lanes
+  const int lanes = a.H * LPR;
+  const bool wide = lanes % 32 == 0 && a.Dh == 8 * LPR;
+  const int block = !wide || lanes % 128 == 0 ? 128 : lanes % 96 == 0 ? 96 : lanes % 64 == 0 ? 64 : 32;
+  const int y = ceil_div(lanes, block), tokens = wide || lanes >= 128 ? 1 : 128 / lanes;
+  const int64_t groups = ((int64_t)a.T + tokens - 1) / tokens;
+  // A token (or group of them) per CTA for a few tokens; else 2048 threads per SM that walk, in bf16 with the registers held to 8 resident
   // CTAs per SM for more rows in flight: 8188 tokens of 16 heads of 128 take 36 us so (5.6 TB/s), 39 with 6 resident
   // CTAs, 44 without a limit, 46 with a token per CTA.  fp32 rows are twice as long and would spill at 8.
-  const int64_t most = (int64_t)num_sms() * kAppendCtas / y;
-  const bool walk = a.T > most;
+  const int64_t most = (int64_t)num_sms() * kAppendThreads / (block * y);
+  const bool walk = groups > most;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(walk ? (most > 0 ? most : 1) : a.T), (unsigned)y);
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3((unsigned)(walk ? (most > 0 ? most : 1) : groups), (unsigned)y);
+  cfg.blockDim = dim3(block);
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -455,8 +475,12 @@ static void launch_append(const QkvArgs& a, const PagedDst& d, cudaStream_t st) 
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   // (a launch error is picked up by check_launch)
-  if (walk) cudaLaunchKernelEx(&cfg, append_vec_kernel<T, LPR, sizeof(T) == 2 ? 8 : 1>, a, d);
-  else cudaLaunchKernelEx(&cfg, append_vec_kernel<T, LPR, 1>, a, d);
+  if (!wide)
+    cudaLaunchKernelEx(&cfg, append_vec_kernel<T, LPR, sizeof(T) == 2 ? 7 : 1, false>, a, d);
+  else if (walk)
+    cudaLaunchKernelEx(&cfg, append_vec_kernel<T, LPR, sizeof(T) == 2 ? 8 : 1, true>, a, d);
+  else
+    cudaLaunchKernelEx(&cfg, append_vec_kernel<T, LPR, 1, true>, a, d);
 }
 
 }  // namespace engpt
@@ -547,7 +571,8 @@ extern "C" int engpt_qkv_append(const void* qkv, int dtype, const float* rho, co
     d.vs[i] = page_strides[3 + i];
   }
   const int esz = dtype == ENGPT_BF16 ? 2 : 4;
-  bool vec = vec_access(a, esz) && H <= 65535;
+  bool vec = Dh % 8 == 0 && Dh <= 256 && vec_aligned(a) && H <= 65535;   // (then half of Dh is a multiple of 4)
+  vec = vec && (rope_half == 0 || rope_half == Dh / 2);
   for (int i = 0; i < 3; ++i) {
     // the stride of an axis of one element is never used, and may be anything
     if ((i == 0 ? num_pages : i == 1 ? H : page_size) == 1) d.ks[i] = d.vs[i] = 0;
@@ -556,20 +581,17 @@ extern "C" int engpt_qkv_append(const void* qkv, int dtype, const float* rho, co
   cudaStream_t st = as_stream(stream);
   if (!vec) return launch_generic<true>(a, d, dtype, "qkv_append", st);
 #define ENGPT_APPEND_LAUNCH(L)                                       \
-  case 8 * L:                                                        \
+  if (Dh <= 8 * L) {                                                 \
     if (dtype == ENGPT_BF16) launch_append<__nv_bfloat16, L>(a, d, st); \
     else launch_append<float, L>(a, d, st);                          \
-    break;
-  switch (Dh) {
-    ENGPT_APPEND_LAUNCH(1)
-    ENGPT_APPEND_LAUNCH(2)
-    ENGPT_APPEND_LAUNCH(4)
-    ENGPT_APPEND_LAUNCH(8)
-    ENGPT_APPEND_LAUNCH(16)
-    ENGPT_APPEND_LAUNCH(32)
-    default:
-      return set_error(ENGPT_ERR_UNSUPPORTED, "qkv_append: head_dim %d", Dh);
+    return check_launch("qkv_append");                               \
   }
+  ENGPT_APPEND_LAUNCH(1)
+  ENGPT_APPEND_LAUNCH(2)
+  ENGPT_APPEND_LAUNCH(4)
+  ENGPT_APPEND_LAUNCH(8)
+  ENGPT_APPEND_LAUNCH(16)
+  ENGPT_APPEND_LAUNCH(32)
 #undef ENGPT_APPEND_LAUNCH
-  return check_launch("qkv_append");
+  return set_error(ENGPT_ERR_UNSUPPORTED, "qkv_append: head_dim %d", Dh);
 }

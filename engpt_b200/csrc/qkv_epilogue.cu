@@ -460,9 +460,11 @@ static void launch_append(const QkvArgs& a, const PagedDst& d, cudaStream_t st) 
   const int block = !wide || lanes % 128 == 0 ? 128 : lanes % 96 == 0 ? 96 : lanes % 64 == 0 ? 64 : 32;
   const int y = ceil_div(lanes, block), tokens = wide || lanes >= 128 ? 1 : 128 / lanes;
   const int64_t groups = ((int64_t)a.T + tokens - 1) / tokens;
-  // A token (or group of them) per CTA for a few tokens; else 2048 threads per SM that walk, in bf16 with the registers held to 8 resident
-  // CTAs per SM for more rows in flight: 8188 tokens of 16 heads of 128 take 36 us so (5.6 TB/s), 39 with 6 resident
-  // CTAs, 44 without a limit, 46 with a token per CTA.  fp32 rows are twice as long and would spill at 8.
+  // A token (or group of them) per CTA for a few tokens; else 2048 threads per SM that walk, with the registers held to
+  // 8 resident CTAs in bf16 (8188 tokens of 16 heads of 128: 36 us = 5.6 TB/s so, 39 with 6, 44 without a limit, 46
+  // with a token per CTA) and to 3 in fp32, whose rows are twice as long (8188 tokens of 16 heads of 64: 34 us with 3
+  // or 4, 39 with 5, 43 with 6).  Several tokens side by side do best at 7 (16384 of 5 heads of 80: 28 us, 32 at 5, 33
+  // at 8).
   const int64_t most = (int64_t)num_sms() * kAppendThreads / (block * y);
   const bool walk = groups > most;
   cudaLaunchConfig_t cfg = {};
@@ -478,7 +480,7 @@ static void launch_append(const QkvArgs& a, const PagedDst& d, cudaStream_t st) 
   if (!wide)
     cudaLaunchKernelEx(&cfg, append_vec_kernel<T, LPR, sizeof(T) == 2 ? 7 : 1, false>, a, d);
   else if (walk)
-    cudaLaunchKernelEx(&cfg, append_vec_kernel<T, LPR, sizeof(T) == 2 ? 8 : 1, true>, a, d);
+    cudaLaunchKernelEx(&cfg, append_vec_kernel<T, LPR, sizeof(T) == 2 ? 8 : 3, true>, a, d);
   else
     cudaLaunchKernelEx(&cfg, append_vec_kernel<T, LPR, 1, true>, a, d);
 }

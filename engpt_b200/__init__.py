@@ -6,8 +6,8 @@ Drop-in names for the reference package:
 * ``EfficientNGPT`` / ``EfficientNGPTBlock`` -- engpt/models.py (same
   ``state_dict`` keys and seeded init; forward runs the fused CUDA engine)
 * ``engpt_b200.kernels`` -- the engpt.kernels hot-path ops on CUDA kernels
-* ``torch.ops.engpt_b200.*`` -- the three hot-path ops as registered
-  PyTorch operators (``engpt_b200.torch_ops``)
+* ``torch.ops.engpt_b200.*`` -- the three hot-path ops and the paged-cache
+  ops as registered PyTorch operators (``engpt_b200.torch_ops``)
 * ``PagedDecoder`` / ``PagedKVCache`` -- generation with a paged key-value
   cache (``engpt_b200.decode``; the reference has none)
 * ``patch_reference(engpt_pkg)`` -- rebinds the hot-path ops inside an
@@ -19,7 +19,7 @@ __version__ = "0.1.0"
 from .config import ModelConfig
 from .models import EfficientNGPT, EfficientNGPTBlock
 from . import kernels
-from . import torch_ops  # registers torch.ops.engpt_b200.{qkv_postprocess_from_carried, causal_sdpa, carried_residual_gauge}
+from . import torch_ops  # registers torch.ops.engpt_b200.*
 from .decode import PagedDecoder, PagedKVCache
 from .integration import patch_reference
 

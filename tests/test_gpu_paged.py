@@ -580,3 +580,21 @@ def test_generation_step_in_a_graph_grows_the_cache(cuda):
     got = torch.stack(outs, 1).float()
     # the same bf16 q, k, v; the whole-sequence op in fp32: one bf16 rounding apart, and some fp32 noise
     assert ((got - want).abs() <= 2.0 ** -8 * want.abs() + 1e-4 * v.float().abs().max()).all()
+
+
+def test_registered_operators_are_the_same_calls(cuda):
+    ops = torch.ops.engpt_b200
+    runs = []
+    for f in (K, ops):
+        t = Tables([5, 0, 40], 16, 4, 12, seed=1)
+        kp, vp = make_pools(12, 4, 16, 64, torch.bfloat16, fill=0.5)
+        new = torch.tensor([1, 3, 2], dtype=torch.int32, device=cuda)
+        slots, pos = f.advance_block_tables(t.lengths, new, t.table, t.free, t.count, page_size=16, max_new=3,
+                                            finished=torch.tensor([False, False, True], device=cuda))
+        qkv, rho, cos, sin, scale, _ = append_inputs(9, 4, 64, torch.bfloat16, 4)
+        q = f.qkv_append_from_carried(qkv.view(3, 3, 3, 4, 64), rho.view(3, 3), cos, sin, scale, 1e-6, pos, slots, kp,
+                                      vp, qk_mult=0.5)
+        f.write_kv_pages(qkv[:2, 1], qkv[:2, 2], torch.tensor([2, 1], dtype=torch.int32, device=cuda), kp, vp)
+        o = f.paged_sdpa(q[:, 0].contiguous(), kp, vp, t.table, t.lengths, scale=0.3)
+        runs.append((slots, pos, t.lengths, t.table, t.free, t.count, kp, vp, q, o))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))

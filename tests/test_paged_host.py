@@ -136,3 +136,30 @@ def test_cache_and_decoder_refuse_the_cpu():
         PagedKVCache(cfg, 2, 4, dtype=torch.float16)
     with pytest.raises(RuntimeError, match="CUDA"):
         EfficientNGPT(cfg).decoder(2, 4)
+
+
+def test_torch_ops_of_the_cache():
+    """Registered operators: schemas with the changed arguments, fake shapes, no CPU kernel."""
+    ops = torch.ops.engpt_b200
+    s = str(ops.advance_block_tables.default._schema)
+    assert "Tensor(a0!) lengths" in s and "Tensor(a2!) block_table" in s and "Tensor? finished" in s, s
+    assert "k_pages" in str(ops.write_kv_pages.default._schema) and "!" in str(ops.write_kv_pages.default._schema)
+    assert "!" not in str(ops.paged_sdpa.default._schema)
+    with cuda_fakes():
+        c = dict(device="cuda")
+        i = torch.empty(3, dtype=torch.int32, **c)
+        table, free = torch.empty(3, 5, dtype=torch.int32, **c), torch.empty(9, dtype=torch.int32, **c)
+        slots, pos = ops.advance_block_tables(i, i.clone(), table, free, i[:1].clone(), page_size=16, max_new=7)
+        assert slots.shape == pos.shape == (3, 7) and slots.dtype == torch.int32
+        kp = torch.empty(8, 2, 16, 64, dtype=torch.bfloat16, **c)
+        q = ops.qkv_append_from_carried(torch.empty(3, 1, 3, 2, 64, dtype=torch.bfloat16, **c),
+                                        torch.empty(3, 1, **c), torch.empty(9, 32, **c), torch.empty(9, 32, **c),
+                                        torch.empty(2, 64, **c), 1e-6, i.view(3, 1), i.view(3, 1).clone(), kp,
+                                        kp.clone())
+        assert q.shape == (3, 1, 2, 64) and q.dtype == torch.bfloat16
+        o = ops.paged_sdpa(torch.empty(3, 4, 64, dtype=torch.bfloat16, **c), kp, kp, table, i, scale=1.0)
+        assert o.shape == (3, 4, 64)
+    x = torch.zeros(4, 2, 16, 64)
+    with pytest.raises(NotImplementedError):
+        ops.paged_sdpa(torch.zeros(1, 2, 64), x, x, torch.zeros(1, 2, dtype=torch.int32),
+                       torch.zeros(1, dtype=torch.int32), scale=1.0)

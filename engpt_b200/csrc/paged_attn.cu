@@ -330,9 +330,9 @@ int dispatch_simt(const AttnArgs& a, bool vec, cudaStream_t st) {
 //
 // A tile is KT keys of one kv head, kTileBytes of keys and as many of values.  The tiles of all (row, kv head) pairs
 // form one list, cut into contiguous ranges of equal cost, one per warp ("worker") of a persistent grid, so the load is
-// even whatever the lengths.  A warp fetches its own tiles through its own ring of kStages tiles in shared memory: TMA
-// boxes of R rows (R divides the page size) at the page that the block table names, 128-byte swizzled, one mbarrier
-// per stage; no warp waits for another one until the end.
+// even whatever the lengths.  A warp fetches its own tiles, one at a time, into its own 16 KB of shared memory:
+// TMA boxes of R rows (R divides the page size) at the page that the block table names, 128-byte swizzled, completing
+// on the warp's mbarrier; no warp waits for another one until the end.
 //
 // Per tile, with up to 8 query heads of the kv head as rows 0-7 of the 16-row mma.sync operand:
 //   S = Q K^T (rows 8-15 are zero), p = 2^(S scale - m), and O += P V with P's bf16 value in rows 0-7 and the
@@ -345,12 +345,12 @@ int dispatch_simt(const AttnArgs& a, bool vec, cudaStream_t st) {
 // of a pair are joined by the warp that holds its first one; a pair that runs over CTAs leaves one part per CTA in
 // the workspace, joined by decode_join_list_kernel.
 //
-// Warps, stages and tiles are what 64 rows of up to 4096 tokens (16 heads of 64) run best with: eight warps with one
-// 16 KB stage each 87 us, which leaves a warp idle while its copies fly but has seven others; 10 or 12 such warps 90
-// and 89, six or four with two stages 101 and 105, eight with two stages of 8 KB 97.
+// Warps and tiles are what 64 rows of up to 4096 tokens (16 heads of 64) run best with: eight warps, each of which idles
+// while its 16 KB fly but has seven others beside it, 87 us; 10 or 12 such warps 90 and 89, six or four with two tiles
+// in flight each 101 and 105, eight with two tiles of 8 KB 97.
 constexpr int kWarps = 8;
-constexpr int kPairWarps = 4;           // of the form with a cluster per pair: several CTAs per SM
-constexpr int kStages = 1;
+constexpr int kPairWarps = 4;           // of the form with a cluster per pair: two CTAs per SM
+constexpr size_t kPairSmem = 80 * 1024;
 constexpr int kTileBytes = 8192;        // one of K, V
 template <int D>
 struct Mma {
@@ -377,7 +377,6 @@ struct MmaArgs {
   uint32_t q_flip;         // sign bits to flip in q for a negative scale
   __nv_bfloat16* o;
   float* work;             // [CTAs][2][rows][D + 2]
-  int stages;
   int tile_units, end_units;   // list form: cost of a tile and of a pair's end
 };
 
@@ -429,9 +428,8 @@ struct Worker {
   using C = Mma<D>;
   const MmaArgs& a;
   const CUtensorMap *mk, *mv;
-  uint32_t ring;            // this warp's stages in shared memory
-  uint32_t bars;            // its mbarriers
-  int* masks;               // copied boxes of the tile in each stage
+  uint32_t tile;            // this warp's tile in shared memory: keys, then values
+  uint32_t bar;             // its mbarrier
   int lane;
 
   __device__ __forceinline__ void enter_row(Cursor& c) const {
@@ -463,19 +461,15 @@ struct Worker {
     return Box{a.table[c.b * a.table_stride + j], key - j * a.ps};
   }
 
-  // Start the copies of the cursor's tile into stage s.
-  __device__ __forceinline__ void issue(const Cursor& c, const Box& x, int s) const {
+  // Start the copies of the cursor's tile; returns which of its boxes are copied.
+  __device__ __forceinline__ uint32_t issue(const Cursor& c, const Box& x) const {
     const bool here = x.off >= 0 && (unsigned)x.page < (unsigned)a.P;
     const uint32_t mask = __ballot_sync(0xffffffffu, here);
-    const uint32_t bar = bars + 8 * s;
     const uint32_t box = a.R * 128;
-    if (lane == 0) {
-      masks[s] = (int)mask;
-      sm100::mbar_expect_tx(bar, __popc(mask) * box * (D / 64) * 2);
-    }
+    if (lane == 0) sm100::mbar_expect_tx(bar, __popc(mask) * box * (D / 64) * 2);
     __syncwarp();
     if (here) {
-      const uint32_t dst = ring + s * 2 * kTileBytes + lane * box;
+      const uint32_t dst = tile + lane * box;
 #pragma unroll
       for (int half = 0; half < D / 64; ++half) {
         sm100::tma_load_4d(dst + half * C::KT * 128, mk, half * 64, x.off, c.hk, x.page, bar);
@@ -485,16 +479,13 @@ struct Worker {
       record_device_error(ENGPT_ERR_ARG, 44);
     }
     __syncwarp();
+    return mask;
   }
 
   // A wait ran out: let the copies still in flight land (bounded) before the CTA's shared memory goes away.
-  __device__ __forceinline__ void drain(int next, int in_flight, uint32_t phases) const {
-    for (int i = 0; i < in_flight; ++i) {
-      const int s = (next + i) % a.stages;
-      const uint64_t t0 = globaltimer_ns();
-      while (!sm100::mbar_try_wait_sleep(bars + 8 * s, (phases >> s) & 1u, 100000u) &&
-             globaltimer_ns() - t0 < kWaitLimitNs) {
-      }
+  __device__ __forceinline__ void drain(uint32_t phase) const {
+    const uint64_t t0 = globaltimer_ns();
+    while (!sm100::mbar_try_wait_sleep(bar, phase, 100000u) && globaltimer_ns() - t0 < kWaitLimitNs) {
     }
   }
 };
@@ -613,7 +604,7 @@ __device__ __forceinline__ void tile_step(const MmaArgs& a, uint32_t sk, const u
       mma16816(st.o[2 * dp + 1], hi[j][0], lo[j][0], hi[j][1], lo[j][1], b[dp][2], b[dp][3]);
     }
   }
-  if (!WHOLE) sm100::fence_proxy_async_smem();   // the zeros above, before a later copy into this stage
+  if (!WHOLE) sm100::fence_proxy_async_smem();   // the zeros above, before a later copy into this memory
 }
 
 // The pair's sums of this lane: o (both halves of the operand added) and l over the row's four lanes; m in base-2 units.
@@ -781,21 +772,17 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(MmaArgs a, con
   using C = Mma<D>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (sm100::smem_u32(smem_raw) + 1023u) & ~1023u;
-  uint8_t* ring_ptr = smem_raw + (base - sm100::smem_u32(smem_raw));
-  const int ring_bytes = a.stages * 2 * kTileBytes;
-  uint8_t* tail = ring_ptr + kWarps * ring_bytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(tail);                       // [kWarps][stages]
+  uint8_t* tiles = smem_raw + (base - sm100::smem_u32(smem_raw));           // one of each warp
+  uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + kWarps * 2 * kTileBytes);   // [kWarps]
   const int pf = part_floats<D>(a.rows);
-  float* s_part = reinterpret_cast<float*>(bars + kWarps * a.stages);       // [kWarps] first part of each warp
-  int* masks = reinterpret_cast<int*>(s_part + kWarps * pf);                // [kWarps][stages]
-  int* s_start = masks + kWarps * a.stages;                                 // [B + 1] first tile of each row
+  float* s_part = reinterpret_cast<float*>(bars + kWarps);                  // [kWarps] first part of each warp
+  int* s_start = reinterpret_cast<int*>(s_part + kWarps * pf);              // [B + 1] first unit of each row
   __shared__ int s_abort, s_scan[kWarps], s_head[kWarps], s_tail[kWarps], s_over[kWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  Worker<D> w{a, &mk, &mv, base + warp * ring_bytes, sm100::smem_u32(bars + warp * a.stages), masks + warp * a.stages,
-              lane};
+  Worker<D> w{a, &mk, &mv, base + warp * 2 * kTileBytes, sm100::smem_u32(bars + warp), lane};
   if (lane == 0) {
-    for (int s = 0; s < a.stages; ++s) sm100::mbar_init(w.bars + 8 * s, 1);
+    sm100::mbar_init(w.bar, 1);
     sm100::fence_mbar_init();
     s_abort = 0;         // (every warp: a wait may set it only seconds later)
     s_head[warp] = s_tail[warp] = -1;
@@ -834,17 +821,14 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(MmaArgs a, con
     w.advance(c);
   }
 
-  // fill the ring: ci is the next tile to fetch
+  // the first tile's copies; ci is the next tile to fetch, box its place
   Cursor ci = c;
-  Box box = ci.u < u1 ? w.find_box(ci) : Box{0, -1};
-  int in_flight = 0;
-  for (; in_flight < a.stages && ci.u < u1; ++in_flight) {
-    Cursor cn = ci;
-    w.advance(cn);
-    const Box next = cn.u < u1 ? w.find_box(cn) : Box{0, -1};
-    w.issue(ci, box, in_flight);
-    ci = cn;
-    box = next;
+  uint32_t mask = 0;
+  Box box{0, -1};
+  if (c.u < u1) {
+    mask = w.issue(ci, w.find_box(ci));
+    w.advance(ci);
+    if (ci.u < u1) box = w.find_box(ci);
   }
 
   // the joining kernel may start: it reads nothing of this one before this one has ended
@@ -859,40 +843,35 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(MmaArgs a, con
   }
 
   float* part = s_part + warp * pf;                                         // a pair that began before this range
-  float* tail_part = reinterpret_cast<float*>(ring_ptr + warp * ring_bytes);   // one that ends behind it (ring unused)
+  float* tail_part = reinterpret_cast<float*>(tiles + warp * 2 * kTileBytes);   // one that ends behind it (no tile left)
   State<D> st;
   st.reset();
   uint32_t qa[C::DK][2];
-  uint32_t phases = 0;
+  uint32_t phase = 0;
   bool fresh = true;                // the next tile begins a segment
   int t0 = 0;
-  int s = 0;
   while (c.u < u1) {
     if (fresh) {
       load_query<D>(a, c.b, c.h, lane, qa);
       t0 = c.t;
       fresh = false;
     }
-    if (!__all_sync(0xffffffffu, sm100::mbar_wait(w.bars + 8 * s, (phases >> s) & 1u, &s_abort, 45))) {
-      w.drain(s, in_flight, phases);
+    if (!__all_sync(0xffffffffu, sm100::mbar_wait(w.bar, phase, &s_abort, 45))) {
+      w.drain(phase);
       break;   // (the pair keeps no part of this warp: its rows are wrong, and the status word says so)
     }
-    phases ^= 1u << s;
-    const uint32_t sk = w.ring + s * 2 * kTileBytes, mask = (uint32_t)w.masks[s];
+    phase ^= 1u;
     const int live = c.len - c.t * C::KT;
     if (live >= C::KT && mask == (1u << (C::KT >> a.r_shift)) - 1u)
-      tile_step<D, true>(a, sk, qa, st, live, mask, lane);
+      tile_step<D, true>(a, w.tile, qa, st, live, mask, lane);
     else
-      tile_step<D, false>(a, sk, qa, st, live, mask, lane);
+      tile_step<D, false>(a, w.tile, qa, st, live, mask, lane);
     __syncwarp();
-    --in_flight;
     if (ci.u < u1) {
-      w.issue(ci, box, s);
-      ++in_flight;
+      mask = w.issue(ci, box);
       w.advance(ci);
-      box = ci.u < u1 ? w.find_box(ci) : Box{0, -1};
+      if (ci.u < u1) box = w.find_box(ci);
     }
-    if (++s == a.stages) s = 0;
     const bool pair_end = c.t + 1 == c.T;
     Cursor cn = c;
     w.advance(cn);
@@ -901,7 +880,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(MmaArgs a, con
       if (t0 == 0 && pair_end) {
         store_rows<D>(a, st, c.b, c.h, lane);
       } else if (t0 == 0) {
-        store_part<D>(a, st, tail_part, lane);   // the last tile of the range: every stage has been read
+        store_part<D>(a, st, tail_part, lane);   // the last tile of the range: nothing is being copied
         if (lane == 0) {
           s_tail[warp] = c.b * a.HQ + c.h;
           // does its last tile begin behind this CTA's units?
@@ -928,7 +907,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(MmaArgs a, con
     const int w0 = max(g, 0);
     int n = g < 0 ? 0 : 1;
     while (w0 + n < kWarps && s_head[w0 + n] == pair) ++n;
-    const float* first = g < 0 ? s_part : reinterpret_cast<const float*>(ring_ptr + g * ring_bytes);
+    const float* first = g < 0 ? s_part : reinterpret_cast<const float*>(tiles + g * 2 * kTileBytes);
     const float* rest = s_part + g * pf;
     float* to = g < 0 ? out : (s_over[g] ? out + pf : nullptr);   // at most one pair runs over the CTA's end
     const int b = pair / a.HQ, h = pair - b * a.HQ;
@@ -952,28 +931,25 @@ __global__ void __launch_bounds__(kPairWarps * 32) decode_pair_kernel(MmaArgs a,
   using C = Mma<D>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (sm100::smem_u32(smem_raw) + 1023u) & ~1023u;
-  uint8_t* ring_ptr = smem_raw + (base - sm100::smem_u32(smem_raw));
-  const int ring_bytes = a.stages * 2 * kTileBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring_ptr + kPairWarps * ring_bytes);   // [kPairWarps][stages]
+  uint8_t* tiles = smem_raw + (base - sm100::smem_u32(smem_raw));           // one of each warp
+  uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + kPairWarps * 2 * kTileBytes);  // [kPairWarps]
   const int pf = part_floats<D>(a.rows);
-  float* s_part = reinterpret_cast<float*>(bars + kPairWarps * a.stages);             // [kPairWarps] the warps' parts
-  float* s_cta = s_part + kPairWarps * pf;                                            // [cs] the CTAs' parts (rank 0)
-  int* masks = reinterpret_cast<int*>(s_cta + cs * pf);                           // [kPairWarps][stages]
+  float* s_part = reinterpret_cast<float*>(bars + kPairWarps);              // [kPairWarps] the warps' parts
+  float* s_cta = s_part + kPairWarps * pf;                                  // [cs] the CTAs' parts (rank 0)
   __shared__ int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (cs > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
   const int pair = blockIdx.x / cs, rank = blockIdx.x - pair * cs;
   const int me = rank * kPairWarps + warp, step = cs * kPairWarps;
-  Worker<D> w{a, &mk, &mv, base + warp * ring_bytes, sm100::smem_u32(bars + warp * a.stages), masks + warp * a.stages,
-              lane};
+  Worker<D> w{a, &mk, &mv, base + warp * 2 * kTileBytes, sm100::smem_u32(bars + warp), lane};
   Cursor c;
   c.b = pair / a.HQ;
   c.h = pair - c.b * a.HQ;
   c.hk = c.h / a.QG;
   c.t = me;
   if (lane == 0) {
-    for (int s = 0; s < a.stages; ++s) sm100::mbar_init(w.bars + 8 * s, 1);
+    sm100::mbar_init(w.bar, 1);
     sm100::fence_mbar_init();
     s_abort = 0;                        // (every warp: a wait may set it only seconds later)
     if (warp == 0) {
@@ -994,37 +970,35 @@ __global__ void __launch_bounds__(kPairWarps * 32) decode_pair_kernel(MmaArgs a,
   if (c.t * C::KT + lane * a.R >= c.len) box.off = -1;
   const int n = c.T > me ? (c.T - me + step - 1) / step : 0;   // this warp's tiles
   Cursor ci = c;
-  for (int i = 0; i < min(n, a.stages); ++i) {
-    w.issue(ci, box, i);
+  uint32_t mask = 0;
+  if (n > 0) {
+    mask = w.issue(ci, box);
     ci.t += step;
-    box = i + 1 < n ? w.find_box(ci) : Box{0, -1};
+    if (n > 1) box = w.find_box(ci);
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   State<D> st;
   st.reset();
-  uint32_t phases = 0;
+  uint32_t phase = 0;
   bool ok = true;
-  int s = 0;
   for (int i = 0; i < n; ++i, c.t += step) {
-    if (!__all_sync(0xffffffffu, sm100::mbar_wait(w.bars + 8 * s, (phases >> s) & 1u, &s_abort, 46))) {
-      w.drain(s, min(n - i, a.stages), phases);
+    if (!__all_sync(0xffffffffu, sm100::mbar_wait(w.bar, phase, &s_abort, 46))) {
+      w.drain(phase);
       ok = false;
       break;
     }
-    phases ^= 1u << s;
-    const uint32_t sk = w.ring + s * 2 * kTileBytes, mask = (uint32_t)w.masks[s];
+    phase ^= 1u;
     const int live = c.len - c.t * C::KT;
     if (live >= C::KT && mask == (1u << (C::KT >> a.r_shift)) - 1u)
-      tile_step<D, true>(a, sk, qa, st, live, mask, lane);
+      tile_step<D, true>(a, w.tile, qa, st, live, mask, lane);
     else
-      tile_step<D, false>(a, sk, qa, st, live, mask, lane);
+      tile_step<D, false>(a, w.tile, qa, st, live, mask, lane);
     __syncwarp();
-    if (i + a.stages < n) {
-      w.issue(ci, box, s);
+    if (i + 1 < n) {
+      mask = w.issue(ci, box);
       ci.t += step;
-      box = i + a.stages + 1 < n ? w.find_box(ci) : Box{0, -1};
+      if (i + 2 < n) box = w.find_box(ci);
     }
-    if (++s == a.stages) s = 0;
   }
   finish_rows<D>(a, st);
 
@@ -1208,13 +1182,15 @@ inline int64_t mma_floats(int H, int Hkv, int D) {
 
 template <int D>
 size_t mma_smem(const MmaArgs& a, int warps, int parts) {
-  return 1024 + (size_t)warps * a.stages * (2 * kTileBytes + 12) + 4 * (size_t)parts * part_floats<D>(a.rows);
+  return 1024 + (size_t)warps * (2 * kTileBytes + 8) + 4 * (size_t)parts * part_floats<D>(a.rows);
 }
 
 template <int D>
 int launch_pair(const MmaArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int cs, cudaStream_t st) {
   auto kern = decode_pair_kernel<D>;
-  const size_t smem = mma_smem<D>(a, kPairWarps, kPairWarps + cs);
+  // Two CTAs per SM and no third one, which would leave other SMs idle (one wave has at most two per SM; 128 pairs of 32
+  // tiles: 15.2 us so, 16.5 if three fit).
+  const size_t needed = mma_smem<D>(a, kPairWarps, kPairWarps + cs), smem = needed > kPairSmem ? needed : kPairSmem;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((int64_t)a.B * a.HQ * cs));
@@ -1294,7 +1270,6 @@ int launch_mma(const AttnArgs& x, int Hkv, cudaStream_t st) {
   if ((rc = page_map(&mk, x.k_pages, x.Dh, x.ps, Hkv, x.P, x.ks, a.R))) return rc;
   if ((rc = page_map(&mv, x.v_pages, x.Dh, x.ps, Hkv, x.P, x.vs, a.R))) return rc;
   const int cs = pair_ctas(x.B, x.H, Hkv, D, x.W, x.ps);
-  a.stages = kStages;
   // The end of a pair costs a worker about half a tile (its sums and stores, and tiles that are partly empty).  It is
   // counted once workers see such ends often (256 rows of 1 to 512 tokens: 51.8 us, 63.8 without); with few pairs the
   // ranges are whole tiles, which cuts fewer pairs (32 rows of 512 tokens, 16 heads: 16.9 us, 18.5 with).

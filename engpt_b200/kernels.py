@@ -406,6 +406,8 @@ def paged_sdpa(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: Tensor,
     query head ``h`` reads kv head ``h // (H // kv_heads)``.  A row of length 0
     gives zeros.  Whatever lies in the cache behind a row's length (stale or
     NaN) has no effect.  ``k_pages`` and ``v_pages`` are ``[num_pages, kv_heads,
-    page_size, Dh]`` with any strides and a contiguous last axis.
+    page_size, Dh]`` with any strides and a contiguous last axis, ``Dh`` at most
+    256.  bf16 with ``Dh`` up to 128 and a multiple of 8, pages of a multiple of 8
+    tokens and 16-byte aligned strides runs on the tensor cores.
     """
     return _lib.native().paged_sdpa(q, k_pages, v_pages, block_table, lengths, scale)

@@ -362,7 +362,8 @@ def advance_block_tables(lengths: Tensor, new_tokens: Tensor, block_table: Tenso
     empty; then every row takes the pages that ``new_tokens[b]`` more tokens
     need, rows in order.  ``slots`` and ``positions`` are int32 ``[B,
     max_new]``: a token's place in the cache (``page * page_size + offset``)
-    and in its sequence; ``-1`` and 0 behind a row's last new token.
+    and in its sequence; ``-1`` and 0 behind a row's last new token.  At most 8192
+    rows.
 
     A row whose request cannot be met (more than ``max_new`` tokens, a table
     row too short, no pages left) is refused whole: its length stays, its

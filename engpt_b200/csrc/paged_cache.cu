@@ -213,30 +213,53 @@ struct WriteArgs {
   void* v_pages;
   int64_t ks[3], vs[3];
   int64_t n_slots;
-  int ps;
+  int ps, ps_shift;   // ps_shift: log2(page size), or -1
 };
 
-// One thread per V-sized piece of a (token, head) row, for k and v.  V: uint4 (16 bytes), or the element itself.
-template <typename V>
+// 32768 tokens of 16 heads of 64 in bf16 (269 MB): 42.3 us = 6.36 TB/s with two pieces and 8 CTAs per SM; 46.7 with one
+// piece, 46.1 with four, 45.4 with 32 CTAs.
+constexpr int kWriteUnroll = 2, kWriteCtas = 8;
+
+// One thread per V-sized piece of a (token, head) row, for k and v, U pieces a grid apart at a time: all their slots,
+// then all their loads are in flight before the first store.  V: uint4 (16 bytes), or the element itself.
+template <typename V, int U>
 __global__ void __launch_bounds__(256) write_pages_kernel(WriteArgs a, int pieces, int esz) {
-  const int64_t per_row = (int64_t)a.H * pieces;
-  const int64_t total = a.n * per_row;
-  const int64_t step = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += step) {
-    const int64_t row = i / per_row;
-    const int rest = (int)(i - row * per_row);
-    const int h = rest / pieces, c = rest - h * pieces;
-    const int slot = a.slots[row];
-    if (slot < 0 || slot >= a.n_slots) {
-      if (slot != -1) record_device_error(ENGPT_ERR_ARG, 43);
-      continue;
+  const uint32_t per_row = (uint32_t)a.H * pieces;
+  const int64_t total = a.n * per_row, step = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t i0 = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i0 < total; i0 += U * step) {
+    int slot[U];
+    int64_t row[U];
+    int h[U], c[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = i0 + u * step;
+      row[u] = total <= 0xffffffffLL ? (uint32_t)i / per_row : i / per_row;
+      const uint32_t rest = (uint32_t)(i - row[u] * per_row);
+      h[u] = (int)(rest / (uint32_t)pieces);
+      c[u] = (int)(rest - h[u] * (uint32_t)pieces);
+      slot[u] = i < total ? a.slots[row[u]] : -1;
     }
-    const int page = slot / a.ps, off = slot - page * a.ps;
-    const int64_t byte = (int64_t)c * sizeof(V);
-    const V kv = *reinterpret_cast<const V*>((const char*)a.k + (row * a.k_row + h * a.k_head) * esz + byte);
-    const V vv = *reinterpret_cast<const V*>((const char*)a.v + (row * a.v_row + h * a.v_head) * esz + byte);
-    *reinterpret_cast<V*>((char*)a.k_pages + (page * a.ks[0] + h * a.ks[1] + off * a.ks[2]) * esz + byte) = kv;
-    *reinterpret_cast<V*>((char*)a.v_pages + (page * a.vs[0] + h * a.vs[1] + off * a.vs[2]) * esz + byte) = vv;
+    V kv[U], vv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (slot[u] >= 0 && slot[u] < a.n_slots) {
+        const int64_t byte = (int64_t)c[u] * sizeof(V);
+        kv[u] = *reinterpret_cast<const V*>((const char*)a.k + (row[u] * a.k_row + h[u] * a.k_head) * esz + byte);
+        vv[u] = *reinterpret_cast<const V*>((const char*)a.v + (row[u] * a.v_row + h[u] * a.v_head) * esz + byte);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (slot[u] >= 0 && slot[u] < a.n_slots) {
+        const int page = a.ps_shift >= 0 ? slot[u] >> a.ps_shift : slot[u] / a.ps;
+        const int off = slot[u] - page * a.ps;
+        const int64_t byte = (int64_t)c[u] * sizeof(V);
+        *reinterpret_cast<V*>((char*)a.k_pages + (page * a.ks[0] + h[u] * a.ks[1] + off * a.ks[2]) * esz + byte) = kv[u];
+        *reinterpret_cast<V*>((char*)a.v_pages + (page * a.vs[0] + h[u] * a.vs[1] + off * a.vs[2]) * esz + byte) = vv[u];
+      } else if (slot[u] != -1) {
+        record_device_error(ENGPT_ERR_ARG, 43);
+      }
+    }
   }
 }
 
@@ -319,6 +342,7 @@ extern "C" int engpt_write_kv_pages(const void* k, const void* v, const int64_t*
   a.v_pages = v_pages;
   a.n_slots = (int64_t)num_pages * page_size;
   a.ps = page_size;
+  a.ps_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size) : -1;
   bool vec = Dh * esz % 16 == 0 && aligned(k, 16) && aligned(v, 16) && aligned(k_pages, 16) && aligned(v_pages, 16);
   for (int i = 0; i < 4; ++i) vec = vec && kv_strides[i] * esz % 16 == 0;
   for (int i = 0; i < 3; ++i) {
@@ -328,11 +352,12 @@ extern "C" int engpt_write_kv_pages(const void* k, const void* v, const int64_t*
   }
   const int pieces = vec ? Dh * esz / 16 : Dh;
   const int64_t total = n * H * pieces;
-  const int64_t want = (total + 255) / 256, cap = (int64_t)num_sms() * 16;
+  ENGPT_REQUIRE((int64_t)H * pieces <= 0x7fffffffLL, ENGPT_ERR_SHAPE, "write_kv_pages: H=%d Dh=%d", H, Dh);
+  const int64_t want = (total + 255) / 256, cap = (int64_t)num_sms() * kWriteCtas;
   const unsigned blocks = (unsigned)(want < cap ? want : cap);
   cudaStream_t st = as_stream(stream);
-  if (vec) write_pages_kernel<uint4><<<blocks, 256, 0, st>>>(a, pieces, esz);
-  else if (esz == 2) write_pages_kernel<unsigned short><<<blocks, 256, 0, st>>>(a, pieces, esz);
-  else write_pages_kernel<float><<<blocks, 256, 0, st>>>(a, pieces, esz);
+  if (vec) write_pages_kernel<uint4, kWriteUnroll><<<blocks, 256, 0, st>>>(a, pieces, esz);
+  else if (esz == 2) write_pages_kernel<unsigned short, 1><<<blocks, 256, 0, st>>>(a, pieces, esz);
+  else write_pages_kernel<float, 1><<<blocks, 256, 0, st>>>(a, pieces, esz);
   return check_launch("write_kv_pages");
 }

@@ -114,9 +114,11 @@ class PagedDecoder:
     """Generates from ``model`` for up to ``max_batch`` requests at a time (see the module's text).
 
     ``dtype`` is the compute type: bfloat16 (as the model under bf16 autocast)
-    or float32.  In bfloat16 the decoder holds its own copies of the linear
-    weights, made when it is built: call ``refresh_weights()`` after the
-    model's parameters have changed.  Requests are rows ``0 .. max_batch - 1``.
+    or float32.  Steps use the parameters that the decoder took when it was built
+    or last refreshed (in bfloat16 its own copies of the linear weights, in both
+    types its own scaled copy of the head): call ``refresh_weights()`` after the
+    model's parameters have changed, in place or for other tensors.  Requests are
+    rows ``0 .. max_batch - 1``.
     """
 
     def __init__(self, model, max_batch: int, num_pages: int, *, page_size: int = 64, max_len: Optional[int] = None,
@@ -136,28 +138,55 @@ class PagedDecoder:
         self._graph: Optional[_StepGraph] = None
         self.cuda_graphs = False
         self._ones = torch.ones(max_batch, dtype=torch.int32, device=p.device)
-        self._w: List[dict] = []
-        self._w_head = torch.empty(0)
+        # what a step reads of each block, and the embedding: held here, so that neither an eager step nor a captured
+        # one can read a tensor that the model has given up, and a step's parameters are all of one refresh
+        self._w: List[dict] = [{} for _ in model.blocks]
+        self._emb = torch.empty(0)
+        self._w_head = torch.zeros(-(-model.cfg.vocab_size // 64) * 64, model.cfg.n_embd, device=self.device,
+                                   dtype=dtype)
         self.refresh_weights()
+
+    def _take(self, name: str, p: Tensor, *shape: int) -> Tensor:
+        if p.device != self.device or p.dtype != torch.float32 or tuple(p.shape) != shape:
+            raise ValueError(f"{name} must be float32 {list(shape)} on {self.device}, got {p.dtype} {list(p.shape)} on "
+                             f"{p.device}")
+        return p.detach().contiguous()
 
     @torch.no_grad()
     def refresh_weights(self) -> None:
-        """Take the model's current parameters (in float32 the linear weights are used in place)."""
+        """Take the model's current parameters (in float32 all but the head are used in place).
+
+        A captured step is captured again if a parameter that it reads in place
+        has become another tensor.
+        """
         m, cfg = self.model, self.cfg
-        names = ("qkv", "out_proj", "up_gate", "down_proj")
-        if not self._w:
-            bf16 = self.dtype == torch.bfloat16
-            self._w = [{n: torch.empty_like(getattr(b, n).weight, dtype=self.dtype) if bf16
-                        else getattr(b, n).weight.detach() for n in names} for b in m.blocks]
-            self._w_head = torch.zeros(-(-cfg.vocab_size // 64) * 64, cfg.n_embd, device=self.device, dtype=self.dtype)
+        d, width = cfg.n_embd, cfg.mlp_width
+        linear = {"qkv": (3 * d, d), "out_proj": (d, d), "up_gate": (2 * width, d), "down_proj": (d, width)}
+        small = {"s_qk": (cfg.n_head, cfg.head_dim), "s_u": (width,), "s_gate": (width,), "alpha_attn_raw": (d,),
+                 "alpha_mlp_raw": (d,)}
+        # everything is looked at before anything is taken
+        emb = self._take("token_emb.weight", m.token_emb.weight, cfg.vocab_size, d)
+        out = self._take("output_emb", m.output_emb, cfg.vocab_size, d)
+        s_z = self._take("s_z", m.s_z, cfg.vocab_size)
+        taken = []
+        for i, b in enumerate(m.blocks):
+            taken.append({n: self._take(f"blocks.{i}.{n}.weight", getattr(b, n).weight, *s) for n, s in linear.items()})
+            taken[i].update((n, self._take(f"blocks.{i}.{n}", getattr(b, n), *s)) for n, s in small.items())
         if self.dtype == torch.bfloat16:
-            for w, b in zip(self._w, m.blocks):
-                for n in names:
-                    w[n].copy_(getattr(b, n).weight)
+            for old, new in zip(self._w, taken):
+                for n in linear:
+                    new[n] = old[n].copy_(new[n]) if old else new[n].to(self.dtype)
+        if self._addresses(emb, taken) != self._addresses(self._emb, self._w):
+            self._graph = None
+        self._emb, self._w = emb, taken
         with torch.cuda.device(self.device):
-            _lib.call("engpt_scale_rows_cast", m.output_emb.data_ptr(), m.s_z.data_ptr(), float(m.logit_mult),
+            _lib.call("engpt_scale_rows_cast", out.data_ptr(), s_z.data_ptr(), float(m.logit_mult),
                       cfg.vocab_size, cfg.n_embd, self._w_head.data_ptr(), _lib.dtype_code(self.dtype),
                       _lib.stream_handle(self.device))
+
+    @staticmethod
+    def _addresses(emb: Tensor, blocks: List[dict]) -> List[int]:
+        return [emb.data_ptr()] + [t.data_ptr() for b in blocks for t in b.values()]
 
     # ---------------------------------------------------------------- requests
     def _rows_mask(self, rows: Sequence[int]) -> Tuple[List[int], Tensor]:
@@ -250,7 +279,7 @@ class PagedDecoder:
         hidden = torch.empty(b, width, device=self.device, dtype=self.dtype)
         slots, positions = cache.advance(new_tokens, 1)
         slots, positions = slots.view(b), positions.view(b)
-        _lib.call("engpt_embed_carried", idx.data_ptr(), m.token_emb.weight.data_ptr(), b, d, cfg.vocab_size,
+        _lib.call("engpt_embed_carried", idx.data_ptr(), self._emb.data_ptr(), b, d, cfg.vocab_size,
                   y.data_ptr(), rho.data_ptr(), x.data_ptr() if bf16 else None, st)
         scale, sqrt_d = K.ngpt_attention_scale(dim), math.sqrt(float(d))
         u_mult = sqrt_d if cfg.scale_mlp_u_by_sqrt_d else 1.0
@@ -258,19 +287,19 @@ class PagedDecoder:
         last = cfg.n_layer - 1
         for i, (blk, w) in enumerate(zip(m.blocks, self._w)):
             qkv = torch.mm(x, w["qkv"].t()).view(b, 3, heads, dim)
-            q = K.qkv_append_from_carried(qkv, rho, self.cos, self.sin, blk.s_qk.detach(), cfg.norm_eps, positions,
+            q = K.qkv_append_from_carried(qkv, rho, self.cos, self.sin, w["s_qk"], cfg.norm_eps, positions,
                                           slots, cache.k_pages[i], cache.v_pages[i], qk_mult=blk.qk_mult)
             attn = K.paged_sdpa(q, cache.k_pages[i], cache.v_pages[i], cache.block_table, cache.lengths, scale=scale)
             branch = torch.mm(attn.view(b, d), w["out_proj"].t())
-            K.carried_residual_into(y, rho, branch, blk.alpha_attn_raw, blk.alpha_mult, True, cfg.norm_eps,
+            K.carried_residual_into(y, rho, branch, w["alpha_attn_raw"], blk.alpha_mult, True, cfg.norm_eps,
                                     cfg.norm_eps, cfg.carried_gauge_max, y, rho, h, aux_h)
             ug = torch.mm(h, w["up_gate"].t())
-            _lib.call("engpt_swiglu", ug.data_ptr(), act, blk.s_u.data_ptr(), blk.s_gate.data_ptr(), float(u_mult),
+            _lib.call("engpt_swiglu", ug.data_ptr(), act, w["s_u"].data_ptr(), w["s_gate"].data_ptr(), float(u_mult),
                       float(sqrt_d), b, width, hidden.data_ptr(), act, st)
             branch = torch.mm(hidden, w["down_proj"].t())
             # what comes next reads Y (the next layer's QKV) or Y / rho (the head)
             aux = aux_h if i == last else (_lib.AUX_BF16_Y if bf16 else _lib.AUX_NONE)
-            K.carried_residual_into(y, rho, branch, blk.alpha_mlp_raw, blk.alpha_mult, True, cfg.norm_eps,
+            K.carried_residual_into(y, rho, branch, w["alpha_mlp_raw"], blk.alpha_mult, True, cfg.norm_eps,
                                     cfg.norm_eps, cfg.carried_gauge_max, y, rho,
                                     None if aux == _lib.AUX_NONE else h, aux)
         return torch.mm(h, self._w_head.t())[:, :cfg.vocab_size]

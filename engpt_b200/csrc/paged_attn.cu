@@ -1353,7 +1353,8 @@ extern "C" int engpt_paged_attention(const void* q, const int64_t* q_strides, co
     positive = positive && a.ks[i] > 0 && a.vs[i] > 0;
   }
   cudaStream_t st = as_stream(stream);
-  if (vec && positive && num_pages > 0 && mma_sizes(dtype, B, H, Hkv, Dh, table_width, page_size))
+  // (the tensor-core kernels write o in pieces of up to 16 bytes, the others element by element)
+  if (vec && positive && aligned(o, 16) && num_pages > 0 && mma_sizes(dtype, B, H, Hkv, Dh, table_width, page_size))
     return mma_width(Dh) == 64 ? launch_mma<64>(a, Hkv, st) : launch_mma<128>(a, Hkv, st);
   return dtype == ENGPT_BF16 ? dispatch_simt<__nv_bfloat16>(a, vec, st) : dispatch_simt<float>(a, vec, st);
 }

@@ -396,7 +396,9 @@ ENGPT_API int engpt_write_kv_pages(const void* k, const void* v, const int64_t* 
  * o[b, h] = sum_j softmax_j(scale q[b, h] . k_j) v_j over the first lengths[b]
  * tokens of request b, query head h reading kv head h / (H / Hkv).  q [B, H,
  * Dh] with element strides q_strides (2 int64: row, head), o [B, H, Dh]
- * contiguous.  A row of length 0 (or below) gives zeros; what lies in the
+ * contiguous; the tensor cores are used where all addresses, o's too, and
+ * strides are multiples of 16 bytes (bf16, Dh <= 128 and a multiple of 8,
+ * page_size a multiple of 8).  A row of length 0 (or below) gives zeros; what lies in the
  * cache behind a row's length is never used.  A length above table_width *
  * page_size (at most 2^31 - 4097) or a page outside the pool is recorded
  * (ENGPT_ERR_ARG, site 44) and its keys count as absent.  Dh <= 256.  workspace: scratch of

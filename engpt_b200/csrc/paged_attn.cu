@@ -607,7 +607,11 @@ __device__ __forceinline__ void tile_step(const MmaArgs& a, uint32_t sk, const u
   if (!WHOLE) sm100::fence_proxy_async_smem();   // the zeros above, before a later copy into this memory
 }
 
-// The pair's sums of this lane: o (both halves of the operand added) and l over the row's four lanes; m in base-2 units.
+// The two halves of the operand added: (sum of bf16(p) v) + (sum of (p - bf16(p)) v).  Where a value is infinite the
+// first half is the result; the second one, with weights of either sign or 0, would turn it into NaN.
+__device__ __forceinline__ float add_halves(float hi, float lo) { return fabsf(hi) == INFINITY ? hi : hi + lo; }
+
+// The pair's sums of this lane: o (both halves) and l over the row's four lanes; m in base-2 units.
 template <int D>
 __device__ __forceinline__ void finish_rows(const MmaArgs& a, State<D>& st) {
   st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
@@ -615,8 +619,8 @@ __device__ __forceinline__ void finish_rows(const MmaArgs& a, State<D>& st) {
   if (st.m != -INFINITY) st.m *= a.scale_log2;
 #pragma unroll
   for (int i = 0; i < Mma<D>::DN; ++i) {
-    st.o[i][0] += st.o[i][2];
-    st.o[i][1] += st.o[i][3];
+    st.o[i][0] = add_halves(st.o[i][0], st.o[i][2]);
+    st.o[i][1] = add_halves(st.o[i][1], st.o[i][3]);
   }
 }
 

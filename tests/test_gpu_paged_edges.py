@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from engpt_b200 import _lib, kernels as K
+from tests import paged_ref as R
 from tests.test_gpu_paged import _clean, attention_inputs, check_attention  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -46,3 +47,32 @@ def test_output_of_any_alignment(cuda, dtype, dim, lengths, shift):
     torch.cuda.synchronize()
     check_attention(args, out)
     assert (buf[:8 + shift] == 7.5).all() and (buf[8 + shift + n:] == 7.5).all()
+
+
+# ------------------------------------------------------------------ infinite values
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (2, 2, 128), (8, 1, 64), (2, 2, 48), (4, 1, 80)])
+@pytest.mark.parametrize("lengths", [[1, 33, 300], [1] * 5 + [17, 0, 64] * 30, [2500]])
+def test_infinite_values_in_use(cuda, dtype, heads, kv_heads, dim, lengths):
+    """An infinite element of a value makes that element of its heads' output infinite and no other; two of opposite
+    signs make it NaN.  The weights here are all far above the smallest normal number."""
+    q, kp, vp, table, lens, scale = attention_inputs(lengths, heads, kv_heads, dim, 16, dtype, seed=dim)
+    b = max(range(len(lengths)), key=lambda i: lengths[i])
+    n, inf = lengths[b], float("inf")
+    marks = [(0, 3, inf), (n - 1, 5, -inf), (n // 2, 5, -inf), (n // 3, dim - 1, inf), (n // 2, dim - 1, -inf)]
+    for key, e, x in marks:
+        vp[int(table[b, key // 16]), 0, key % 16, e] = x
+    if lengths[0] == 1:
+        vp[int(table[0, 0]), 0, 0, 7] = inf
+    out = K.paged_sdpa(q, kp, vp, table, lens, scale=scale).cpu().double()
+    group = heads // kv_heads
+    want = torch.zeros_like(out)
+    want[b, :group, 3], want[b, :group, 5], want[b, :group, dim - 1] = inf, -inf, float("nan")
+    if lengths[0] == 1:
+        want[0, :group, 7] = inf
+    marked = want != 0
+    assert torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(out[marked].nan_to_num(0.0), want[marked].nan_to_num(0.0))
+    ref, vmax, smax = R.attention(q, kp, vp.nan_to_num(nan=0.0, posinf=0.0, neginf=0.0), table, lens, scale)
+    tol = R.attention_tolerance(dtype, ref, vmax, smax, dim, max(lengths))
+    assert ((out - ref).abs() <= tol)[~marked].all()

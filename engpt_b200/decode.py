@@ -243,8 +243,9 @@ class PagedDecoder:
         """Append token ``idx[b]`` to every request and return the logits ``[max_batch, V]`` that follow it.
 
         ``active`` (bool ``[max_batch]``) leaves the other rows' requests as they
-        are; their logits mean nothing.  With CUDA graphs the returned logits are
-        overwritten by the next step.
+        are; their logits mean nothing.  A request that has ``block_size`` tokens
+        already, or fills the cache's capacity, is refused (``advance_block_tables``).  With
+        CUDA graphs the returned logits are overwritten by the next step.
         """
         b = self.cache.max_batch
         if tuple(idx.shape) != (b,):
@@ -277,6 +278,9 @@ class PagedDecoder:
         x = torch.empty(b, d, device=self.device, dtype=self.dtype) if bf16 else y
         h = x if bf16 else torch.empty_like(y)     # operand Y / rho of the MLP and the head
         hidden = torch.empty(b, width, device=self.device, dtype=self.dtype)
+        if cache.capacity > cfg.block_size:
+            # whole pages may leave room behind the block size: two tokens where one may be asked for are refused
+            new_tokens = torch.where(cache.lengths < cfg.block_size, new_tokens, 2 * new_tokens)
         slots, positions = cache.advance(new_tokens, 1)
         slots, positions = slots.view(b), positions.view(b)
         _lib.call("engpt_embed_carried", idx.data_ptr(), self._emb.data_ptr(), b, d, cfg.vocab_size,

@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from engpt_b200 import _lib
 from tests.helpers import seeded_model
 from tests.test_gpu_decode import CFGS, TOL, _clean, forward_logits, model_on, row_err, tokens  # noqa: F401
 
@@ -63,3 +64,27 @@ def test_refresh_refuses_other_types_and_shapes(cuda):
         dec.refresh_weights()
         dec.cache.reset()
         assert torch.equal(dec.step(idx[:, 0]), want)
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+def test_steps_stop_at_the_block_size(cuda, graphs):
+    """A cache of whole pages has room behind the model's block size; a step there is refused as a forward is."""
+    model = seeded_model(dict(CFGS["dh64"], block_size=20), 0).to(cuda).requires_grad_(False)
+    idx = tokens(CFGS["dh64"], (3, 21), 3)
+    full = forward_logits(model, idx[:, :20], torch.float32)
+    dec = model.decoder(3, 6, page_size=16, dtype=torch.float32)
+    assert dec.cache.capacity == 32
+    dec.enable_cuda_graphs(graphs)
+    dec.prefill(idx[:, :19], lengths=[19, 10, 19])
+    on = torch.tensor([True, True, False])
+    logits = dec.step(torch.stack([idx[0, 19], idx[1, 10], idx[2, 19]]), on)
+    assert row_err(logits[:1], full[0, 19][None]) < TOL[torch.float32]
+    assert row_err(logits[1:2], full[1, 10][None]) < TOL[torch.float32]
+    _lib.raise_on_device_status()
+    logits = dec.step(torch.stack([idx[0, 20], idx[1, 11], idx[2, 19]]), on)
+    assert dec.cache.lengths.tolist() == [20, 12, 19]
+    assert row_err(logits[1:2], full[1, 11][None]) < TOL[torch.float32]
+    with pytest.raises(_lib.EngptError, match="site 40"):
+        _lib.raise_on_device_status()
+    dec.step(torch.stack([idx[0, 20], idx[1, 12], idx[2, 19]]), torch.tensor([False, True, True]))
+    assert dec.cache.lengths.tolist() == [20, 13, 20]      # a full row that is not asked to grow is no error

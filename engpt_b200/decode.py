@@ -211,7 +211,8 @@ class PagedDecoder:
         ``lengths`` gives the prompts' lengths (1 to T, default T; what is behind
         them in ``idx`` is ignored but must be valid token ids).  Whatever the rows
         held before is released.  Returns the logits ``[n, V]`` after each prompt's
-        last token.
+        last token.  A prompt that finds too few pages is refused
+        (``advance_block_tables``): its row stays empty and its logits are zeros.
         """
         if idx.dim() != 2 or idx.shape[0] == 0 or idx.shape[1] == 0:
             raise ValueError("idx must have shape [requests, tokens]")
@@ -228,6 +229,7 @@ class PagedDecoder:
         with torch.cuda.device(self.device):
             slots, _ = cache.advance(new.to(self.device, non_blocking=True), seq_len, mask)
             slots = slots.index_select(0, torch.tensor(rows).to(self.device, non_blocking=True))
+            refused = slots[:, :1] < 0
             last = torch.tensor([b * seq_len + x - 1 for b, x in enumerate(lens)]).to(self.device, non_blocking=True)
 
             def keep(layer: int, k: Tensor, v: Tensor) -> None:
@@ -235,7 +237,7 @@ class PagedDecoder:
 
             with torch.autocast("cuda", dtype=torch.bfloat16, enabled=self.dtype == torch.bfloat16):
                 logits, _ = self.model._run(idx=idx, kv_callback=keep, head_rows=last)
-        return logits
+        return logits.masked_fill_(refused, 0.0)
 
     # ---------------------------------------------------------------- one token
     @torch.no_grad()
@@ -243,9 +245,10 @@ class PagedDecoder:
         """Append token ``idx[b]`` to every request and return the logits ``[max_batch, V]`` that follow it.
 
         ``active`` (bool ``[max_batch]``) leaves the other rows' requests as they
-        are; their logits mean nothing.  A request that has ``block_size`` tokens
-        already, or fills the cache's capacity, is refused (``advance_block_tables``).  With
-        CUDA graphs the returned logits are overwritten by the next step.
+        are; their logits are zeros.  A request that finds no page, has ``block_size``
+        tokens already or fills the cache's capacity is refused
+        (``advance_block_tables``): its token is not kept, its logits are zeros too.
+        With CUDA graphs the returned logits are overwritten by the next step.
         """
         b = self.cache.max_batch
         if tuple(idx.shape) != (b,):
@@ -306,6 +309,7 @@ class PagedDecoder:
             K.carried_residual_into(y, rho, branch, w["alpha_mlp_raw"], blk.alpha_mult, True, cfg.norm_eps,
                                     cfg.norm_eps, cfg.carried_gauge_max, y, rho,
                                     None if aux == _lib.AUX_NONE else h, aux)
+        h.masked_fill_((slots < 0).unsqueeze(1), 0.0)    # refused rows (and inactive ones)
         return torch.mm(h, self._w_head.t())[:, :cfg.vocab_size]
 
     # ---------------------------------------------------------------- generation

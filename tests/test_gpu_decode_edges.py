@@ -88,3 +88,29 @@ def test_steps_stop_at_the_block_size(cuda, graphs):
         _lib.raise_on_device_status()
     dec.step(torch.stack([idx[0, 20], idx[1, 12], idx[2, 19]]), torch.tensor([False, True, True]))
     assert dec.cache.lengths.tolist() == [20, 13, 20]      # a full row that is not asked to grow is no error
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_refused_rows_have_zero_logits(cuda, dtype):
+    """A prompt or a step that finds no pages: the row's cache is as the refusal left it, its logits are zeros, and the
+    other rows are served."""
+    model = model_on(cuda, "dh64")
+    idx = tokens(CFGS["dh64"], (3, 40), 6)
+    full = forward_logits(model, idx, dtype)
+    dec = model.decoder(3, 4, page_size=16, dtype=dtype)
+    logits = dec.prefill(idx[:, :30], lengths=[16, 30, 20]).float()      # one page, two, and two where one is left
+    assert dec.cache.lengths.tolist() == [16, 30, 0] and int(dec.cache.free_count) == 1
+    assert row_err(logits[:1], full[0, 15][None]) < TOL[dtype] and row_err(logits[1:2], full[1, 29][None]) < TOL[dtype]
+    assert (logits[2] == 0).all()
+    with pytest.raises(_lib.EngptError, match="site 41"):
+        _lib.raise_on_device_status()
+    dec.step(torch.tensor([0, 0, 0]), torch.tensor([True, False, False]))     # row 0 takes the last page
+    _lib.raise_on_device_status()
+    dec.release([0])
+    dec.prefill(idx[:1, :32], rows=[0])
+    logits = dec.step(torch.stack([idx[0, 32], idx[1, 30], idx[2, 0]])).float()
+    assert dec.cache.lengths.tolist() == [32, 31, 0]
+    assert (logits[0] == 0).all() and (logits[2] == 0).all()
+    assert row_err(logits[1:2], full[1, 30][None]) < TOL[dtype]
+    with pytest.raises(_lib.EngptError, match="site 41"):
+        _lib.raise_on_device_status()

@@ -352,6 +352,7 @@ constexpr int kWarps = 8;
 constexpr int kPairWarps = 4;           // of the form with a cluster per pair: two CTAs per SM
 constexpr size_t kPairSmem = 80 * 1024;
 constexpr int kTileBytes = 8192;        // one of K, V
+constexpr int kMaxListRows = 8192;      // of the list form: an int of shared memory each
 template <int D>
 struct Mma {
   static constexpr int KT = kTileBytes / (2 * D);
@@ -1152,7 +1153,7 @@ inline int64_t most_tiles(int D, int table_width, int page_size) {
 
 // Does a launch of these sizes go to the tensor-core kernel (strides and alignment apart)?
 inline bool mma_sizes(int dtype, int B, int H, int Hkv, int D, int table_width, int page_size) {
-  return dtype == ENGPT_BF16 && D <= 128 && D % 8 == 0 && page_size % 8 == 0 && B <= 8192 &&
+  return dtype == ENGPT_BF16 && D <= 128 && D % 8 == 0 && page_size % 8 == 0 && B <= kMaxListRows &&
          B * (int64_t)H * (2 * most_tiles(D, table_width, page_size) + 1) < (1ll << 31);
 }
 
@@ -1185,8 +1186,8 @@ inline int64_t mma_floats(int H, int Hkv, int D) {
 }
 
 template <int D>
-size_t mma_smem(const MmaArgs& a, int warps, int parts) {
-  return 1024 + (size_t)warps * (2 * kTileBytes + 8) + 4 * (size_t)parts * part_floats<D>(a.rows);
+size_t mma_smem(int rows, int warps, int parts) {
+  return 1024 + (size_t)warps * (2 * kTileBytes + 8) + 4 * (size_t)parts * part_floats<D>(rows);
 }
 
 template <int D>
@@ -1194,8 +1195,11 @@ int launch_pair(const MmaArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, 
   auto kern = decode_pair_kernel<D>;
   // Two CTAs per SM and no third one, which would leave other SMs idle (one wave has at most two per SM; 128 pairs of 32
   // tiles: 15.2 us so, 16.5 if three fit).
-  const size_t needed = mma_smem<D>(a, kPairWarps, kPairWarps + cs), smem = needed > kPairSmem ? needed : kPairSmem;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  const size_t needed = mma_smem<D>(a.rows, kPairWarps, kPairWarps + cs), smem = needed > kPairSmem ? needed : kPairSmem;
+  // (the attribute is the kernel's, not the launch's: every call sets it to the same, largest size, so that a call on
+  // another host thread cannot lower it between here and the launch)
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)mma_smem<D>(8, kPairWarps, kPairWarps + 8));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((int64_t)a.B * a.HQ * cs));
   cfg.blockDim = dim3(kPairWarps * 32);
@@ -1217,8 +1221,9 @@ int launch_pair(const MmaArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, 
 template <int D>
 int launch_list(const MmaArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t st) {
   auto kern = decode_list_kernel<D>;
-  const size_t smem = mma_smem<D>(a, kWarps, kWarps) + 4 * ((size_t)a.B + 1);
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  const size_t smem = mma_smem<D>(a.rows, kWarps, kWarps) + 4 * ((size_t)a.B + 1);
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,   // as in launch_pair
+                                       (int)(mma_smem<D>(8, kWarps, kWarps) + 4 * ((size_t)kMaxListRows + 1)));
   if (e != cudaSuccess) return set_error(ENGPT_ERR_LAUNCH, "paged_attention: %s", cudaGetErrorString(e));
   // both kernels may be started before what runs ahead of them has ended; they wait for it on the device
   cudaLaunchConfig_t cfg = {};

@@ -296,8 +296,11 @@ extern "C" int engpt_advance_block_tables(int* lengths, const int* new_tokens, c
   const int ctas = small ? 1 : kTableCluster;
   const size_t smem = sizeof(int) * 5 * (size_t)B;
   auto kern = vec ? advance_tables_kernel<4> : advance_tables_kernel<1>;
+  // (the attribute is the kernel's, not the launch's: every call that needs it sets the same, largest size, so that a
+  // call on another host thread cannot lower it between here and the launch)
   cudaError_t e = cudaSuccess;
-  if (smem > 40 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (smem > 40 * 1024)
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(int) * 5 * kMaxRows);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(small ? 256 : 1024);

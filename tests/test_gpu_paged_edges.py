@@ -1,7 +1,9 @@
 """Paged key-value cache operators on B200, at their edges: what the tests of ordinary calls do not reach."""
 
 import ctypes
+import threading
 
+import numpy as np
 import pytest
 import torch
 
@@ -76,3 +78,63 @@ def test_infinite_values_in_use(cuda, dtype, heads, kv_heads, dim, lengths):
     ref, vmax, smax = R.attention(q, kp, vp.nan_to_num(nan=0.0, posinf=0.0, neginf=0.0), table, lens, scale)
     tol = R.attention_tolerance(dtype, ref, vmax, smax, dim, max(lengths))
     assert ((out - ref).abs() <= tol)[~marked].all()
+
+
+# ------------------------------------------------------------------ calls from several host threads
+def run_threads(calls, times):
+    """Each call `times` times in a thread of its own, all at once, through the C boundary (which holds no lock): the
+    status codes of each."""
+    codes, gate = [set() for _ in calls], threading.Barrier(len(calls))
+
+    def work(i):
+        torch.cuda.synchronize()
+        gate.wait()
+        for _ in range(times):
+            codes[i].add(calls[i]())
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(calls))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    return codes
+
+
+def test_attention_from_several_threads(cuda):
+    """Calls whose kernels need different amounts of shared memory."""
+    lib, calls, outs = _lib.load(), [], []
+    for seed, (bsz, heads) in enumerate([(8000, 2), (300, 2), (300, 16)]):
+        rng = np.random.default_rng(seed)
+        lengths = rng.integers(0, 20, bsz).tolist()
+        lengths[3] = 700
+        pool = sum(R.pages_of(n, 16) for n in lengths)
+        table, _ = R.random_table(lengths, 16, 44, pool, rng)
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        kp, vp = (torch.randn(pool, 2, 16, 64, generator=gen, device="cuda").bfloat16() for _ in range(2))
+        q = torch.randn(bsz, heads, 64, generator=gen, device="cuda").bfloat16()
+        args = (q, kp, vp, table.cuda(), torch.tensor(lengths, dtype=torch.int32, device=cuda), 0.125)
+        out = torch.empty_like(q)
+        call, keep = attention_call(args, out, torch.cuda.Stream())
+        calls.append(lambda c=call: lib.engpt_paged_attention(*c))
+        outs.append((K.paged_sdpa(*args[:5], scale=args[5]), out, keep))
+    torch.cuda.synchronize()
+    assert run_threads(calls, 500) == [{0}] * 3
+    assert all(torch.equal(want, out) for want, out, _ in outs)
+
+
+def test_tables_from_several_threads(cuda):
+    lib, calls, keep = _lib.load(), [], []
+    i32 = dict(dtype=torch.int32, device=cuda)
+    for bsz in (8192, 2500, 4000):
+        t = dict(lengths=torch.zeros(bsz, **i32), new=torch.zeros(bsz, **i32), table=torch.zeros(bsz, 2, **i32),
+                 free=torch.arange(bsz, **i32), count=torch.tensor([bsz], **i32), slots=torch.empty(bsz, **i32),
+                 pos=torch.empty(bsz, **i32))
+        p, stream = {k: v.data_ptr() for k, v in t.items()}, torch.cuda.Stream()
+        call = (p["lengths"], p["new"], None, bsz, p["table"], 2, 2, p["free"], bsz, p["count"], 16, 1, p["slots"],
+                p["pos"], stream.cuda_stream)
+        calls.append(lambda c=call: lib.engpt_advance_block_tables(*c))
+        keep.append((t, stream))
+    torch.cuda.synchronize()
+    assert run_threads(calls, 1000) == [{0}] * 3
+    assert all(int(t["count"]) == len(t["free"]) and (t["slots"] == -1).all() for t, _ in keep)

@@ -27,6 +27,17 @@ int check_launch(const char* what) {
   return ENGPT_OK;
 }
 
+int bind_thread_context() {
+  static thread_local bool bound = false;
+  if (bound) return ENGPT_OK;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaSetDevice(dev);
+  if (e != cudaSuccess) return set_error(ENGPT_ERR_LAUNCH, "no CUDA context: %s", cudaGetErrorString(e));
+  bound = true;
+  return ENGPT_OK;
+}
+
 __device__ int g_device_status = 0;
 
 int num_sms() {

@@ -1084,6 +1084,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 static PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 
 static int get_encode() {
+  if (int rc = bind_thread_context()) return rc;
   if (g_encode) return ENGPT_OK;
   void* fn = nullptr;
   cudaDriverEntryPointQueryResult q;

@@ -15,6 +15,9 @@ namespace engpt {
 int set_error(int code, const char* fmt, ...);
 void clear_error();
 int check_launch(const char* what);
+// Makes the current device's context current on a host thread that has made no CUDA call yet: kernel launches do that
+// by themselves, cuTensorMapEncodeTiled fails without one.
+int bind_thread_context();
 // Mean of row_loss over the rows whose target is not -100 (F.cross_entropy's reduction) into loss_out[0].
 int launch_mean_loss(const float* row_loss, const int64_t* targets, int64_t rows, float* loss_out, cudaStream_t st);
 

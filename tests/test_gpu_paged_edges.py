@@ -138,3 +138,44 @@ def test_tables_from_several_threads(cuda):
     torch.cuda.synchronize()
     assert run_threads(calls, 1000) == [{0}] * 3
     assert all(int(t["count"]) == len(t["free"]) and (t["slots"] == -1).all() for t, _ in keep)
+
+
+@pytest.mark.parametrize("bsz", [2, 300])
+def test_attention_as_the_first_cuda_call_of_a_thread(cuda, bsz):
+    """A thread that has made no CUDA call has no context of its own yet: both forms on the tensor cores."""
+    lib = _lib.load()
+    args = attention_inputs([70] + [1] * (bsz - 1), 2, 2, 64, 16, torch.bfloat16)
+    out = torch.empty_like(args[0])
+    call, keep = attention_call(args, out)
+    torch.cuda.synchronize()
+    codes = []
+    t = threading.Thread(target=lambda: codes.append(lib.engpt_paged_attention(*call)))
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert codes == [0]
+    check_attention(args, out)
+
+
+def test_other_tensor_map_kernels_as_the_first_cuda_call_of_a_thread(cuda):
+    lib = _lib.load()
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v = (torch.randn(1, 256, 2, 64, generator=gen, device="cuda").bfloat16() for _ in range(3))
+    want, out = K.causal_sdpa(q, k, v, scale=0.125, dropout_p=0.0, impl="tcgen05"), torch.empty_like(q)
+    strides = K.attention_strides(q, k, v, out, head_major=False)
+    w, x = (torch.randn(n, 256, generator=gen, device="cuda").bfloat16() for n in (512, 300))
+    y, stream = torch.empty(300, 512, device=cuda, dtype=torch.bfloat16), torch.cuda.current_stream().cuda_stream
+    calls = [lambda: lib.engpt_causal_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 1, 1, 256, 2, 64,
+                                                0.125, strides.data_ptr(), _lib.ATTN_TCGEN05, stream),
+             lambda: lib.engpt_gemm_bf16(x.data_ptr(), 256, w.data_ptr(), 256, y.data_ptr(), 512, 300, 512, 256, stream)]
+    torch.cuda.synchronize()
+    codes = []
+    for call in calls:
+        t = threading.Thread(target=lambda: codes.append(call()))
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    assert codes == [0, 0]
+    assert torch.equal(out, want)
+    ref = x.double() @ w.double().t()      # 256 products of fp32 sums, one rounding
+    assert ((y.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -16 * (x.abs().double() @ w.abs().double().t())).all()

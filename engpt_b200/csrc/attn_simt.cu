@@ -143,17 +143,20 @@ int launch_attn_simt(const void* q, const void* k, const void* v, void* o, int d
   const int nqb = (T + kSimtQ - 1) / kSimtQ;
   const int64_t blocks = (int64_t)nqb * B * H;
   ENGPT_REQUIRE(blocks <= 0x7fffffffLL, ENGPT_ERR_SHAPE, "attention (simt): grid too large");
-  const size_t smem = sizeof(float) * (size_t)(2 * kSimtK * (Dh + 1) + kSimtQ * Dh);
+  const auto smem_bytes = [](int dim) { return sizeof(float) * (size_t)(2 * kSimtK * (dim + 1) + kSimtQ * dim); };
+  const size_t smem = smem_bytes(Dh);
+  // the limit is the kernel's, not the launch's: every call sets the largest, as another host thread may set it too
+  const int most_smem = (int)smem_bytes(256);
   const int maxv = (Dh + 31) / 32;
 #define ENGPT_SIMT_CASE(MV)                                                                              \
   if (maxv <= MV) {                                                                                      \
     if (dtype == ENGPT_BF16) {                                                                           \
       auto kern = attn_simt_kernel<__nv_bfloat16, MV>;                                                   \
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);                \
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem);                  \
       kern<<<(unsigned)blocks, kSimtWarps * 32, smem, st>>>(a);                                          \
     } else {                                                                                             \
       auto kern = attn_simt_kernel<float, MV>;                                                           \
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);                \
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem);                  \
       kern<<<(unsigned)blocks, kSimtWarps * 32, smem, st>>>(a);                                          \
     }                                                                                                    \
     return check_launch("attention (simt)");                                                             \

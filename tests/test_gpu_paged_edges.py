@@ -140,6 +140,23 @@ def test_tables_from_several_threads(cuda):
     assert all(int(t["count"]) == len(t["free"]) and (t["slots"] == -1).all() for t, _ in keep)
 
 
+def test_whole_sequence_attention_from_several_threads(cuda):
+    """The CUDA-core kernel at head dims of one instantiation that need different amounts of shared memory."""
+    lib, calls, outs = _lib.load(), [], []
+    for dim in (136, 200, 256):
+        gen = torch.Generator(device="cuda").manual_seed(dim)
+        q, k, v = (torch.randn(1, 40, 2, dim, generator=gen, device="cuda") for _ in range(3))
+        want, out, stream = K.causal_sdpa(q, k, v, scale=0.1, dropout_p=0.0), torch.empty_like(q), torch.cuda.Stream()
+        strides = K.attention_strides(q, k, v, out, head_major=False)
+        call = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _lib.F32, 1, 40, 2, dim, 0.1, strides.data_ptr(),
+                _lib.ATTN_SIMT, stream.cuda_stream)
+        calls.append(lambda c=call: lib.engpt_causal_attention(*c))
+        outs.append((want, out, (q, k, v, strides, stream)))
+    torch.cuda.synchronize()
+    assert run_threads(calls, 500) == [{0}] * 3
+    assert all(torch.equal(want, out) for want, out, _ in outs)
+
+
 @pytest.mark.parametrize("bsz", [2, 300])
 def test_attention_as_the_first_cuda_call_of_a_thread(cuda, bsz):
     """A thread that has made no CUDA call has no context of its own yet: both forms on the tensor cores."""

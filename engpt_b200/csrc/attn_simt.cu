@@ -152,11 +152,11 @@ int launch_attn_simt(const void* q, const void* k, const void* v, void* o, int d
   if (maxv <= MV) {                                                                                      \
     if (dtype == ENGPT_BF16) {                                                                           \
       auto kern = attn_simt_kernel<__nv_bfloat16, MV>;                                                   \
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem);                  \
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem);                \
       kern<<<(unsigned)blocks, kSimtWarps * 32, smem, st>>>(a);                                          \
     } else {                                                                                             \
       auto kern = attn_simt_kernel<float, MV>;                                                           \
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem);                  \
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem);                \
       kern<<<(unsigned)blocks, kSimtWarps * 32, smem, st>>>(a);                                          \
     }                                                                                                    \
     return check_launch("attention (simt)");                                                             \

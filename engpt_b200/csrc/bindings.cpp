@@ -136,7 +136,7 @@ Tensor qkv_append(const Tensor& qkv_in, const Tensor& rho, const Tensor& cos, co
   const Pools p = check_pools(k_pages, v_pages);
   const auto dev = k_pages.device();
   for (const Tensor* t : {&qkv_in, &rho, &cos, &sin, &qk_scale}) require_device(*t, dev);
-  forward_only({&qkv_in, &rho, &cos, &sin, &qk_scale});
+  forward_only({&qkv_in, &rho, &cos, &sin, &qk_scale, &k_pages, &v_pages});
   const int64_t nd = qkv_in.dim();
   TORCH_CHECK_VALUE(nd >= 3 && qkv_in.size(nd - 3) == 3 && qkv_in.size(nd - 2) == p.heads &&
                         qkv_in.size(nd - 1) == p.dim && qkv_in.scalar_type() == k_pages.scalar_type(),
@@ -178,6 +178,7 @@ void write_kv_pages(const Tensor& k_in, const Tensor& v_in, const Tensor& slots,
   const auto dev = k_pages.device();
   require_device(k_in, dev);
   require_device(v_in, dev);
+  forward_only({&k_in, &v_in, &k_pages, &v_pages});
   const int64_t nd = k_in.dim();
   TORCH_CHECK_VALUE(nd >= 2 && k_in.sizes() == v_in.sizes() && k_in.size(nd - 2) == p.heads &&
                         k_in.size(nd - 1) == p.dim,

@@ -38,6 +38,13 @@ void forward_only(std::initializer_list<const Tensor*> ts) {
                                 "engpt_b200 kernels are forward-only; call under torch.no_grad()");
 }
 
+// Tensors that a call has written through their addresses: counted as torch's own in-place operators are, so that
+// autograd notices where it kept one of them.
+void written(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 int dtype_code(const Tensor& t) {
   const auto dt = t.scalar_type();
   TORCH_CHECK_NOT_IMPLEMENTED(dt == at::kBFloat16 || dt == at::kFloat,
@@ -127,6 +134,7 @@ py::tuple advance_block_tables(const Tensor& lengths, const Tensor& new_tokens, 
                    (int*)free_pages.data_ptr(), to_int(free_pages.size(0), "num_pages"), (int*)free_count.data_ptr(),
                    to_int(page_size, "page_size"), to_int(max_new, "max_new"), (int*)slots.data_ptr(),
                    (int*)positions.data_ptr(), stream_of(dev)));
+  written({&lengths, &block_table, &free_pages, &free_count});
   return py::make_tuple(slots, positions);
 }
 
@@ -163,6 +171,7 @@ Tensor qkv_append(const Tensor& qkv_in, const Tensor& rho, const Tensor& cos, co
                                 p.dim, (const int*)positions.data_ptr(), (const int*)slots.data_ptr(), q.data_ptr(),
                                 k_pages.data_ptr(), v_pages.data_ptr(), p.strides, p.num_pages, p.page_size,
                                 stream_of(dev)));
+  written({&k_pages, &v_pages});
   return q;
 }
 
@@ -195,6 +204,7 @@ void write_kv_pages(const Tensor& k_in, const Tensor& v_in, const Tensor& slots,
                engpt_write_kv_pages(k.data_ptr(), v.data_ptr(), strides, p.code, k.size(0), p.heads, p.dim,
                                     (const int*)slots.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), p.strides,
                                     p.num_pages, p.page_size, stream_of(dev)));
+  written({&k_pages, &v_pages});
 }
 
 Tensor paged_sdpa(const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,

@@ -9,7 +9,7 @@ import torch
 
 from engpt_b200 import _lib, kernels as K
 from tests import paged_ref as R
-from tests.test_gpu_paged import _clean, attention_inputs, check_attention  # noqa: F401
+from tests.test_gpu_paged import _clean, append_inputs, attention_inputs, check_attention, make_pools  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -196,3 +196,41 @@ def test_other_tensor_map_kernels_as_the_first_cuda_call_of_a_thread(cuda):
     assert torch.equal(out, want)
     ref = x.double() @ w.double().t()      # 256 products of fp32 sums, one rounding
     assert ((y.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -16 * (x.abs().double() @ w.abs().double().t())).all()
+
+
+# ------------------------------------------------------------------ in-place writes and autograd
+def test_writes_are_counted(cuda):
+    """The tensors that a call changes in place get a new version, views of them too; inference tensors have none."""
+    def state():
+        i32 = dict(dtype=torch.int32, device=cuda)
+        kp, vp = make_pools(2, 2, 4, 64, torch.bfloat16)
+        return dict(lengths=torch.zeros(1, **i32), table=torch.zeros(1, 2, **i32), free=torch.tensor([1, 0], **i32),
+                    count=torch.tensor([2], **i32), kp=kp, vp=vp, new=torch.ones(1, **i32))
+
+    def calls(t):
+        qkv, rho, cos, sin, scale, pos = append_inputs(1, 2, 64, torch.bfloat16, 1)
+        slots, _ = K.advance_block_tables(t["lengths"], t["new"], t["table"], t["free"], t["count"], page_size=4,
+                                          max_new=1)
+        yield ("lengths", "table", "free", "count")
+        K.qkv_append_from_carried(qkv, rho, cos, sin, scale, 1e-6, pos, slots.view(1), t["kp"], t["vp"])
+        yield ("kp", "vp")
+        K.write_kv_pages(qkv[:, 1], qkv[:, 2], slots.view(1), t["kp"], t["vp"])
+        yield ("kp", "vp")
+        K.paged_sdpa(qkv[:, 0], t["kp"], t["vp"], t["table"], t["lengths"], scale=1.0)
+        yield ()
+
+    t = state()
+    before = {k: v._version for k, v in t.items()}
+    for changed in calls(t):
+        now = {k: v._version for k, v in t.items()}
+        assert {k for k in now if now[k] > before[k]} == set(changed)
+        before = now
+    with torch.enable_grad():
+        x = torch.ones(64, device=cuda, dtype=torch.bfloat16, requires_grad=True)
+        y = (x * t["kp"]).sum()
+    K.write_kv_pages(t["kp"][:1, :, 0], t["kp"][:1, :, 0], t["new"], t["kp"], t["vp"])
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+    with torch.inference_mode():
+        t = state()
+    assert len(list(calls(t))) == 4

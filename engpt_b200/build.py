@@ -2,12 +2,14 @@
 
 The library is built in-tree next to this file so that it travels with the
 source tree.  ``python -m engpt_b200.build`` (or ``build()``) recompiles the
-objects whose sources or headers changed and relinks.
+objects whose sources or headers changed and relinks.  Without torch (``python
+engpt_b200/build.py``) the library alone is built.
 """
 
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -80,7 +82,8 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> str:
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
         os.replace(tmp, LIB)
-    build_native(force)
+    if importlib.util.find_spec("torch") is not None:   # the library alone, for callers of the C ABI, needs no torch
+        build_native(force)
     return LIB
 
 

@@ -1,10 +1,14 @@
 """Refusals of the paged key-value cache operators (no GPU) next to those of tests/test_paged_host.py."""
 
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
-from engpt_b200 import kernels as K
+from engpt_b200 import build as B, kernels as K
 
 
 def test_writes_are_forward_only():
@@ -27,3 +31,15 @@ def test_writes_are_forward_only():
                 with pytest.raises(NotImplementedError, match="forward-only"):
                     call()
                 t.requires_grad_(False)
+
+
+def test_the_library_builds_without_torch():
+    """Callers of the C ABI alone have no torch: the build then leaves the Python binding out."""
+    assert os.path.exists(B.LIB)
+    code = ("import sys, runpy; sys.modules['torch'] = None\n"
+            "import importlib.util as u; find = u.find_spec\n"
+            "u.find_spec = lambda name, *a: None if name == 'torch' else find(name, *a)\n"
+            f"ns = runpy.run_path({B.__file__!r})\n"
+            "print(ns['build']())")
+    res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert res.returncode == 0 and res.stdout.strip() == B.LIB, res.stderr

@@ -32,6 +32,7 @@ from torch import Tensor
 from . import _lib
 from . import kernels as K
 from .config import ModelConfig
+from .models import plain_tensors
 
 __all__ = ["PagedKVCache", "PagedDecoder"]
 
@@ -47,6 +48,7 @@ class PagedKVCache:
     ``block_size``), rounded up to whole pages.
     """
 
+    @plain_tensors
     def __init__(self, cfg: ModelConfig, max_batch: int, num_pages: int, *, page_size: int = 64,
                  max_len: Optional[int] = None, dtype: torch.dtype = torch.bfloat16,
                  device: Optional[torch.device] = None) -> None:
@@ -90,6 +92,7 @@ class PagedKVCache:
 class _StepGraph:
     """A captured step: static inputs, the graph and its logits."""
 
+    @plain_tensors
     def __init__(self, dec: "PagedDecoder") -> None:
         b, dev = dec.cache.max_batch, dec.device
         self.idx = torch.zeros(b, dtype=torch.int64, device=dev)
@@ -121,6 +124,7 @@ class PagedDecoder:
     rows ``0 .. max_batch - 1``.
     """
 
+    @plain_tensors
     def __init__(self, model, max_batch: int, num_pages: int, *, page_size: int = 64, max_len: Optional[int] = None,
                  dtype: torch.dtype = torch.bfloat16) -> None:
         p = model.token_emb.weight
@@ -152,7 +156,7 @@ class PagedDecoder:
                              f"{p.device}")
         return p.detach().contiguous()
 
-    @torch.no_grad()
+    @plain_tensors
     def refresh_weights(self) -> None:
         """Take the model's current parameters (in float32 all but the head are used in place).
 

@@ -134,9 +134,16 @@ class EfficientNGPTBlock(nn.Module):
         _normalize_columns_(self.down_proj.weight, eps)
 
 
+# Buffers that are kept between calls are made as plain tensors, also where the call that makes them is under
+# torch.inference_mode: an inference tensor could not be written again outside of it.
+def plain_tensors(f):
+    return torch.inference_mode(False)(torch.no_grad()(f))
+
+
 class _Workspace:
     """Activation buffers for one (batch, seq_len, precision) shape on one device."""
 
+    @plain_tensors
     def __init__(self, cfg: ModelConfig, bsz: int, seq_len: int, device: torch.device, bf16: bool,
                  fuse_mlp: bool = True, split: Optional[HeadSplit] = None):
         d, Dh, W_full = cfg.n_embd, cfg.head_dim, cfg.mlp_width
@@ -185,6 +192,7 @@ class _Workspace:
         self._lse_shape = (-(-cfg.vocab_size // 256) * n * 2,)
         self._device = device
 
+    @plain_tensors
     def lse_partials(self) -> torch.Tensor:
         """Scratch of the fused head: one (max, sum) pair per row and 256-column logits tile."""
         if self._lse is None:
@@ -199,6 +207,7 @@ class _GraphedForward:
     pointers into it), whatever the model's current workspace becomes.
     """
 
+    @plain_tensors
     def __init__(self, model: "EfficientNGPT", shape: tuple, has_targets: bool, dev: torch.device) -> None:
         self.idx = torch.zeros(shape, dtype=torch.int64, device=dev)
         self.targets = torch.zeros(shape, dtype=torch.int64, device=dev) if has_targets else None

@@ -114,3 +114,33 @@ def test_refused_rows_have_zero_logits(cuda, dtype):
     assert row_err(logits[1:2], full[1, 30][None]) < TOL[dtype]
     with pytest.raises(_lib.EngptError, match="site 41"):
         _lib.raise_on_device_status()
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_inside_and_outside_inference_mode(cuda, dtype, graphs):
+    """What is made in a call under inference_mode (the decoder, its captured step, the model's workspace) serves calls
+    outside of it, and the other way round."""
+    idx = tokens(CFGS["dh64"], (2, 12), 5)
+    runs = []
+    for modes in ((False,) * 5, (True, False) * 3, (False, True) * 3):
+        with torch.inference_mode(modes[0]), torch.no_grad():
+            model = model_on(cuda, "dh64")
+            model.enable_cuda_graphs(graphs)
+            dec = model.decoder(2, 8, page_size=16, dtype=dtype)
+            dec.enable_cuda_graphs(graphs)
+        out = []
+        for i, inside in enumerate(modes[1:5]):
+            with torch.inference_mode(inside), torch.no_grad():
+                dec.refresh_weights()
+                dec.cache.reset()
+                out.append(dec.prefill(idx[:, :9]).clone())
+                out.append(dec.step(idx[:, 9]).clone())
+                out.append(dec.generate(idx[:, :9], 3).clone())
+                out.append(forward_logits(model, idx, dtype).clone())
+                if dtype == torch.bfloat16:     # with targets: the fused head's scratch is kept too
+                    with torch.autocast("cuda", dtype=torch.bfloat16):
+                        out.append(model(idx.cuda(), idx.cuda())[1].clone())
+        runs.append(out)
+    for other in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], other))

@@ -324,7 +324,7 @@ class PagedDecoder:
 
         ``pick`` chooses the next tokens ``[n]`` from the logits ``[n, V]``
         (default: the largest).  The requests take rows ``0 .. n-1`` and are released
-        at the end.  Raises if a token id was out of range or the pages ran out.
+        at the end, also if ``pick`` raises.  Raises if a token id was out of range or the pages ran out.
         """
         n, b = idx.shape[0], self.cache.max_batch
         if n > b:
@@ -340,12 +340,14 @@ class PagedDecoder:
         logits = self.prefill(idx, lengths=lengths)
         out = torch.empty(n, max_new_tokens, dtype=torch.int64, device=self.device)
         tokens = torch.zeros(b, dtype=torch.int64, device=self.device)
-        for t in range(max_new_tokens):
-            out[:, t] = pick(logits)
-            if t + 1 < max_new_tokens:
-                tokens[:n] = out[:, t]
-                logits = self.step(tokens, active)[:n]
-        self.release(range(n))
+        try:
+            for t in range(max_new_tokens):
+                out[:, t] = pick(logits)
+                if t + 1 < max_new_tokens:
+                    tokens[:n] = out[:, t]
+                    logits = self.step(tokens, active)[:n]
+        finally:
+            self.release(range(n))
         with torch.cuda.device(self.device):
             _lib.raise_on_device_status()
         return out

@@ -144,3 +144,25 @@ def test_inside_and_outside_inference_mode(cuda, dtype, graphs):
         runs.append(out)
     for other in runs[1:]:
         assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+
+
+def test_generate_releases_its_rows_when_pick_raises(cuda):
+    model = model_on(cuda, "dh64")
+    idx = tokens(CFGS["dh64"], (2, 20), 5)
+    dec = model.decoder(3, 9, page_size=16, dtype=torch.float32)
+    dec.prefill(idx[:1], rows=[2])
+    for at in (1, 3):
+        seen = []
+
+        def pick(z):
+            seen.append(z)
+            if len(seen) == at:
+                raise KeyError("stop")
+            return z.argmax(-1)
+
+        with pytest.raises(KeyError):
+            dec.generate(idx, 8, pick=pick)
+        assert dec.cache.lengths.tolist() == [0, 0, 20] and int(dec.cache.free_count) == 7
+    with pytest.raises(ValueError):
+        dec.generate(idx, 8, lengths=[21, 3])
+    assert dec.cache.lengths.tolist() == [0, 0, 20]

@@ -257,8 +257,9 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(AttnArgs a) {
   join_parts<T>(a, a.work + (int64_t)blockIdx.x * a.splits * (a.Dh + 2), blockIdx.x);
 }
 
-// Key splits of a launch: about four CTAs per SM, at least 64 keys each at the longest length the table holds.  One
-// cluster rather than a second launch where that leaves a CTA no more than 256 keys.
+// Key splits of a launch: about four CTAs per SM if every query head had one of its own (heads that share a reading of
+// their kv head's keys leave a half or a quarter as many), at least 64 keys each at the longest length the table holds.
+// One cluster rather than a second launch where that leaves a CTA no more than 256 keys.
 inline int simt_splits(int B, int H, int64_t most) {
   const int64_t rows = (int64_t)B * H;
   int64_t s = rows > 0 ? (4 * (int64_t)num_sms() + rows - 1) / rows : 1;

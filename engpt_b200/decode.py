@@ -121,7 +121,8 @@ class PagedDecoder:
     or last refreshed (in bfloat16 its own copies of the linear weights, in both
     types its own scaled copy of the head): call ``refresh_weights()`` after the
     model's parameters have changed, in place or for other tensors.  Requests are
-    rows ``0 .. max_batch - 1``.
+    rows ``0 .. max_batch - 1``.  ``prefill`` uses the model's parameters and
+    activation buffers, as its forward does: one stream at a time.
     """
 
     @plain_tensors

@@ -410,5 +410,9 @@ def paged_sdpa(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: Tensor,
     page_size, Dh]`` with any strides and a contiguous last axis, ``Dh`` at most
     256.  bf16 with ``Dh`` up to 128 and a multiple of 8, pages of a multiple of 8
     tokens and 16-byte aligned strides runs on the tensor cores.
+
+    How the work is split follows from the width of ``block_table``, as the
+    lengths are on the device: where they are known to be short, a table cut to
+    them (``block_table[:, :n]``) is faster than a wide one.
     """
     return _lib.native().paged_sdpa(q, k_pages, v_pages, block_table, lengths, scale)

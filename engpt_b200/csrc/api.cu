@@ -4,6 +4,7 @@
 // token cross-entropy.
 #include "common.cuh"
 
+#include <cuda.h>
 #include <string.h>
 
 
@@ -30,10 +31,19 @@ int check_launch(const char* what) {
 int bind_thread_context() {
   static thread_local bool bound = false;
   if (bound) return ENGPT_OK;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaSetDevice(dev);
-  if (e != cudaSuccess) return set_error(ENGPT_ERR_LAUNCH, "no CUDA context: %s", cudaGetErrorString(e));
+  // (a caller's own driver context stays: only where there is none does the device's primary one become current)
+  void* fn = nullptr;
+  cudaDriverEntryPointQueryResult q;
+  cudaError_t e = cudaGetDriverEntryPoint("cuCtxGetCurrent", &fn, cudaEnableDefault, &q);
+  CUcontext ctx = nullptr;
+  if (e == cudaSuccess && q == cudaDriverEntryPointSuccess && fn)
+    if (reinterpret_cast<CUresult (*)(CUcontext*)>(fn)(&ctx) != CUDA_SUCCESS) ctx = nullptr;
+  if (!ctx) {
+    int dev = 0;
+    e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaSetDevice(dev);
+    if (e != cudaSuccess) return set_error(ENGPT_ERR_LAUNCH, "no CUDA context: %s", cudaGetErrorString(e));
+  }
   bound = true;
   return ENGPT_OK;
 }

@@ -216,7 +216,7 @@ struct WriteArgs {
   int ps, ps_shift;   // ps_shift: log2(page size), or -1
 };
 
-// 32768 tokens of 16 heads of 64 in bf16, 30720 of them with a slot (252 MB move): 42.3 us = 5.95 TB/s with two pieces and
+// 32768 tokens of 16 heads of 64 in bf16, 15 of 16 with a slot (252 MB move): 42.3 us = 5.95 TB/s with two pieces and
 // 8 CTAs per SM; 46.7 with one piece, 46.1 with four, 45.4 with 32 CTAs.  All 32768 with one (268 MB): 44.2 us = 6.07 TB/s.
 constexpr int kWriteUnroll = 2, kWriteCtas = 8;
 

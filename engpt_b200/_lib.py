@@ -68,6 +68,13 @@ SIGNATURES = {
     "engpt_paged_attention_floats": (_i64, [_i, _i, _i, _i, _i, _i, _i]),
     "engpt_paged_attention": (_i, [_p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _i64, _i, _p, _f, _p, _p,
                                    _p]),
+    "engpt_write_kv_pages_q8": (_i, [_p, _p, _p, _i, _i64, _i, _i, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p]),
+    "engpt_qkv_append_q8": (_i, [_p, _i, _p, _p, _p, _i, _i, _p, _f, _f, _i64, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p,
+                                 _p, _i, _i, _i, _i, _p]),
+    "engpt_read_kv_pages_q8": (_i, [_p, _i64, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p, _p, _i, _p]),
+    "engpt_paged_attention_q8_floats": (_i64, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "engpt_paged_attention_q8": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _i64, _i,
+                                      _p, _f, _p, _p, _p]),
 }
 CE_NOALLOC_MAX_ROWS = 262144
 

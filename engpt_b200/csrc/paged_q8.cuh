@@ -1,0 +1,74 @@
+// The paged cache in 8 bits: codes and their scales.
+#pragma once
+
+#include "common.cuh"
+
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <math.h>
+
+namespace engpt {
+namespace paged {
+
+// One cache: k (0) and v (1).
+struct Q8Cache {
+  void* codes[2];
+  float* scales[2];
+  int64_t cs[2][3];       // element strides of the codes: page, head, slot
+  int64_t ss[2][3];       // of the scales: page, head, block
+  int H, Dh;
+  int ps, block;          // tokens of a page, and of a block (which divides it)
+  int64_t n_slots;        // num_pages * page_size
+
+  // codes of (slot, head) and scale of (slot, head), as offsets
+  __device__ __forceinline__ int64_t code_at(int part, int slot, int h) const {
+    const int page = slot / ps, off = slot - page * ps;
+    return page * cs[part][0] + h * cs[part][1] + off * cs[part][2];
+  }
+  __device__ __forceinline__ int64_t scale_at(int part, int slot, int h) const {
+    const int page = slot / ps, off = slot - page * ps;
+    return page * ss[part][0] + h * ss[part][1] + off / block * ss[part][2];
+  }
+};
+
+// Codes.  kTop: the largest one.  encode: of a number that the scale has brought within +-kTop (up to rounding), to the
+// nearest code, even ones in the middle; NaN gives some code.
+struct Int8Code {
+  static constexpr float kTop = 127.f;
+  static __device__ __forceinline__ float decode(uint8_t c) { return (float)(int8_t)c; }
+  static __device__ __forceinline__ uint8_t encode(float x) {
+    int r;
+    asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(r) : "f"(x));
+    return (uint8_t)r;
+  }
+};
+
+struct E4m3Code {
+  static constexpr float kTop = 448.f;
+  static __device__ __forceinline__ float decode(uint8_t c) {
+    const __half_raw h = __nv_cvt_fp8_to_halfraw(c, __NV_E4M3);
+    return __half2float(__half(h));
+  }
+  static __device__ __forceinline__ uint8_t encode(float x) {
+    return (uint8_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+  }
+};
+
+// The scale that a block needs for numbers of at most |x| = `amax`, given as bits (so that the largest of them in
+// whole-number order is the largest magnitude, infinities and NaN above all): NaN if they are not finite, and never so
+// small that its reciprocal is infinite.
+constexpr float kLeastAmax = 7.888609052210118e-31f;   // 2^-100
+template <typename Code>
+__device__ __forceinline__ float needed_scale(uint32_t amax) {
+  if (amax >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+  return __fdiv_rn(fmaxf(__uint_as_float(amax), kLeastAmax), Code::kTop);
+}
+
+// Scale of a block that held tokens with scale `old` before.  NaN stays.
+__device__ __forceinline__ float raised_scale(float old, float need) {
+  if (isnan(old) || isnan(need)) return __uint_as_float(0x7fc00000u);
+  return fmaxf(old, need);
+}
+
+}  // namespace paged
+}  // namespace engpt

@@ -41,6 +41,10 @@ __all__ = [
     "qkv_append_from_carried",
     "write_kv_pages",
     "paged_sdpa",
+    "write_kv_pages_q8",
+    "qkv_append_from_carried_q8",
+    "read_kv_pages_q8",
+    "paged_sdpa_q8",
 ]
 
 
@@ -416,3 +420,58 @@ def paged_sdpa(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: Tensor,
     them (``block_table[:, :n]``) is faster than a wide one.
     """
     return _lib.native().paged_sdpa(q, k_pages, v_pages, block_table, lengths, scale)
+
+
+# ------------------------------------------------------------ the paged cache in 8 bits
+# k_pages / v_pages: int8 or float8_e4m3fn [num_pages, kv_heads, page_size, Dh]; k_scales / v_scales: float32 [num_pages,
+# kv_heads, blocks per page].  A block is page_size / blocks tokens of one page and kv head; a number is code * scale.
+def write_kv_pages_q8(k: Tensor, v: Tensor, slots: Tensor, k_pages: Tensor, v_pages: Tensor, k_scales: Tensor,
+                      v_scales: Tensor) -> None:
+    """Quantise finished k and v ``[..., H, Dh]`` (bf16 or fp32) into their cache slots (``-1``: none).
+
+    The tokens that one call puts into a block are quantised together.  If one of
+    them is the block's first token the block starts anew with the scale that they
+    need, ``max(max |x|, 2^-100) / top`` (``top`` 127 for int8, 448 for e4m3);
+    otherwise it keeps the larger one of that and its scale so far, and where
+    that grows, the codes of its other tokens become ``round(code * (scale before
+    / scale))``.  Codes are ``round(x / scale)``.  An infinity or NaN makes the
+    block's scale NaN until the block starts anew.
+
+    Slots other than ``-1`` must be distinct, and those of one block stand side by
+    side in ``slots`` (seen as one row), in ascending order, as ``advance_block_tables``
+    gives them.  Where they do not, that block's numbers are undefined.
+    """
+    _lib.native().write_kv_pages_q8(k, v, slots, k_pages, v_pages, k_scales, v_scales)
+
+
+def qkv_append_from_carried_q8(qkv: Tensor, rho: Tensor, cos: Tensor, sin: Tensor, qk_scale: Tensor, norm_eps: float,
+                               positions: Tensor, slots: Tensor, k_pages: Tensor, v_pages: Tensor, k_scales: Tensor,
+                               v_scales: Tensor, *, qk_mult: float = 1.0) -> Tensor:
+    """``qkv_append_from_carried`` into a cache of 8 bits (the rules of ``write_kv_pages_q8``).
+
+    k and v are quantised from their fp32 values, without a rounding to
+    ``qkv``'s type in between.  Returns q ``[..., H, Dh]`` in ``qkv``'s type.
+    """
+    return _lib.native().qkv_append_q8(qkv, rho, cos, sin, qk_scale, norm_eps, positions, slots, k_pages, v_pages,
+                                       k_scales, v_scales, qk_mult)
+
+
+def read_kv_pages_q8(slots: Tensor, k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor, *,
+                     dtype: torch.dtype = torch.bfloat16) -> Tuple[Tensor, Tensor]:
+    """The numbers ``code * scale`` of given cache slots (int32 ``[...]``; ``-1`` gives zeros).
+
+    Returns k and v ``[..., H, Dh]`` in ``dtype`` (bfloat16 or float32).
+    """
+    return _lib.native().read_kv_pages_q8(slots, k_pages, v_pages, k_scales, v_scales, dtype)
+
+
+def paged_sdpa_q8(q: Tensor, k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor,
+                  block_table: Tensor, lengths: Tensor, *, scale: float) -> Tensor:
+    """``paged_sdpa`` over a cache of 8 bits: ``softmax(scale * q k^T) v`` with k and v the numbers that it stands for.
+
+    q ``[B, H, Dh]`` and the result are bf16 or fp32.  Codes and scales behind a
+    row's length have no effect, whatever they are.  The tensor cores are used for
+    ``Dh`` up to 128 and a multiple of 16, pages and blocks of a multiple of 8
+    tokens and 16-byte aligned strides.
+    """
+    return _lib.native().paged_sdpa_q8(q, k_pages, v_pages, k_scales, v_scales, block_table, lengths, scale)

@@ -20,6 +20,8 @@ and those of the paged key-value cache (no counterpart in the reference; the arg
   qk_mult=1.0) -> q`` (changes ``k_pages`` and ``v_pages``)
 * ``engpt_b200::write_kv_pages(k, v, slots, k_pages, v_pages)`` (the same)
 * ``engpt_b200::paged_sdpa(q, k_pages, v_pages, block_table, lengths, *, scale) -> o``
+* ``engpt_b200::write_kv_pages_q8``, ``qkv_append_from_carried_q8``, ``read_kv_pages_q8`` and ``paged_sdpa_q8``: the
+  same on a cache of 8 bits (``k_pages, v_pages, k_scales, v_scales``; the writing ones change all four)
 
 Only CUDA implementations are registered: a CPU tensor finds no kernel and
 the dispatcher raises (there is no CPU fallback).  Like the underlying ops
@@ -118,6 +120,56 @@ def paged_sdpa(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: Tensor,
 
 @paged_sdpa.register_fake
 def _paged_sdpa_fake(q, k_pages, v_pages, block_table, lengths, *, scale):
+    return q.new_empty(q.shape)
+
+
+_Q8_CACHE = ("k_pages", "v_pages", "k_scales", "v_scales")
+
+
+@torch.library.custom_op(f"{NAMESPACE}::write_kv_pages_q8", mutates_args=_Q8_CACHE, device_types="cuda")
+def write_kv_pages_q8(k: Tensor, v: Tensor, slots: Tensor, k_pages: Tensor, v_pages: Tensor, k_scales: Tensor,
+                      v_scales: Tensor) -> None:
+    K.write_kv_pages_q8(k, v, slots, k_pages, v_pages, k_scales, v_scales)
+
+
+@write_kv_pages_q8.register_fake
+def _write_q8_fake(k, v, slots, k_pages, v_pages, k_scales, v_scales):
+    return None
+
+
+@torch.library.custom_op(f"{NAMESPACE}::qkv_append_from_carried_q8", mutates_args=_Q8_CACHE, device_types="cuda")
+def qkv_append_from_carried_q8(qkv: Tensor, rho: Tensor, cos: Tensor, sin: Tensor, qk_scale: Tensor, norm_eps: float,
+                               positions: Tensor, slots: Tensor, k_pages: Tensor, v_pages: Tensor, k_scales: Tensor,
+                               v_scales: Tensor, *, qk_mult: float = 1.0) -> Tensor:
+    return K.qkv_append_from_carried_q8(qkv, rho, cos, sin, qk_scale, norm_eps, positions, slots, k_pages, v_pages,
+                                        k_scales, v_scales, qk_mult=qk_mult)
+
+
+@qkv_append_from_carried_q8.register_fake
+def _append_q8_fake(qkv, rho, cos, sin, qk_scale, norm_eps, positions, slots, k_pages, v_pages, k_scales, v_scales, *,
+                    qk_mult=1.0):
+    return qkv.new_empty(*qkv.shape[:-3], *qkv.shape[-2:])
+
+
+@torch.library.custom_op(f"{NAMESPACE}::read_kv_pages_q8", mutates_args=(), device_types="cuda")
+def read_kv_pages_q8(slots: Tensor, k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor, *,
+                     dtype: torch.dtype = torch.bfloat16) -> Tuple[Tensor, Tensor]:
+    return K.read_kv_pages_q8(slots, k_pages, v_pages, k_scales, v_scales, dtype=dtype)
+
+
+@read_kv_pages_q8.register_fake
+def _read_q8_fake(slots, k_pages, v_pages, k_scales, v_scales, *, dtype=torch.bfloat16):
+    return tuple(k_scales.new_empty(*slots.shape, k_pages.shape[1], k_pages.shape[3], dtype=dtype) for _ in range(2))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::paged_sdpa_q8", mutates_args=(), device_types="cuda")
+def paged_sdpa_q8(q: Tensor, k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor,
+                  block_table: Tensor, lengths: Tensor, *, scale: float) -> Tensor:
+    return K.paged_sdpa_q8(q, k_pages, v_pages, k_scales, v_scales, block_table, lengths, scale=scale)
+
+
+@paged_sdpa_q8.register_fake
+def _paged_sdpa_q8_fake(q, k_pages, v_pages, k_scales, v_scales, block_table, lengths, *, scale):
     return q.new_empty(q.shape)
 
 

@@ -413,6 +413,75 @@ ENGPT_API int engpt_paged_attention(const void* q, const int64_t* q_strides, con
                                     int64_t table_stride, int table_width, const int* lengths, float scale, void* o,
                                     float* workspace, void* stream);
 
+/*
+ * The paged cache in 8 bits.  k_pages and v_pages hold one-byte codes (`code`:
+ * ENGPT_CODE_INT8 or ENGPT_CODE_E4M3, element strides page_strides as above);
+ * a block of `block` tokens (a divisor of page_size) of one page and kv head
+ * has one fp32 scale, k_scales and v_scales [num_pages, kv heads, page_size /
+ * block] with element strides scale_strides (6 int64: k page, head, block,
+ * then v).  A number is code * scale.
+ *
+ * Writing quantises all tokens that a call puts into a block together:
+ *   need  = max(max |x|, 2^-100) / top     (top: 127 for int8, 448 for e4m3)
+ *   scale = need if one of them is the block's first token (the block starts
+ *           anew: what its other slots held is void), else max(scale, need);
+ *           where that raises it, the block's other codes become
+ *           round(code * (scale before / scale))
+ *   code  = round(x / scale), ties to even codes
+ * An infinity or NaN among them makes the block's scale NaN until the block
+ * starts anew.  The tokens of one block must stand side by side in `slots`, in
+ * the order of their slots (as engpt_advance_block_tables gives them); a call
+ * in which they do not leaves some of that block's numbers undefined.
+ */
+typedef enum engpt_code {
+  ENGPT_CODE_INT8 = 0,
+  ENGPT_CODE_E4M3 = 1
+} engpt_code;
+
+/* engpt_write_kv_pages with such a cache; dtype is that of k and v. */
+ENGPT_API int engpt_write_kv_pages_q8(const void* k, const void* v, const int64_t* kv_strides, int dtype, int64_t n,
+                                      int H, int Dh, const int* slots, void* k_pages, void* v_pages, float* k_scales,
+                                      float* v_scales, const int64_t* page_strides, const int64_t* scale_strides,
+                                      int code, int num_pages, int page_size, int block, void* stream);
+
+/*
+ * engpt_qkv_append with such a cache; dtype is that of qkv and q_out.  k and v
+ * are quantised from their fp32 values.  A token whose position is out of
+ * range is not kept, and has no part in its block's scale.
+ */
+ENGPT_API int engpt_qkv_append_q8(const void* qkv, int dtype, const float* rho, const float* cos_tab,
+                                  const float* sin_tab, int rope_rows, int rope_half, const float* qk_scale,
+                                  float qk_mult, float norm_eps, int64_t n, int H, int Dh, const int* positions,
+                                  const int* slots, void* q_out, void* k_pages, void* v_pages, float* k_scales,
+                                  float* v_scales, const int64_t* page_strides, const int64_t* scale_strides,
+                                  int code, int num_pages, int page_size, int block, void* stream);
+
+/*
+ * The numbers of given slots [n]: k_out and v_out [n, H, Dh] of type dtype,
+ * contiguous.  Zeros for a slot of -1 and for one outside the pool, which is
+ * recorded (ENGPT_ERR_ARG, site 43).
+ */
+ENGPT_API int engpt_read_kv_pages_q8(const int* slots, int64_t n, const void* k_pages, const void* v_pages,
+                                     const float* k_scales, const float* v_scales, const int64_t* page_strides,
+                                     const int64_t* scale_strides, int code, int H, int Dh, int num_pages,
+                                     int page_size, int block, void* k_out, void* v_out, int dtype, void* stream);
+
+/*
+ * engpt_paged_attention with such a cache; dtype is that of q and o.  What
+ * lies behind a row's length, codes and scales, is never used.  The tensor
+ * cores are used for Dh <= 128 and a multiple of 16, page_size and block
+ * multiples of 8, and addresses (q, codes, o) and strides of multiples of 16
+ * bytes.
+ */
+ENGPT_API int64_t engpt_paged_attention_q8_floats(int dtype, int B, int H, int Hkv, int Dh, int table_width,
+                                                  int page_size, int block);
+ENGPT_API int engpt_paged_attention_q8(const void* q, const int64_t* q_strides, const void* k_pages,
+                                       const void* v_pages, const float* k_scales, const float* v_scales,
+                                       const int64_t* page_strides, const int64_t* scale_strides, int dtype, int code,
+                                       int B, int H, int Hkv, int Dh, int num_pages, int page_size, int block,
+                                       const int* block_table, int64_t table_stride, int table_width,
+                                       const int* lengths, float scale, void* o, float* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -56,6 +56,363 @@ int dispatch_simt_q8(const Q8AttnArgs& a, bool vec, cudaStream_t st) {
   return launch_simt<Kv, 1, 32, 1, 1>(a, st);
 }
 
+// ------------------------------------------------------------------ tensor-core kernel (head_dim up to 128)
+//
+// The codes are exact in fp16 (int8: integers up to 127; e4m3: 4 significant bits, 2^-9 to 448), so both products run on
+// fp16 operands with fp32 sums:
+//   S = Q K^T with q brought to [1, 2) by a power of two of its row, which the row's score factor takes back; a
+//   fp32 q is two fp16 numbers, the second one (what the first left, times 2^11) in the otherwise idle rows 8-15;
+//   O += P V with p vs / vref in fp16, vref the largest value scale so far (raised like the running maximum of the
+//   softmax): at most 2^14 as scaled, so that what is 2^-28 of the largest weight is still a normal number; the
+//   remainder of that rounding, again fp16, in rows 8-15.  Weights have 22 bits so.
+//
+// The columns of a product may come in any order that both operands share, and keys and columns of O in any order at
+// all: a 16-byte row of 8-bit codes that ldmatrix distributes (4 bytes a lane, in place of two 16-bit numbers) becomes the
+// fragments of two steps or tiles by byte permutations, with no transposition of bytes.
+template <typename C>
+struct CodePairs;
+// Two codes of w, at the bytes that SEL names in the permutation's order, as fp16.
+template <>
+struct CodePairs<Int8Code> {
+  // With the sign bit flipped a code is c + 128, and 0x6400 + that the fp16 number 1024 + 128 + c.
+  static __device__ __forceinline__ uint32_t prepare(uint32_t w) { return w ^ 0x80808080u; }
+  template <int A, int B>
+  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
+    const uint32_t x = __byte_perm(w, 0x64646464u, 0x4040 | A | B << 8);
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&y);
+  }
+};
+template <>
+struct CodePairs<E4m3Code> {
+  static __device__ __forceinline__ uint32_t prepare(uint32_t w) { return w; }
+  template <int A, int B>
+  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
+    uint32_t y;
+    const uint16_t x = (uint16_t)__byte_perm(w, 0, A | B << 4);
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(y) : "h"(x));
+    return y;
+  }
+};
+
+__device__ __forceinline__ void mma16816_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// x and y as fp16, and what that left of them.
+__device__ __forceinline__ uint32_t split_half2(float& x, float& y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  x -= f.x;
+  y -= f.y;
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+struct Q8MmaArgs : MmaArgs {
+  const float* scales[2];   // k, v
+  int64_t ss[2][3];
+  int block;                // a multiple of 8
+};
+
+template <int Width, typename C, typename Type>
+struct Q8Tile {
+  static constexpr int D = Width;
+  static constexpr int KT = kTileBytes / D;
+  static constexpr int NG = KT / 8;       // groups of 8 keys, which share their scales
+  static constexpr int NT = 8;            // of a step's 64 keys: 8-key tiles
+  static constexpr int KC = 4;            // 16-key steps of P V
+  static constexpr int DK = D / 16;       // 16-dim steps of Q K^T
+  static constexpr int DN = D / 8;        // 8-dim tiles of O
+  static constexpr int kCodeBytes = 1, kBoxes = 1, kBoxRow = D;
+  static constexpr CUtensorMapDataType kMapType = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  static constexpr CUtensorMapSwizzle kSwizzle = D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+  static constexpr bool kTwoParts = sizeof(Type) == 4;   // of q
+  static constexpr float kWeightTop = 16384.f;
+  using T = Type;
+  using Args = Q8MmaArgs;
+  using Pairs = CodePairs<C>;
+  // Lane i < NG looks after the key scale of group i of the tile, lane NG + i after its value scale.
+  struct Spot {
+    int page, off;   // off -1: no such key
+  };
+  struct Side {
+    float scale;     // 0 without a key
+  };
+  struct Query {
+    uint32_t hi[DK][2], lo[kTwoParts ? DK : 1][2];
+    float factor;    // base-2 score of a sum of products
+  };
+  struct State {
+    float o[DN][4];  // tile 2c: columns 16 c + 2 i, tile 2c + 1: 16 c + 2 i + 1, in units of vref / kWeightTop
+    float m, l, vref, factor;
+    __device__ __forceinline__ void reset() {
+#pragma unroll
+      for (int i = 0; i < DN; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+      m = -INFINITY;
+      l = vref = 0.f;
+      factor = 1.f;
+    }
+  };
+
+  static __device__ __forceinline__ Spot find(const Args& a, const Cursor& c, int lane) {
+    const int key = c.t * KT + lane % NG * 8;
+    if (lane >= 2 * NG || key >= c.len) return Spot{0, -1};
+    const int j = a.ps_shift >= 0 ? key >> a.ps_shift : key / a.ps;
+    return Spot{a.table[c.b * a.table_stride + j], key - j * a.ps};
+  }
+
+  static __device__ __forceinline__ void fetch(const Args& a, const Cursor& c, const Spot& x, Side& side) {
+    const int lane = threadIdx.x & 31, part = lane / NG;
+    side.scale = 0.f;
+    if (x.off < 0 || c.t * KT + lane % NG * 8 >= c.len || (unsigned)x.page >= (unsigned)a.P) return;
+    const float* p = part == 0 ? a.scales[0] : a.scales[1];
+    const int64_t* s = part == 0 ? a.ss[0] : a.ss[1];
+    side.scale = p[x.page * s[0] + c.hk * s[1] + x.off / a.block * s[2]];
+  }
+
+  static __device__ __forceinline__ void load_query(const Args& a, int b, int h, int lane, Query& x) {
+    const int g = lane >> 2, t = lane & 3;
+    const int head = (h / a.QG) * a.G + (h % a.QG) * 8 + g;
+    const bool live = g < a.rows && (h % a.QG) * 8 + g < a.G;
+    const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_row + head * a.q_head + 4 * t;
+    float v[DK][4];
+    uint32_t most = 0;
+#pragma unroll
+    for (int k = 0; k < DK; ++k) {
+      if (live && k * 16 < a.dim) {
+        if constexpr (sizeof(T) == 2) {
+          const uint2 r = *reinterpret_cast<const uint2*>(q + k * 16);
+          v[k][0] = __uint_as_float(r.x << 16);
+          v[k][1] = __uint_as_float(r.x & 0xffff0000u);
+          v[k][2] = __uint_as_float(r.y << 16);
+          v[k][3] = __uint_as_float(r.y & 0xffff0000u);
+        } else {
+          const float4 r = *reinterpret_cast<const float4*>(q + k * 16);
+          v[k][0] = r.x;
+          v[k][1] = r.y;
+          v[k][2] = r.z;
+          v[k][3] = r.w;
+        }
+      } else {
+        v[k][0] = v[k][1] = v[k][2] = v[k][3] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) most = max(most, __float_as_uint(v[k][i]) & 0x7fffffffu);
+    }
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    const uint32_t e = min(max(most >> 23, 1u), 253u);   // the row's largest |q| is in [1, 2) 2^(e - 127), for most rows
+    const float down = __uint_as_float((254u - e) << 23), up = __uint_as_float(e << 23);
+    x.factor = a.scale_log2 * up;
+    const float f = a.negative ? -down : down;
+#pragma unroll
+    for (int k = 0; k < DK; ++k) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[k][i] *= f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        x.hi[k][i] = split_half2(v[k][2 * i], v[k][2 * i + 1]);
+        if constexpr (kTwoParts) x.lo[k][i] = pack_half2(v[k][2 * i] * 2048.f, v[k][2 * i + 1] * 2048.f);
+      }
+    }
+  }
+
+  // Address of 16-byte piece c of a key's row in shared memory, as TMA has swizzled it.
+  static __device__ __forceinline__ uint32_t piece(uint32_t base, int key, int c) {
+    return D == 64 ? base + key * 64 + ((c ^ ((key >> 1) & 3)) << 4) : base + key * 128 + ((c ^ (key & 7)) << 4);
+  }
+
+  // One tile: per 64 keys scores, softmax step, P V.  WHOLE: all its keys count.  Otherwise `live` keys from the tile's
+  // start are below the length, and boxes whose bit of `mask` is unset were not copied.
+  template <bool WHOLE>
+  static __device__ __forceinline__ void step(const Args& a, uint32_t sk, const Query& x, const Side& side, State& st,
+                                              int live, uint32_t mask, int lane) {
+    const uint32_t sv = sk + kTileBytes;
+    const int r8 = lane & 7, q4 = lane >> 3, t = lane & 3;
+    if (!WHOLE && C::kHasNan) {
+      // absent values become 0: their weight 0 would not cancel a stale NaN
+      for (int i = lane; i < KT * (D / 16); i += 32) {
+        const int key = i / (D / 16);
+        if (key >= live || !((mask >> (key >> a.r_shift)) & 1u))
+          asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(sv + i * 16), "r"(0u) : "memory");
+      }
+      __syncwarp();
+    }
+    st.factor = x.factor;
+    // value scales relative to the largest one so far; a NaN is above all, and makes the rows NaN
+    const uint32_t top = __reduce_max_sync(0xffffffffu, lane >= NG ? __float_as_uint(side.scale) & 0x7fffffffu : 0u);
+    if (top > __float_as_uint(st.vref)) {
+      const float corr = st.vref / __uint_as_float(top);
+      st.vref = __uint_as_float(top);
+#pragma unroll
+      for (int i = 0; i < DN; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) st.o[i][j] *= corr;
+    }
+    const float weight = top == 0u ? 0.f : side.scale / st.vref * kWeightTop;   // (0 / 0 for dead groups alone)
+#pragma unroll
+    for (int k0 = 0; k0 < KT; k0 += 64) {
+      float s[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          uint32_t w[4];
+          ldsm4(piece(sk, k0 + n * 8 + r8, c * 4 + q4), w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = c * 4 + i;
+            const uint32_t y = Pairs::prepare(w[i]);
+            mma16816_f16(s[n], x.hi[k][0], kTwoParts ? x.lo[k][0] : 0u, x.hi[k][1], kTwoParts ? x.lo[k][1] : 0u,
+                         Pairs::template pair<0, 1>(y), Pairs::template pair<2, 3>(y));
+          }
+        }
+        const float ks = __shfl_sync(0xffffffffu, side.scale, k0 / 8 + n);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if constexpr (kTwoParts) s[n][i] = fmaf(s[n][2 + i], 1.f / 2048.f, s[n][i]);
+          s[n][i] *= ks;
+          if (!WHOLE) {
+            const int key = k0 + n * 8 + 2 * t + i;
+            if (key >= live || !((mask >> (key >> a.r_shift)) & 1u)) s[n][i] = -INFINITY;
+          }
+        }
+      }
+      float mx = st.m;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mx = fmaxf(mx, fmaxf(s[n][0], s[n][1]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float ms = mx == -INFINITY ? 0.f : mx * st.factor;
+      if (__any_sync(0xffffffffu, mx > st.m)) {
+        const float corr = st.m == -INFINITY ? 0.f : sm100::ex2_approx(st.m * st.factor - ms);
+#pragma unroll
+        for (int i = 0; i < DN; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) st.o[i][j] *= corr;
+        st.l *= corr;
+        st.m = mx;
+      }
+      uint32_t hi[KC][2], lo[KC][2];
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float w = __shfl_sync(0xffffffffu, weight, NG + k0 / 8 + n);
+        float p[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          p[i] = sm100::ex2_approx(fmaf(s[n][i], st.factor, -ms));
+          if (!WHOLE && s[n][i] == -INFINITY) p[i] = 0.f;   // (the product is NaN for a scale of 0)
+          sum[i] += p[i];
+          p[i] *= w;
+        }
+        hi[n >> 1][n & 1] = split_half2(p[0], p[1]);
+        lo[n >> 1][n & 1] = pack_half2(p[0], p[1]);
+      }
+      st.l += sum[0] + sum[1];
+#pragma unroll
+      for (int j = 0; j < KC; ++j) {
+        const int key = k0 + j * 16 + (q4 & 1) * 8 + r8;
+#pragma unroll
+        for (int dp = 0; dp < D / 32; ++dp) {
+          uint32_t w[4];
+          ldsm4_t(piece(sv, key, 2 * dp + (q4 >> 1)), w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = Pairs::prepare(w[i]);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            mma16816_f16(st.o[4 * dp + 2 * c], hi[j][0], lo[j][0], hi[j][1], lo[j][1],
+                         Pairs::template pair<0, 2>(w[2 * c]), Pairs::template pair<0, 2>(w[2 * c + 1]));
+            mma16816_f16(st.o[4 * dp + 2 * c + 1], hi[j][0], lo[j][0], hi[j][1], lo[j][1],
+                         Pairs::template pair<1, 3>(w[2 * c]), Pairs::template pair<1, 3>(w[2 * c + 1]));
+          }
+        }
+      }
+    }
+    if (!WHOLE && C::kHasNan) sm100::fence_proxy_async_smem();   // the zeros above, before a later copy into this memory
+  }
+
+  // The pair's sums of this lane: o (both halves, in its own units) and l over the row's four lanes; m in base-2 units.
+  static __device__ __forceinline__ void finish(const Args&, State& st) {
+    st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
+    st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
+    if (st.m != -INFINITY) st.m *= st.factor;
+    const float unit = st.vref * (1.f / kWeightTop);
+#pragma unroll
+    for (int i = 0; i < DN; ++i) {
+      st.o[i][0] = (st.o[i][0] + st.o[i][2]) * unit;
+      st.o[i][1] = (st.o[i][1] + st.o[i][3]) * unit;
+    }
+  }
+
+  static __device__ __forceinline__ void store_part(const Args& a, const State& st, float* part, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    if (g >= a.rows) return;
+    float* p = part + g * (D + 2);
+#pragma unroll
+    for (int i = 0; i < DN; i += 2) {
+      *reinterpret_cast<float2*>(p + i * 8 + 4 * t) = make_float2(st.o[i][0], st.o[i + 1][0]);
+      *reinterpret_cast<float2*>(p + i * 8 + 4 * t + 2) = make_float2(st.o[i][1], st.o[i + 1][1]);
+    }
+    if (t == 0) *reinterpret_cast<float2*>(p + D) = make_float2(st.m, st.l);
+  }
+
+  static __device__ __forceinline__ void store_rows(const Args& a, const State& st, int b, int h, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    const int in = (h % a.QG) * 8 + g;
+    if (g >= a.rows || in >= a.G) return;
+    T* o = reinterpret_cast<T*>(a.o) + ((int64_t)b * a.H + (h / a.QG) * a.G + in) * a.dim + 4 * t;
+    const float inv = st.l == 0.f ? 0.f : 1.f / st.l;
+#pragma unroll
+    for (int i = 0; i < DN; i += 2) {
+      if (i * 8 >= a.dim) break;
+      const float v[4] = {st.o[i][0] * inv, st.o[i + 1][0] * inv, st.o[i][1] * inv, st.o[i + 1][1] * inv};
+      if constexpr (sizeof(T) == 2)
+        *reinterpret_cast<uint2*>(o + i * 8) = make_uint2(sm100::pack_bf16x2(v[0], v[1]), sm100::pack_bf16x2(v[2], v[3]));
+      else
+        *reinterpret_cast<float4*>(o + i * 8) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+  }
+};
+
+template <int D, typename C, typename T>
+int launch_mma_q8(const Q8AttnArgs& x, int Hkv, cudaStream_t st) {
+  Q8MmaArgs a;
+  a.scales[0] = x.k_scales;
+  a.scales[1] = x.v_scales;
+  for (int i = 0; i < 3; ++i) {
+    a.ss[0][i] = x.kss[i];
+    a.ss[1][i] = x.vss[i];
+  }
+  a.block = x.block;
+  return launch_mma<Q8Tile<D, C, T>>(a, x, Hkv, st);
+}
+
+// Keys of a tile of the tensor-core kernels for a head_dim.
+inline int tile_keys_q8(int dim) { return kTileBytes / mma_width(dim); }
+
+// Does a launch of these sizes go to the tensor-core kernel (strides and alignment apart)?
+inline bool mma_sizes_q8(int B, int H, int D, int table_width, int page_size, int block) {
+  return D <= 128 && D % 16 == 0 && page_size % 8 == 0 && block % 8 == 0 &&
+         list_fits(B, H, tile_keys_q8(D), table_width, page_size);
+}
+
+template <typename T, typename C>
+int dispatch_q8(const Q8AttnArgs& a, bool mma, bool vec, int Hkv, cudaStream_t st) {
+  if (mma) return mma_width(a.Dh) == 64 ? launch_mma_q8<64, C, T>(a, Hkv, st) : launch_mma_q8<128, C, T>(a, Hkv, st);
+  return dispatch_simt_q8<T, C>(a, vec, st);
+}
+
 }  // namespace paged
 }  // namespace engpt
 
@@ -67,7 +424,12 @@ extern "C" int64_t engpt_paged_attention_q8_floats(int dtype, int B, int H, int 
   (void)dtype;
   if (B <= 0 || H <= 0 || Hkv <= 0 || Dh <= 0 || table_width < 0 || page_size <= 0 || block <= 0) return 0;
   const int splits = simt_splits(B, H, (int64_t)table_width * page_size);
-  return splits > kSimtCluster ? (int64_t)B * H * splits * (Dh + 2) : 0;
+  const int64_t simt = splits > kSimtCluster ? (int64_t)B * H * splits * (Dh + 2) : 0;
+  if (H % Hkv != 0 || !mma_sizes_q8(B, H, Dh, table_width, page_size, block)) return simt;
+  // strides and alignment decide at the call which of the two kernels runs
+  const int64_t mma =
+      pair_ctas(B, H, Hkv, tile_keys_q8(Dh), table_width, page_size) == 0 ? mma_floats(H, Hkv, Dh) : 0;
+  return simt > mma ? simt : mma;
 }
 
 extern "C" int engpt_paged_attention_q8(const void* q, const int64_t* q_strides, const void* k_pages,
@@ -136,10 +498,14 @@ extern "C" int engpt_paged_attention_q8(const void* q, const int64_t* q_strides,
     if ((i == 0 ? num_pages : i == 1 ? Hkv : page_size / block) == 1) a.kss[i] = a.vss[i] = 1;
     vec = vec && a.ks[i] % 8 == 0 && a.vs[i] % 8 == 0;
   }
+  // (the copies of TMA want multiples of 16 bytes; outputs are written in pieces of up to 16)
+  bool mma = vec && aligned(k_pages, 16) && aligned(v_pages, 16) && aligned(o, 16) && num_pages > 0 &&
+             mma_sizes_q8(B, H, Dh, table_width, page_size, block);
+  for (int i = 0; i < 3; ++i) mma = mma && a.ks[i] > 0 && a.vs[i] > 0 && a.ks[i] % 16 == 0 && a.vs[i] % 16 == 0;
   cudaStream_t st = as_stream(stream);
   if (dtype == ENGPT_BF16)
-    return code == ENGPT_CODE_INT8 ? dispatch_simt_q8<__nv_bfloat16, Int8Code>(a, vec, st)
-                                   : dispatch_simt_q8<__nv_bfloat16, E4m3Code>(a, vec, st);
-  return code == ENGPT_CODE_INT8 ? dispatch_simt_q8<float, Int8Code>(a, vec, st)
-                                 : dispatch_simt_q8<float, E4m3Code>(a, vec, st);
+    return code == ENGPT_CODE_INT8 ? dispatch_q8<__nv_bfloat16, Int8Code>(a, mma, vec, Hkv, st)
+                                   : dispatch_q8<__nv_bfloat16, E4m3Code>(a, mma, vec, Hkv, st);
+  return code == ENGPT_CODE_INT8 ? dispatch_q8<float, Int8Code>(a, mma, vec, Hkv, st)
+                                 : dispatch_q8<float, E4m3Code>(a, mma, vec, Hkv, st);
 }

@@ -48,10 +48,15 @@ __device__ __forceinline__ float add_halves(float hi, float lo) { return fabsf(h
 //   S = Q K^T (rows 8-15 are zero), p = 2^(S scale - m), and O += P V with P's bf16 value in rows 0-7 and the
 //   remainder p - bf16(p), again as bf16, in rows 8-15: adding the two halves of O at the end gives the product
 //   with weights of 16 mantissa bits for the price of the otherwise idle half of the operand.
+//
+// Warps and tiles are what 64 rows of up to 4096 tokens (16 heads of 64, bf16) run best with: eight warps, each of which
+// idles while its 16 KB fly but has seven others beside it, 87 us; 10 or 12 such warps 90 and 89, six or four with two
+// tiles in flight each 101 and 105, eight with two tiles of 8 KB 97.
 template <int Width>
 struct Bf16Tile {
   static constexpr int D = Width;
-  static constexpr int KT = kTileBytes / (2 * D);
+  static constexpr int kTile = 8192, kWarps = 8, kPairWarps = 4;
+  static constexpr int KT = kTile / (2 * D);
   static constexpr int NT = KT / 8;     // 8-key tiles
   static constexpr int KC = KT / 16;    // 16-key steps of P V
   static constexpr int DK = D / 16;     // 16-dim steps of Q K^T
@@ -102,7 +107,7 @@ struct Bf16Tile {
   template <bool WHOLE>
   static __device__ __forceinline__ void step(const MmaArgs& a, uint32_t sk, const Query& x, const Side&, State& st,
                                               int live, uint32_t mask, int lane) {
-    const uint32_t sv = sk + kTileBytes;
+    const uint32_t sv = sk + kTile;
     const int r8 = lane & 7, q4 = lane >> 3, t = lane & 3;
     if (!WHOLE) {
       // absent values become 0: their weight 0 would not cancel a stale NaN or infinity
@@ -217,13 +222,10 @@ struct Bf16Tile {
   }
 };
 
-// Keys of a tile of the tensor-core kernels for a head_dim.
-inline int tile_keys(int dim) { return kTileBytes / (2 * mma_width(dim)); }
-
 // Does a launch of these sizes go to the tensor-core kernel (strides and alignment apart)?
 inline bool mma_sizes(int dtype, int B, int H, int D, int table_width, int page_size) {
   return dtype == ENGPT_BF16 && D <= 128 && D % 8 == 0 && page_size % 8 == 0 &&
-         list_fits(B, H, tile_keys(D), table_width, page_size);
+         list_fits(B, H, mma_width(D) == 64 ? Bf16Tile<64>::KT : Bf16Tile<128>::KT, table_width, page_size);
 }
 
 }  // namespace paged
@@ -239,7 +241,9 @@ extern "C" int64_t engpt_paged_attention_floats(int dtype, int B, int H, int Hkv
   const int64_t simt = splits > kSimtCluster ? (int64_t)B * H * splits * (Dh + 2) : 0;
   if (!mma_sizes(dtype, B, H, Dh, table_width, page_size)) return simt;
   // strides and alignment decide at the call which of the two kernels runs
-  const int64_t mma = pair_ctas(B, H, Hkv, tile_keys(Dh), table_width, page_size) == 0 ? mma_floats(H, Hkv, Dh) : 0;
+  const int cs = mma_width(Dh) == 64 ? pair_ctas<Bf16Tile<64>>(B, H, Hkv, table_width, page_size)
+                                     : pair_ctas<Bf16Tile<128>>(B, H, Hkv, table_width, page_size);
+  const int64_t mma = cs == 0 ? mma_floats(H, Hkv, Dh) : 0;
   return simt > mma ? simt : mma;
 }
 

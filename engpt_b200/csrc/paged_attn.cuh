@@ -335,14 +335,15 @@ int launch_simt_heads(const typename KV::Args& a, cudaStream_t st) {
 
 // ------------------------------------------------------------------ tensor-core kernels
 //
-// A tile is KT keys of one kv head, kTileBytes of keys and as many of values.  The tiles of all (row, kv head) pairs
+// A tile is KT keys of one kv head, kTile bytes of keys and as many of values.  The tiles of all (row, kv head) pairs
 // form one list, cut into contiguous ranges of equal cost, one per warp ("worker") of a persistent grid, so the load is
-// even whatever the lengths.  A warp fetches its own tiles, one at a time, into its own 16 KB of shared memory:
+// even whatever the lengths.  A warp fetches its own tiles, one at a time, into its own 2 kTile bytes of shared memory:
 // TMA boxes of R rows (R divides the page size) at the page that the block table names, swizzled, completing
 // on the warp's mbarrier; no warp waits for another one until the end.
 //
 // What a tile holds and how it is used is the business of a class F:
 //   D, KT              width (a smaller head_dim is padded with zeros by TMA, in shared memory only), keys of a tile
+//   kTile, kWarps, kPairWarps    bytes of a tile's keys, warps of a CTA of the list form and of the pair form
 //   T, Args            type of q and o; kernel arguments (MmaArgs and what F adds)
 //   kBoxes, kBoxRow    boxes of 64 columns of a group of R keys, bytes of a row of one
 //   Spot, find         a look-up that is made a tile ahead of the tile's copies
@@ -356,14 +357,7 @@ int launch_simt_heads(const typename KV::Args& a, cudaStream_t st) {
 // A range that begins or ends inside a pair leaves a part (o, m, l) in shared memory.  After a CTA barrier the parts
 // of a pair are joined by the warp that holds its first one; a pair that runs over CTAs leaves one part per CTA in
 // the workspace, joined by decode_join_list_kernel.
-//
-// Warps and tiles are what 64 rows of up to 4096 tokens (16 heads of 64, bf16) run best with: eight warps, each of which
-// idles while its 16 KB fly but has seven others beside it, 87 us; 10 or 12 such warps 90 and 89, six or four with two
-// tiles in flight each 101 and 105, eight with two tiles of 8 KB 97.
-constexpr int kWarps = 8;
-constexpr int kPairWarps = 4;           // of the form with a cluster per pair: two CTAs per SM
-constexpr size_t kPairSmem = 80 * 1024;
-constexpr int kTileBytes = 8192;        // one of K, V
+constexpr size_t kPairSmem = 80 * 1024;  // of the form with a cluster per pair, at least: two CTAs per SM
 constexpr int kMaxListRows = 8192;      // of the list form: an int of shared memory each
 
 struct MmaArgs {
@@ -468,7 +462,7 @@ struct Worker {
 #pragma unroll
       for (int half = 0; half < F::kBoxes; ++half) {
         sm100::tma_load_4d(dst + half * F::KT * F::kBoxRow, mk, half * 64, x.off, c.hk, x.page, bar);
-        sm100::tma_load_4d(dst + half * F::KT * F::kBoxRow + kTileBytes, mv, half * 64, x.off, c.hk, x.page, bar);
+        sm100::tma_load_4d(dst + half * F::KT * F::kBoxRow + F::kTile, mv, half * 64, x.off, c.hk, x.page, bar);
       }
     } else if (x.off >= 0) {   // a page outside the pool
       record_device_error(ENGPT_ERR_ARG, 44);
@@ -491,6 +485,7 @@ struct Worker {
 template <typename F, int N, typename Part>
 __device__ __forceinline__ void join_row(const MmaArgs& a, int b, int h, int r, int n, Part part, float* to, int lane) {
   constexpr int D = F::D, E = D / 32;
+  constexpr int half = N > 16 ? 16 : N > 8 ? 8 : N > 4 ? 4 : N > 2 ? 2 : 1;   // of the lanes that hold a part
   if ((h % a.QG) * 8 + r >= a.G) return;
   float m = -INFINITY, l = 0.f;
   if (lane < n) {
@@ -500,12 +495,12 @@ __device__ __forceinline__ void join_row(const MmaArgs& a, int b, int h, int r, 
   }
   float mx = m;
 #pragma unroll
-  for (int k = N / 2; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+  for (int k = half; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
   mx = __shfl_sync(0xffffffffu, mx, 0);
   const float w = join_weight(m, mx);
   l *= w;
 #pragma unroll
-  for (int k = N / 2; k > 0; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
+  for (int k = half; k > 0; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
   l = __shfl_sync(0xffffffffu, l, 0);
   float x[N][E], o[E] = {};
 #pragma unroll
@@ -544,7 +539,7 @@ __host__ __device__ constexpr int part_floats(int rows) {
 // First unit of every row, s_start[0 .. B] (exclusive prefix sums of a row's units times HQ), by a CTA of `threads`
 // threads; returns their number.  For up to 32 rows every warp forms the same sums for itself (the warps write the
 // same numbers) and keeps row `lane`'s length and first tile in `len` and `start`: no barrier before the first copy.
-template <int KT>
+template <typename F>
 __device__ __forceinline__ int list_starts(const MmaArgs& a, int* s_start, int* s_scan, int threads, bool record,
                                            int& len, int& start) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -557,7 +552,7 @@ __device__ __forceinline__ int list_starts(const MmaArgs& a, int* s_start, int* 
       if (record && len > (int64_t)a.W * a.ps) record_device_error(ENGPT_ERR_ARG, 44);
       len = clip_length(a, len);
     }
-    const int v = pair_units(a, (len + KT - 1) / KT) * a.HQ;
+    const int v = pair_units(a, (len + F::KT - 1) / F::KT) * a.HQ;
     int x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -576,7 +571,7 @@ __device__ __forceinline__ int list_starts(const MmaArgs& a, int* s_start, int* 
     __syncthreads();
     int before = carry, total = 0;
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
+    for (int i = 0; i < F::kWarps; ++i) {
       if (i < warp) before += s_scan[i];
       total += s_scan[i];
     }
@@ -590,8 +585,9 @@ __device__ __forceinline__ int list_starts(const MmaArgs& a, int* s_start, int* 
 }
 
 // Units of a worker; at least a tile's, so that no worker between two others of a pair is without one of its tiles.
+template <typename F>
 __device__ __forceinline__ int worker_units(const MmaArgs& a, int total, int ctas) {
-  const uint32_t workers = ctas * kWarps;
+  const uint32_t workers = ctas * F::kWarps;
   return max(a.tile_units, (int)(((uint32_t)total + workers - 1) / workers));
 }
 
@@ -611,21 +607,21 @@ __device__ __forceinline__ int list_row(const MmaArgs& a, const int* s_start, in
 
 // The persistent form over the list of tiles.
 template <typename F>
-__global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(typename F::Args a,
+__global__ void __launch_bounds__(F::kWarps * 32) decode_list_kernel(typename F::Args a,
                                                                  const __grid_constant__ CUtensorMap mk,
                                                                  const __grid_constant__ CUtensorMap mv) {
   constexpr int D = F::D;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (sm100::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* tiles = smem_raw + (base - sm100::smem_u32(smem_raw));           // one of each warp
-  uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + kWarps * 2 * kTileBytes);   // [kWarps]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + F::kWarps * 2 * F::kTile);   // [F::kWarps]
   const int pf = part_floats<D>(a.rows);
-  float* s_part = reinterpret_cast<float*>(bars + kWarps);                  // [kWarps] first part of each warp
-  int* s_start = reinterpret_cast<int*>(s_part + kWarps * pf);              // [B + 1] first unit of each row
-  __shared__ int s_abort, s_scan[kWarps], s_head[kWarps], s_tail[kWarps], s_over[kWarps];
+  float* s_part = reinterpret_cast<float*>(bars + F::kWarps);                  // [F::kWarps] first part of each warp
+  int* s_start = reinterpret_cast<int*>(s_part + F::kWarps * pf);              // [B + 1] first unit of each row
+  __shared__ int s_abort, s_scan[F::kWarps], s_head[F::kWarps], s_tail[F::kWarps], s_over[F::kWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  Worker<F> w{a, &mk, &mv, base + warp * 2 * kTileBytes, sm100::smem_u32(bars + warp), lane};
+  Worker<F> w{a, &mk, &mv, base + warp * 2 * F::kTile, sm100::smem_u32(bars + warp), lane};
   if (lane == 0) {
     sm100::mbar_init(w.bar, 1);
     sm100::fence_mbar_init();
@@ -640,10 +636,10 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(typename F::Ar
   asm volatile("griddepcontrol.wait;" ::: "memory");   // nothing of an earlier kernel has been touched before
 
   // this worker's range [u0, u1) of the list's units and its first tile: the tiles that begin in the range are its own
-  const int worker = blockIdx.x * kWarps + warp;
+  const int worker = blockIdx.x * F::kWarps + warp;
   int row_len = 0, row_start = 0;
-  const int total = list_starts<F::KT>(a, s_start, s_scan, kWarps * 32, blockIdx.x == 0, row_len, row_start);
-  const int per = worker_units(a, total, gridDim.x);
+  const int total = list_starts<F>(a, s_start, s_scan, F::kWarps * 32, blockIdx.x == 0, row_len, row_start);
+  const int per = worker_units<F>(a, total, gridDim.x);
   const int u0 = (int)min((int64_t)total, (int64_t)worker * per), u1 = (int)min((int64_t)total, (int64_t)u0 + per);
   Cursor c;
   c.b = list_row(a, s_start, u0, row_start);
@@ -681,8 +677,8 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(typename F::Ar
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // rows without keys
-  for (int64_t i = blockIdx.x * (int64_t)(kWarps * 32) + tid; i < (int64_t)a.B * a.H;
-       i += (int64_t)gridDim.x * kWarps * 32) {
+  for (int64_t i = blockIdx.x * (int64_t)(F::kWarps * 32) + tid; i < (int64_t)a.B * a.H;
+       i += (int64_t)gridDim.x * F::kWarps * 32) {
     const int b = (int)(i / a.H);
     if (s_start[b + 1] == s_start[b])
       for (int e = 0; e < a.dim; e += 16 / (int)sizeof(typename F::T))
@@ -690,7 +686,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(typename F::Ar
   }
 
   float* part = s_part + warp * pf;                                         // a pair that began before this range
-  float* tail_part = reinterpret_cast<float*>(tiles + warp * 2 * kTileBytes);   // one that ends behind it (no tile left)
+  float* tail_part = reinterpret_cast<float*>(tiles + warp * 2 * F::kTile);   // one that ends behind it (no tile left)
   typename F::State st;
   st.reset();
   typename F::Query qa;
@@ -731,7 +727,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(typename F::Ar
         if (lane == 0) {
           s_tail[warp] = c.b * a.HQ + c.h;
           // does its last tile begin behind this CTA's units?
-          s_over[warp] = (int64_t)c.u + (c.T - 1 - c.t) * a.tile_units >= (int64_t)(blockIdx.x + 1) * kWarps * per;
+          s_over[warp] = (int64_t)c.u + (c.T - 1 - c.t) * a.tile_units >= (int64_t)(blockIdx.x + 1) * F::kWarps * per;
         }
       } else {
         F::store_part(a, st, part, lane);
@@ -753,44 +749,44 @@ __global__ void __launch_bounds__(kWarps * 32) decode_list_kernel(typename F::Ar
     if (pair < 0) return;
     const int w0 = max(g, 0);
     int n = g < 0 ? 0 : 1;
-    while (w0 + n < kWarps && s_head[w0 + n] == pair) ++n;
-    const float* first = g < 0 ? s_part : reinterpret_cast<const float*>(tiles + g * 2 * kTileBytes);
+    while (w0 + n < F::kWarps && s_head[w0 + n] == pair) ++n;
+    const float* first = g < 0 ? s_part : reinterpret_cast<const float*>(tiles + g * 2 * F::kTile);
     const float* rest = s_part + g * pf;
     float* to = g < 0 ? out : (s_over[g] ? out + pf : nullptr);   // at most one pair runs over the CTA's end
     const int b = pair / a.HQ, h = pair - b * a.HQ;
     for (int r = r0; r < a.rows; r += step)
-      join_row<F, kWarps>(a, b, h, r, n, [=](int i) { return i == 0 ? first : (g < 0 ? first : rest) + i * pf; }, to, lane);
+      join_row<F, F::kWarps>(a, b, h, r, n, [=](int i) { return i == 0 ? first : (g < 0 ? first : rest) + i * pf; }, to, lane);
   };
-  if (a.rows < kWarps) {
+  if (a.rows < F::kWarps) {
     join_group(warp, 0, 1);
-    if (warp == kWarps - 1) join_group(-1, 0, 1);
+    if (warp == F::kWarps - 1) join_group(-1, 0, 1);
   } else {
-    for (int g = -1; g < kWarps; ++g) join_group(g, warp, kWarps);
+    for (int g = -1; g < F::kWarps; ++g) join_group(g, warp, F::kWarps);
   }
 }
 
-// One cluster of `cs` CTAs per pair: tile t goes to warp t mod (cs * kPairWarps) of the cluster, whose parts are joined
+// One cluster of `cs` CTAs per pair: tile t goes to warp t mod (cs * F::kPairWarps) of the cluster, whose parts are joined
 // through shared memory, then through the shared memory of the cluster's first CTA.  No prefix sums, no second
 // launch, and the first page look-up does not wait for the length: the form for short rows and for few pairs.
 template <typename F>
-__global__ void __launch_bounds__(kPairWarps * 32) decode_pair_kernel(typename F::Args a,
+__global__ void __launch_bounds__(F::kPairWarps * 32) decode_pair_kernel(typename F::Args a,
                                                                      const __grid_constant__ CUtensorMap mk,
                                                                      const __grid_constant__ CUtensorMap mv, int cs) {
   constexpr int D = F::D;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (sm100::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* tiles = smem_raw + (base - sm100::smem_u32(smem_raw));           // one of each warp
-  uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + kPairWarps * 2 * kTileBytes);  // [kPairWarps]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + F::kPairWarps * 2 * F::kTile);  // [F::kPairWarps]
   const int pf = part_floats<D>(a.rows);
-  float* s_part = reinterpret_cast<float*>(bars + kPairWarps);              // [kPairWarps] the warps' parts
-  float* s_cta = s_part + kPairWarps * pf;                                  // [cs] the CTAs' parts (rank 0)
+  float* s_part = reinterpret_cast<float*>(bars + F::kPairWarps);              // [F::kPairWarps] the warps' parts
+  float* s_cta = s_part + F::kPairWarps * pf;                                  // [cs] the CTAs' parts (rank 0)
   __shared__ int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (cs > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
   const int pair = blockIdx.x / cs, rank = blockIdx.x - pair * cs;
-  const int me = rank * kPairWarps + warp, step = cs * kPairWarps;
-  Worker<F> w{a, &mk, &mv, base + warp * 2 * kTileBytes, sm100::smem_u32(bars + warp), lane};
+  const int me = rank * F::kPairWarps + warp, step = cs * F::kPairWarps;
+  Worker<F> w{a, &mk, &mv, base + warp * 2 * F::kTile, sm100::smem_u32(bars + warp), lane};
   Cursor c;
   c.b = pair / a.HQ;
   c.h = pair - c.b * a.HQ;
@@ -856,27 +852,27 @@ __global__ void __launch_bounds__(kPairWarps * 32) decode_pair_kernel(typename F
     if (cs > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     return;
   }
-  const int mine = min(max(c.T - rank * kPairWarps, 0), kPairWarps);   // this CTA's warps with tiles
+  const int mine = min(max(c.T - rank * F::kPairWarps, 0), F::kPairWarps);   // this CTA's warps with tiles
   if (warp < mine && ok) F::store_part(a, st, s_part + warp * pf, lane);
   __syncthreads();
   const float* parts = s_part;
   if (cs == 1) {
-    for (int r = warp; r < a.rows; r += kPairWarps)
-      join_row<F, kPairWarps>(a, c.b, c.h, r, mine, [=](int i) { return parts + i * pf; }, nullptr, lane);
+    for (int r = warp; r < a.rows; r += F::kPairWarps)
+      join_row<F, F::kPairWarps>(a, c.b, c.h, r, mine, [=](int i) { return parts + i * pf; }, nullptr, lane);
     return;
   }
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // every CTA of the cluster has started
   if (mine > 0) {
     float* to;
     asm("mapa.u64 %0, %1, %2;" : "=l"(to) : "l"(s_cta + rank * pf), "r"(0));
-    for (int r = warp; r < a.rows; r += kPairWarps)
-      join_row<F, kPairWarps>(a, c.b, c.h, r, mine, [=](int i) { return parts + i * pf; }, to, lane);
+    for (int r = warp; r < a.rows; r += F::kPairWarps)
+      join_row<F, F::kPairWarps>(a, c.b, c.h, r, mine, [=](int i) { return parts + i * pf; }, to, lane);
   }
   sm100::cluster_sync_all();
   if (rank == 0) {
     const float* ctas = s_cta;
-    const int k = min(cs, (c.T + kPairWarps - 1) / kPairWarps);                 // CTAs with tiles
-    for (int r = warp; r < a.rows; r += kPairWarps)
+    const int k = min(cs, (c.T + F::kPairWarps - 1) / F::kPairWarps);                 // CTAs with tiles
+    for (int r = warp; r < a.rows; r += F::kPairWarps)
       join_row<F, 8>(a, c.b, c.h, r, k, [=](int i) { return ctas + i * pf; }, nullptr, lane);
   }
 }
@@ -886,17 +882,17 @@ __global__ void __launch_bounds__(kPairWarps * 32) decode_pair_kernel(typename F
 // It starts while that kernel runs (whose CTAs have by then waited for all earlier work) and finds its pair from the
 // lengths; only the parts have to wait.
 template <typename F>
-__global__ void __launch_bounds__(kWarps * 32) decode_join_list_kernel(MmaArgs a, int ctas) {
+__global__ void __launch_bounds__(F::kWarps * 32) decode_join_list_kernel(MmaArgs a, int ctas) {
   constexpr int D = F::D, E = D / 32;
   extern __shared__ int s_start[];
-  __shared__ float s_o[kWarps][D];
-  __shared__ float s_m[kWarps], s_l[kWarps];
-  __shared__ int s_scan[kWarps];
+  __shared__ float s_o[F::kWarps][D];
+  __shared__ float s_m[F::kWarps], s_l[F::kWarps];
+  __shared__ int s_scan[F::kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   int row_len = 0, row_start = 0;
-  const int total = list_starts<F::KT>(a, s_start, s_scan, kWarps * 32, false, row_len, row_start);
-  const int64_t per = (int64_t)kWarps * worker_units(a, total, ctas);   // of a CTA
+  const int total = list_starts<F>(a, s_start, s_scan, F::kWarps * 32, false, row_len, row_start);
+  const int64_t per = (int64_t)F::kWarps * worker_units<F>(a, total, ctas);   // of a CTA
   int first = 0, n = 0, b = 0, h = 0;
   if ((int)gridDim.x < ctas) {                        // pair blockIdx.x
     b = blockIdx.x / a.HQ;
@@ -926,7 +922,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_join_list_kernel(MmaArgs a
   if (n > 0 && (h % a.QG) * 8 + r < a.G) {
     float m = -INFINITY, l = 0.f, o[E] = {};
 #pragma unroll 4
-    for (int i = warp; i < n; i += kWarps) {
+    for (int i = warp; i < n; i += F::kWarps) {
       const float* p = a.work + ((int64_t)(first + i) * 2 + (i == 0 ? 1 : 0)) * pf + r * (D + 2);
       const float2 ml = *reinterpret_cast<const float2*>(p + D);
       const float mx = fmaxf(m, ml.x);
@@ -946,10 +942,10 @@ __global__ void __launch_bounds__(kWarps * 32) decode_join_list_kernel(MmaArgs a
     if (threadIdx.x < a.dim) {
       float mx = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < kWarps; ++i) mx = fmaxf(mx, s_m[i]);
+      for (int i = 0; i < F::kWarps; ++i) mx = fmaxf(mx, s_m[i]);
       float lx = 0.f, ox = 0.f;
 #pragma unroll
-      for (int i = 0; i < kWarps; ++i) {
+      for (int i = 0; i < F::kWarps; ++i) {
         const float wgt = join_weight(s_m[i], mx);
         lx = fmaf(s_l[i], wgt, lx);
         ox = fmaf(s_o[i][threadIdx.x], wgt, ox);
@@ -1014,14 +1010,15 @@ inline bool list_fits(int B, int H, int KT, int table_width, int page_size) {
 // tiles / 380 (16 pairs of 128 tiles: 12.3 against 13.0 us, 8 pairs of 128: 10.7 against 9.6, 16 pairs of 256: 19.2
 // against 18.5), and, as the rows of a batch may differ and the longest one decides, with at most 4 tiles per warp if
 // there are several rows (8 rows of 16 pairs of 32 tiles: 15.4 us against the list's 17.0 if all are that long).
-inline int pair_ctas(int B, int H, int Hkv, int KT, int table_width, int page_size) {
+template <typename F>
+int pair_ctas(int B, int H, int Hkv, int table_width, int page_size) {
   const int64_t pairs = (int64_t)B * Hkv * ((H / Hkv + 7) / 8);
-  const int64_t tiles = most_tiles(KT, table_width, page_size);
+  const int64_t tiles = most_tiles(F::KT, table_width, page_size);
   const int sms = num_sms();
   if (pairs > 2 * sms) return 0;
   int cs = pairs * 8 <= sms ? 8 : pairs * 4 <= 2 * sms ? 4 : pairs * 2 <= 2 * sms ? 2 : 1;
-  while (cs > 1 && tiles <= kPairWarps * (cs / 2)) cs >>= 1;
-  const int64_t per_warp = (tiles + kPairWarps * cs - 1) / (kPairWarps * cs);
+  while (cs > 1 && tiles <= F::kPairWarps * (cs / 2)) cs >>= 1;
+  const int64_t per_warp = (tiles + F::kPairWarps * cs - 1) / (F::kPairWarps * cs);
   if (B > 1 && per_warp > 4) return 0;
   return 2 * (per_warp - 1) <= 2 + pairs * tiles / 380 ? cs : 0;
 }
@@ -1032,9 +1029,9 @@ inline int64_t mma_floats(int H, int Hkv, int D) {
   return (int64_t)num_sms() * 2 * rows * (mma_width(D) + 2);
 }
 
-template <int D>
+template <typename F>
 size_t mma_smem(int rows, int warps, int parts) {
-  return 1024 + (size_t)warps * (2 * kTileBytes + 8) + 4 * (size_t)parts * part_floats<D>(rows);
+  return 1024 + (size_t)warps * (2 * F::kTile + 8) + 4 * (size_t)parts * part_floats<F::D>(rows);
 }
 
 template <typename F>
@@ -1042,14 +1039,16 @@ int launch_pair(const typename F::Args& a, const CUtensorMap& mk, const CUtensor
   auto kern = decode_pair_kernel<F>;
   // Two CTAs per SM and no third one, which would leave other SMs idle (one wave has at most two per SM; 128 pairs of 32
   // tiles: 15.2 us so, 16.5 if three fit).
-  const size_t needed = mma_smem<F::D>(a.rows, kPairWarps, kPairWarps + cs), smem = needed > kPairSmem ? needed : kPairSmem;
+  constexpr size_t floor = kPairSmem;
+  const size_t needed = mma_smem<F>(a.rows, F::kPairWarps, F::kPairWarps + cs), smem = needed > floor ? needed : floor;
   // (the attribute is the kernel's, not the launch's: every call sets it to the same, largest size, so that a call on
   // another host thread cannot lower it between here and the launch)
+  const size_t most = mma_smem<F>(8, F::kPairWarps, F::kPairWarps + 8);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)mma_smem<F::D>(8, kPairWarps, kPairWarps + 8));
+                                       (int)(most > floor ? most : floor));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((int64_t)a.B * a.HQ * cs));
-  cfg.blockDim = dim3(kPairWarps * 32);
+  cfg.blockDim = dim3(F::kPairWarps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -1068,14 +1067,14 @@ int launch_pair(const typename F::Args& a, const CUtensorMap& mk, const CUtensor
 template <typename F>
 int launch_list(const typename F::Args& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t st) {
   auto kern = decode_list_kernel<F>;
-  const size_t smem = mma_smem<F::D>(a.rows, kWarps, kWarps) + 4 * ((size_t)a.B + 1);
+  const size_t smem = mma_smem<F>(a.rows, F::kWarps, F::kWarps) + 4 * ((size_t)a.B + 1);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,   // as in launch_pair
-                                       (int)(mma_smem<F::D>(8, kWarps, kWarps) + 4 * ((size_t)kMaxListRows + 1)));
+                                       (int)(mma_smem<F>(8, F::kWarps, F::kWarps) + 4 * ((size_t)kMaxListRows + 1)));
   if (e != cudaSuccess) return set_error(ENGPT_ERR_LAUNCH, "paged_attention: %s", cudaGetErrorString(e));
   // both kernels may be started before what runs ahead of them has ended; they wait for it on the device
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)num_sms());
-  cfg.blockDim = dim3(kWarps * 32);
+  cfg.blockDim = dim3(F::kWarps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr;
@@ -1128,11 +1127,11 @@ int launch_mma(typename F::Args a, const AttnArgs& x, int Hkv, cudaStream_t st) 
     return rc;
   if ((rc = page_map(&mv, x.v_pages, F::kMapType, esz, F::kBoxRow, F::kSwizzle, x.Dh, x.ps, Hkv, x.P, x.vs, a.R)))
     return rc;
-  const int cs = pair_ctas(x.B, x.H, Hkv, F::KT, x.W, x.ps);
+  const int cs = pair_ctas<F>(x.B, x.H, Hkv, x.W, x.ps);
   // The end of a pair costs a worker about half a tile (its sums and stores, and tiles that are partly empty).  It is
   // counted once workers see such ends often (256 rows of 1 to 512 tokens: 51.8 us, 63.8 without); with few pairs the
   // ranges are whole tiles, which cuts fewer pairs (32 rows of 512 tokens, 16 heads: 16.9 us, 18.5 with).
-  const bool ends = 2 * (int64_t)x.B * a.HQ > (int64_t)num_sms() * kWarps;
+  const bool ends = 2 * (int64_t)x.B * a.HQ > (int64_t)num_sms() * F::kWarps;
   a.tile_units = ends ? 2 : 1;
   a.end_units = ends ? 1 : 0;
   if (cs == 0) return launch_list<F>(a, mk, mv, st);

@@ -58,17 +58,24 @@ int dispatch_simt_q8(const Q8AttnArgs& a, bool vec, cudaStream_t st) {
 
 // ------------------------------------------------------------------ tensor-core kernel (head_dim up to 128)
 //
-// The codes are exact in fp16 (int8: integers up to 127; e4m3: 4 significant bits, 2^-9 to 448), so both products run on
-// fp16 operands with fp32 sums:
+// Scores of int8 codes are products of whole numbers (mma.sync on 8-bit integers, 32-bit sums, exact): a row of q, times a
+// power of two, is rounded to 16 bits (fp32 q: 24), which are two (three) digits of 8 bits; the first two are rows 0-7
+// and 8-15 of one operand, so the second one is free.  What that rounding takes from q is below 2^-15 (2^-23) of the row's
+// largest element; the codes themselves are that of a number rounded to 2^-8 of a block's largest one.
+//
+// e4m3 codes, and all values, are exact in fp16 (4 significant bits, 2^-9 to 448; integers up to 127), so these products run
+// on fp16 operands with fp32 sums:
 //   S = Q K^T with q brought to [1, 2) by a power of two of its row, which the row's score factor takes back; a
 //   fp32 q is two fp16 numbers, the second one (what the first left, times 2^11) in the otherwise idle rows 8-15;
-//   O += P V with p vs / vref in fp16, vref the largest value scale so far (raised like the running maximum of the
-//   softmax): at most 2^14 as scaled, so that what is 2^-28 of the largest weight is still a normal number; the
-//   remainder of that rounding, again fp16, in rows 8-15.  Weights have 22 bits so.
+//   O^T += V^T P^T with p vs / vref in fp16, vref the largest value scale so far (raised like the running maximum of the
+//   softmax): at most 2^14 as scaled, so that what is 2^-28 of the largest weight is still a normal number.  That
+//   rounding is 2^-11 of a weight, an eighth of that of a bf16 result; for fp32 results what it left is multiplied
+//   too.  (O^T because its 16-row operand is full of values, where that of O would be half empty.)
 //
 // The columns of a product may come in any order that both operands share, and keys and columns of O in any order at
-// all: a 16-byte row of 8-bit codes that ldmatrix distributes (4 bytes a lane, in place of two 16-bit numbers) becomes the
-// fragments of two steps or tiles by byte permutations, with no transposition of bytes.
+// all: a 16-byte row of 8-bit codes that ldmatrix distributes (4 bytes a lane, in place of two 16-bit numbers) is the
+// fragment of an 8-bit product, or becomes those of two steps or tiles by byte permutations, with no transposition of
+// bytes.
 template <typename C>
 struct CodePairs;
 // Two codes of w, at the bytes that SEL names in the permutation's order, as fp16.
@@ -102,6 +109,13 @@ __device__ __forceinline__ void mma16816_f16(float* c, uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void mma16832_s8(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                            uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 __device__ __forceinline__ uint32_t pack_half2(float x, float y) {
   const __half2 h = __floats2half2_rn(x, y);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -124,16 +138,18 @@ struct Q8MmaArgs : MmaArgs {
 template <int Width, typename C, typename Type>
 struct Q8Tile {
   static constexpr int D = Width;
-  static constexpr int KT = kTileBytes / D;
+  static constexpr int kTile = 8192, kWarps = 8, kPairWarps = 4;
+  static constexpr int KT = kTile / D;
   static constexpr int NG = KT / 8;       // groups of 8 keys, which share their scales
-  static constexpr int NT = 8;            // of a step's 64 keys: 8-key tiles
-  static constexpr int KC = 4;            // 16-key steps of P V
-  static constexpr int DK = D / 16;       // 16-dim steps of Q K^T
-  static constexpr int DN = D / 8;        // 8-dim tiles of O
+  static constexpr int kStep = KT < 64 ? KT : 64;   // keys of a softmax step
+  static constexpr int NT = kStep / 8;    // 8-key tiles of a step
+  static constexpr int KC = kStep / 16;   // 16-key steps of P V
+  static constexpr int DC = D / 16;       // 16-byte pieces of a row
+  static constexpr bool kInt = C::kInteger;
   static constexpr int kCodeBytes = 1, kBoxes = 1, kBoxRow = D;
   static constexpr CUtensorMapDataType kMapType = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   static constexpr CUtensorMapSwizzle kSwizzle = D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
-  static constexpr bool kTwoParts = sizeof(Type) == 4;   // of q
+  static constexpr bool kFine = sizeof(Type) == 4;   // three digits or two parts of q, two parts of a weight
   static constexpr float kWeightTop = 16384.f;
   using T = Type;
   using Args = Q8MmaArgs;
@@ -146,20 +162,34 @@ struct Q8Tile {
     float scale;     // 0 without a key
   };
   struct Query {
-    uint32_t hi[DK][2], lo[kTwoParts ? DK : 1][2];
+    uint32_t a[DC], b[kInt || kFine ? DC : 1], c[kInt && kFine ? DC : 1];   // int8: the digits; else see load_query
+    uint32_t a2[kInt ? 1 : DC], b2[!kInt && kFine ? DC : 1];
     float factor;    // base-2 score of a sum of products
   };
   struct State {
-    float o[DN][4];  // tile 2c: columns 16 c + 2 i, tile 2c + 1: 16 c + 2 i + 1, in units of vref / kWeightTop
+    // piece c, row of O^T: columns 16 c + 2 g and 16 c + 2 g + 1 (0, 1 and 2, 3) of heads 2 t and 2 t + 1 of the group, in
+    // units of vref / kWeightTop, where g = lane / 4 and t = lane % 4.  m and l are those of head g.
+    float o[DC][4];
     float m, l, vref, factor;
     __device__ __forceinline__ void reset() {
 #pragma unroll
-      for (int i = 0; i < DN; ++i)
+      for (int i = 0; i < DC; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
       m = -INFINITY;
       l = vref = 0.f;
       factor = 1.f;
+    }
+    // Every column of O^T times its head's x.
+    __device__ __forceinline__ void scale_heads(float x, int lane) {
+      const float x0 = __shfl_sync(0xffffffffu, x, 8 * (lane & 3)), x1 = __shfl_sync(0xffffffffu, x, 8 * (lane & 3) + 4);
+#pragma unroll
+      for (int i = 0; i < DC; ++i) {
+        o[i][0] *= x0;
+        o[i][1] *= x1;
+        o[i][2] *= x0;
+        o[i][3] *= x1;
+      }
     }
   };
 
@@ -184,10 +214,10 @@ struct Q8Tile {
     const int head = (h / a.QG) * a.G + (h % a.QG) * 8 + g;
     const bool live = g < a.rows && (h % a.QG) * 8 + g < a.G;
     const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_row + head * a.q_head + 4 * t;
-    float v[DK][4];
+    float v[DC][4];
     uint32_t most = 0;
 #pragma unroll
-    for (int k = 0; k < DK; ++k) {
+    for (int k = 0; k < DC; ++k) {
       if (live && k * 16 < a.dim) {
         if constexpr (sizeof(T) == 2) {
           const uint2 r = *reinterpret_cast<const uint2*>(q + k * 16);
@@ -210,19 +240,80 @@ struct Q8Tile {
     }
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    const uint32_t e = min(max(most >> 23, 1u), 253u);   // the row's largest |q| is in [1, 2) 2^(e - 127), for most rows
-    const float down = __uint_as_float((254u - e) << 23), up = __uint_as_float(e << 23);
-    x.factor = a.scale_log2 * up;
-    const float f = a.negative ? -down : down;
+    if constexpr (kInt) {
+      // round(q 2^(bits - e)): the row's largest element comes to 2^bits up to 2^(bits + 1), but not so near to that that
+      // its first digit would be above 127.  (Rows that are nearly zero, below 2^-100, are brought less far up.)
+      constexpr int bits = kFine ? 22 : 14;
+      const uint32_t e = min(max((most + 0x20000u) >> 23, 27u), 253u);
+      const float up = __uint_as_float((uint32_t)(254 + bits - e) << 23);
+      x.factor = most >= 0x7f800000u ? __uint_as_float(0x7fc00000u)
+                                     : a.scale_log2 * __uint_as_float((uint32_t)(e - bits) << 23);
+      const float f = a.negative ? -up : up;
 #pragma unroll
-    for (int k = 0; k < DK; ++k) {
+      for (int k = 0; k < DC; ++k) {
+        int d[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[k][i] *= f;
+        for (int i = 0; i < 4; ++i) d[i] = __float2int_rn(v[k][i] * f);
+        uint32_t* digits[3] = {&x.a[k], &x.b[k], &x.c[kFine ? k : 0]};
+#pragma unroll
+        for (int n = kFine ? 2 : 1; n >= 0; --n) {
+          *digits[n] = __byte_perm(__byte_perm(d[0], d[1], 0x0040), __byte_perm(d[2], d[3], 0x0040), 0x5410);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d[i] = (d[i] - (int)(int8_t)d[i]) >> 8;
+        }
+      }
+    } else {
+      const uint32_t e = min(max(most >> 23, 1u), 253u);   // the largest |q| is in [1, 2) 2^(e - 127), for most rows
+      const float down = __uint_as_float((254u - e) << 23);
+      x.factor = a.scale_log2 * __uint_as_float(e << 23);
+      const float f = a.negative ? -down : down;
+#pragma unroll
+      for (int k = 0; k < DC; ++k) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[k][i] *= f;
+        x.a[k] = split_half2(v[k][0], v[k][1]);
+        x.a2[k] = split_half2(v[k][2], v[k][3]);
+        if constexpr (kFine) {
+          x.b[k] = pack_half2(v[k][0] * 2048.f, v[k][1] * 2048.f);
+          x.b2[k] = pack_half2(v[k][2] * 2048.f, v[k][3] * 2048.f);
+        }
+      }
+    }
+  }
+
+  // Scores of the 8 keys from `key` on, as sums of products: this lane's two of head g.
+  static __device__ __forceinline__ void scores(const Query& x, uint32_t sk, int key, int lane, float* s) {
+    const int r8 = lane & 7, q4 = lane >> 3;
+    if constexpr (kInt) {
+      int c[4] = {0, 0, 0, 0}, last[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int p = 0; p < DC; p += 4) {
+        uint32_t w[4];
+        ldsm4(piece(sk, key + r8, p + q4), w);
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          mma16832_s8(c, x.a[p + i], x.b[p + i], x.a[p + i + 1], x.b[p + i + 1], w[i], w[i + 1]);
+          if constexpr (kFine) mma16832_s8(last, x.c[p + i], 0u, x.c[p + i + 1], 0u, w[i], w[i + 1]);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        x.hi[k][i] = split_half2(v[k][2 * i], v[k][2 * i + 1]);
-        if constexpr (kTwoParts) x.lo[k][i] = pack_half2(v[k][2 * i] * 2048.f, v[k][2 * i + 1] * 2048.f);
+        s[i] = (float)(c[i] * 256 + c[2 + i]);     // below 2^29
+        if constexpr (kFine) s[i] = fmaf(s[i], 256.f, (float)last[i]);
       }
+    } else {
+      float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int p = 0; p < DC; p += 4) {
+        uint32_t w[4];
+        ldsm4(piece(sk, key + r8, p + q4), w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          mma16816_f16(c, x.a[p + i], kFine ? x.b[p + i] : 0u, x.a2[p + i], kFine ? x.b2[p + i] : 0u,
+                       Pairs::template pair<0, 1>(w[i]), Pairs::template pair<2, 3>(w[i]));
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) s[i] = kFine ? fmaf(c[2 + i], 1.f / 2048.f, c[i]) : c[i];
     }
   }
 
@@ -231,12 +322,12 @@ struct Q8Tile {
     return D == 64 ? base + key * 64 + ((c ^ ((key >> 1) & 3)) << 4) : base + key * 128 + ((c ^ (key & 7)) << 4);
   }
 
-  // One tile: per 64 keys scores, softmax step, P V.  WHOLE: all its keys count.  Otherwise `live` keys from the tile's
+  // One tile: per kStep keys scores, softmax step, P V.  WHOLE: all its keys count.  Otherwise `live` keys from the tile's
   // start are below the length, and boxes whose bit of `mask` is unset were not copied.
   template <bool WHOLE>
   static __device__ __forceinline__ void step(const Args& a, uint32_t sk, const Query& x, const Side& side, State& st,
                                               int live, uint32_t mask, int lane) {
-    const uint32_t sv = sk + kTileBytes;
+    const uint32_t sv = sk + kTile;
     const int r8 = lane & 7, q4 = lane >> 3, t = lane & 3;
     if (!WHOLE && C::kHasNan) {
       // absent values become 0: their weight 0 would not cancel a stale NaN
@@ -254,33 +345,20 @@ struct Q8Tile {
       const float corr = st.vref / __uint_as_float(top);
       st.vref = __uint_as_float(top);
 #pragma unroll
-      for (int i = 0; i < DN; ++i)
+      for (int i = 0; i < DC; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) st.o[i][j] *= corr;
     }
     const float weight = top == 0u ? 0.f : side.scale / st.vref * kWeightTop;   // (0 / 0 for dead groups alone)
 #pragma unroll
-    for (int k0 = 0; k0 < KT; k0 += 64) {
-      float s[NT][4];
+    for (int k0 = 0; k0 < KT; k0 += kStep) {
+      float s[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          uint32_t w[4];
-          ldsm4(piece(sk, k0 + n * 8 + r8, c * 4 + q4), w);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int k = c * 4 + i;
-            const uint32_t y = Pairs::prepare(w[i]);
-            mma16816_f16(s[n], x.hi[k][0], kTwoParts ? x.lo[k][0] : 0u, x.hi[k][1], kTwoParts ? x.lo[k][1] : 0u,
-                         Pairs::template pair<0, 1>(y), Pairs::template pair<2, 3>(y));
-          }
-        }
+        scores(x, sk, k0 + n * 8, lane, s[n]);
         const float ks = __shfl_sync(0xffffffffu, side.scale, k0 / 8 + n);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          if constexpr (kTwoParts) s[n][i] = fmaf(s[n][2 + i], 1.f / 2048.f, s[n][i]);
           s[n][i] *= ks;
           if (!WHOLE) {
             const int key = k0 + n * 8 + 2 * t + i;
@@ -296,14 +374,11 @@ struct Q8Tile {
       const float ms = mx == -INFINITY ? 0.f : mx * st.factor;
       if (__any_sync(0xffffffffu, mx > st.m)) {
         const float corr = st.m == -INFINITY ? 0.f : sm100::ex2_approx(st.m * st.factor - ms);
-#pragma unroll
-        for (int i = 0; i < DN; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) st.o[i][j] *= corr;
+        st.scale_heads(corr, lane);
         st.l *= corr;
         st.m = mx;
       }
-      uint32_t hi[KC][2], lo[KC][2];
+      uint32_t hi[NT], lo[kFine ? NT : 1];
       float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -316,25 +391,28 @@ struct Q8Tile {
           sum[i] += p[i];
           p[i] *= w;
         }
-        hi[n >> 1][n & 1] = split_half2(p[0], p[1]);
-        lo[n >> 1][n & 1] = pack_half2(p[0], p[1]);
+        if constexpr (kFine) {
+          hi[n] = split_half2(p[0], p[1]);
+          lo[n] = pack_half2(p[0], p[1]);
+        } else {
+          hi[n] = pack_half2(p[0], p[1]);
+        }
       }
       st.l += sum[0] + sum[1];
 #pragma unroll
-      for (int j = 0; j < KC; ++j) {
-        const int key = k0 + j * 16 + (q4 & 1) * 8 + r8;
+      for (int j = 0; j < NT; j += 2) {
+        const int key = k0 + j * 8 + (q4 & 1) * 8 + r8;
 #pragma unroll
-        for (int dp = 0; dp < D / 32; ++dp) {
+        for (int c = 0; c < DC; c += 2) {
           uint32_t w[4];
-          ldsm4_t(piece(sv, key, 2 * dp + (q4 >> 1)), w);
+          ldsm4_t(piece(sv, key, c + (q4 >> 1)), w);   // keys 0-7 and 8-15 of piece c, then of piece c + 1
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = Pairs::prepare(w[i]);
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            mma16816_f16(st.o[4 * dp + 2 * c], hi[j][0], lo[j][0], hi[j][1], lo[j][1],
-                         Pairs::template pair<0, 2>(w[2 * c]), Pairs::template pair<0, 2>(w[2 * c + 1]));
-            mma16816_f16(st.o[4 * dp + 2 * c + 1], hi[j][0], lo[j][0], hi[j][1], lo[j][1],
-                         Pairs::template pair<1, 3>(w[2 * c]), Pairs::template pair<1, 3>(w[2 * c + 1]));
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t y0 = Pairs::prepare(w[2 * i]), y1 = Pairs::prepare(w[2 * i + 1]);
+            const uint32_t a0 = Pairs::template pair<0, 2>(y0), a1 = Pairs::template pair<1, 3>(y0),
+                           a2 = Pairs::template pair<0, 2>(y1), a3 = Pairs::template pair<1, 3>(y1);
+            mma16816_f16(st.o[c + i], a0, a1, a2, a3, hi[j], hi[j + 1]);
+            if constexpr (kFine) mma16816_f16(st.o[c + i], a0, a1, a2, a3, lo[j], lo[j + 1]);
           }
         }
       }
@@ -342,45 +420,46 @@ struct Q8Tile {
     if (!WHOLE && C::kHasNan) sm100::fence_proxy_async_smem();   // the zeros above, before a later copy into this memory
   }
 
-  // The pair's sums of this lane: o (both halves, in its own units) and l over the row's four lanes; m in base-2 units.
+  // The pair's sums of this lane: o in its own units and l over the head's four lanes; m in base-2 units.
   static __device__ __forceinline__ void finish(const Args&, State& st) {
     st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
     st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
     if (st.m != -INFINITY) st.m *= st.factor;
     const float unit = st.vref * (1.f / kWeightTop);
 #pragma unroll
-    for (int i = 0; i < DN; ++i) {
-      st.o[i][0] = (st.o[i][0] + st.o[i][2]) * unit;
-      st.o[i][1] = (st.o[i][1] + st.o[i][3]) * unit;
-    }
+    for (int i = 0; i < DC; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) st.o[i][j] *= unit;
   }
 
   static __device__ __forceinline__ void store_part(const Args& a, const State& st, float* part, int lane) {
     const int g = lane >> 2, t = lane & 3;
-    if (g >= a.rows) return;
-    float* p = part + g * (D + 2);
 #pragma unroll
-    for (int i = 0; i < DN; i += 2) {
-      *reinterpret_cast<float2*>(p + i * 8 + 4 * t) = make_float2(st.o[i][0], st.o[i + 1][0]);
-      *reinterpret_cast<float2*>(p + i * 8 + 4 * t + 2) = make_float2(st.o[i][1], st.o[i + 1][1]);
+    for (int r = 0; r < 2; ++r) {
+      if (2 * t + r >= a.rows) break;
+      float* p = part + (2 * t + r) * (D + 2) + 2 * g;
+#pragma unroll
+      for (int i = 0; i < DC; ++i) *reinterpret_cast<float2*>(p + i * 16) = make_float2(st.o[i][r], st.o[i][2 + r]);
     }
-    if (t == 0) *reinterpret_cast<float2*>(p + D) = make_float2(st.m, st.l);
+    if (t == 0 && g < a.rows) *reinterpret_cast<float2*>(part + g * (D + 2) + D) = make_float2(st.m, st.l);
   }
 
-  static __device__ __forceinline__ void store_rows(const Args& a, const State& st, int b, int h, int lane) {
+  static __device__ __forceinline__ void store_rows(const Args& a, State& st, int b, int h, int lane) {
     const int g = lane >> 2, t = lane & 3;
-    const int in = (h % a.QG) * 8 + g;
-    if (g >= a.rows || in >= a.G) return;
-    T* o = reinterpret_cast<T*>(a.o) + ((int64_t)b * a.H + (h / a.QG) * a.G + in) * a.dim + 4 * t;
-    const float inv = st.l == 0.f ? 0.f : 1.f / st.l;
+    st.scale_heads(st.l == 0.f ? 0.f : 1.f / st.l, lane);
 #pragma unroll
-    for (int i = 0; i < DN; i += 2) {
-      if (i * 8 >= a.dim) break;
-      const float v[4] = {st.o[i][0] * inv, st.o[i + 1][0] * inv, st.o[i][1] * inv, st.o[i + 1][1] * inv};
-      if constexpr (sizeof(T) == 2)
-        *reinterpret_cast<uint2*>(o + i * 8) = make_uint2(sm100::pack_bf16x2(v[0], v[1]), sm100::pack_bf16x2(v[2], v[3]));
-      else
-        *reinterpret_cast<float4*>(o + i * 8) = make_float4(v[0], v[1], v[2], v[3]);
+    for (int r = 0; r < 2; ++r) {
+      const int in = (h % a.QG) * 8 + 2 * t + r;
+      if (2 * t + r >= a.rows || in >= a.G) break;
+      T* o = reinterpret_cast<T*>(a.o) + ((int64_t)b * a.H + (h / a.QG) * a.G + in) * a.dim + 2 * g;
+#pragma unroll
+      for (int i = 0; i < DC; ++i) {
+        if (i * 16 >= a.dim) break;
+        if constexpr (sizeof(T) == 2)
+          *reinterpret_cast<uint32_t*>(o + i * 16) = sm100::pack_bf16x2(st.o[i][r], st.o[i][2 + r]);
+        else
+          *reinterpret_cast<float2*>(o + i * 16) = make_float2(st.o[i][r], st.o[i][2 + r]);
+      }
     }
   }
 };
@@ -398,13 +477,14 @@ int launch_mma_q8(const Q8AttnArgs& x, int Hkv, cudaStream_t st) {
   return launch_mma<Q8Tile<D, C, T>>(a, x, Hkv, st);
 }
 
-// Keys of a tile of the tensor-core kernels for a head_dim.
-inline int tile_keys_q8(int dim) { return kTileBytes / mma_width(dim); }
+// (sizes and forms do not depend on the type of the codes, or of q)
+using Q8Tile64 = Q8Tile<64, Int8Code, __nv_bfloat16>;
+using Q8Tile128 = Q8Tile<128, Int8Code, __nv_bfloat16>;
 
 // Does a launch of these sizes go to the tensor-core kernel (strides and alignment apart)?
 inline bool mma_sizes_q8(int B, int H, int D, int table_width, int page_size, int block) {
   return D <= 128 && D % 16 == 0 && page_size % 8 == 0 && block % 8 == 0 &&
-         list_fits(B, H, tile_keys_q8(D), table_width, page_size);
+         list_fits(B, H, mma_width(D) == 64 ? Q8Tile64::KT : Q8Tile128::KT, table_width, page_size);
 }
 
 template <typename T, typename C>
@@ -427,8 +507,9 @@ extern "C" int64_t engpt_paged_attention_q8_floats(int dtype, int B, int H, int 
   const int64_t simt = splits > kSimtCluster ? (int64_t)B * H * splits * (Dh + 2) : 0;
   if (H % Hkv != 0 || !mma_sizes_q8(B, H, Dh, table_width, page_size, block)) return simt;
   // strides and alignment decide at the call which of the two kernels runs
-  const int64_t mma =
-      pair_ctas(B, H, Hkv, tile_keys_q8(Dh), table_width, page_size) == 0 ? mma_floats(H, Hkv, Dh) : 0;
+  const int cs = mma_width(Dh) == 64 ? pair_ctas<Q8Tile64>(B, H, Hkv, table_width, page_size)
+                                     : pair_ctas<Q8Tile128>(B, H, Hkv, table_width, page_size);
+  const int64_t mma = cs == 0 ? mma_floats(H, Hkv, Dh) : 0;
   return simt > mma ? simt : mma;
 }
 

@@ -35,7 +35,7 @@ struct Q8Cache {
 // nearest code, even ones in the middle; NaN gives some code.
 struct Int8Code {
   static constexpr float kTop = 127.f;
-  static constexpr bool kHasNan = false;
+  static constexpr bool kHasNan = false, kInteger = true;
   static __device__ __forceinline__ float decode(uint8_t c) { return (float)(int8_t)c; }
   static __device__ __forceinline__ uint8_t encode(float x) {
     int r;
@@ -46,7 +46,7 @@ struct Int8Code {
 
 struct E4m3Code {
   static constexpr float kTop = 448.f;
-  static constexpr bool kHasNan = true;
+  static constexpr bool kHasNan = true, kInteger = false;
   static __device__ __forceinline__ float decode(uint8_t c) {
     const __half_raw h = __nv_cvt_fp8_to_halfraw(c, __NV_E4M3);
     return __half2float(__half(h));

@@ -145,34 +145,60 @@ def check_store(codes, scales, before, scales_before, x, slots, err=0.0, dead=()
     assert torch.equal(now[untouched], old[untouched])
 
 
-def attention_tolerance(q, ref, vmax, smax, kmax, scale, n):
+def query_error(q, kind):
+    """How far the kernels' form of each element of q may be from it.
+
+    For int8 codes a row is rounded to whole multiples of 2^-22 (fp32) or 2^-14
+    (bf16) of a power of two that its largest element is about at least (0.992):
+    half a step is 2^-23 or 2^-15 of the largest.  A bf16 element of at least 2^-6
+    of it is exact (8 bits from there down are multiples of 2^-14).  For e4m3
+    codes it is two fp16 parts of 11 bits each (fp32: 2^-22, and 2^-35 of the
+    largest for what is too small for them) or one (bf16: its 8 bits fit, but
+    for what lies below 2^-24 of the largest).
+    """
+    x = q.cpu().double().abs()
+    most = x.amax(-1, keepdim=True)
+    if kind == torch.int8:
+        if q.dtype == torch.float32:
+            return (1.01 * 2.0 ** -23 * most).expand(x.shape)
+        return torch.where(x < 2.0 ** -6 * most, torch.minimum(x, 1.01 * 2.0 ** -15 * most), torch.zeros_like(x))
+    if q.dtype == torch.float32:
+        return 2.0 ** -22 * x + 2.0 ** -35 * most
+    return torch.where(x < 2.0 ** -16 * most, torch.minimum(x, 2.0 ** -24 * most), torch.zeros_like(x))
+
+
+def attention_tolerance(q, ref, vmax, smax, dmax, scale, n):
     """How far paged_sdpa_q8 may be from the 64-bit result on the cache's numbers.
 
-    As paged_ref.attention_tolerance (fp32 dot products, exponentials, sums
-    over n terms, one rounding of the result), with: the products with the
-    scales (4 roundings of 2^-24 on scores and weights); q as one or two
-    fp16 numbers of its row's power of two (2^-22 of each element, 2^-24 of
-    the row's largest one); weights as two fp16 parts (2^-21).
-    kmax: the largest sum |k_i| of a key.
+    As paged_ref.attention_tolerance (fp32 dot products of dim terms,
+    exponentials, sums over n terms, one rounding of the result), with the
+    products with the scales (up to 8 roundings of 2^-24 on scores and
+    weights) and the rounding of q (dmax: the largest sum of |k_i| times what q_i
+    may be off by).  The weights of the values are fp16 numbers: for an fp32
+    result two of them, 2^-21; for a bf16 result one, half a step 2^-11, in
+    the sum over the values alone (the weights' own sum is of fp32 numbers), so
+    the weighted mean moves by at most 2^-11 vmax.
     """
     dim = q.shape[2]
-    qmax = q.cpu().double().abs().amax(-1, keepdim=True)
-    score = ((dim + 8) * 2.0 ** -24 + 2.0 ** -22) * smax + 2.0 ** -24 * qmax * kmax * abs(scale)
+    score = (dim + 8) * 2.0 ** -24 * smax + dmax * abs(scale)
     weight = 1.45 * score + 2.0 ** -20 + 2 * n * 2.0 ** -24
-    return torch.finfo(q.dtype).eps / 2 * ref.abs() + 2 * weight * vmax + 1e-30
+    rounded = 0.0 if q.dtype == torch.float32 else 2.0 ** -11
+    return torch.finfo(q.dtype).eps / 2 * ref.abs() + (2 * weight + rounded) * vmax + 1e-30
 
 
 def attention(q, cache, table, lengths, scale):
     """The 64-bit result and its tolerance."""
     k, v = values(cache[0], cache[2]), values(cache[1], cache[3])
     ref, vmax, smax = R.attention(q, k, v, table, lengths, scale)
-    kmax = torch.zeros_like(vmax)
+    off = query_error(q, cache[0].dtype)
+    dmax = torch.zeros_like(vmax)
     group = q.shape[1] // k.shape[1]
     for b, n in enumerate(int(x) for x in lengths.cpu()):
         if n > 0:
-            kmax[b, :, 0] = R.gather_rows(k, table.cpu()[b], n).abs().sum(-1).amax(0).repeat_interleave(group)
+            rows = R.gather_rows(k, table.cpu()[b], n).abs().repeat_interleave(group, dim=1)
+            dmax[b, :, 0] = torch.einsum("nhd,hd->nh", rows, off[b]).amax(0)
     n = max(1, int(lengths.max()) if lengths.numel() else 1)
-    return ref, attention_tolerance(q, ref, vmax, smax, kmax, scale, n)
+    return ref, attention_tolerance(q, ref, vmax, smax, dmax, scale, n)
 
 
 def prompt_slots(first, tokens, page, pool, seed, pad=()):

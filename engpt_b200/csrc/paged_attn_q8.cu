@@ -131,8 +131,8 @@ __device__ __forceinline__ uint32_t split_half2(float& x, float& y) {
 
 struct Q8MmaArgs : MmaArgs {
   const float* scales[2];   // k, v
-  int64_t ss[2][3];
-  int block;                // a multiple of 8
+  int ss[2][3];             // element strides: page, head, block
+  int block, block_shift;   // tokens of a block, a multiple of 8; its logarithm, or -1
 };
 
 template <int Width, typename C, typename Type>
@@ -150,7 +150,7 @@ struct Q8Tile {
   static constexpr CUtensorMapDataType kMapType = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   static constexpr CUtensorMapSwizzle kSwizzle = D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
   static constexpr bool kFine = sizeof(Type) == 4;   // three digits or two parts of q, two parts of a weight
-  static constexpr float kWeightTop = 16384.f;
+  static constexpr float kWeightTop = 16384.f, kLeastScale = 7.52316384526264e-37f;   // 2^-120
   using T = Type;
   using Args = Q8MmaArgs;
   using Pairs = CodePairs<C>;
@@ -170,14 +170,16 @@ struct Q8Tile {
     // piece c, row of O^T: columns 16 c + 2 g and 16 c + 2 g + 1 (0, 1 and 2, 3) of heads 2 t and 2 t + 1 of the group, in
     // units of vref / kWeightTop, where g = lane / 4 and t = lane % 4.  m and l are those of head g.
     float o[DC][4];
-    float m, l, vref, factor;
+    float m, l, vref, per_vref, factor;
     __device__ __forceinline__ void reset() {
 #pragma unroll
       for (int i = 0; i < DC; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
       m = -INFINITY;
-      l = vref = 0.f;
+      l = 0.f;
+      vref = kLeastScale;
+      per_vref = kWeightTop / kLeastScale;
       factor = 1.f;
     }
     // Every column of O^T times its head's x.
@@ -204,9 +206,12 @@ struct Q8Tile {
     const int lane = threadIdx.x & 31, part = lane / NG;
     side.scale = 0.f;
     if (x.off < 0 || c.t * KT + lane % NG * 8 >= c.len || (unsigned)x.page >= (unsigned)a.P) return;
+    const int block = a.block_shift >= 0 ? x.off >> a.block_shift : x.off / a.block;
     const float* p = part == 0 ? a.scales[0] : a.scales[1];
-    const int64_t* s = part == 0 ? a.ss[0] : a.ss[1];
-    side.scale = p[x.page * s[0] + c.hk * s[1] + x.off / a.block * s[2]];
+    p += (int64_t)x.page * (part == 0 ? a.ss[0][0] : a.ss[1][0]);
+    p += (int64_t)c.hk * (part == 0 ? a.ss[0][1] : a.ss[1][1]);
+    p += (int64_t)block * (part == 0 ? a.ss[0][2] : a.ss[1][2]);
+    side.scale = *p;
   }
 
   static __device__ __forceinline__ void load_query(const Args& a, int b, int h, int lane, Query& x) {
@@ -344,12 +349,13 @@ struct Q8Tile {
     if (top > __float_as_uint(st.vref)) {
       const float corr = st.vref / __uint_as_float(top);
       st.vref = __uint_as_float(top);
+      st.per_vref = kWeightTop / st.vref;
 #pragma unroll
       for (int i = 0; i < DC; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) st.o[i][j] *= corr;
     }
-    const float weight = top == 0u ? 0.f : side.scale / st.vref * kWeightTop;   // (0 / 0 for dead groups alone)
+    const float weight = side.scale * st.per_vref;
 #pragma unroll
     for (int k0 = 0; k0 < KT; k0 += kStep) {
       float s[NT][2];
@@ -470,10 +476,11 @@ int launch_mma_q8(const Q8AttnArgs& x, int Hkv, cudaStream_t st) {
   a.scales[0] = x.k_scales;
   a.scales[1] = x.v_scales;
   for (int i = 0; i < 3; ++i) {
-    a.ss[0][i] = x.kss[i];
-    a.ss[1][i] = x.vss[i];
+    a.ss[0][i] = (int)x.kss[i];
+    a.ss[1][i] = (int)x.vss[i];
   }
   a.block = x.block;
+  a.block_shift = (x.block & (x.block - 1)) == 0 ? __builtin_ctz((unsigned)x.block) : -1;
   return launch_mma<Q8Tile<D, C, T>>(a, x, Hkv, st);
 }
 
@@ -582,7 +589,10 @@ extern "C" int engpt_paged_attention_q8(const void* q, const int64_t* q_strides,
   // (the copies of TMA want multiples of 16 bytes; outputs are written in pieces of up to 16)
   bool mma = vec && aligned(k_pages, 16) && aligned(v_pages, 16) && aligned(o, 16) && num_pages > 0 &&
              mma_sizes_q8(B, H, Dh, table_width, page_size, block);
-  for (int i = 0; i < 3; ++i) mma = mma && a.ks[i] > 0 && a.vs[i] > 0 && a.ks[i] % 16 == 0 && a.vs[i] % 16 == 0;
+  for (int i = 0; i < 3; ++i) {
+    mma = mma && a.ks[i] > 0 && a.vs[i] > 0 && a.ks[i] % 16 == 0 && a.vs[i] % 16 == 0;
+    mma = mma && a.kss[i] == (int)a.kss[i] && a.vss[i] == (int)a.vss[i];   // (any scales of less than 2^31 numbers)
+  }
   cudaStream_t st = as_stream(stream);
   if (dtype == ENGPT_BF16)
     return code == ENGPT_CODE_INT8 ? dispatch_q8<__nv_bfloat16, Int8Code>(a, mma, vec, Hkv, st)

@@ -42,6 +42,22 @@ struct Int8Code {
     asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(r) : "f"(x));
     return (uint8_t)r;
   }
+  // The codes of four numbers times f: the sum of a product and 1.5 2^23, rounded once, has the rounded product in its
+  // low bits.
+  static __device__ __forceinline__ uint32_t encode4(const float* x, float f) {
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(fmaf(x[i], f, 12582912.f));
+    return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+  }
+  static __device__ __forceinline__ void decode4(uint32_t w, float* x) {
+    // (with the sign bit flipped a code is c + 128)
+    const uint32_t y = w ^ 0x80808080u;
+    x[0] = __uint_as_float(__byte_perm(y, 0x4b000000u, 0x7440)) - 8388736.f;
+    x[1] = __uint_as_float(__byte_perm(y, 0x4b000000u, 0x7441)) - 8388736.f;
+    x[2] = __uint_as_float(__byte_perm(y, 0x4b000000u, 0x7442)) - 8388736.f;
+    x[3] = __uint_as_float(__byte_perm(y, 0x4b000000u, 0x7443)) - 8388736.f;
+  }
 };
 
 struct E4m3Code {
@@ -53,6 +69,22 @@ struct E4m3Code {
   }
   static __device__ __forceinline__ uint8_t encode(float x) {
     return (uint8_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+  }
+  static __device__ __forceinline__ uint32_t encode4(const float* x, float f) {
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(x[1] * f), "f"(x[0] * f));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(x[3] * f), "f"(x[2] * f));
+    return (uint32_t)lo | (uint32_t)hi << 16;
+  }
+  static __device__ __forceinline__ void decode4(uint32_t w, float* x) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t y;
+      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(y) : "h"((uint16_t)(w >> (16 * i))));
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&y));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
   }
 };
 

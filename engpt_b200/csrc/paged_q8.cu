@@ -14,6 +14,8 @@
 // All of it is a pass over the numbers with a maximum in between, bound by HBM.
 #include "paged_q8.cuh"
 
+#include <type_traits>
+
 namespace engpt {
 namespace paged {
 
@@ -45,6 +47,11 @@ template <typename T>
 __device__ __forceinline__ T from_f32(float v) {
   if constexpr (sizeof(T) == 2) return __float2bfloat16_rn(v);
   else return v;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
@@ -177,168 +184,273 @@ __global__ void __launch_bounds__(256) store_generic_kernel(StoreArgs a) {
 // ------------------------------------------------------------------ store, 8 elements a lane
 //
 // head_dim a multiple of 8, aligned.  LPR lanes (a power of two) share a row, 8 elements each; a warp has 32 / LPR rows
-// of a run beside each other and kSteps such steps in registers, all their loads in flight before the first is used.  W
-// warps share a run, so that it fits the registers of one team: its numbers are read once.  (A longer run is read twice.)
+// of a run beside each other and kSteps such steps, of k and of v, all loads in flight before the first is used.  They
+// stay in registers as they were loaded; the post-processed k waits for its scale in shared memory, as fp32.  W warps
+// share a run, so that it fits one team and its numbers are read once; a longer run is read twice.
 //
-// A team looks after the runs that begin in a window of `window` tokens of one head and one of k, v (and, appending, q):
-// a block's worth in a long call, which is one run then, a single token in a short one or where requests add a token
-// each.
-constexpr int kSteps = 4;
+// A team looks after the runs that begin in a window of `window` tokens, of one head: a block's worth in a long call,
+// which is one run then, a single token in a short one or where requests add a token each.
+template <typename T>
+constexpr int kSteps = sizeof(T) == 2 ? 4 : 2;
 
-// Eight elements of a row: as loaded, where the numbers are those of the cache, or as computed.
-template <typename T, bool APPEND>
-struct Held {
-  float x[8];
-  __device__ __forceinline__ void get(float* y) const {
+// The largest of m >= 0 and the magnitudes of x and y; NaN if one is.
+__device__ __forceinline__ float most3(float m, float x, float y) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float most8(float m, const float* x) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = x[i];
+  for (int i = 0; i < 8; i += 2) m = most3(m, x[i], x[i + 1]);
+  return m;
+}
+
+// Eight elements as loaded.
+template <typename T>
+struct Raw {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
   }
-  __device__ __forceinline__ uint32_t most(uint32_t m) const {
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, abs_bits(x[i]));
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = ld_once(p + i * (16 / sizeof(T)));
+  }
+  __device__ __forceinline__ void get(float* x) const {
+    if constexpr (sizeof(T) == 2) {
+      unpack8(v[0], x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        x[4 * i] = __uint_as_float(v[i].x);
+        x[4 * i + 1] = __uint_as_float(v[i].y);
+        x[4 * i + 2] = __uint_as_float(v[i].z);
+        x[4 * i + 3] = __uint_as_float(v[i].w);
+      }
+    }
+  }
+  __device__ __forceinline__ float most() const {
+    if constexpr (sizeof(T) == 2) {
+      // (magnitudes of bf16 numbers, infinities and NaN above them, are in the order of their 15 bits)
+      const uint32_t a = __vmaxu2(__vmaxu2(v[0].x & 0x7fff7fffu, v[0].y & 0x7fff7fffu),
+                                  __vmaxu2(v[0].z & 0x7fff7fffu, v[0].w & 0x7fff7fffu));
+      return __uint_as_float(max(a << 16, a & 0xffff0000u));
+    } else {
+      float x[8];
+      get(x);
+      return most8(0.f, x);
+    }
+  }
+};
+
+// The post-process of engpt_qkv_append of this lane's slice (elements from e0 on) of a q or k row.
+template <typename T>
+struct PostProcess {
+  static constexpr bool kFast = sizeof(T) == 2;   // bf16 rows use the approximate reciprocals (2 ulp)
+  const StoreArgs& a;
+  int p0;                  // first rotary pair, a multiple of 4 like rope_half: 4 pairs rotate together or not at all
+  float scl[8];
+  __device__ __forceinline__ PostProcess(const StoreArgs& args, int h, int e0) : a(args), p0(e0 >> 1) {
+    const float* scale = args.qk_scale + (int64_t)h * args.c.Dh + e0;
+    const float4 s0 = __ldg(reinterpret_cast<const float4*>(scale)), s1 = __ldg(reinterpret_cast<const float4*>(scale + 4));
+    const float v[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) scl[k] = v[k] * a.qk_mult;
+  }
+
+  static __device__ __forceinline__ float per_rho(float rho) { return kFast ? __fdividef(1.0f, rho) : 1.0f / rho; }
+
+  // x: the raw slice, then the post-processed one; by a whole warp.  Bit for bit what engpt_qkv_append does.
+  template <int LPR>
+  __device__ __forceinline__ void apply(float* x, float rho, int pos) const {
+    float c[4] = {1.f, 1.f, 1.f, 1.f}, sn[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool rot = p0 < a.rope_half;
+    if (rot && (unsigned)pos < (unsigned)a.rope_rows) {
+      const int64_t at = (int64_t)pos * a.rope_half + p0;
+      const float4 c4 = __ldg(reinterpret_cast<const float4*>(a.cos_tab + at));
+      const float4 s4 = __ldg(reinterpret_cast<const float4*>(a.sin_tab + at));
+      c[0] = c4.x; c[1] = c4.y; c[2] = c4.z; c[3] = c4.w;
+      sn[0] = s4.x; sn[1] = s4.y; sn[2] = s4.z; sn[3] = s4.w;
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) ss = fmaf(x[k], x[k], ss);
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    float inv;
+    if (kFast) {
+      inv = rsqrtf(ss);
+      if (a.eps > 0.f) inv = fminf(inv, __fdividef(1.0f, rho * a.eps));
+    } else {
+      float den = sqrtf(ss);
+      if (a.eps > 0.f) den = fmaxf(den, rho * a.eps);
+      inv = 1.0f / den;
+    }
+    if (rot) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float xe = x[2 * k], xo = x[2 * k + 1];
+        x[2 * k] = ((xe * c[k] - xo * sn[k]) * inv) * scl[2 * k];
+        x[2 * k + 1] = ((xe * sn[k] + xo * c[k]) * inv) * scl[2 * k + 1];
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = (x[k] * inv) * scl[k];
+    }
+  }
+};
+struct NoPostProcess {
+  __device__ __forceinline__ NoPostProcess(const StoreArgs&, int, int) {}
+};
+
+// This lane's slices of kSteps rows of a run, k and v.
+template <typename T, bool APPEND, int LPR, int W>
+struct Rows {
+  static constexpr int S = kSteps<T>, kRows = W * (32 / LPR);   // rows of the team's step
+  using Post = std::conditional_t<APPEND, PostProcess<T>, NoPostProcess>;
+  Raw<T> v[S], k[APPEND ? 1 : S];
+  float4* s_k;             // appending: this lane's part of the warp's shared memory, [S][2][32]
+  float v_mult[APPEND ? S : 1];
+  uint32_t live;           // bit s: the row of step s is there, and its position in range
+
+  // Rows 0, kRows, ... from this lane's first one on, `left` of the run behind it; n: that one's token; k0, v0: this
+  // lane's elements of it.
+  __device__ __forceinline__ void load(const StoreArgs& a, const Post& post, const T* k0, const T* v0, int64_t n, int left,
+                                       bool mine) {
+    Raw<T> kr[S];
+    float rho[APPEND ? S : 1];
+    int pos[APPEND ? S : 1];
+    const int* pos_p = a.positions + n;
+    const float* rho_p = a.rho + n;
+    live = 0;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const bool in = s * kRows < left;
+      kr[s].clear();
+      v[s].clear();
+      if (in && mine) {
+        kr[s].load(k0);
+        v[s].load(v0);
+      }
+      k0 += kRows * a.row[0];
+      v0 += kRows * a.row[1];
+      if constexpr (APPEND) {
+        pos[s] = in ? pos_p[s * kRows] : -1;
+        rho[s] = in ? rho_p[s * kRows] : 1.f;
+        if ((unsigned)pos[s] < (unsigned)a.rope_rows) live |= 1u << s;
+      } else {
+        live |= in ? 1u << s : 0u;
+        k[s] = kr[s];
+      }
+    }
+    if constexpr (APPEND) {
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        float x[8];
+        kr[s].get(x);
+        post.template apply<LPR>(x, rho[s], pos[s]);
+        const bool on = mine && ((live >> s) & 1u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = on ? x[e] : 0.f;
+        s_k[s * 64] = make_float4(x[0], x[1], x[2], x[3]);
+        s_k[s * 64 + 32] = make_float4(x[4], x[5], x[6], x[7]);
+        most_k = most8(s == 0 ? 0.f : most_k, x);
+        v_mult[s] = PostProcess<T>::per_rho(rho[s]);
+        if (!on) v[s].clear();
+      }
+    }
+  }
+  float most_k;
+  __device__ __forceinline__ float largest(int p) const {
+    float m = APPEND && p == 0 ? most_k : 0.f;
+#pragma unroll
+    for (int s = 0; s < S; s += 1) {
+      if (APPEND && p == 0) break;
+      // (a product with 1 / rho rounds in the order of the magnitudes: the largest one's is the largest)
+      const float x = p == 0 ? k[APPEND ? 0 : s].most() : v[s].most() * (APPEND ? v_mult[APPEND ? s : 0] : 1.f);
+      m = most3(m, x, 0.f);
+    }
     return m;
   }
-};
-template <>
-struct Held<__nv_bfloat16, false> {
-  uint4 v;
-  __device__ __forceinline__ void get(float* y) const { unpack8(v, y); }
-  __device__ __forceinline__ uint32_t most(uint32_t m) const {
-    // (magnitudes of bf16 numbers are in the order of their 16 bits, like those of fp32)
-    const uint32_t a = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
-                                __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
-    return max(m, max(a << 16, a & 0xffff0000u));
+  // The codes of part p (0: k, 1: v) of step s, for 1 / scale.
+  template <typename Code>
+  __device__ __forceinline__ uint2 codes(int p, int s, float inv) const {
+    float x[8];
+    if (APPEND && p == 0) {
+      const float4 a = s_k[s * 64], b = s_k[s * 64 + 32];
+      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+      x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else if (p == 0) {
+      k[APPEND ? 0 : s].get(x);
+    } else {
+      v[s].get(x);
+      if constexpr (APPEND) inv *= v_mult[s];          // (x / rho / scale, with one rounding in another place)
+    }
+    return make_uint2(Code::encode4(x, inv), Code::encode4(x + 4, inv));
   }
 };
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* x) {
-  if constexpr (sizeof(T) == 2) {
-    unpack8(ld_once(p), x);
-  } else {
-    const uint4 a = ld_once(p), b = ld_once(p + 4);
-    x[0] = __uint_as_float(a.x); x[1] = __uint_as_float(a.y); x[2] = __uint_as_float(a.z); x[3] = __uint_as_float(a.w);
-    x[4] = __uint_as_float(b.x); x[5] = __uint_as_float(b.y); x[6] = __uint_as_float(b.z); x[7] = __uint_as_float(b.w);
+// q of a window of tokens (appending).
+template <typename T, int LPR, int W>
+__device__ __forceinline__ void store_q(const StoreArgs& a, int h, int64_t w0, int64_t w1, int me, int lane) {
+  constexpr int S = kSteps<T>, RPW = 32 / LPR, kRows = W * RPW;
+  int e0 = (lane % LPR) * 8;
+  const bool mine = e0 < a.c.Dh;
+  if (!mine) e0 = 0;
+  const PostProcess<T> post(a, h, e0);
+  const int width = a.c.H * a.c.Dh;
+  int64_t n = w0 + me * RPW + lane / LPR;
+  for (int left = (int)(w1 - n); __any_sync(0xffffffffu, left > 0); left -= S * kRows, n += S * kRows) {
+    const T* src = reinterpret_cast<const T*>(a.qkv) + n * 3 * width + (int64_t)h * a.c.Dh + e0;
+    T* dst = reinterpret_cast<T*>(a.q) + n * width + (int64_t)h * a.c.Dh + e0;
+    const int* pos_p = a.positions + n;
+    const float* rho_p = a.rho + n;
+    Raw<T> raw[S];
+    int pos[S];
+    float rho[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const bool in = s * kRows < left;
+      raw[s].clear();
+      if (in && mine) raw[s].load(src);
+      src += (int64_t)(3 * kRows) * width;
+      pos[s] = in ? pos_p[s * kRows] : -1;
+      rho[s] = in ? rho_p[s * kRows] : 1.f;
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      float x[8];
+      raw[s].get(x);
+      post.template apply<LPR>(x, rho[s], pos[s]);
+      if (s * kRows < left && mine) {
+        if ((unsigned)pos[s] >= (unsigned)a.rope_rows) {
+          if (h == 0 && e0 == 0) record_device_error(ENGPT_ERR_ARG, 42);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = 0.f;
+        }
+        if constexpr (sizeof(T) == 2) {
+          *reinterpret_cast<uint4*>(dst) = pack8(x);
+        } else {
+          *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<float4*>(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        }
+      }
+      dst += (int64_t)kRows * width;
+    }
   }
 }
 
-// What a lane needs for its slice of the rows of one head and part.
-template <typename T, int LPR, bool APPEND>
-struct Slice {
-  const StoreArgs& a;
-  const T* src;            // its first element in token 0
-  int64_t row;             // elements from token to token
-  int part, e0;            // 0: k, 1: v, 2: q; first element
-  bool mine;               // e0 is within the row
-  float scl[8];
-  __device__ __forceinline__ Slice(const StoreArgs& args, int h, int p, int lane) : a(args), part(p) {
-    e0 = (lane % LPR) * 8;
-    mine = e0 < a.c.Dh;
-    if (!mine) e0 = 0;
-    if constexpr (APPEND) {
-      row = (int64_t)3 * a.c.H * a.c.Dh;
-      src = reinterpret_cast<const T*>(a.qkv) + ((int64_t)(p + 1) % 3 * a.c.H + h) * a.c.Dh + e0;
-      const float* s = a.qk_scale + (int64_t)h * a.c.Dh + e0;
-      const float4 s0 = __ldg(reinterpret_cast<const float4*>(s)), s1 = __ldg(reinterpret_cast<const float4*>(s + 4));
-      const float v[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) scl[i] = v[i] * a.qk_mult;
-    } else {
-      row = a.row[p];
-      src = reinterpret_cast<const T*>(a.x[p]) + h * a.head[p] + e0;
-    }
-  }
-
-  // The slice of N tokens, token n[i] if in[i]; by a whole warp.  live: the numbers are there (its position is not
-  // out of range).  The arithmetic of engpt_qkv_append, bit for bit.
-  template <int N>
-  __device__ __forceinline__ void load(const int64_t* n, const bool* in, Held<T, APPEND>* out, bool* live) const {
-    if constexpr (!APPEND) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        live[i] = in[i] && mine;
-        if constexpr (sizeof(T) == 2) {
-          out[i].v = make_uint4(0u, 0u, 0u, 0u);
-          if (live[i]) out[i].v = ld_once(src + n[i] * row);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) out[i].x[k] = 0.f;
-          if (live[i]) load8(src + n[i] * row, out[i].x);
-        }
-      }
-    } else {
-      constexpr bool kFast = sizeof(T) == 2;
-      float rho[N];
-      float4 c4[N], s4[N];
-      const int p0 = e0 >> 1;
-      const bool rot = part != 1 && p0 < a.rope_half;   // rope_half is a multiple of 4: 4 pairs rotate together or not
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int pos = in[i] ? a.positions[n[i]] : -1;
-        live[i] = (unsigned)pos < (unsigned)a.rope_rows;
-        rho[i] = 1.f;
-        c4[i] = make_float4(1.f, 1.f, 1.f, 1.f);
-        s4[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) out[i].x[k] = 0.f;
-        if (in[i]) {
-          rho[i] = a.rho[n[i]];
-          if (mine) load8(src + n[i] * row, out[i].x);
-        }
-        if (rot && live[i]) {
-          c4[i] = __ldg(reinterpret_cast<const float4*>(a.cos_tab + (int64_t)pos * a.rope_half + p0));
-          s4[i] = __ldg(reinterpret_cast<const float4*>(a.sin_tab + (int64_t)pos * a.rope_half + p0));
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        float* x = out[i].x;
-        if (part == 1) {
-          const float inv_rho = kFast ? __fdividef(1.0f, rho[i]) : 1.0f / rho[i];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] *= inv_rho;
-        } else {
-          float ss = 0.f;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) ss = fmaf(x[k], x[k], ss);
-#pragma unroll
-          for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          float inv_den;
-          if (kFast) {
-            inv_den = rsqrtf(ss);
-            if (a.eps > 0.f) inv_den = fminf(inv_den, __fdividef(1.0f, rho[i] * a.eps));
-          } else {
-            float den = sqrtf(ss);
-            if (a.eps > 0.f) den = fmaxf(den, rho[i] * a.eps);
-            inv_den = 1.0f / den;
-          }
-          if (rot) {
-            const float c[4] = {c4[i].x, c4[i].y, c4[i].z, c4[i].w}, sn[4] = {s4[i].x, s4[i].y, s4[i].z, s4[i].w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float xe = x[2 * k], xo = x[2 * k + 1];
-              x[2 * k] = ((xe * c[k] - xo * sn[k]) * inv_den) * scl[2 * k];
-              x[2 * k + 1] = ((xe * sn[k] + xo * c[k]) * inv_den) * scl[2 * k + 1];
-            }
-          } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = (x[k] * inv_den) * scl[k];
-          }
-        }
-        if (!live[i] || !mine) {      // (a row of length 0 may have given NaN behind the head_dim)
-#pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] = 0.f;
-        }
-        live[i] = live[i] && mine;
-      }
-    }
-  }
-};
+// CTAs of four warps per SM that the registers leave room for.
+template <bool APPEND>
+constexpr int kStoreCtas = APPEND ? 6 : 7;
 
 template <typename T, typename Code, bool APPEND, int LPR, int W>
-__global__ void __launch_bounds__(W > 4 ? 32 * W : 128) store_runs_kernel(StoreArgs a, int window) {
-  constexpr int RPW = 32 / LPR, kRows = W * RPW;       // rows of a warp's step, of the team's
-  __shared__ uint32_t s_most[W > 1 ? W : 1];
+__global__ void __launch_bounds__(W > 4 ? 32 * W : 128, kStoreCtas<APPEND> * 4 / (W > 4 ? W : 4))
+store_runs_kernel(StoreArgs a, int window) {
+  constexpr int RPW = 32 / LPR, kRows = W * RPW, S = kSteps<T>;
+  __shared__ uint32_t s_most[W > 1 ? W : 1][2];
+  __shared__ float4 s_k[APPEND ? (W > 4 ? W : 4) : 1][APPEND ? S * 64 : 1];
   if constexpr (APPEND) {
     // started ahead of the end of what runs before (usually the projection), and so may be what follows
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -346,50 +458,37 @@ __global__ void __launch_bounds__(W > 4 ? 32 * W : 128) store_runs_kernel(StoreA
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int me = W > 1 ? warp : 0;                     // this warp of its team
-  const int parts = APPEND ? 3 : 2;
   const int64_t item = W > 1 ? blockIdx.x : blockIdx.x * 4ll + warp;
   const int64_t windows = (a.n + window - 1) / window;
-  if (item >= windows * parts * a.c.H) return;         // (of the last CTA of single warps only)
-  const int h = (int)(item % a.c.H);
-  const int64_t wp = item / a.c.H;
-  const int part = (int)(wp % parts);
-  const int64_t w0 = wp / parts * window, w1 = min(a.n, w0 + window);
-  const Slice<T, LPR, APPEND> slice(a, h, part, lane);
-  const int sub = lane / LPR;
-
+  if (item >= windows * (APPEND ? 2 : 1) * a.c.H) return;   // (of the last CTA of single warps only)
+  const int64_t wp = item <= 0xffffffffLL ? (int64_t)((uint32_t)item / (uint32_t)a.c.H) : item / a.c.H;
+  const int h = (int)(item - wp * a.c.H);
+  const int64_t w0 = (APPEND ? wp >> 1 : wp) * window, w1 = min(a.n, w0 + window);
   if constexpr (APPEND) {
-    if (part == 2) {
-      T* q = reinterpret_cast<T*>(a.q) + (int64_t)h * a.c.Dh + slice.e0;
-      for (int64_t t = w0 + me * RPW; t < w1; t += kRows) {
-        const int64_t n = t + sub;
-        const bool in = n < w1;
-        Held<T, APPEND> x;
-        bool live;
-        slice.template load<1>(&n, &in, &x, &live);
-        if (!in || !slice.mine) continue;
-        if (!live && h == 0 && lane % LPR == 0) record_device_error(ENGPT_ERR_ARG, 42);
-        T* dst = q + n * a.c.H * a.c.Dh;
-        if constexpr (sizeof(T) == 2) {
-          *reinterpret_cast<uint4*>(dst) = pack8(x.x);
-        } else {
-          *reinterpret_cast<float4*>(dst) = make_float4(x.x[0], x.x[1], x.x[2], x.x[3]);
-          *reinterpret_cast<float4*>(dst + 4) = make_float4(x.x[4], x.x[5], x.x[6], x.x[7]);
-        }
-      }
+    if (wp & 1) {
+      store_q<T, LPR, W>(a, h, w0, w1, me, lane);
       return;
     }
   }
-  uint8_t* const codes = reinterpret_cast<uint8_t*>(a.c.codes[part]) + h * a.c.cs[part][1] + slice.e0;
-  float* const scales = a.c.scales[part] + h * a.c.ss[part][1];
+  int e0 = (lane % LPR) * 8;
+  const bool mine = e0 < a.c.Dh;
+  if (!mine) e0 = 0;
+  const typename Rows<T, APPEND, LPR, W>::Post post(a, h, e0);
+  const T* const src_k = reinterpret_cast<const T*>(a.x[0]) + h * a.head[0] + e0;
+  const T* const src_v = reinterpret_cast<const T*>(a.x[1]) + h * a.head[1] + e0;
+  const int row0 = me * RPW + lane / LPR;              // this lane's first row of a run
+  Rows<T, APPEND, LPR, W> rows;
+  rows.s_k = &s_k[APPEND ? warp : 0][APPEND ? lane : 0];
 
   for (int64_t t0 = w0; t0 < w1; t0 += 32) {
     // the slots of 32 tokens, and which of them begin a run (of those in the window)
     const int64_t mine_n = t0 + lane;
-    const int raw = mine_n < a.n ? a.slots[mine_n] : -1;
-    const int before = mine_n > 0 && mine_n <= a.n ? a.slots[mine_n - 1] : -1;
+    const int given = mine_n < a.n ? a.slots[mine_n] : -1;
+    int before = __shfl_up_sync(0xffffffffu, given, 1);
+    if (lane == 0) before = mine_n > 0 ? a.slots[mine_n - 1] : -1;
     const bool window_token = mine_n < w1;
-    const int slot = checked_slot(a, raw, window_token && part == 0 && h == 0 && me == 0);
-    const int my_off = (int)((uint32_t)max(slot, 0) % (uint32_t)a.c.block);
+    const int slot = checked_slot(a, given, window_token && h == 0 && me == 0);
+    const int my_off = max(slot, 0) - a.c.block_of(max(slot, 0)) * a.c.block;   // (blocks divide pages)
     uint32_t heads = __ballot_sync(0xffffffffu, window_token && slot >= 0 && !(my_off > 0 && before == slot - 1));
     while (heads) {
       const int i = __ffs(heads) - 1;
@@ -411,88 +510,79 @@ __global__ void __launch_bounds__(W > 4 ? 32 * W : 128) store_runs_kernel(StoreA
           if (k < 32) break;
         }
       }
-      const int page = first / a.c.ps, in_page = first - page * a.c.ps;
-      float* const scale_p = scales + page * a.c.ss[part][0] + in_page / a.c.block * a.c.ss[part][2];
-      const float old = off > 0 ? *scale_p : 0.f;
-      uint8_t* const block_p = codes + page * a.c.cs[part][0] + (in_page - off) * a.c.cs[part][2];   // the block's first row
-
-      // the largest magnitude, with the numbers of the last kSteps steps kept
-      Held<T, APPEND> x[kSteps];
-      bool live[kSteps];
-      const bool all = run <= kSteps * kRows;          // kept whole
-      uint32_t most = 0;
-      bool any = false;
-      for (int r0 = 0; r0 < run; r0 += kSteps * kRows) {
-        int64_t n[kSteps];
-        bool in[kSteps];
+      const int64_t n1 = n0 + row0;                    // this lane's first token
+      const T *k = src_k + n1 * a.row[0], *v = src_v + n1 * a.row[1];
+      rows.load(a, post, k, v, n1, run - row0, mine);
+      const int page = a.c.page_of(first), in_page = first - page * a.c.ps, block = a.c.block_of(in_page);
+      float* scale_p[2];
+      float old[2];
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          const int r = r0 + (s * W + me) * RPW + sub;
-          in[s] = r < run;
-          n[s] = n0 + r;
-        }
-        slice.template load<kSteps>(n, in, x, live);
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          most = x[s].most(most);
-          any = any || live[s];
-        }
+      for (int p = 0; p < 2; ++p) {
+        scale_p[p] = a.c.scales[p] + page * a.c.ss[p][0] + h * a.c.ss[p][1] + block * a.c.ss[p][2];
+        old[p] = off > 0 ? *scale_p[p] : 0.f;
       }
-      most = __reduce_max_sync(0xffffffffu, most);
-      if (APPEND) any = __any_sync(0xffffffffu, any);
-      if constexpr (W > 1) {
-        // (most is a magnitude: its top bit says whether there is any number at all)
-        if (lane == 0) s_most[warp] = most | (any ? 0x80000000u : 0u);
-        __syncthreads();
-        uint32_t m = 0;
-        any = false;
+      float largest[2] = {rows.largest(0), rows.largest(1)};
+      uint32_t any = rows.live;
+      for (int r0 = S * kRows; r0 < run; r0 += S * kRows) {
+        rows.load(a, post, k + r0 * a.row[0], v + r0 * a.row[1], n1 + r0, run - row0 - r0, mine);
+        largest[0] = most3(largest[0], rows.largest(0), 0.f);
+        largest[1] = most3(largest[1], rows.largest(1), 0.f);
+        any |= rows.live;
+      }
+      uint32_t most[2];
 #pragma unroll
-        for (int k = 0; k < W; ++k) {
-          m = max(m, s_most[k] & 0x7fffffffu);
-          any = any || (s_most[k] & 0x80000000u);
-        }
-        most = m;
+      for (int p = 0; p < 2; ++p) most[p] = __reduce_max_sync(0xffffffffu, __float_as_uint(largest[p]));
+      if (APPEND) any = __any_sync(0xffffffffu, any != 0);
+      if constexpr (W > 1) {
+        // (a magnitude's top bit is free: whether there is any number at all)
+        if (lane < 2) s_most[warp][lane] = (lane == 0 ? most[0] : most[1]) | (any ? 0x80000000u : 0u);
+        __syncthreads();
+        const uint32_t m = s_most[lane % W][(lane / W) & 1];   // lanes 0 .. W - 1: k, the next W: v
+        most[0] = __reduce_max_sync(0xffffffffu, lane < W ? m & 0x7fffffffu : 0u);
+        most[1] = __reduce_max_sync(0xffffffffu, lane >= W && lane < 2 * W ? m & 0x7fffffffu : 0u);
+        any = __any_sync(0xffffffffu, m >> 31);
         __syncthreads();                               // before the next run's maxima
       }
       if (APPEND && !any) continue;
-      const float need = needed_scale<Code>(most);
-      const float scale = off > 0 ? raised_scale(old, need) : need;
-      if (off > 0 && scale > old) {                    // (not for NaN)
-        const float ratio = __fdiv_rn(old, scale);
-        for (int j = me * RPW + sub; j < a.c.block; j += kRows) {
-          if ((j >= off && j < off + run) || !slice.mine) continue;
-          uint2* p = reinterpret_cast<uint2*>(block_p + j * a.c.cs[part][2]);
-          const uint2 w = *p;
-          float y[8];
-          Code::decode4(w.x, y);
-          Code::decode4(w.y, y + 4);
-          *p = make_uint2(Code::encode4(y, ratio), Code::encode4(y + 4, ratio));
-        }
-      }
-      const float inv = isnan(scale) ? 0.f : __fdiv_rn(1.f, scale);
-      for (int r0 = 0; r0 < run; r0 += kSteps * kRows) {
-        if (!all) {
-          int64_t n[kSteps];
-          bool in[kSteps];
+      float inv[2];
+      uint8_t* code_p[2];                              // this lane's codes of its first row
 #pragma unroll
-          for (int s = 0; s < kSteps; ++s) {
-            const int r = r0 + (s * W + me) * RPW + sub;
-            in[s] = r < run;
-            n[s] = n0 + r;
+      for (int p = 0; p < 2; ++p) {
+        const int64_t row = a.c.cs[p][2];
+        uint8_t* at = reinterpret_cast<uint8_t*>(a.c.codes[p]) + page * a.c.cs[p][0] + h * a.c.cs[p][1] +
+                      (in_page - off + row0) * row + e0;       // row row0 of the block
+        const float need = needed_scale<Code>(most[p]);
+        const float scale = off > 0 ? raised_scale(old[p], need) : need;
+        if (off > 0 && scale > old[p]) {               // (not for NaN)
+          const float ratio = __fdiv_rn(old[p], scale);
+          uint8_t* to = at;
+          for (int j = row0; j < a.c.block; j += kRows, to += kRows * row) {
+            if ((j >= off && j < off + run) || !mine) continue;
+            uint2* c = reinterpret_cast<uint2*>(to);
+            const uint2 w = *c;
+            float y[8];
+            Code::decode4(w.x, y);
+            Code::decode4(w.y, y + 4);
+            *c = make_uint2(Code::encode4(y, ratio), Code::encode4(y + 4, ratio));
           }
-          slice.template load<kSteps>(n, in, x, live);
         }
+        inv[p] = isnan(scale) ? 0.f : __fdiv_rn(1.f, scale);
+        code_p[p] = at + off * row;
+        if (lane == 0 && me == 0) *scale_p[p] = scale;
+      }
+      // (a run of one load is still there)
+      for (int r0 = 0; r0 < run; r0 += S * kRows) {
+        if (run > S * kRows) rows.load(a, post, k + r0 * a.row[0], v + r0 * a.row[1], n1 + r0, run - row0 - r0, mine);
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          if (!live[s]) continue;
-          const int r = r0 + (s * W + me) * RPW + sub;
-          float y[8];
-          x[s].get(y);
-          *reinterpret_cast<uint2*>(block_p + (off + r) * a.c.cs[part][2]) =
-              make_uint2(Code::encode4(y, inv), Code::encode4(y + 4, inv));
+        for (int s = 0; s < S; ++s) {
+          const bool here = ((rows.live >> s) & 1u) && mine;
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            if (here) *reinterpret_cast<uint2*>(code_p[p]) = rows.template codes<Code>(p, s, inv[p]);
+            code_p[p] += kRows * a.c.cs[p][2];
+          }
         }
       }
-      if (lane == 0 && me == 0) *scale_p = scale;
     }
   }
 }
@@ -526,6 +616,88 @@ __global__ void __launch_bounds__(256) read_generic_kernel(ReadArgs a) {
   }
 }
 
+// Head_dim a multiple of N = 8 or 16, aligned.  A thread owns N codes of a row (k and v) and walks over tokens; a CTA
+// takes several tokens beside each other where a row has fewer pieces than it has threads.  The slot of the next token
+// is on its way while this one's numbers are.
+constexpr int kReadCtas = 6;
+
+template <typename T>
+__device__ __forceinline__ void store_row(T* p, const float* x, int n) {
+#pragma unroll
+  for (int i = 0; i < n; i += 32 / (int)sizeof(T)) {
+    uint32_t w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      w[k] = sizeof(T) == 2 ? pack_bf16(x[i + 2 * k], x[i + 2 * k + 1]) : __float_as_uint(x[i + k]);
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p + i), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  }
+}
+
+template <typename T, typename Code, int N>
+__global__ void __launch_bounds__(256, kReadCtas) read_vec_kernel(ReadArgs a, int pieces) {
+  const int row = a.c.H * pieces, tokens = row >= (int)blockDim.x ? 1 : blockDim.x / row;
+  const int idx = blockIdx.y * blockDim.x + threadIdx.x, sub = tokens > 1 ? idx / row : 0, at = idx - sub * row;
+  if (sub >= tokens || at >= row) return;
+  const int h = at / pieces, e = (at - h * pieces) * N;
+  const char* codes[2];
+  const float* scales[2];
+  T* out[2];
+  const int64_t step = (int64_t)gridDim.x * tokens, n0 = (int64_t)blockIdx.x * tokens + sub, width = (int64_t)row * N;
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    codes[p] = (const char*)a.c.codes[p] + h * a.c.cs[p][1] + e;
+    scales[p] = a.c.scales[p] + h * a.c.ss[p][1];
+    out[p] = reinterpret_cast<T*>(a.out[p]) + n0 * width + (int64_t)at * N;
+  }
+  int next = n0 < a.n ? a.slots[n0] : -1;
+  for (int64_t n = n0; n < a.n; n += step) {
+    int slot = next;
+    if (n + step < a.n) next = a.slots[n + step];
+    if ((uint32_t)slot >= (uint64_t)a.c.n_slots) {
+      if (slot != -1 && at == 0) record_device_error(ENGPT_ERR_ARG, 43);
+      slot = -1;
+    }
+    uint32_t w[2][N / 4];
+    float scale[2];
+    const int page = a.c.page_of(slot), off = slot - page * a.c.ps, block = a.c.block_of(off);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) w[p][i] = 0u;
+      scale[p] = 0.f;
+      if (slot >= 0) {
+        const char* c = codes[p] + page * a.c.cs[p][0] + off * a.c.cs[p][2];
+        if constexpr (N == 16) {
+          const uint4 r = ld_once(c);
+          w[p][0] = r.x; w[p][1] = r.y; w[p][2] = r.z; w[p][3] = r.w;
+        } else {
+          asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(w[p][0]), "=r"(w[p][1]) : "l"(c));
+        }
+        scale[p] = scales[p][page * a.c.ss[p][0] + block * a.c.ss[p][2]];
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      float x[N];
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) Code::decode4(w[p][i], x + 4 * i);
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[k] *= scale[p];   // (both are 0 without a slot)
+      if constexpr (N == 16) {
+        store_row<T>(out[p], x, N);
+      } else if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint4*>(out[p]) = pack8(x);
+      } else {
+        *reinterpret_cast<float4*>(out[p]) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4*>(out[p] + 4) = make_float4(x[4], x[5], x[6], x[7]);
+      }
+      out[p] += step * width;
+    }
+  }
+}
+
 // Checks of a cache's description, common to all entry points; fills `c`.
 int fill_q8_cache(const char* what, Q8Cache& c, void* k_pages, void* v_pages, float* k_scales, float* v_scales,
                   const int64_t* page_strides, const int64_t* scale_strides, int code, int H, int Dh, int num_pages,
@@ -552,6 +724,8 @@ int fill_q8_cache(const char* what, Q8Cache& c, void* k_pages, void* v_pages, fl
   c.Dh = Dh;
   c.ps = page_size;
   c.block = block;
+  c.ps_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size) : -1;
+  c.block_shift = (block & (block - 1)) == 0 ? __builtin_ctz((unsigned)block) : -1;
   c.n_slots = (int64_t)num_pages * page_size;
   return ENGPT_OK;
 }
@@ -566,7 +740,7 @@ int launch_store_generic(const StoreArgs& a, const char* what, cudaStream_t st) 
 
 template <typename T, typename Code, bool APPEND, int LPR, int W>
 int launch_store_runs(const StoreArgs& a, int window, const char* what, cudaStream_t st) {
-  const int64_t items = (a.n + window - 1) / window * (APPEND ? 3 : 2) * a.c.H, blocks = W > 1 ? items : (items + 3) / 4;
+  const int64_t items = (a.n + window - 1) / window * (APPEND ? 2 : 1) * a.c.H, blocks = W > 1 ? items : (items + 3) / 4;
   ENGPT_REQUIRE(blocks <= 0x7fffffffLL, ENGPT_ERR_SHAPE, "%s: too large", what);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
@@ -584,9 +758,9 @@ int launch_store_runs(const StoreArgs& a, int window, const char* what, cudaStre
 
 template <typename T, typename Code, bool APPEND, int LPR>
 int launch_store_team(const StoreArgs& a, const char* what, cudaStream_t st) {
-  const int rows = kSteps * 32 / LPR;                  // that a warp holds
+  const int rows = kSteps<T> * 32 / LPR;               // that a warp holds
   // a token per window while that makes no more warps than run at once some times over
-  const bool single = a.n * (APPEND ? 3 : 2) * a.c.H <= (int64_t)num_sms() * 128;
+  const bool single = a.n * (APPEND ? 2 : 1) * a.c.H <= (int64_t)num_sms() * 64;
   if (single) return launch_store_runs<T, Code, APPEND, LPR, 1>(a, 1, what, st);
   if (a.c.block <= rows) return launch_store_runs<T, Code, APPEND, LPR, 1>(a, a.c.block, what, st);
   if (a.c.block <= 4 * rows) return launch_store_runs<T, Code, APPEND, LPR, 4>(a, a.c.block, what, st);
@@ -618,13 +792,36 @@ int launch_store(const StoreArgs& a, int code, bool vec, const char* what, cudaS
                                  : launch_store_code<T, E4m3Code, APPEND>(a, vec, what, st);
 }
 
+template <typename T, typename Code>
+int launch_read_code(const ReadArgs& a, cudaStream_t st) {
+  bool vec = a.c.Dh % 8 == 0, wide = a.c.Dh % 16 == 0;
+  for (int p = 0; p < 2; ++p) {
+    vec = vec && aligned(a.c.codes[p], 8) && aligned(a.out[p], 16);
+    wide = wide && aligned(a.c.codes[p], 16) && aligned(a.out[p], 32);
+    for (int i = 0; i < 3; ++i) {
+      vec = vec && a.c.cs[p][i] % 8 == 0;
+      wide = wide && a.c.cs[p][i] % 16 == 0;
+    }
+  }
+  const int64_t most = (int64_t)num_sms() * kReadCtas;
+  if (!vec) {
+    const int64_t want = (a.n * a.c.H * a.c.Dh + 255) / 256;
+    read_generic_kernel<T, Code><<<(unsigned)(want < most ? want : most), 256, 0, st>>>(a);
+    return check_launch("read_kv_pages_q8");
+  }
+  const int pieces = a.c.Dh / (wide ? 16 : 8), row = a.c.H * pieces, y = (row + 255) / 256;
+  const int tokens = row >= 256 ? 1 : 256 / row;
+  ENGPT_REQUIRE(y <= 65535, ENGPT_ERR_SHAPE, "read_kv_pages_q8: H=%d Dh=%d", a.c.H, a.c.Dh);
+  const int64_t groups = (a.n + tokens - 1) / tokens, cap = most / y > 0 ? most / y : 1;
+  const dim3 grid((unsigned)(groups < cap ? groups : cap), (unsigned)y);
+  if (wide) read_vec_kernel<T, Code, 16><<<grid, 256, 0, st>>>(a, pieces);
+  else read_vec_kernel<T, Code, 8><<<grid, 256, 0, st>>>(a, pieces);
+  return check_launch("read_kv_pages_q8");
+}
+
 template <typename T>
 int launch_read(const ReadArgs& a, int code, cudaStream_t st) {
-  const int64_t want = (a.n * a.c.H * a.c.Dh + 255) / 256, cap = (int64_t)num_sms() * 8;
-  const unsigned blocks = (unsigned)(want < cap ? want : cap);
-  if (code == ENGPT_CODE_INT8) read_generic_kernel<T, Int8Code><<<blocks, 256, 0, st>>>(a);
-  else read_generic_kernel<T, E4m3Code><<<blocks, 256, 0, st>>>(a);
-  return check_launch("read_kv_pages_q8");
+  return code == ENGPT_CODE_INT8 ? launch_read_code<T, Int8Code>(a, st) : launch_read_code<T, E4m3Code>(a, st);
 }
 
 }  // namespace paged
@@ -679,6 +876,11 @@ extern "C" int engpt_qkv_append_q8(const void* qkv, int dtype, const float* rho,
   a.slots = slots;
   a.n = n;
   a.qkv = qkv;
+  for (int i = 0; i < 2; ++i) {                        // (k and v as rows of the projection)
+    a.x[i] = static_cast<const char*>(qkv) + (size_t)(i + 1) * H * Dh * (dtype == ENGPT_BF16 ? 2 : 4);
+    a.row[i] = (int64_t)3 * H * Dh;
+    a.head[i] = Dh;
+  }
   a.rho = rho;
   a.cos_tab = cos_tab;
   a.sin_tab = sin_tab;

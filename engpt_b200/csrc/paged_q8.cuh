@@ -18,16 +18,20 @@ struct Q8Cache {
   int64_t ss[2][3];       // of the scales: page, head, block
   int H, Dh;
   int ps, block;          // tokens of a page, and of a block (which divides it)
+  int ps_shift, block_shift;   // their logarithms, or -1
   int64_t n_slots;        // num_pages * page_size
+
+  __device__ __forceinline__ int page_of(int slot) const { return ps_shift >= 0 ? slot >> ps_shift : slot / ps; }
+  __device__ __forceinline__ int block_of(int slot) const { return block_shift >= 0 ? slot >> block_shift : slot / block; }
 
   // codes of (slot, head) and scale of (slot, head), as offsets
   __device__ __forceinline__ int64_t code_at(int part, int slot, int h) const {
-    const int page = slot / ps, off = slot - page * ps;
+    const int page = page_of(slot), off = slot - page * ps;
     return page * cs[part][0] + h * cs[part][1] + off * cs[part][2];
   }
   __device__ __forceinline__ int64_t scale_at(int part, int slot, int h) const {
-    const int page = slot / ps, off = slot - page * ps;
-    return page * ss[part][0] + h * ss[part][1] + off / block * ss[part][2];
+    const int page = page_of(slot), off = slot - page * ps;
+    return page * ss[part][0] + h * ss[part][1] + block_of(off) * ss[part][2];
   }
 };
 

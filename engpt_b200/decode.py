@@ -16,6 +16,11 @@ them, and a ``PagedDecoder`` runs the model over it:
     Y, rho   = carried residual of attn @ W_o^T                engpt_carried_residual_gauge
     Y, rho   = carried residual of SwiGLU(..) @ W_down^T       cuBLAS, engpt_swiglu
 
+The cache can be held in 8 bits (int8 or float8_e4m3fn codes with a scale for
+each head and block of tokens): k and v are quantised as they are written and
+the attention reads the codes (the ``_q8`` forms of the three operators).  A
+prompt's own attention sees its k and v before that.
+
 Pages are handed out and taken back on the GPU
 (``kernels.advance_block_tables``), so a step makes no host synchronisation
 and can be captured: ``enable_cuda_graphs()`` replays the whole step.
@@ -36,6 +41,8 @@ from .models import plain_tensors
 
 __all__ = ["PagedKVCache", "PagedDecoder"]
 
+_CODES = (torch.int8, torch.float8_e4m3fn)
+
 
 class PagedKVCache:
     """Page pools of all layers and the page allocator's state for ``max_batch`` requests.
@@ -46,16 +53,29 @@ class PagedKVCache:
     views of one buffer.  A page holds ``page_size`` tokens of one request in
     every layer.  A request has at most ``max_len`` tokens (default
     ``block_size``), rounded up to whole pages.
+
+    With ``dtype`` int8 or float8_e4m3fn the pools hold codes, and ``k_scales`` /
+    ``v_scales`` float32 ``[layers, num_pages, heads, page_size / scale_block]`` their
+    scales, one for every ``scale_block`` tokens of a page (a divisor of
+    ``page_size``; default 16, or 8, if it is one, else the page).
     """
 
     @plain_tensors
     def __init__(self, cfg: ModelConfig, max_batch: int, num_pages: int, *, page_size: int = 64,
                  max_len: Optional[int] = None, dtype: torch.dtype = torch.bfloat16,
-                 device: Optional[torch.device] = None) -> None:
+                 scale_block: Optional[int] = None, device: Optional[torch.device] = None) -> None:
         if min(max_batch, num_pages, page_size) < 1:
             raise ValueError("max_batch, num_pages and page_size must be positive")
-        if dtype not in (torch.bfloat16, torch.float32):
-            raise NotImplementedError(f"engpt_b200 kernels support float32 and bfloat16, got {dtype}")
+        if dtype not in (torch.bfloat16, torch.float32, *_CODES):
+            raise NotImplementedError("a paged cache holds float32, bfloat16, int8 or float8_e4m3fn, got "
+                                      f"{dtype}")
+        if dtype in _CODES:
+            if scale_block is None:
+                scale_block = next((b for b in (16, 8) if page_size % b == 0), page_size)
+            if scale_block < 1 or page_size % scale_block:
+                raise ValueError(f"scale_block must divide page_size {page_size}, got {scale_block}")
+        elif scale_block is not None:
+            raise ValueError(f"a cache of {dtype} has no scales")
         device = torch.device("cuda") if device is None else torch.device(device)
         if device.type != "cuda":
             raise RuntimeError("engpt_b200 ops run on CUDA tensors only (no CPU fallback)")
@@ -64,6 +84,12 @@ class PagedKVCache:
         shape = (cfg.n_layer, num_pages, cfg.n_head, page_size, cfg.head_dim)
         self.k_pages = torch.empty(shape, dtype=dtype, device=device)
         self.v_pages = torch.empty(shape, dtype=dtype, device=device)
+        self.scale_block = scale_block
+        self.k_scales = self.v_scales = None
+        if self.quantised:
+            shape = shape[:3] + (page_size // scale_block,)
+            self.k_scales = torch.zeros(shape, dtype=torch.float32, device=device)
+            self.v_scales = torch.zeros(shape, dtype=torch.float32, device=device)
         state = torch.empty(max_batch + 1 + num_pages + max_batch * self.pages_per_request, dtype=torch.int32,
                             device=device)
         self.lengths, self.free_count, self.free_pages, table = state.split(
@@ -75,6 +101,36 @@ class PagedKVCache:
     def capacity(self) -> int:
         """Tokens that one request can have."""
         return self.pages_per_request * self.page_size
+
+    @property
+    def quantised(self) -> bool:
+        """Whether the pools hold 8-bit codes."""
+        return self.k_pages.dtype in _CODES
+
+    def layer(self, i: int) -> Tuple[Tensor, ...]:
+        """Pools of layer ``i``: k and v pages, and their scales if they hold codes."""
+        if not self.quantised:
+            return self.k_pages[i], self.v_pages[i]
+        return self.k_pages[i], self.v_pages[i], self.k_scales[i], self.v_scales[i]
+
+    @torch.no_grad()
+    def read(self, layer: int, row: int, n: int, *, dtype: Optional[torch.dtype] = None) -> Tuple[Tensor, Tensor]:
+        """k and v ``[n, heads, Dh]`` of the first ``n`` tokens of request ``row`` in a layer, zeros behind its length.
+
+        ``dtype`` is bfloat16 or float32 (default: the pools' own, bfloat16 for codes).
+        """
+        if not 0 <= row < self.max_batch or not 0 <= n <= self.capacity:
+            raise ValueError(f"row must be in [0, {self.max_batch}) and n in [0, {self.capacity}], got {row} and {n}")
+        pos = torch.arange(n, device=self.lengths.device)
+        page = self.block_table[row].index_select(0, pos // self.page_size)
+        there = pos < self.lengths[row]
+        slots = torch.where(there, page * self.page_size + pos % self.page_size, -1).to(torch.int32)
+        pools = self.layer(layer)
+        if self.quantised:
+            return K.read_kv_pages_q8(slots, *pools, dtype=torch.bfloat16 if dtype is None else dtype)
+        at = slots.clamp(min=0).long()
+        return tuple(p[at // self.page_size, :, at % self.page_size].masked_fill_(~there[:, None, None], 0.0).to(
+            p.dtype if dtype is None else dtype) for p in pools)
 
     def reset(self) -> None:
         """Drop all requests: every page is free."""
@@ -120,14 +176,17 @@ class PagedDecoder:
     or float32.  Steps use the parameters that the decoder took when it was built
     or last refreshed (in bfloat16 its own copies of the linear weights, in both
     types its own scaled copy of the head): call ``refresh_weights()`` after the
-    model's parameters have changed, in place or for other tensors.  Requests are
+    model's parameters have changed, in place or for other tensors.  ``cache_dtype``
+    (default: ``dtype``) int8 or float8_e4m3fn holds the cache in 8 bits, with a
+    scale for every ``scale_block`` tokens (``PagedKVCache``).  Requests are
     rows ``0 .. max_batch - 1``.  ``prefill`` uses the model's parameters and
     activation buffers, as its forward does: one stream at a time.
     """
 
     @plain_tensors
     def __init__(self, model, max_batch: int, num_pages: int, *, page_size: int = 64, max_len: Optional[int] = None,
-                 dtype: torch.dtype = torch.bfloat16) -> None:
+                 dtype: torch.dtype = torch.bfloat16, cache_dtype: Optional[torch.dtype] = None,
+                 scale_block: Optional[int] = None) -> None:
         p = model.token_emb.weight
         if not p.is_cuda:
             raise RuntimeError("engpt_b200 EfficientNGPT runs on CUDA only (no CPU fallback); call .cuda()")
@@ -136,7 +195,12 @@ class PagedDecoder:
         if model.head_split is not None:
             raise NotImplementedError("a head-split model cannot decode from a paged cache")
         self.model, self.cfg, self.device, self.dtype = model, model.cfg, p.device, dtype
-        self.cache = PagedKVCache(model.cfg, max_batch, num_pages, page_size=page_size, max_len=max_len, dtype=dtype,
+        if dtype not in (torch.bfloat16, torch.float32):
+            raise NotImplementedError(f"engpt_b200 kernels support float32 and bfloat16, got {dtype}")
+        if cache_dtype is not None and cache_dtype != dtype and cache_dtype not in _CODES:
+            raise NotImplementedError(f"the cache holds the compute type {dtype}, int8 or float8_e4m3fn, got {cache_dtype}")
+        self.cache = PagedKVCache(model.cfg, max_batch, num_pages, page_size=page_size, max_len=max_len,
+                                  dtype=dtype if cache_dtype is None else cache_dtype, scale_block=scale_block,
                                   device=p.device)
         self.cos, self.sin = K.rotary_frequencies(self.cache.capacity, model.cfg.head_dim, device=p.device,
                                                   dtype=torch.float32, theta=model.cfg.rope_theta)
@@ -237,8 +301,10 @@ class PagedDecoder:
             refused = slots[:, :1] < 0
             last = torch.tensor([b * seq_len + x - 1 for b, x in enumerate(lens)]).to(self.device, non_blocking=True)
 
+            write = K.write_kv_pages_q8 if cache.quantised else K.write_kv_pages
+
             def keep(layer: int, k: Tensor, v: Tensor) -> None:
-                K.write_kv_pages(k, v, slots, cache.k_pages[layer], cache.v_pages[layer])
+                write(k, v, slots, *cache.layer(layer))
 
             with torch.autocast("cuda", dtype=torch.bfloat16, enabled=self.dtype == torch.bfloat16):
                 logits, _ = self.model._run(idx=idx, kv_callback=keep, head_rows=last)
@@ -297,11 +363,14 @@ class PagedDecoder:
         u_mult = sqrt_d if cfg.scale_mlp_u_by_sqrt_d else 1.0
         act, aux_h = _lib.dtype_code(self.dtype), _lib.AUX_BF16_H if bf16 else _lib.AUX_F32_H
         last = cfg.n_layer - 1
+        append, attend = ((K.qkv_append_from_carried_q8, K.paged_sdpa_q8) if cache.quantised else
+                          (K.qkv_append_from_carried, K.paged_sdpa))
         for i, (blk, w) in enumerate(zip(m.blocks, self._w)):
             qkv = torch.mm(x, w["qkv"].t()).view(b, 3, heads, dim)
-            q = K.qkv_append_from_carried(qkv, rho, self.cos, self.sin, w["s_qk"], cfg.norm_eps, positions,
-                                          slots, cache.k_pages[i], cache.v_pages[i], qk_mult=blk.qk_mult)
-            attn = K.paged_sdpa(q, cache.k_pages[i], cache.v_pages[i], cache.block_table, cache.lengths, scale=scale)
+            pools = cache.layer(i)
+            q = append(qkv, rho, self.cos, self.sin, w["s_qk"], cfg.norm_eps, positions, slots, *pools,
+                       qk_mult=blk.qk_mult)
+            attn = attend(q, *pools, cache.block_table, cache.lengths, scale=scale)
             branch = torch.mm(attn.view(b, d), w["out_proj"].t())
             K.carried_residual_into(y, rho, branch, w["alpha_attn_raw"], blk.alpha_mult, True, cfg.norm_eps,
                                     cfg.norm_eps, cfg.carried_gauge_max, y, rho, h, aux_h)

@@ -183,3 +183,20 @@ def test_the_reference_store_finds_a_wrong_code():
     wrong[2, 0, 0] *= 1.001
     with pytest.raises(AssertionError):
         Q.check_store(cache[0], wrong, before, scales, x, slots)
+
+
+def test_cache_and_decoder_refusals():
+    from engpt_b200 import EfficientNGPT, ModelConfig, PagedKVCache
+    from tests.helpers import SMALL
+    cfg = ModelConfig(**SMALL)
+    for block in (0, -1, 5, 128):
+        with pytest.raises(ValueError, match="scale_block"):
+            PagedKVCache(cfg, 2, 4, page_size=64, dtype=torch.int8, scale_block=block)
+    with pytest.raises(ValueError, match="no scales"):
+        PagedKVCache(cfg, 2, 4, scale_block=16)
+    with pytest.raises(NotImplementedError, match="int8 or float8"):
+        PagedKVCache(cfg, 2, 4, dtype=torch.float8_e5m2)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        PagedKVCache(cfg, 2, 4, dtype=torch.int8, device="cpu")
+    with pytest.raises(RuntimeError, match="CUDA"):
+        EfficientNGPT(cfg).decoder(2, 4, cache_dtype=torch.int8)

@@ -55,7 +55,7 @@ __device__ __forceinline__ float add_halves(float hi, float lo) { return fabsf(h
 template <int Width>
 struct Bf16Tile {
   static constexpr int D = Width;
-  static constexpr int kTile = 8192, kWarps = 8, kPairWarps = 4;
+  static constexpr int kTile = 8192, kWarps = 8, kPairWarps = 4, kPairPerSm = 2, kTileUs = 2;
   static constexpr int KT = kTile / (2 * D);
   static constexpr int NT = KT / 8;     // 8-key tiles
   static constexpr int KC = KT / 16;    // 16-key steps of P V

@@ -357,7 +357,7 @@ int launch_simt_heads(const typename KV::Args& a, cudaStream_t st) {
 // A range that begins or ends inside a pair leaves a part (o, m, l) in shared memory.  After a CTA barrier the parts
 // of a pair are joined by the warp that holds its first one; a pair that runs over CTAs leaves one part per CTA in
 // the workspace, joined by decode_join_list_kernel.
-constexpr size_t kPairSmem = 80 * 1024;  // of the form with a cluster per pair, at least: two CTAs per SM
+constexpr size_t kPairSmem = 80 * 1024;  // of the form with a cluster per pair, at least: no more than two CTAs per SM
 constexpr int kMaxListRows = 8192;      // of the list form: an int of shared memory each
 
 struct MmaArgs {
@@ -742,9 +742,8 @@ __global__ void __launch_bounds__(F::kWarps * 32) decode_list_kernel(typename F:
   float* out = a.work + (int64_t)blockIdx.x * 2 * pf;
   __syncthreads();   // every worker's parts are written
   // Groups of parts of one pair: those that begin in warp g, and the one that comes in from an earlier CTA (g = -1:
-  // warps 0, 1, ..).  With few rows a warp joins its own group (the last warp the incoming one too); with 8 all warps
-  // share each group's rows.
-  auto join_group = [&](int g, int r0, int step) {
+  // warps 0, 1, ..).  The warps share the rows of all groups.
+  auto join_group = [&](int g, int r) {
     const int pair = g < 0 ? s_head[0] : s_tail[g];
     if (pair < 0) return;
     const int w0 = max(g, 0);
@@ -754,14 +753,11 @@ __global__ void __launch_bounds__(F::kWarps * 32) decode_list_kernel(typename F:
     const float* rest = s_part + g * pf;
     float* to = g < 0 ? out : (s_over[g] ? out + pf : nullptr);   // at most one pair runs over the CTA's end
     const int b = pair / a.HQ, h = pair - b * a.HQ;
-    for (int r = r0; r < a.rows; r += step)
-      join_row<F, F::kWarps>(a, b, h, r, n, [=](int i) { return i == 0 ? first : (g < 0 ? first : rest) + i * pf; }, to, lane);
+    join_row<F, F::kWarps>(a, b, h, r, n, [=](int i) { return i == 0 ? first : (g < 0 ? first : rest) + i * pf; }, to, lane);
   };
-  if (a.rows < F::kWarps) {
-    join_group(warp, 0, 1);
-    if (warp == F::kWarps - 1) join_group(-1, 0, 1);
-  } else {
-    for (int g = -1; g < F::kWarps; ++g) join_group(g, warp, F::kWarps);
+  for (int i = warp; i < (F::kWarps + 1) * a.rows; i += F::kWarps) {
+    const int g = i / a.rows;
+    join_group(g - 1, i - g * a.rows);
   }
 }
 
@@ -778,8 +774,7 @@ __global__ void __launch_bounds__(F::kPairWarps * 32) decode_pair_kernel(typenam
   uint8_t* tiles = smem_raw + (base - sm100::smem_u32(smem_raw));           // one of each warp
   uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + F::kPairWarps * 2 * F::kTile);  // [F::kPairWarps]
   const int pf = part_floats<D>(a.rows);
-  float* s_part = reinterpret_cast<float*>(bars + F::kPairWarps);              // [F::kPairWarps] the warps' parts
-  float* s_cta = s_part + F::kPairWarps * pf;                                  // [cs] the CTAs' parts (rank 0)
+  float* s_cta = reinterpret_cast<float*>(bars + F::kPairWarps);                // [cs] the CTAs' parts (rank 0)
   __shared__ int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (cs > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
@@ -853,12 +848,14 @@ __global__ void __launch_bounds__(F::kPairWarps * 32) decode_pair_kernel(typenam
     return;
   }
   const int mine = min(max(c.T - rank * F::kPairWarps, 0), F::kPairWarps);   // this CTA's warps with tiles
-  if (warp < mine && ok) F::store_part(a, st, s_part + warp * pf, lane);
+  // (a warp's part goes where its tiles were: nothing is being copied any more)
+  if (warp < mine && ok) F::store_part(a, st, reinterpret_cast<float*>(tiles + warp * 2 * F::kTile), lane);
   __syncthreads();
-  const float* parts = s_part;
+  const float* parts = reinterpret_cast<const float*>(tiles);
+  constexpr int per_warp = 2 * F::kTile / 4;
   if (cs == 1) {
     for (int r = warp; r < a.rows; r += F::kPairWarps)
-      join_row<F, F::kPairWarps>(a, c.b, c.h, r, mine, [=](int i) { return parts + i * pf; }, nullptr, lane);
+      join_row<F, F::kPairWarps>(a, c.b, c.h, r, mine, [=](int i) { return parts + i * per_warp; }, nullptr, lane);
     return;
   }
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // every CTA of the cluster has started
@@ -866,7 +863,7 @@ __global__ void __launch_bounds__(F::kPairWarps * 32) decode_pair_kernel(typenam
     float* to;
     asm("mapa.u64 %0, %1, %2;" : "=l"(to) : "l"(s_cta + rank * pf), "r"(0));
     for (int r = warp; r < a.rows; r += F::kPairWarps)
-      join_row<F, F::kPairWarps>(a, c.b, c.h, r, mine, [=](int i) { return parts + i * pf; }, to, lane);
+      join_row<F, F::kPairWarps>(a, c.b, c.h, r, mine, [=](int i) { return parts + i * per_warp; }, to, lane);
   }
   sm100::cluster_sync_all();
   if (rank == 0) {
@@ -1015,12 +1012,13 @@ int pair_ctas(int B, int H, int Hkv, int table_width, int page_size) {
   const int64_t pairs = (int64_t)B * Hkv * ((H / Hkv + 7) / 8);
   const int64_t tiles = most_tiles(F::KT, table_width, page_size);
   const int sms = num_sms();
-  if (pairs > 2 * sms) return 0;
-  int cs = pairs * 8 <= sms ? 8 : pairs * 4 <= 2 * sms ? 4 : pairs * 2 <= 2 * sms ? 2 : 1;
+  const int slots = F::kPairPerSm * sms;
+  if (pairs > slots) return 0;
+  int cs = pairs * 8 <= sms ? 8 : pairs * 4 <= slots ? 4 : pairs * 2 <= slots ? 2 : 1;
   while (cs > 1 && tiles <= F::kPairWarps * (cs / 2)) cs >>= 1;
   const int64_t per_warp = (tiles + F::kPairWarps * cs - 1) / (F::kPairWarps * cs);
   if (B > 1 && per_warp > 4) return 0;
-  return 2 * (per_warp - 1) <= 2 + pairs * tiles / 380 ? cs : 0;
+  return F::kTileUs * (per_warp - 1) <= 2 + pairs * tiles * (2 * F::kTile) / 6200000 ? cs : 0;
 }
 
 // Floats of workspace of the list form.
@@ -1040,10 +1038,10 @@ int launch_pair(const typename F::Args& a, const CUtensorMap& mk, const CUtensor
   // Two CTAs per SM and no third one, which would leave other SMs idle (one wave has at most two per SM; 128 pairs of 32
   // tiles: 15.2 us so, 16.5 if three fit).
   constexpr size_t floor = kPairSmem;
-  const size_t needed = mma_smem<F>(a.rows, F::kPairWarps, F::kPairWarps + cs), smem = needed > floor ? needed : floor;
+  const size_t needed = mma_smem<F>(a.rows, F::kPairWarps, cs), smem = needed > floor ? needed : floor;
   // (the attribute is the kernel's, not the launch's: every call sets it to the same, largest size, so that a call on
   // another host thread cannot lower it between here and the launch)
-  const size_t most = mma_smem<F>(8, F::kPairWarps, F::kPairWarps + 8);
+  const size_t most = mma_smem<F>(8, F::kPairWarps, 8);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        (int)(most > floor ? most : floor));
   cudaLaunchConfig_t cfg = {};

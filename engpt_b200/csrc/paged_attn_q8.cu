@@ -138,7 +138,7 @@ struct Q8MmaArgs : MmaArgs {
 template <int Width, typename C, typename Type>
 struct Q8Tile {
   static constexpr int D = Width;
-  static constexpr int kTile = 8192, kWarps = 8, kPairWarps = 4;
+  static constexpr int kTile = 4096, kWarps = 16, kPairWarps = 8, kPairPerSm = 2, kTileUs = 2;
   static constexpr int KT = kTile / D;
   static constexpr int NG = KT / 8;       // groups of 8 keys, which share their scales
   static constexpr int kStep = KT < 64 ? KT : 64;   // keys of a softmax step

@@ -62,6 +62,7 @@ struct Bf16Tile {
   static constexpr int DK = D / 16;     // 16-dim steps of Q K^T
   static constexpr int DN = D / 8;      // 8-dim tiles of O
   static constexpr int kCodeBytes = 2, kBoxes = D / 64, kBoxRow = 128;
+  static constexpr bool kFlat = false;
   static constexpr CUtensorMapDataType kMapType = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   static constexpr CUtensorMapSwizzle kSwizzle = CU_TENSOR_MAP_SWIZZLE_128B;
   using T = __nv_bfloat16;

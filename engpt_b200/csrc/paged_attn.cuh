@@ -346,6 +346,7 @@ int launch_simt_heads(const typename KV::Args& a, cudaStream_t st) {
 //   kTile, kWarps, kPairWarps    bytes of a tile's keys, warps of a CTA of the list form and of the pair form
 //   T, Args            type of q and o; kernel arguments (MmaArgs and what F adds)
 //   kBoxes, kBoxRow    boxes of 64 columns of a group of R keys, bytes of a row of one
+//   kFlat, rows_at     rows that are one behind the other in a page are copied as they are, in one piece
 //   Spot, find         a look-up that is made a tile ahead of the tile's copies
 //   Side, fetch        loads that start with the tile's copies
 //   Query, load_query  a pair's query heads, up to 8, as rows 0-7 of the 16-row mma.sync operand
@@ -459,8 +460,12 @@ struct Worker {
     __syncwarp();
     if (here) {
       const uint32_t dst = tile + lane * box;
+      if constexpr (F::kFlat) {
+        sm100::bulk_load(dst, F::rows_at(a, 0, x.page, c.hk, x.off), box, bar);
+        sm100::bulk_load(dst + F::kTile, F::rows_at(a, 1, x.page, c.hk, x.off), box, bar);
+      }
 #pragma unroll
-      for (int half = 0; half < F::kBoxes; ++half) {
+      for (int half = 0; !F::kFlat && half < F::kBoxes; ++half) {
         sm100::tma_load_4d(dst + half * F::KT * F::kBoxRow, mk, half * 64, x.off, c.hk, x.page, bar);
         sm100::tma_load_4d(dst + half * F::KT * F::kBoxRow + F::kTile, mv, half * 64, x.off, c.hk, x.page, bar);
       }
@@ -628,7 +633,7 @@ __global__ void __launch_bounds__(F::kWarps * 32) decode_list_kernel(typename F:
     s_abort = 0;         // (every warp: a wait may set it only seconds later)
     s_head[warp] = s_tail[warp] = -1;
   }
-  if (tid == 0) {
+  if (!F::kFlat && tid == 0) {
     sm100::tma_prefetch_desc(&mk);
     sm100::tma_prefetch_desc(&mv);
   }
@@ -791,7 +796,7 @@ __global__ void __launch_bounds__(F::kPairWarps * 32) decode_pair_kernel(typenam
     sm100::mbar_init(w.bar, 1);
     sm100::fence_mbar_init();
     s_abort = 0;                        // (every warp: a wait may set it only seconds later)
-    if (warp == 0) {
+    if (!F::kFlat && warp == 0) {
       sm100::tma_prefetch_desc(&mk);
       sm100::tma_prefetch_desc(&mv);
     }
@@ -1093,7 +1098,7 @@ int launch_list(const typename F::Args& a, const CUtensorMap& mk, const CUtensor
 // Everything of a launch but what F adds to its arguments.
 template <typename F>
 int launch_mma(typename F::Args a, const AttnArgs& x, int Hkv, cudaStream_t st) {
-  int rc = get_encode();
+  int rc = F::kFlat ? ENGPT_OK : get_encode();
   if (rc) return rc;
   a.q = x.q;
   a.q_row = x.q_row;
@@ -1119,12 +1124,14 @@ int launch_mma(typename F::Args a, const AttnArgs& x, int Hkv, cudaStream_t st) 
   a.negative = x.scale_log2 < 0.f;
   a.o = x.o;
   a.work = x.work;
-  CUtensorMap mk, mv;
-  constexpr int esz = F::kCodeBytes;
-  if ((rc = page_map(&mk, x.k_pages, F::kMapType, esz, F::kBoxRow, F::kSwizzle, x.Dh, x.ps, Hkv, x.P, x.ks, a.R)))
-    return rc;
-  if ((rc = page_map(&mv, x.v_pages, F::kMapType, esz, F::kBoxRow, F::kSwizzle, x.Dh, x.ps, Hkv, x.P, x.vs, a.R)))
-    return rc;
+  CUtensorMap mk = {}, mv = {};
+  if constexpr (!F::kFlat) {
+    constexpr int esz = F::kCodeBytes;
+    if ((rc = page_map(&mk, x.k_pages, F::kMapType, esz, F::kBoxRow, F::kSwizzle, x.Dh, x.ps, Hkv, x.P, x.ks, a.R)))
+      return rc;
+    if ((rc = page_map(&mv, x.v_pages, F::kMapType, esz, F::kBoxRow, F::kSwizzle, x.Dh, x.ps, Hkv, x.P, x.vs, a.R)))
+      return rc;
+  }
   const int cs = pair_ctas<F>(x.B, x.H, Hkv, x.W, x.ps);
   // The end of a pair costs a worker about half a tile (its sums and stores, and tiles that are partly empty).  It is
   // counted once workers see such ends often (256 rows of 1 to 512 tokens: 51.8 us, 63.8 without); with few pairs the

@@ -762,16 +762,17 @@ int launch_store_team(const StoreArgs& a, const char* what, cudaStream_t st) {
   // a token per window while that makes no more warps than run at once some times over
   const bool single = a.n * (APPEND ? 2 : 1) * a.c.H <= (int64_t)num_sms() * 64;
   if (single) return launch_store_runs<T, Code, APPEND, LPR, 1>(a, 1, what, st);
-  if (a.c.block <= rows) return launch_store_runs<T, Code, APPEND, LPR, 1>(a, a.c.block, what, st);
-  if (a.c.block <= 4 * rows) return launch_store_runs<T, Code, APPEND, LPR, 4>(a, a.c.block, what, st);
-  return launch_store_runs<T, Code, APPEND, LPR, 8>(a, a.c.block, what, st);
+  if constexpr (LPR >= 8) {                            // (a warp has room for 64 shorter rows)
+    if (a.c.block > 4 * rows) return launch_store_runs<T, Code, APPEND, LPR, 8>(a, a.c.block, what, st);
+    if (a.c.block > rows) return launch_store_runs<T, Code, APPEND, LPR, 4>(a, a.c.block, what, st);
+  }
+  return launch_store_runs<T, Code, APPEND, LPR, 1>(a, a.c.block, what, st);
 }
 
 template <typename T, typename Code, bool APPEND>
 int launch_store_code(const StoreArgs& a, bool vec, const char* what, cudaStream_t st) {
   const int Dh = a.c.Dh;
   if (!vec) return launch_store_generic<T, Code, APPEND>(a, what, st);
-  if (Dh <= 8) return launch_store_team<T, Code, APPEND, 1>(a, what, st);
   if (Dh <= 16) return launch_store_team<T, Code, APPEND, 2>(a, what, st);
   if (Dh <= 32) return launch_store_team<T, Code, APPEND, 4>(a, what, st);
   if (Dh <= 64) return launch_store_team<T, Code, APPEND, 8>(a, what, st);

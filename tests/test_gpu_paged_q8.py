@@ -373,10 +373,24 @@ def test_attention_head_groups(cuda, dtype, kind, heads, kv_heads, dim):
     check_attention(attention_inputs([70, 0, 513, 1], heads, kv_heads, dim, 16, 8, dtype, kind, seed=heads))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv_heads", [(4, 4), (16, 2)])
+@pytest.mark.parametrize("dim", [16, 32, 48, 80, 96, 112])
+@pytest.mark.parametrize("bsz,width_tokens", [(1, 100), (1, 3000), (9, 700), (60, 400)])
+def test_attention_widths_of_any_number_of_pieces(cuda, dtype, kind, heads, kv_heads, dim, bsz, width_tokens):
+    """Head dims of 1, 2, 3, 5, 6 and 7 pieces of 16 codes, in every form of a launch."""
+    page = 24 if dim == 48 else 32
+    rng = np.random.default_rng(bsz)
+    lengths = [int(x) for x in rng.integers(0, width_tokens + 1, bsz)]
+    lengths[-1] = width_tokens
+    check_attention(attention_inputs(lengths, heads, kv_heads, dim, page, 8, dtype, kind, seed=dim))
+
+
 @pytest.mark.parametrize("layout", ["token", "both", "odd"])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("dim,page", [(64, 16), (128, 32), (48, 16)])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 32), (48, 16), (80, 64), (16, 16)])
 def test_attention_cache_layouts(cuda, dtype, kind, layout, dim, page):
     check_attention(attention_inputs([90, 300, 33], 6, 3, dim, page, 16, dtype, kind, layout=layout, seed=dim))
 

@@ -184,15 +184,12 @@ __global__ void __launch_bounds__(256) store_generic_kernel(StoreArgs a) {
 // ------------------------------------------------------------------ store, 8 elements a lane
 //
 // head_dim a multiple of 8, aligned.  LPR lanes (a power of two) share a row, 8 elements each; a warp has 32 / LPR rows
-// of a run beside each other and kSteps such steps, of k and of v, all loads in flight before the first is used.  They
-// stay in registers as they were loaded; the post-processed k waits for its scale in shared memory, as fp32.  W warps
-// share a run, so that it fits one team and its numbers are read once; a longer run is read twice.
+// of a run beside each other and S such steps, of k and of v, all loads in flight before the first is used.  They stay in
+// registers as they were loaded; the post-processed k waits for its scale in shared memory, as fp32.  W warps share a
+// run, so that it fits one team and its numbers are read once; a longer run is read twice.
 //
 // A team looks after the runs that begin in a window of `window` tokens, of one head: a block's worth in a long call,
 // which is one run then, a single token in a short one or where requests add a token each.
-template <typename T>
-constexpr int kSteps = sizeof(T) == 2 ? 4 : 2;
-
 // The largest of m >= 0 and the magnitudes of x and y; NaN if one is.
 __device__ __forceinline__ float most3(float m, float x, float y) {
   float r;
@@ -304,10 +301,10 @@ struct NoPostProcess {
   __device__ __forceinline__ NoPostProcess(const StoreArgs&, int, int) {}
 };
 
-// This lane's slices of kSteps rows of a run, k and v.
-template <typename T, bool APPEND, int LPR, int W>
+// This lane's slices of S rows of a run, k and v.
+template <typename T, bool APPEND, int LPR, int S, int W>
 struct Rows {
-  static constexpr int S = kSteps<T>, kRows = W * (32 / LPR);   // rows of the team's step
+  static constexpr int kRows = W * (32 / LPR);   // rows of the team's step
   using Post = std::conditional_t<APPEND, PostProcess<T>, NoPostProcess>;
   Raw<T> v[S], k[APPEND ? 1 : S];
   float4* s_k;             // appending: this lane's part of the warp's shared memory, [S][2][32]
@@ -392,9 +389,9 @@ struct Rows {
 };
 
 // q of a window of tokens (appending).
-template <typename T, int LPR, int W>
+template <typename T, int LPR, int S, int W>
 __device__ __forceinline__ void store_q(const StoreArgs& a, int h, int64_t w0, int64_t w1, int me, int lane) {
-  constexpr int S = kSteps<T>, RPW = 32 / LPR, kRows = W * RPW;
+  constexpr int RPW = 32 / LPR, kRows = W * RPW;
   int e0 = (lane % LPR) * 8;
   const bool mine = e0 < a.c.Dh;
   if (!mine) e0 = 0;
@@ -442,15 +439,16 @@ __device__ __forceinline__ void store_q(const StoreArgs& a, int h, int64_t w0, i
 }
 
 // CTAs of four warps per SM that the registers leave room for.
-template <bool APPEND>
-constexpr int kStoreCtas = APPEND ? 6 : 7;
+template <bool APPEND, int BYTES>
+constexpr int kStoreCtas = BYTES > 8 ? (APPEND ? 3 : 4) : APPEND ? 5 : 7;
 
-template <typename T, typename Code, bool APPEND, int LPR, int W>
-__global__ void __launch_bounds__(W > 4 ? 32 * W : 128, kStoreCtas<APPEND> * 4 / (W > 4 ? W : 4))
+template <typename T, typename Code, bool APPEND, int LPR, int S, int W>
+__global__ void __launch_bounds__(128, kStoreCtas<APPEND, S * (int)sizeof(T)>)
 store_runs_kernel(StoreArgs a, int window) {
-  constexpr int RPW = 32 / LPR, kRows = W * RPW, S = kSteps<T>;
+  static_assert(W == 1 || W == 4, "a team is a warp or the CTA");
+  constexpr int RPW = 32 / LPR, kRows = W * RPW;
   __shared__ uint32_t s_most[W > 1 ? W : 1][2];
-  __shared__ float4 s_k[APPEND ? (W > 4 ? W : 4) : 1][APPEND ? S * 64 : 1];
+  __shared__ float4 s_k[APPEND ? 4 : 1][APPEND ? S * 64 : 1];
   if constexpr (APPEND) {
     // started ahead of the end of what runs before (usually the projection), and so may be what follows
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -460,24 +458,23 @@ store_runs_kernel(StoreArgs a, int window) {
   const int me = W > 1 ? warp : 0;                     // this warp of its team
   const int64_t item = W > 1 ? blockIdx.x : blockIdx.x * 4ll + warp;
   const int64_t windows = (a.n + window - 1) / window;
-  if (item >= windows * (APPEND ? 2 : 1) * a.c.H) return;   // (of the last CTA of single warps only)
+  constexpr bool kApart = APPEND && S == 1;            // q is an item of its own
+  if (item >= windows * (kApart ? 2 : 1) * a.c.H) return;   // (of the last CTA of single warps only)
   const int64_t wp = item <= 0xffffffffLL ? (int64_t)((uint32_t)item / (uint32_t)a.c.H) : item / a.c.H;
   const int h = (int)(item - wp * a.c.H);
-  const int64_t w0 = (APPEND ? wp >> 1 : wp) * window, w1 = min(a.n, w0 + window);
+  const int64_t w0 = (kApart ? wp >> 1 : wp) * window, w1 = min(a.n, w0 + window);
   if constexpr (APPEND) {
-    if (wp & 1) {
-      store_q<T, LPR, W>(a, h, w0, w1, me, lane);
-      return;
-    }
+    if (!kApart || (wp & 1)) store_q<T, LPR, S, W>(a, h, w0, w1, me, lane);
+    if (kApart && (wp & 1)) return;
   }
   int e0 = (lane % LPR) * 8;
   const bool mine = e0 < a.c.Dh;
   if (!mine) e0 = 0;
-  const typename Rows<T, APPEND, LPR, W>::Post post(a, h, e0);
+  const typename Rows<T, APPEND, LPR, S, W>::Post post(a, h, e0);
   const T* const src_k = reinterpret_cast<const T*>(a.x[0]) + h * a.head[0] + e0;
   const T* const src_v = reinterpret_cast<const T*>(a.x[1]) + h * a.head[1] + e0;
   const int row0 = me * RPW + lane / LPR;              // this lane's first row of a run
-  Rows<T, APPEND, LPR, W> rows;
+  Rows<T, APPEND, LPR, S, W> rows;
   rows.s_k = &s_k[APPEND ? warp : 0][APPEND ? lane : 0];
 
   for (int64_t t0 = w0; t0 < w1; t0 += 32) {
@@ -738,35 +735,33 @@ int launch_store_generic(const StoreArgs& a, const char* what, cudaStream_t st) 
   return check_launch(what);
 }
 
-template <typename T, typename Code, bool APPEND, int LPR, int W>
+template <typename T, typename Code, bool APPEND, int LPR, int S, int W>
 int launch_store_runs(const StoreArgs& a, int window, const char* what, cudaStream_t st) {
-  const int64_t items = (a.n + window - 1) / window * (APPEND ? 2 : 1) * a.c.H, blocks = W > 1 ? items : (items + 3) / 4;
+  const int64_t items = (a.n + window - 1) / window * (APPEND && S == 1 ? 2 : 1) * a.c.H, blocks = W > 1 ? items : (items + 3) / 4;
   ENGPT_REQUIRE(blocks <= 0x7fffffffLL, ENGPT_ERR_SHAPE, "%s: too large", what);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3(W > 4 ? 32 * W : 128);
+  cfg.blockDim = dim3(128);
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = APPEND ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, store_runs_kernel<T, Code, APPEND, LPR, W>, a, window);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, store_runs_kernel<T, Code, APPEND, LPR, S, W>, a, window);
   if (e != cudaSuccess) return set_error(ENGPT_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
   return check_launch(what);
 }
 
 template <typename T, typename Code, bool APPEND, int LPR>
 int launch_store_team(const StoreArgs& a, const char* what, cudaStream_t st) {
-  const int rows = kSteps<T> * 32 / LPR;               // that a warp holds
+  constexpr int kHeld = 8 / sizeof(T), RPW = 32 / LPR;    // steps: 4 of bf16 rows, 2 of fp32 ones, or twice as many
   // a token per window while that makes no more warps than run at once some times over
-  const bool single = a.n * (APPEND ? 2 : 1) * a.c.H <= (int64_t)num_sms() * 64;
-  if (single) return launch_store_runs<T, Code, APPEND, LPR, 1>(a, 1, what, st);
-  if constexpr (LPR >= 8) {                            // (a warp has room for 64 shorter rows)
-    if (a.c.block > 4 * rows) return launch_store_runs<T, Code, APPEND, LPR, 8>(a, a.c.block, what, st);
-    if (a.c.block > rows) return launch_store_runs<T, Code, APPEND, LPR, 4>(a, a.c.block, what, st);
-  }
-  return launch_store_runs<T, Code, APPEND, LPR, 1>(a, a.c.block, what, st);
+  const bool single = a.n * (APPEND ? 2 : 1) * a.c.H <= (int64_t)num_sms() * (APPEND ? 256 : 64);
+  if (single) return launch_store_runs<T, Code, APPEND, LPR, 1, 1>(a, 1, what, st);
+  if (a.c.block > 2 * kHeld * RPW) return launch_store_runs<T, Code, APPEND, LPR, 2 * kHeld, 4>(a, a.c.block, what, st);
+  if (a.c.block > kHeld * RPW) return launch_store_runs<T, Code, APPEND, LPR, 2 * kHeld, 1>(a, a.c.block, what, st);
+  return launch_store_runs<T, Code, APPEND, LPR, kHeld, 1>(a, a.c.block, what, st);
 }
 
 template <typename T, typename Code, bool APPEND>

@@ -328,10 +328,10 @@ struct Rows {
       v[s].clear();
       if (in && mine) {
         kr[s].load(k0);
-        v[s].load(v0);
+        if (!APPEND) v[s].load(v0);
       }
       k0 += kRows * a.row[0];
-      v0 += kRows * a.row[1];
+      if (!APPEND) v0 += kRows * a.row[1];
       if constexpr (APPEND) {
         pos[s] = in ? pos_p[s * kRows] : -1;
         rho[s] = in ? rho_p[s * kRows] : 1.f;
@@ -354,7 +354,12 @@ struct Rows {
         s_k[s * 64 + 32] = make_float4(x[4], x[5], x[6], x[7]);
         most_k = most8(s == 0 ? 0.f : most_k, x);
         v_mult[s] = PostProcess<T>::per_rho(rho[s]);
-        if (!on) v[s].clear();
+      }
+      // (v follows when k has given its registers up: more warps instead of more loads in flight per warp)
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        if (mine && ((live >> s) & 1u)) v[s].load(v0);
+        v0 += kRows * a.row[1];
       }
     }
   }
@@ -440,7 +445,7 @@ __device__ __forceinline__ void store_q(const StoreArgs& a, int h, int64_t w0, i
 
 // CTAs of four warps per SM that the registers leave room for.
 template <bool APPEND, int BYTES>
-constexpr int kStoreCtas = BYTES > 8 ? (APPEND ? 3 : 4) : APPEND ? 5 : 7;
+constexpr int kStoreCtas = BYTES > 8 ? 4 : APPEND ? 6 : 7;
 
 template <typename T, typename Code, bool APPEND, int LPR, int S, int W>
 __global__ void __launch_bounds__(128, kStoreCtas<APPEND, S * (int)sizeof(T)>)

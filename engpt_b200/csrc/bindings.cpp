@@ -282,7 +282,7 @@ void write_kv_pages_q8(const Tensor& k_in, const Tensor& v_in, const Tensor& slo
   const auto dev = k_pages.device();
   require_device(k_in, dev);
   require_device(v_in, dev);
-  forward_only({&k_in, &v_in, &k_scales, &v_scales});
+  forward_only({&k_in, &v_in, &k_pages, &v_pages, &k_scales, &v_scales});
   const int64_t nd = k_in.dim();
   TORCH_CHECK_VALUE(nd >= 2 && k_in.sizes() == v_in.sizes() && k_in.scalar_type() == v_in.scalar_type() &&
                         k_in.size(nd - 2) == p.heads && k_in.size(nd - 1) == p.dim,
@@ -309,7 +309,7 @@ Tensor qkv_append_q8(const Tensor& qkv_in, const Tensor& rho, const Tensor& cos,
   const Q8Pools p = check_q8_pools(k_pages, v_pages, k_scales, v_scales);
   const auto dev = k_pages.device();
   for (const Tensor* t : {&qkv_in, &rho, &cos, &sin, &qk_scale}) require_device(*t, dev);
-  forward_only({&qkv_in, &rho, &cos, &sin, &qk_scale, &k_scales, &v_scales});
+  forward_only({&qkv_in, &rho, &cos, &sin, &qk_scale, &k_pages, &v_pages, &k_scales, &v_scales});
   const int64_t nd = qkv_in.dim();
   TORCH_CHECK_VALUE(nd >= 3 && qkv_in.size(nd - 3) == 3 && qkv_in.size(nd - 2) == p.heads &&
                         qkv_in.size(nd - 1) == p.dim,
@@ -346,7 +346,7 @@ py::tuple read_kv_pages_q8(const Tensor& slots, const Tensor& k_pages, const Ten
                            const Tensor& v_scales, at::ScalarType dtype) {
   const Q8Pools p = check_q8_pools(k_pages, v_pages, k_scales, v_scales);
   const auto dev = k_pages.device();
-  forward_only({&k_scales, &v_scales});
+  forward_only({&k_pages, &v_pages, &k_scales, &v_scales});
   TORCH_CHECK_NOT_IMPLEMENTED(dtype == at::kBFloat16 || dtype == at::kFloat,
                               "engpt_b200 kernels support float32 and bfloat16, got ", dtype);
   check_index(slots, "slots", slots.sizes(), dev);
@@ -369,7 +369,7 @@ Tensor paged_sdpa_q8(const Tensor& q_in, const Tensor& k_pages, const Tensor& v_
   const Q8Pools p = check_q8_pools(k_pages, v_pages, k_scales, v_scales);
   const auto dev = k_pages.device();
   require_device(q_in, dev);
-  forward_only({&q_in, &k_scales, &v_scales});
+  forward_only({&q_in, &k_pages, &v_pages, &k_scales, &v_scales});
   TORCH_CHECK_VALUE(q_in.dim() == 3 && q_in.size(2) == p.dim,
                     "q must have shape [batch, n_head, head_dim] and the cache's head_dim");
   const int code = dtype_code(q_in);

@@ -1010,7 +1010,7 @@ inline bool list_fits(int B, int H, int KT, int table_width, int page_size) {
 // without a tile.  Its warps take their tiles one after the other, 2 us each, where the list form spreads them over all
 // SMs at 16 KB / 6.2 TB/s = 1/380 us each: with t tiles per warp the pair form is taken while 2 (t - 1) <= 2 + pairs *
 // tiles / 380 (16 pairs of 128 tiles: 12.3 against 13.0 us, 8 pairs of 128: 10.7 against 9.6, 16 pairs of 256: 19.2
-// against 18.5), and, as the rows of a batch may differ and the longest one decides, with at most 4 tiles per warp if
+// against 18.5; an F gives the time of its own tiles in kTileUs), and, as the rows of a batch may differ and the longest one decides, with at most 4 tiles per warp if
 // there are several rows (8 rows of 16 pairs of 32 tiles: 15.4 us against the list's 17.0 if all are that long).
 template <typename F>
 int pair_ctas(int B, int H, int Hkv, int table_width, int page_size) {

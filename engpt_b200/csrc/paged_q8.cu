@@ -190,6 +190,12 @@ __global__ void __launch_bounds__(256) store_generic_kernel(StoreArgs a) {
 //
 // A team looks after the runs that begin in a window of `window` tokens, of one head: a block's worth in a long call,
 // which is one run then, a single token in a short one or where requests add a token each.
+//
+// 32768 tokens of 16 heads of 64, 15 of 16 with a slot, bf16 to int8 (190 MB move): 42.6 us = 4.5 TB/s, bound by the
+// latency of a run's chain (slots, rows, maximum, codes) at 28 warps per SM.  The append of 8188 tokens of 16 heads of 128
+// in blocks of 64 (168 MB): 56 us = 3.0 TB/s, the same at 16 warps per SM, with 28 M instructions at 40 % of the issue
+// slots; 72 with 8 warps and 4 steps, 80 with the post-process applied twice in place of the shared memory, 66 with v
+// loaded beside k.
 // The largest of m >= 0 and the magnitudes of x and y; NaN if one is.
 __device__ __forceinline__ float most3(float m, float x, float y) {
   float r;
@@ -443,7 +449,8 @@ __device__ __forceinline__ void store_q(const StoreArgs& a, int h, int64_t w0, i
   }
 }
 
-// CTAs of four warps per SM that the registers leave room for.
+// CTAs of four warps per SM that the registers leave room for.  The write above: 42.6 us with 7, 43.9 with 6, 51 with 4,
+// 55 with 10 (registers spill); the append: 56 with 4 in its 8-step form, 65 with 3, 74 with 5.
 template <bool APPEND, int BYTES>
 constexpr int kStoreCtas = BYTES > 8 ? 4 : APPEND ? 6 : 7;
 
@@ -620,7 +627,9 @@ __global__ void __launch_bounds__(256) read_generic_kernel(ReadArgs a) {
 
 // Head_dim a multiple of N = 8 or 16, aligned.  A thread owns N codes of a row (k and v) and walks over tokens; a CTA
 // takes several tokens beside each other where a row has fewer pieces than it has threads.  The slot of the next token
-// is on its way while this one's numbers are.
+// is on its way while this one's numbers are.  16 x 2048 tokens, half of them with a slot, 16 heads of 64, int8 to bf16
+// (168 MB move): 32.4 us = 5.2 TB/s with the registers held to 6 CTAs per SM; 33.9 with 5, 36.7 with 7, 39 with 3; 8 codes
+// a thread 47.
 constexpr int kReadCtas = 6;
 
 template <typename T>
@@ -761,7 +770,10 @@ int launch_store_runs(const StoreArgs& a, int window, const char* what, cudaStre
 template <typename T, typename Code, bool APPEND, int LPR>
 int launch_store_team(const StoreArgs& a, const char* what, cudaStream_t st) {
   constexpr int kHeld = 8 / sizeof(T), RPW = 32 / LPR;    // steps: 4 of bf16 rows, 2 of fp32 ones, or twice as many
-  // a token per window while that makes no more warps than run at once some times over
+  // A token per window while that makes no more warps than run at once some times over.  Appending, the calls that
+  // matter add a token per request, and a window of a block's tokens would be as many runs one after the other: 999
+  // requests, 16 heads of 64: 23 us so, 61 in windows of 16 (one prompt of 1100 tokens: 27 us so, 8 in windows); a write
+  // is a prompt's (2047 tokens: 6.3 us in windows, 17 a token each).
   const bool single = a.n * (APPEND ? 2 : 1) * a.c.H <= (int64_t)num_sms() * (APPEND ? 256 : 64);
   if (single) return launch_store_runs<T, Code, APPEND, LPR, 1, 1>(a, 1, what, st);
   if (a.c.block > 2 * kHeld * RPW) return launch_store_runs<T, Code, APPEND, LPR, 2 * kHeld, 4>(a, a.c.block, what, st);

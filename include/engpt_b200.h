@@ -447,7 +447,8 @@ ENGPT_API int engpt_write_kv_pages_q8(const void* k, const void* v, const int64_
 /*
  * engpt_qkv_append with such a cache; dtype is that of qkv and q_out.  k and v
  * are quantised from their fp32 values.  A token whose position is out of
- * range is not kept, and has no part in its block's scale.
+ * range is not kept, and has no part in its block's scale; what its slot held
+ * is void where that scale changes.
  */
 ENGPT_API int engpt_qkv_append_q8(const void* qkv, int dtype, const float* rho, const float* cos_tab,
                                   const float* sin_tab, int rope_rows, int rope_half, const float* qk_scale,

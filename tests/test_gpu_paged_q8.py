@@ -535,3 +535,101 @@ def test_attention_strided_q(cuda, dtype):
     odd = torch.zeros(3, 6, 65, dtype=dtype, device=cuda)[..., 1:]
     odd.copy_(args[0])
     check_attention((odd,) + args[1:], attend((odd,) + args[1:]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 80, 33])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_attention_of_a_query_that_is_no_number(cuda, dtype, kind, dim, bad):
+    """Its own result is NaN; the other heads of its row and kv head, and the other rows, are untouched."""
+    args = attention_inputs([50, 400], 8, 2, dim, 16, 8, dtype, kind, seed=3)
+    clean = check_attention(args)
+    q = args[0].clone()
+    q[1, 2, 5] = bad
+    out = attend((q,) + args[1:])
+    assert out[1, 2].isnan().all()
+    keep = torch.ones(2, 8, dtype=torch.bool, device=cuda)
+    keep[1, 2] = False
+    assert torch.equal(out[keep], clean[keep])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [128, 80, 112])
+def test_attention_most_rows_that_the_list_takes(cuda, dtype, dim):
+    """8192 rows with eight query heads on a kv head: the most shared memory that a launch asks for."""
+    rng = np.random.default_rng(2)
+    lengths = rng.integers(0, 20, 8192).tolist()
+    lengths[4000] = 130
+    check_attention(attention_inputs(lengths, 8, 1, dim, 16, 16, dtype, "int8", seed=1))
+
+
+def test_attention_far_into_a_large_pool(cuda):
+    """Codes more than 2^31 bytes behind the pool's start, scales of strides that are not their shape's."""
+    page, heads, dim, pool = 64, 8, 128, 36000                        # 2.36e9 codes each
+    if torch.cuda.mem_get_info()[0] < 12e9:
+        pytest.skip("needs 12 GB")
+    k = torch.zeros(pool, heads, page, dim, dtype=torch.int8, device=cuda)
+    v = torch.zeros_like(k)
+    ks, vs = (torch.zeros(heads, 4, pool, device=cuda).permute(2, 0, 1) for _ in range(2))
+    n = 200
+    pages = torch.tensor([pool - 1, 3, pool - 2, 17], dtype=torch.int32)
+    slots = torch.tensor([int(pages[p // page]) * page + p % page for p in range(n)], dtype=torch.int32, device=cuda)
+    kr, vr = rows(n, heads, dim, torch.bfloat16, 5)
+    K.write_kv_pages_q8(kr, vr, slots, k, v, ks, vs)
+    back = K.read_kv_pages_q8(slots, k, v, ks, vs, dtype=torch.float32)
+    small = [x[pages.long().to(cuda)].contiguous() for x in (k, v, ks, vs)]
+    near = torch.tensor([(p // page) * page + p % page for p in range(n)], dtype=torch.int32, device=cuda)
+    for a, b in zip(back, K.read_kv_pages_q8(near, *small, dtype=torch.float32)):
+        assert torch.equal(a, b) and (a != 0).any()
+    q = torch.randn(1, 16, dim, device=cuda).bfloat16()
+    lens = torch.tensor([n], dtype=torch.int32, device=cuda)
+    out = K.paged_sdpa_q8(q, k, v, ks, vs, pages[None].to(cuda), lens, scale=0.1)
+    check_attention((q, small, torch.arange(4, dtype=torch.int32, device=cuda)[None], lens, 0.1), out)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_calls_on_two_streams_and_in_graphs(cuda, kind):
+    """Calls at the same time on two streams, and replays of one captured graph of all four operators, give what they give
+    alone."""
+    heads, dim, page, block, n = 4, 64, 16, 16, 60
+    sets = []
+    for seed in range(2):
+        qkv, rho, cos, sin, scale, pos = append_inputs(n, heads, dim, torch.bfloat16, seed)
+        cache = Q.make_pools(n, heads, page, dim, block, kind)
+        Q.fill_pools(cache, seed)
+        slots = Q.prompt_slots([3] * 4, n // 4, page, n, seed).flatten().to(cuda)
+        k, v = rows(n, heads, dim, torch.bfloat16, seed)
+        table = (slots.view(4, -1)[:, [0, -1]] // page).contiguous()
+        lens = torch.tensor([18] * 4, dtype=torch.int32, device=cuda)
+        sets.append((qkv, rho, cos, sin, scale, pos, cache, [c.clone() for c in cache], slots, k, v, table, lens))
+
+    def run(s):
+        qkv, rho, cos, sin, scale, pos, cache, first, slots, k, v, table, lens = s
+        for c, f in zip(cache, first):
+            c.copy_(f)
+        K.write_kv_pages_q8(k, v, slots, *cache)
+        q = K.qkv_append_from_carried_q8(qkv, rho, cos, sin, scale, 1e-6, pos, slots, *cache)
+        o = K.paged_sdpa_q8(q[:4].contiguous(), *cache, table, lens, scale=0.125)
+        return (q, o, *K.read_kv_pages_q8(slots, *cache))
+
+    want = [[x.clone() for x in run(s)] for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(run(sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+    with torch.cuda.stream(streams[0]):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=streams[0]):
+            out = run(sets[0])
+        for _ in range(3):
+            graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want[0]))

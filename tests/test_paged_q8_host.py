@@ -87,6 +87,19 @@ def test_forward_only():
             calls(i.long(), cache)[0]()
 
 
+def test_forward_only_in_every_tensor():
+    """(float8 pools can ask for a gradient too)"""
+    with FakeTensorMode():
+        i, kp, vp, ks, vs = fakes()
+        cache = [kp.view(torch.float8_e4m3fn), vp.view(torch.float8_e4m3fn), ks, vs]
+        for t in cache:
+            t.requires_grad_(True)
+            for call in calls(i, cache):
+                with pytest.raises(NotImplementedError, match="forward-only"):
+                    call()
+            t.requires_grad_(False)
+
+
 def i64(*v):
     return (ctypes.c_int64 * len(v))(*v)
 

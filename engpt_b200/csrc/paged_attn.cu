@@ -56,6 +56,7 @@ template <int Width>
 struct Bf16Tile {
   static constexpr int D = Width;
   static constexpr int kTile = 8192, kWarps = 8, kPairWarps = 4, kPairPerSm = 2, kTileUs = 2;
+  static constexpr bool kPartsOver = false;
   static constexpr int KT = kTile / (2 * D);
   static constexpr int NT = KT / 8;     // 8-key tiles
   static constexpr int KC = KT / 16;    // 16-key steps of P V

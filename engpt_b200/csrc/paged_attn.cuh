@@ -344,6 +344,7 @@ int launch_simt_heads(const typename KV::Args& a, cudaStream_t st) {
 // What a tile holds and how it is used is the business of a class F:
 //   D, KT              width (a smaller head_dim is padded with zeros by TMA, in shared memory only), keys of a tile
 //   kTile, kWarps, kPairWarps    bytes of a tile's keys, warps of a CTA of the list form and of the pair form
+//   kPairPerSm, kTileUs, kPartsOver    of the pair form: CTAs per SM, time of a tile, parts that go where the tiles were
 //   T, Args            type of q and o; kernel arguments (MmaArgs and what F adds)
 //   kBoxes, kBoxRow    boxes of 64 columns of a group of R keys, bytes of a row of one
 //   kFlat, rows_at     rows that are one behind the other in a page are copied as they are, in one piece
@@ -779,7 +780,11 @@ __global__ void __launch_bounds__(F::kPairWarps * 32) decode_pair_kernel(typenam
   uint8_t* tiles = smem_raw + (base - sm100::smem_u32(smem_raw));           // one of each warp
   uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + F::kPairWarps * 2 * F::kTile);  // [F::kPairWarps]
   const int pf = part_floats<D>(a.rows);
-  float* s_cta = reinterpret_cast<float*>(bars + F::kPairWarps);                // [cs] the CTAs' parts (rank 0)
+  // the warps' parts: where their tiles were, or [F::kPairWarps] of their own; then [cs] the CTAs' parts (rank 0)
+  constexpr bool over = F::kPartsOver;
+  float* parts = over ? reinterpret_cast<float*>(tiles) : reinterpret_cast<float*>(bars + F::kPairWarps);
+  const int per_warp = over ? 2 * F::kTile / 4 : pf;
+  float* s_cta = reinterpret_cast<float*>(bars + F::kPairWarps) + (over ? 0 : F::kPairWarps * pf);
   __shared__ int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (cs > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
@@ -853,11 +858,8 @@ __global__ void __launch_bounds__(F::kPairWarps * 32) decode_pair_kernel(typenam
     return;
   }
   const int mine = min(max(c.T - rank * F::kPairWarps, 0), F::kPairWarps);   // this CTA's warps with tiles
-  // (a warp's part goes where its tiles were: nothing is being copied any more)
-  if (warp < mine && ok) F::store_part(a, st, reinterpret_cast<float*>(tiles + warp * 2 * F::kTile), lane);
+  if (warp < mine && ok) F::store_part(a, st, parts + warp * per_warp, lane);   // (nothing is being copied any more)
   __syncthreads();
-  const float* parts = reinterpret_cast<const float*>(tiles);
-  constexpr int per_warp = 2 * F::kTile / 4;
   if (cs == 1) {
     for (int r = warp; r < a.rows; r += F::kPairWarps)
       join_row<F, F::kPairWarps>(a, c.b, c.h, r, mine, [=](int i) { return parts + i * per_warp; }, nullptr, lane);
@@ -1043,10 +1045,11 @@ int launch_pair(const typename F::Args& a, const CUtensorMap& mk, const CUtensor
   // Two CTAs per SM and no third one, which would leave other SMs idle (one wave has at most two per SM; 128 pairs of 32
   // tiles: 15.2 us so, 16.5 if three fit).
   constexpr size_t floor = kPairSmem;
-  const size_t needed = mma_smem<F>(a.rows, F::kPairWarps, cs), smem = needed > floor ? needed : floor;
+  constexpr int own = F::kPartsOver ? 0 : F::kPairWarps;
+  const size_t needed = mma_smem<F>(a.rows, F::kPairWarps, own + cs), smem = needed > floor ? needed : floor;
   // (the attribute is the kernel's, not the launch's: every call sets it to the same, largest size, so that a call on
   // another host thread cannot lower it between here and the launch)
-  const size_t most = mma_smem<F>(8, F::kPairWarps, 8);
+  const size_t most = mma_smem<F>(8, F::kPairWarps, own + 8);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        (int)(most > floor ? most : floor));
   cudaLaunchConfig_t cfg = {};

@@ -120,6 +120,7 @@ struct Q8Tile {
   static constexpr int KT = !Flat ? 256 / DC : DC <= 2 ? 128 : DC <= 5 ? 64 : 32;
   static constexpr int kTile = KT * kWidth, kWarps = Flat && DC == 5 ? 14 : 16;
   static constexpr int kPairWarps = 8, kPairPerSm = 2, kTileUs = 2;
+  static constexpr bool kPartsOver = true;          // (so that two CTAs fit an SM with eight query heads of 128 too)
   static constexpr int NG = KT / 8;       // groups of 8 keys, which share their scales
   static constexpr int kStep = KT < 64 ? KT : 64;   // keys of a softmax step
   static constexpr int NT = kStep / 8;    // 8-key tiles of a step

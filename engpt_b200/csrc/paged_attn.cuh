@@ -748,8 +748,9 @@ __global__ void __launch_bounds__(F::kWarps * 32) decode_list_kernel(typename F:
   float* out = a.work + (int64_t)blockIdx.x * 2 * pf;
   __syncthreads();   // every worker's parts are written
   // Groups of parts of one pair: those that begin in warp g, and the one that comes in from an earlier CTA (g = -1:
-  // warps 0, 1, ..).  The warps share the rows of all groups.
-  auto join_group = [&](int g, int r) {
+  // warps 0, 1, ..).  Eight warps with few rows join their own groups (the last warp the incoming one too), and share
+  // each group's rows with 8; more warps share the rows of all groups.
+  auto join_group = [&](int g, int r0, int step) {
     const int pair = g < 0 ? s_head[0] : s_tail[g];
     if (pair < 0) return;
     const int w0 = max(g, 0);
@@ -759,11 +760,19 @@ __global__ void __launch_bounds__(F::kWarps * 32) decode_list_kernel(typename F:
     const float* rest = s_part + g * pf;
     float* to = g < 0 ? out : (s_over[g] ? out + pf : nullptr);   // at most one pair runs over the CTA's end
     const int b = pair / a.HQ, h = pair - b * a.HQ;
-    join_row<F, F::kWarps>(a, b, h, r, n, [=](int i) { return i == 0 ? first : (g < 0 ? first : rest) + i * pf; }, to, lane);
+    for (int r = r0; r < a.rows; r += step)
+      join_row<F, F::kWarps>(a, b, h, r, n, [=](int i) { return i == 0 ? first : (g < 0 ? first : rest) + i * pf; }, to, lane);
   };
-  for (int i = warp; i < (F::kWarps + 1) * a.rows; i += F::kWarps) {
-    const int g = i / a.rows;
-    join_group(g - 1, i - g * a.rows);
+  if constexpr (F::kWarps > 8) {
+    for (int i = warp; i < (F::kWarps + 1) * a.rows; i += F::kWarps) {
+      const int g = i / a.rows;
+      join_group(g - 1, i - g * a.rows, a.rows);
+    }
+  } else if (a.rows < F::kWarps) {
+    join_group(warp, 0, 1);
+    if (warp == F::kWarps - 1) join_group(-1, 0, 1);
+  } else {
+    for (int g = -1; g < F::kWarps; ++g) join_group(g, warp, F::kWarps);
   }
 }
 

@@ -633,3 +633,31 @@ def test_calls_on_two_streams_and_in_graphs(cuda, kind):
             graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(out, want[0]))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("block", [16, 64])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("tokens", [1, 64, 2048])
+def test_numbers_that_are_none_in_bf16(cuda, kind, block, bad, tokens):
+    """One bad element of a bf16 row, in the write and in the append, whatever form the call takes: its head's block of its
+    pool is NaN (of k and q's row where it is in k or q), every other number is one."""
+    heads, dim, page, pool = 8, 128, 64, tokens // 64 + 2
+    slots = torch.arange(tokens, dtype=torch.int32, device=cuda)
+    at, h = tokens * 2 // 3, 5
+    blk = slice(at // block * block, min(tokens, at // block * block + block))
+    k, v = (torch.randn(tokens, heads, dim, device=cuda).bfloat16() for _ in range(2))
+    v[at, h, 77] = bad
+    cache = Q.make_pools(pool, heads, page, dim, block, kind)
+    K.write_kv_pages_q8(k, v, slots, *cache)
+    got_k, got_v = K.read_kv_pages_q8(slots, *cache)
+    nan = torch.zeros(tokens, heads, dim, dtype=torch.bool, device=cuda)
+    nan[blk, h] = True
+    assert torch.equal(got_v.isnan(), nan) and got_k.isfinite().all()
+
+    qkv, rho, cos, sin, scale, pos = append_inputs(tokens, heads, dim, torch.bfloat16, 3)
+    qkv[at, 1, h, 3] = bad
+    cache = Q.make_pools(pool, heads, page, dim, block, kind)
+    q = K.qkv_append_from_carried_q8(qkv, rho, cos, sin, scale, 1e-6, pos, slots, *cache)
+    got_k, got_v = K.read_kv_pages_q8(slots, *cache)
+    assert torch.equal(got_k.isnan(), nan) and got_v.isfinite().all() and q.isfinite().all()

@@ -107,7 +107,7 @@ struct Q8MmaArgs : MmaArgs {
 // 8 to 9 cycles for 80 bytes and no fewer for 16, where it moves whole pieces of a page at the rate of memory: 64 rows
 // of 2048 tokens, 8 heads of 80: 64 us padded, 38 so.
 //
-// A tile costs some 650 instructions of a warp (64 keys of 64: 16 products of scores, 16 of values, 96 instructions that
+// A tile costs some 700 instructions of a warp (64 keys of 64: 16 products of scores, 16 of values, 96 instructions that
 // make fp16 of the values' codes, 180 of the softmax, the rest its bookkeeping), and 16 warps with 8 KB each cover
 // memory and each other best: 64 rows of up to 4096 tokens, 16 heads of 64, 57.5 us; 12 warps with 16 KB 56.9, but 256
 // rows of 1 to 512 tokens 48 us there, 37 so, and eight query heads of 128 have no room; 8 warps with 16 KB 60 and 56.

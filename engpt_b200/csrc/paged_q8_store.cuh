@@ -395,7 +395,11 @@ struct Rows {
       k[APPEND ? 0 : s].get(x);
     } else {
       v[s].get(x);
-      if constexpr (APPEND) inv *= v_mult[s];          // (x / rho / scale, with one rounding in another place)
+      if constexpr (APPEND) {
+        // (one by one: the product of the two factors can be infinite where x / rho is 0, or next to nothing)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= v_mult[s];
+      }
     }
     return make_uint2(Code::encode4(x, inv), Code::encode4(x + 4, inv));
   }

@@ -361,7 +361,8 @@ struct Rows {
         s_k[s * 64] = make_float4(x[0], x[1], x[2], x[3]);
         s_k[s * 64 + 32] = make_float4(x[4], x[5], x[6], x[7]);
         most_k = most8(s == 0 ? 0.f : most_k, x);
-        v_mult[s] = PostProcess<T>::per_rho(rho[s]);
+        // (a token that is left out has zeros for v, and any number for rho)
+        v_mult[s] = (live >> s) & 1u ? PostProcess<T>::per_rho(rho[s]) : 0.f;
       }
       // (v follows when k has given its registers up: more warps instead of more loads in flight per warp)
 #pragma unroll

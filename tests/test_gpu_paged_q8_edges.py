@@ -6,7 +6,7 @@ import torch
 
 from engpt_b200 import _lib, kernels as K
 from tests import paged_q8_blocks as B, paged_q8_ref as Q
-from tests.test_gpu_paged_q8 import DTYPES, KINDS, append_error, append_inputs
+from tests.test_gpu_paged_q8 import DTYPES, KINDS, append_error, append_inputs, expect_status
 from tests.test_gpu_paged_q8_large import check_both, sizes, state
 
 pytestmark = pytest.mark.gpu
@@ -77,3 +77,29 @@ def test_append_values_below_the_least_scale(cuda, dtype, kind, dim, block, n):
     K.qkv_append_from_carried_q8(qkv, rho, cos, sin, scale, 1e-6, pos, slots, *cache)
     _, rk, rv = B.postprocess(qkv, rho, cos, sin, scale, 1e-6, pos)
     check_both(cache, before, rk, rv, slots, append_error(rk), append_error(rv))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,block,n", CALLS)
+@pytest.mark.parametrize("radius", [0.0, float("nan"), float("inf"), 1e-38, -1.0])
+def test_append_radii_of_tokens_that_are_left_out(cuda, dtype, kind, dim, block, n, radius):
+    """A token with a bad position has no part in its block's scales, whatever its rho and its numbers."""
+    heads, page = 16, 64
+    n = tokens_of(n, heads)
+    qkv, rho, cos, sin, scale, pos = append_inputs(n, heads, dim, dtype, 9, table=50)
+    at = torch.arange(n, device=cuda)
+    dead = (at % 7 == 3) | ((at + 3) // block % 5 == 4)           # in runs of others, and whole runs
+    pos = torch.where(dead, torch.where(at % 2 == 0, 50, -1), pos).to(torch.int32)
+    rho = torch.where(dead, radius, rho)
+    qkv[dead & (at % 3 == 0)] = float("nan")
+    slots = torch.arange(3, n + 3, dtype=torch.int32, device=cuda)
+    cache = Q.make_pools(n // page + 1, heads, page, dim, block, kind)
+    Q.fill_pools(cache, 2)
+    before = state(cache)
+    q = K.qkv_append_from_carried_q8(qkv, rho, cos, sin, scale, 1e-6, pos, slots, *cache)
+    expect_status(42)
+    assert (q[dead] == 0).all() and q.isfinite().all()
+    _, rk, rv = B.postprocess(qkv, rho, cos, sin, scale, 1e-6, pos.clamp(0, 49))
+    rk[dead], rv[dead] = 0.0, 0.0
+    check_both(cache, before, rk, rv, slots, append_error(rk), append_error(rv), dead)

@@ -130,7 +130,8 @@ struct Q8Tile {
   static constexpr CUtensorMapDataType kMapType = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   static constexpr CUtensorMapSwizzle kSwizzle = DC == 4 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
   static constexpr bool kFine = sizeof(Type) == 4;   // three digits or two parts of q, two parts of a weight
-  static constexpr float kWeightTop = 16384.f, kLeastScale = 7.52316384526264e-37f;   // 2^-120
+  // (2^14 and 2^-112: their quotient has to be finite, as it meets scales of 0)
+  static constexpr float kWeightTop = 16384.f, kLeastScale = 1.925929944387236e-34f;
   using T = Type;
   using Args = Q8MmaArgs;
   using Pairs = CodePairs<C>;

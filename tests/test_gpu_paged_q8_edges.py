@@ -5,8 +5,9 @@ import pytest
 import torch
 
 from engpt_b200 import _lib, kernels as K
-from tests import paged_q8_blocks as B, paged_q8_ref as Q
-from tests.test_gpu_paged_q8 import DTYPES, KINDS, append_error, append_inputs, expect_status
+from tests import paged_q8_blocks as B, paged_q8_ref as Q, paged_ref as R
+from tests.test_gpu_paged_q8 import (DTYPES, KINDS, append_error, append_inputs, attend, attention_inputs,
+                                     expect_status)
 from tests.test_gpu_paged_q8_large import check_both, sizes, state
 
 pytestmark = pytest.mark.gpu
@@ -103,3 +104,89 @@ def test_append_radii_of_tokens_that_are_left_out(cuda, dtype, kind, dim, block,
     _, rk, rv = B.postprocess(qkv, rho, cos, sin, scale, 1e-6, pos.clamp(0, 49))
     rk[dead], rv[dead] = 0.0, 0.0
     check_both(cache, before, rk, rv, slots, append_error(rk), append_error(rv), dead)
+
+
+# ------------------------------------------------------------------ attention
+def weighted(args):
+    """The 64-bit result, and the tolerance of check_weighted."""
+    q, cache, table, lengths, scale = args
+    k, v = Q.values(cache[0], cache[2]), Q.values(cache[1], cache[3])
+    step = cache[3].cpu().double().abs().repeat_interleave(cache[1].shape[2] // cache[3].shape[2], dim=2)[..., None]
+    off = Q.query_error(q, cache[0].dtype)
+    qd, table = q.cpu().double(), table.cpu()
+    heads, dim = q.shape[1:]
+    group = heads // k.shape[1]
+    out, tol = torch.zeros_like(qd), torch.zeros_like(qd)
+    top = Q.TOP[cache[0].dtype]
+    for b, n in enumerate(lengths.tolist()):
+        if n <= 0:
+            continue
+        rows, vals, steps = (R.gather_rows(x, table[b], n) for x in (k, v, step))
+        for h in range(heads):
+            kh, vh, sh = rows[:, h // group], vals[:, h // group], steps[:, h // group, 0]
+            p = torch.softmax(kh @ qd[b, h] * scale, dim=0)
+            out[b, h] = p @ vh
+            score = ((dim + 8) * 2.0 ** -24 * (kh.abs() @ qd[b, h].abs()).max() + (kh.abs() @ off[b, h]).max()) * abs(scale)
+            weight = 1.45 * score + 2.0 ** -20 + 2 * n * 2.0 ** -24
+            spread = p @ vh.abs()
+            small = n * 2.0 ** -39 * (p * sh).max() * top
+            tol[b, h] = (torch.finfo(q.dtype).eps / 2 * out[b, h].abs() + weight * (spread + out[b, h].abs()) +
+                         (2.0 ** -21 if q.dtype == torch.float32 else 2.0 ** -11) * spread + small + 1e-37)
+    return out, tol
+
+
+def check_weighted(args, out=None):
+    """Against the 64-bit result, with a tolerance that follows the values with their weights.
+
+    As paged_q8_ref.attention_tolerance, but what the values' weights are off by is taken on sum p |v|, not on the largest
+    value of the row: a relative error of a weight (of the scores, the exponentials and the sums) moves numerator and
+    denominator by as much of sum p |v| and of the result.  A weight p vs (vs: the value's scale) is one fp16 number, half a
+    step 2^-11 (fp32 results: two, 2^-21), or half of 2^-24 where it is below fp16's normal numbers: the head's largest
+    p vs is at least 2^14 there, so that is 2^-39 of it, times a code, for each of n keys.
+    """
+    out = attend(args) if out is None else out
+    ref, tol = weighted(args)
+    err = (out.cpu().double() - ref).abs()
+    assert (err <= tol).all(), f"max error {err.max().item()}, over its tolerance by {(err / tol).max().item()}"
+    return out
+
+
+FORMS = [([400, 130, 64, 7], 2, 2, 16), ([300] * 150, 2, 2, 32), ([3000], 8, 1, 64), ([333, 64, 65], 12, 2, 24)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 80, 33])
+@pytest.mark.parametrize("lengths,heads,kv_heads,page", FORMS)
+@pytest.mark.parametrize("least", [0.0, 1e-43, 2.0 ** -121, 2.0 ** -115])
+def test_attention_scales_of_nearly_nothing(cuda, dtype, kind, dim, lengths, heads, kv_heads, page, least):
+    """Value scales of 0 (a block that was never written, a foreign cache), or too small to be one of the quantising write,
+    first in a row, everywhere, or everywhere but at its end."""
+    args = attention_inputs(lengths, heads, kv_heads, dim, page, 8, dtype, kind, seed=dim)
+    q, cache, table, lens, scale = args
+    for b, n in enumerate(lengths):
+        pages = table[b, :R.pages_of(n, page)].long()
+        last = pages[-1:] if b % 2 else pages[:0]
+        keep = cache[3][last].clone()
+        cache[3][pages] = torch.where(cache[3][pages].isnan(), cache[3][pages], least)
+        cache[3][last] = keep
+    out = check_weighted(args)
+    if least == 0.0:
+        assert (out[::2] == 0).all()
+    for i in range(0, len(lengths), 2):
+        cache[2][table[i, 0]] = 0.0                                # scores of 0 too
+    check_weighted(args)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 80, 33])
+def test_attention_whole_tiles_of_bad_pages(cuda, dtype, kind, dim):
+    """The pages of a row's first tiles are outside the pool: they count as absent."""
+    page = 64
+    q, cache, table, lens, scale = attention_inputs([500, 300, 190], 4, 2, dim, page, 8, dtype, kind, seed=2)
+    bad = table.clone()
+    bad[:, :2] = torch.tensor([-1, cache[0].shape[0]], dtype=torch.int32, device=cuda)
+    out = attend((q, cache, bad, lens, scale))
+    expect_status(44)
+    check_weighted((q, cache, table[:, 2:].contiguous(), lens - 2 * page, scale), out)

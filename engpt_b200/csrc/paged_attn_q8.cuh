@@ -230,7 +230,7 @@ struct Q8Tile {
       // round(q 2^(bits - e)): the row's largest element comes to 2^bits up to 2^(bits + 1), but not so near to that that
       // its first digit would be above 127.  (Rows that are nearly zero, below 2^-100, are brought less far up.)
       constexpr int bits = kFine ? 22 : 14;
-      const uint32_t e = min(max((most + 0x20000u) >> 23, 27u), 253u);
+      const uint32_t e = min(max((most + 0x20000u) >> 23, 27u), 255u);
       const float up = __uint_as_float((uint32_t)(254 + bits - e) << 23);
       x.factor = most >= 0x7f800000u ? __uint_as_float(0x7fc00000u)
                                      : a.scale_log2 * __uint_as_float((uint32_t)(e - bits) << 23);

@@ -190,3 +190,18 @@ def test_attention_whole_tiles_of_bad_pages(cuda, dtype, kind, dim):
     out = attend((q, cache, bad, lens, scale))
     expect_status(44)
     check_weighted((q, cache, table[:, 2:].contiguous(), lens - 2 * page, scale), out)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 48, 128])
+@pytest.mark.parametrize("top", [1.6e38, 1.72e38, 2.5e38, 3.38e38])
+def test_attention_of_the_largest_queries(cuda, dtype, kind, dim, top):
+    """Elements of q up to the end of the range, over keys so small that the scores are ordinary ones."""
+    args = attention_inputs([100, 300, 1], 4, 2, dim, 16, 16, dtype, kind, seed=6)
+    q, cache, table, lens, _ = args
+    q.copy_(torch.randn(q.shape, device=cuda).clamp(-3, 3) / 3 * top)
+    q[0, :, 3], q[1, :, 5] = top, -top
+    cache[2].mul_(1e-36)
+    check_weighted((q, cache, table, lens, 0.05))
+    check_weighted((q, cache, table, lens, -0.05))

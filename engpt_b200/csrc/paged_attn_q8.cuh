@@ -31,10 +31,11 @@ struct Q8AttnArgs : AttnArgs {
 // on fp16 operands with fp32 sums:
 //   S = Q K^T with q brought to [1, 2) by a power of two of its row, which the row's score factor takes back; a
 //   fp32 q is two fp16 numbers, the second one (what the first left, times 2^11) in the otherwise idle rows 8-15;
-//   O^T += V^T P^T with p vs / vref in fp16, vref the largest value scale so far (raised like the running maximum of the
-//   softmax): at most 2^14 as scaled, so that what is 2^-28 of the largest weight is still a normal number.  That
-//   rounding is 2^-11 of a weight, an eighth of that of a bf16 result; for fp32 results what it left is multiplied
-//   too.  (O^T because its 16-row operand is full of values, where that of O would be half empty.)
+//   O^T += V^T P^T with weights p vs / ref in fp16, ref the largest p vs of the head so far (it shrinks with p when the
+//   running maximum of the scores rises): at most 2^15 as scaled, so that what is 2^-28 of the head's largest weight is
+//   still a normal number, whatever the scales of keys that have no weight.  That rounding is 2^-11 of a weight, an
+//   eighth of that of a bf16 result; for fp32 results what it left is multiplied too.  (O^T because its 16-row operand
+//   is full of values, where that of O would be half empty.)
 //
 // The columns of a product may come in any order that both operands share, and keys and columns of O in any order at
 // all: a 16-byte row of 8-bit codes that ldmatrix distributes (4 bytes a lane, in place of two 16-bit numbers) is the
@@ -131,7 +132,7 @@ struct Q8Tile {
   static constexpr CUtensorMapSwizzle kSwizzle = DC == 4 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
   static constexpr bool kFine = sizeof(Type) == 4;   // three digits or two parts of q, two parts of a weight
   // (2^14 and 2^-112: their quotient has to be finite, as it meets scales of 0)
-  static constexpr float kWeightTop = 16384.f, kLeastScale = 1.925929944387236e-34f;
+  static constexpr float kWeightTop = 16384.f, kLeastRef = 1.925929944387236e-34f;
   using T = Type;
   using Args = Q8MmaArgs;
   using Pairs = CodePairs<C>;
@@ -149,9 +150,10 @@ struct Q8Tile {
   };
   struct State {
     // piece c, row of O^T: columns 16 c + 2 g and 16 c + 2 g + 1 (0, 1 and 2, 3) of heads 2 t and 2 t + 1 of the group, in
-    // units of vref / kWeightTop, where g = lane / 4 and t = lane % 4.  m and l are those of head g.
+    // units of their heads' ref / kWeightTop, where g = lane / 4 and t = lane % 4.  m, l, ref and per_ref (kWeightTop / ref)
+    // are those of head g.
     float o[DC][4];
-    float m, l, vref, per_vref, factor;
+    float m, l, ref, per_ref, factor;
     __device__ __forceinline__ void reset() {
 #pragma unroll
       for (int i = 0; i < DC; ++i)
@@ -159,8 +161,8 @@ struct Q8Tile {
         for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
       m = -INFINITY;
       l = 0.f;
-      vref = kLeastScale;
-      per_vref = kWeightTop / kLeastScale;
+      ref = kLeastRef;
+      per_ref = kWeightTop / kLeastRef;
       factor = 1.f;
     }
     // Every column of O^T times its head's x.
@@ -333,18 +335,6 @@ struct Q8Tile {
       __syncwarp();
     }
     st.factor = x.factor;
-    // value scales relative to the largest one so far; a NaN is above all, and makes the rows NaN
-    const uint32_t top = __reduce_max_sync(0xffffffffu, lane >= NG ? __float_as_uint(side.scale) & 0x7fffffffu : 0u);
-    if (top > __float_as_uint(st.vref)) {
-      const float corr = st.vref / __uint_as_float(top);
-      st.vref = __uint_as_float(top);
-      st.per_vref = kWeightTop / st.vref;
-#pragma unroll
-      for (int i = 0; i < DC; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) st.o[i][j] *= corr;
-    }
-    const float weight = side.scale * st.per_vref;
 #pragma unroll
     for (int k0 = 0; k0 < KT; k0 += kStep) {
       float s[NT][2];
@@ -367,33 +357,50 @@ struct Q8Tile {
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       const float ms = mx == -INFINITY ? 0.f : mx * st.factor;
-      if (__any_sync(0xffffffffu, mx > st.m)) {
+      const bool rises = mx > st.m;
+      if (rises) {
+        // (O stays as it is in its units, which shrink with the weights that are in it)
         const float corr = st.m == -INFINITY ? 0.f : sm100::ex2_approx(st.m * st.factor - ms);
-        st.scale_heads(corr, lane);
+        st.ref *= corr;
         st.l *= corr;
         st.m = mx;
       }
-      uint32_t hi[NT], lo[kFine ? NT : 1];
-      float sum[2] = {0.f, 0.f};
+      float sum[2] = {0.f, 0.f}, most = 0.f;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const float w = __shfl_sync(0xffffffffu, weight, NG + k0 / 8 + n);
-        float p[2];
+        const float vs = __shfl_sync(0xffffffffu, side.scale, NG + k0 / 8 + n);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          p[i] = sm100::ex2_approx(fmaf(s[n][i], st.factor, -ms));
-          if (!WHOLE && s[n][i] == -INFINITY) p[i] = 0.f;   // (the product is NaN for a scale of 0)
-          sum[i] += p[i];
-          p[i] *= w;
-        }
-        if constexpr (kFine) {
-          hi[n] = split_half2(p[0], p[1]);
-          lo[n] = pack_half2(p[0], p[1]);
-        } else {
-          hi[n] = pack_half2(p[0], p[1]);
+          float p = sm100::ex2_approx(fmaf(s[n][i], st.factor, -ms));
+          if (!WHOLE && s[n][i] == -INFINITY) p = 0.f;      // (the product is NaN for a scale of 0)
+          sum[i] += p;
+          s[n][i] = p * vs;
+          most = fmaxf(most, fabsf(s[n][i]));
         }
       }
       st.l += sum[0] + sum[1];
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const bool other = rises || most > 2.f * st.ref;
+      if (__any_sync(0xffffffffu, other)) {
+        // (a head's numbers do not depend on the others': the quotient is 1 where its ref stays)
+        const float ref = other ? fmaxf(fmaxf(st.ref, most), kLeastRef) : st.ref;
+        st.scale_heads(st.ref / ref, lane);
+        st.ref = ref;
+        st.per_ref = kWeightTop / ref;
+      }
+      uint32_t hi[NT], lo[kFine ? NT : 1];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        s[n][0] *= st.per_ref;
+        s[n][1] *= st.per_ref;
+        if constexpr (kFine) {
+          hi[n] = split_half2(s[n][0], s[n][1]);
+          lo[n] = pack_half2(s[n][0], s[n][1]);
+        } else {
+          hi[n] = pack_half2(s[n][0], s[n][1]);
+        }
+      }
 #pragma unroll
       for (int j = 0; j < NT; j += 2) {
         const int key = k0 + j * 8 + (q4 & 1) * 8 + r8;
@@ -421,11 +428,7 @@ struct Q8Tile {
     st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
     st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
     if (st.m != -INFINITY) st.m *= st.factor;
-    const float unit = st.vref * (1.f / kWeightTop);
-#pragma unroll
-    for (int i = 0; i < DC; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) st.o[i][j] *= unit;
+    st.scale_heads(st.ref * (1.f / kWeightTop), threadIdx.x & 31);
   }
 
   static __device__ __forceinline__ void store_part(const Args& a, const State& st, float* part, int lane) {

@@ -6,8 +6,7 @@ import torch
 
 from engpt_b200 import _lib, kernels as K
 from tests import paged_q8_blocks as B, paged_q8_ref as Q, paged_ref as R
-from tests.test_gpu_paged_q8 import (DTYPES, KINDS, append_error, append_inputs, attend, attention_inputs,
-                                     expect_status)
+from tests.test_gpu_paged_q8 import (DTYPES, KINDS, append_error, append_inputs, attend, attention_inputs, expect_status)
 from tests.test_gpu_paged_q8_large import check_both, sizes, state
 
 pytestmark = pytest.mark.gpu
@@ -152,6 +151,45 @@ def check_weighted(args, out=None):
 
 
 FORMS = [([400, 130, 64, 7], 2, 2, 16), ([300] * 150, 2, 2, 32), ([3000], 8, 1, 64), ([333, 64, 65], 12, 2, 24)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 80, 33])
+@pytest.mark.parametrize("lengths,heads,kv_heads,page", FORMS)
+@pytest.mark.parametrize("ratio", [2.0 ** 20, 2.0 ** 33, 2.0 ** 90])
+def test_attention_large_values_without_weight(cuda, dtype, kind, dim, lengths, heads, kv_heads, page, ratio):
+    """Keys that get next to no weight have values of far larger scale than the others: these keep their bits."""
+    args = attention_inputs(lengths, heads, kv_heads, dim, page, 8, dtype, kind, seed=dim)
+    q, cache, table, lens, _ = args
+    scale = 1.0
+    q.copy_(0.05 * torch.randn(q.shape, device=cuda))
+    for b, n in enumerate(lengths):
+        for j in range(0, n, 8):
+            if j // 8 % 5 != 2 or j // 8 in (0, (n - 1) // 8):
+                continue
+            pg, bl = int(table[b, j // page]), j % page // 8
+            cache[3][pg, :, bl] *= ratio
+            # the key is against the first kv head's queries: a score of some -150 for all of its group
+            cache[2][pg, :, bl] = 1.0
+            cache[0].view(torch.uint8)[pg, :, bl * 8:bl * 8 + 8] = 0
+            cache[0].view(torch.uint8)[pg, :, bl * 8:bl * 8 + 8, 0] = 0x85 if kind == "int8" else 0xf6   # -123, -224
+    q[..., 0] = 1.25 if kind == "int8" else 0.7
+    check_weighted((q, cache, table, lens, scale))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 80, 33])
+@pytest.mark.parametrize("lengths,heads,kv_heads,page", FORMS)
+def test_attention_scales_far_apart(cuda, dtype, kind, dim, lengths, heads, kv_heads, page):
+    """Values of very different scale beside each other, with weights that are as far apart."""
+    args = attention_inputs(lengths, heads, kv_heads, dim, page, 8, dtype, kind, seed=dim + 1, spread=20.0)
+    cache = args[1]
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    e = torch.rand(cache[3].shape, generator=gen, device="cuda") * 60 - 30
+    cache[3].copy_(torch.where(cache[3].isnan(), cache[3], torch.exp2(e.round())))
+    check_weighted(args)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -1015,7 +1015,8 @@ inline bool list_fits(int B, int H, int KT, int table_width, int page_size) {
 // CTAs per pair of the pair form, or 0 for the list form.
 //
 // The pair form starts and ends faster (an empty launch takes some 3 us, the list form's two 5.5) but does not balance
-// rows of different length, so it has to be one wave of CTAs.  Its clusters are the widest that run at once: 8 CTAs up
+// rows of different length, so it is meant to be one wave of CTAs (it is for kPairPerSm CTAs per SM, if F's registers
+// leave room for as many).  Its clusters are the widest that run at once: 8 CTAs up
 // to one per SM in all (16 pairs of 32 tiles: 4.9 us with 8, 5.8 with 4, 8.3 with 2), 4 or 2 up to two per SM (64 pairs
 // of 32 tiles: 10.6 us with 4, 12.1 with 2, 15.3 with 8 in three waves; list 13.1); narrower where a warp would be
 // without a tile.  Its warps take their tiles one after the other, 2 us each, where the list form spreads them over all

@@ -108,11 +108,12 @@ struct Q8MmaArgs : MmaArgs {
 // 8 to 9 cycles for 80 bytes and no fewer for 16, where it moves whole pieces of a page at the rate of memory: 64 rows
 // of 2048 tokens, 8 heads of 80: 64 us padded, 38 so.
 //
-// A tile costs some 700 instructions of a warp (64 keys of 64: 16 products of scores, 16 of values, 96 instructions that
-// make fp16 of the values' codes, 180 of the softmax, the rest its bookkeeping), and 16 warps with 8 KB each cover
-// memory and each other best: 64 rows of up to 4096 tokens, 16 heads of 64, 57.5 us; 12 warps with 16 KB 56.9, but 256
-// rows of 1 to 512 tokens 48 us there, 37 so, and eight query heads of 128 have no room; 8 warps with 16 KB 60 and 56.
-// Without any arithmetic on the tiles the first is 50 us.
+// A tile costs some 730 instructions of a warp (64 keys of 64: 16 products of scores, 16 of values, 96 instructions that
+// make fp16 of the values' codes, 210 of the softmax, the rest its bookkeeping), and 16 warps with 8 KB each cover
+// memory and each other best, although their 128 registers spill 4 to 260 bytes in nearly every form (fp32 q the most):
+// 64 rows of up to 4096 tokens, 16 heads of 64, 58 us.  Measured before weights had a reference per head (57.5 then): 12
+// warps with 16 KB 56.9, but 256 rows of 1 to 512 tokens 48 us there, 37 so, and eight query heads of 128 have no room; 8
+// warps with 16 KB 60 and 56.  Without any arithmetic on the tiles the first is 50 us.
 template <int Pieces, bool Flat, typename C, typename Type>
 struct Q8Tile {
   static constexpr int DC = Pieces;                 // 16-byte pieces of a row
@@ -121,7 +122,11 @@ struct Q8Tile {
   static constexpr int KT = !Flat ? 256 / DC : DC <= 2 ? 128 : DC <= 5 ? 64 : 32;
   static constexpr int kTile = KT * kWidth, kWarps = Flat && DC == 5 ? 14 : 16;
   static constexpr int kPairWarps = 8, kPairPerSm = 2, kTileUs = 2;
-  static constexpr bool kPartsOver = true;          // (so that two CTAs fit an SM with eight query heads of 128 too)
+  // (Shared memory has room for two CTAs of the pair form per SM, with eight query heads of 128 too.  Registers have where
+  // the kernel takes no more than 128: int8 codes and bf16 q at head_dim 64, and a few of the flat forms.  The others, 130 to
+  // 200, run one at a time, so a launch of more CTAs than SMs is two waves: 4 rows of 1024 tokens, 16 heads of 128, 13.3 us
+  // where 2 rows take 7.1.)
+  static constexpr bool kPartsOver = true;
   static constexpr int NG = KT / 8;       // groups of 8 keys, which share their scales
   static constexpr int kStep = KT < 64 ? KT : 64;   // keys of a softmax step
   static constexpr int NT = kStep / 8;    // 8-key tiles of a step

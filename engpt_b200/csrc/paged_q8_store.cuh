@@ -7,6 +7,8 @@
 //   scale = need if the run holds the block's first slot, else max(scale, need)
 //   code  = round(x / scale)
 //
+// (x / scale as the product with the rounded reciprocal of the scale: an x within 2^-23 of the middle between two codes,
+// such as half of the block's largest, may go to either)
 // and where the scale of a block that is not started anew grows, its codes
 // outside the run become round(code * (scale before / scale)): the values
 // stay, as far as the coarser step allows.
@@ -187,16 +189,17 @@ __global__ void __launch_bounds__(256) store_generic_kernel(StoreArgs a) {
 //
 // head_dim a multiple of 8, aligned.  LPR lanes (a power of two) share a row, 8 elements each; a warp has 32 / LPR rows
 // of a run beside each other and S such steps, of k and of v, all loads in flight before the first is used.  They stay in
-// registers as they were loaded; the post-processed k waits for its scale in shared memory, as fp32.  W warps share a
-// run, so that it fits one team and its numbers are read once; a longer run is read twice.
+// registers as they were loaded (those with four bf16 or two fp32 rows a lane spill 40 to 136 bytes of them); the
+// post-processed k waits for its scale in shared memory, as fp32.  W warps share a run, so that it fits one team and its
+// numbers are read once; a longer run is read twice.
 //
 // A team looks after the runs that begin in a window of `window` tokens, of one head: a block's worth in a long call,
 // which is one run then, a single token in a short one or where requests add a token each.
 //
 // 32768 tokens of 16 heads of 64, 15 of 16 with a slot, bf16 to int8 (190 MB move): 42.6 us = 4.5 TB/s, bound by the
 // latency of a run's chain (slots, rows, maximum, codes) at 28 warps per SM.  The append of 8188 tokens of 16 heads of 128
-// in blocks of 64 (168 MB): 56 us = 3.0 TB/s, the same at 16 warps per SM, with 28 M instructions at 40 % of the issue
-// slots; 72 with 8 warps and 4 steps, 80 with the post-process applied twice in place of the shared memory, 66 with v
+// in blocks of 64 (168 MB): 57 us = 3.0 TB/s, bound by the same latency at 16 warps per SM, a window's q ahead of its slots
+// (29 M instructions, 46 % of the issue slots); 72 with 8 warps and 4 steps, 80 with the post-process applied twice in place of the shared memory, 66 with v
 // loaded beside k.
 // The largest of m >= 0 and the magnitudes of x and y; NaN if one is.
 __device__ __forceinline__ float most3(float m, float x, float y) {
@@ -457,7 +460,7 @@ __device__ __forceinline__ void store_q(const StoreArgs& a, int h, int64_t w0, i
 }
 
 // CTAs of four warps per SM that the registers leave room for.  The write above: 42.6 us with 7, 43.9 with 6, 51 with 4,
-// 55 with 10 (registers spill); the append: 56 with 4 in its 8-step form, 65 with 3, 74 with 5.
+// 55 with 10 (more of them spill); the append: 56 with 4 in its 8-step form, 65 with 3, 74 with 5.
 template <bool APPEND, int BYTES>
 constexpr int kStoreCtas = BYTES > 8 ? 4 : APPEND ? 6 : 7;
 
@@ -667,7 +670,8 @@ int launch_store_team(const StoreArgs& a, const char* what, cudaStream_t st) {
   // A token per window while that makes no more warps than run at once some times over.  Appending, the calls that
   // matter add a token per request, and a window of a block's tokens would be as many runs one after the other: 999
   // requests, 16 heads of 64: 23 us so, 61 in windows of 16 (one prompt of 1100 tokens: 27 us so, 8 in windows); a write
-  // is a prompt's (2047 tokens: 6.3 us in windows, 17 a token each).
+  // is a prompt's (2047 tokens: 6.3 us in windows, 17 a token each).  The rule sees the number of tokens alone: a step of
+  // more than 1184 requests with 16 heads goes in windows too (4096: 130 us).
   const bool single = a.n * (APPEND ? 2 : 1) * a.c.H <= (int64_t)num_sms() * (APPEND ? 256 : 64);
   if (single) return launch_store_runs<T, Code, APPEND, LPR, 1, 1>(a, 1, what, st);
   if (a.c.block > 2 * kHeld * RPW) return launch_store_runs<T, Code, APPEND, LPR, 2 * kHeld, 4>(a, a.c.block, what, st);

@@ -434,8 +434,9 @@ def write_kv_pages_q8(k: Tensor, v: Tensor, slots: Tensor, k_pages: Tensor, v_pa
     need, ``max(max |x|, 2^-100) / top`` (``top`` 127 for int8, 448 for e4m3);
     otherwise it keeps the larger one of that and its scale so far, and where
     that grows, the codes of its other tokens become ``round(code * (scale before
-    / scale))``.  Codes are ``round(x / scale)``.  An infinity or NaN makes the
-    block's scale NaN until the block starts anew.
+    / scale))``.  Codes are ``round(x / scale)``, with the quotient as a product
+    of fp32 numbers: next to the middle between two codes either may be taken.
+    An infinity or NaN makes the block's scale NaN until the block starts anew.
 
     Slots other than ``-1`` must be distinct, and those of one block stand side by
     side in ``slots`` (seen as one row), in ascending order, as ``advance_block_tables``
@@ -472,6 +473,8 @@ def paged_sdpa_q8(q: Tensor, k_pages: Tensor, v_pages: Tensor, k_scales: Tensor,
     q ``[B, H, Dh]`` and the result are bf16 or fp32.  Codes and scales behind a
     row's length have no effect, whatever they are.  The tensor cores are used for
     ``Dh`` up to 128 and a multiple of 16, pages and blocks of a multiple of 8
-    tokens and 16-byte aligned strides.
+    tokens and 16-byte aligned strides.  There an element of q is good to 2^-15
+    (fp32: 2^-23) of its row's largest one over int8 codes, and a weight of a
+    value to 2^-11 (fp32: 2^-21), or 2^-39 of its head's largest.
     """
     return _lib.native().paged_sdpa_q8(q, k_pages, v_pages, k_scales, v_scales, block_table, lengths, scale)

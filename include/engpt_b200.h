@@ -427,7 +427,8 @@ ENGPT_API int engpt_paged_attention(const void* q, const int64_t* q_strides, con
  *           anew: what its other slots held is void), else max(scale, need);
  *           where that raises it, the block's other codes become
  *           round(code * (scale before / scale))
- *   code  = round(x / scale), ties to even codes
+ *   code  = round(x / scale), the quotient as a product of fp32 numbers: next
+ *           to the middle between two codes either may be taken
  * An infinity or NaN among them makes the block's scale NaN until the block
  * starts anew.  The tokens of one block must stand side by side in `slots`, in
  * the order of their slots (as engpt_advance_block_tables gives them); a call

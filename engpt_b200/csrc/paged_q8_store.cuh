@@ -1,7 +1,7 @@
 // Writing the paged key-value cache in 8 bits (paged_q8.cu: finished rows; paged_q8_append.cu: the post-process).
 //
 // The tokens that one call puts into a block of the cache stand side by side
-// in it, in the order of their slots; such a run is quantised as a whole:
+// in it, in slots that follow one another; such a run is quantised as a whole:
 //
 //   need  = max(max |x|, 2^-100) / top        (top: 127 for int8, 448 for e4m3)
 //   scale = need if the run holds the block's first slot, else max(scale, need)
@@ -12,6 +12,9 @@
 // and where the scale of a block that is not started anew grows, its codes
 // outside the run become round(code * (scale before / scale)): the values
 // stay, as far as the coarser step allows.
+//
+// Tokens that go on in the same block but not in the next slot would be a second run of it, in a race with the first one:
+// they are recorded and left out.
 //
 // All of it is a pass over the numbers with a maximum in between, bound by HBM.
 #pragma once
@@ -65,6 +68,11 @@ __device__ __forceinline__ int checked_slot(const StoreArgs& a, int slot, bool r
   if (slot >= 0 && slot < a.c.n_slots) return slot;
   if (slot != -1 && record) record_device_error(ENGPT_ERR_ARG, 43);
   return -1;
+}
+
+// Is slot `before` in the block that begins with slot `first` (0 or more)?  Negative ones are in none.
+__device__ __forceinline__ bool in_block(const StoreArgs& a, int before, int first) {
+  return before >= first && before - first < a.c.block;
 }
 
 // Numbers of one (token, head) row, as they go into the cache before the quantisation.
@@ -147,7 +155,10 @@ __global__ void __launch_bounds__(256) store_generic_kernel(StoreArgs a) {
   const int slot = checked_slot(a, a.slots[n], part == 0 && h == 0 && lane == 0);
   if (slot < 0) return;
   const int off = slot % a.c.block, first = slot - off;   // (the block size divides the page size)
-  if (off > 0 && n > 0 && a.slots[n - 1] == slot - 1) return;
+  if (n > 0 && in_block(a, a.slots[n - 1], first)) {   // of an earlier token's run, or astray
+    if (a.slots[n - 1] != slot - 1 && part == 0 && h == 0 && lane == 0) record_device_error(ENGPT_ERR_ARG, 43);
+    return;
+  }
   int run = 1;
   while (off + run < a.c.block && n + run < a.n && a.slots[n + run] == slot + run) ++run;
 
@@ -508,7 +519,9 @@ store_runs_kernel(StoreArgs a, int window) {
     const bool window_token = mine_n < w1;
     const int slot = checked_slot(a, given, window_token && h == 0 && me == 0);
     const int my_off = max(slot, 0) - a.c.block_of(max(slot, 0)) * a.c.block;   // (blocks divide pages)
-    uint32_t heads = __ballot_sync(0xffffffffu, window_token && slot >= 0 && !(my_off > 0 && before == slot - 1));
+    const bool goes_on = in_block(a, before, slot - my_off);   // an earlier token's run, or is astray
+    uint32_t heads = __ballot_sync(0xffffffffu, window_token && slot >= 0 && !goes_on);
+    if (h == 0 && window_token && slot >= 0 && goes_on && before != slot - 1) record_device_error(ENGPT_ERR_ARG, 43);
     while (heads) {
       const int i = __ffs(heads) - 1;
       heads &= heads - 1;

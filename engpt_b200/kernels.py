@@ -439,8 +439,11 @@ def write_kv_pages_q8(k: Tensor, v: Tensor, slots: Tensor, k_pages: Tensor, v_pa
     An infinity or NaN makes the block's scale NaN until the block starts anew.
 
     Slots other than ``-1`` must be distinct, and those of one block stand side by
-    side in ``slots`` (seen as one row), in ascending order, as ``advance_block_tables``
-    gives them.  Where they do not, that block's numbers are undefined.
+    side in ``slots`` (seen as one row) and follow one another, ``s, s + 1, s + 2``, as
+    ``advance_block_tables`` gives them.  A token beside another one of its block, but
+    not in the next slot, is left out with those that follow it, and
+    ``engpt_b200._lib.raise_on_device_status`` reports it.  Where tokens of other blocks or
+    ``-1`` stand between those of one block, its numbers are undefined.
     """
     _lib.native().write_kv_pages_q8(k, v, slots, k_pages, v_pages, k_scales, v_scales)
 

@@ -431,8 +431,11 @@ ENGPT_API int engpt_paged_attention(const void* q, const int64_t* q_strides, con
  *           to the middle between two codes either may be taken
  * An infinity or NaN among them makes the block's scale NaN until the block
  * starts anew.  The tokens of one block must stand side by side in `slots`, in
- * the order of their slots (as engpt_advance_block_tables gives them); a call
- * in which they do not leaves some of that block's numbers undefined.
+ * slots that follow one another (s, s + 1, ..; as engpt_advance_block_tables
+ * gives them).  A token beside another one of its block that is not in the next
+ * slot is recorded (ENGPT_ERR_ARG, site 43) and left out, with those that follow
+ * it; with tokens of other blocks or slots of -1 between those of one block,
+ * that block's numbers are undefined.
  */
 typedef enum engpt_code {
   ENGPT_CODE_INT8 = 0,

@@ -6,7 +6,8 @@ import torch
 
 from engpt_b200 import _lib, kernels as K
 from tests import paged_q8_blocks as B, paged_q8_ref as Q, paged_ref as R
-from tests.test_gpu_paged_q8 import (DTYPES, KINDS, append_error, append_inputs, attend, attention_inputs, expect_status)
+from tests.test_gpu_paged_q8 import (DTYPES, KINDS, append_error, append_inputs, attend, attention_inputs,
+                                     expect_status, rows)
 from tests.test_gpu_paged_q8_large import check_both, sizes, state
 
 pytestmark = pytest.mark.gpu
@@ -103,6 +104,46 @@ def test_append_radii_of_tokens_that_are_left_out(cuda, dtype, kind, dim, block,
     _, rk, rv = B.postprocess(qkv, rho, cos, sin, scale, 1e-6, pos.clamp(0, 49))
     rk[dead], rv[dead] = 0.0, 0.0
     check_both(cache, before, rk, rv, slots, append_error(rk), append_error(rv), dead)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("append", [False, True])
+@pytest.mark.parametrize("dim,block,n", CALLS)
+@pytest.mark.parametrize("step", ["gap", "down", "twice"])
+def test_slots_that_do_not_follow_one_another(cuda, dtype, kind, append, dim, block, n, step):
+    """A token beside another one of its block, but not in the next slot, is recorded and left out with those behind it; the
+    tokens before it, and the other blocks, are written as if it were not there."""
+    heads, page = 16, 64
+    n = tokens_of(n, heads)
+    slots = torch.arange(n, dtype=torch.int32, device=cuda)
+    given, kept = slots.clone(), slots.clone()
+    for b in range(1, n // block, 3):
+        at = b * block + 3
+        if step == "gap":                                          # .., 2, 4, 5, ..
+            given[at:at + block - 4] += 1
+            given[b * block + block - 1] = -1
+        elif step == "down":                                       # .., 2, 1 (the rest -1)
+            given[at] = at - 2
+            given[at + 1:(b + 1) * block] = -1
+        else:                                                      # .., 2, 2, 3, ..
+            given[at:(b + 1) * block] -= 1
+        kept[at:(b + 1) * block] = -1
+    cache = Q.make_pools(n // page, heads, page, dim, block, kind)
+    Q.fill_pools(cache, 4)
+    before = state(cache)
+    if append:
+        qkv, rho, cos, sin, scale, pos = append_inputs(n, heads, dim, dtype, 5)
+        q = K.qkv_append_from_carried_q8(qkv, rho, cos, sin, scale, 1e-6, pos, given, *cache)
+        rq, rk, rv = B.postprocess(qkv, rho, cos, sin, scale, 1e-6, pos)
+        assert ((q.double() - rq).abs() <= torch.finfo(dtype).eps / 2 * rq.abs() + append_error(rq)).all()
+        err = append_error(rk), append_error(rv)
+    else:
+        k, v = rows(n, heads, dim, dtype, 5)
+        K.write_kv_pages_q8(k, v, given, *cache)
+        rk, rv, err = k.double(), v.double(), (0.0, 0.0)
+    expect_status(43)
+    check_both(cache, before, rk, rv, kept, *err)
 
 
 # ------------------------------------------------------------------ attention
